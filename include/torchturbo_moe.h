@@ -409,6 +409,86 @@ int tt_moe_experts_fwd(const void* x, int dtype, int64_t num_tokens, int64_t hid
                        int act, float limit, int clamp_after, int64_t* tokens_per_expert,
                        void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Dense products of the layer ----------------------------------------
+ * A shared expert's linears (moe_layer.py:175-182; the products, adds and gates
+ * around them are separate torch calls in the reference). Tensors are row-major
+ * and contiguous, x [m, k] and w [rows, k] (out x in) share `dtype` (f32, bf16,
+ * f16); a bias and a row scale may each have any of the three. Sums run in
+ * fp32 and are rounded once, where they are stored. Any size, 0 included; 16-bit
+ * operands whose k and n are multiples of 8 and whose addresses are multiples of
+ * 16 run on the 16-bit matrix instructions, all others on the fp32 ones.
+ * activation: 0 none, 1 SiLU, 2 GELU (erf form).
+ *
+ * tt_linear_workspace: bytes of scratch for an op of these sizes (0: none). With
+ * less, TT_LINEAR_ACT / _GATED / _RESIDUAL / _WGRAD do not split their reductions.
+ *
+ * tt_linear_act_fwd: a = x w^T + bias; y [m, n] = act(a), w [n, k]; gated: y =
+ *   act(a[:, :n]) * a[:, n:], w [2n, k], the gate's rows first. pre (or NULL): a in
+ *   fp32, [m, n] or [m, 2n], for the backward.
+ * tt_linear_act_bwd: da [m, n or 2n] (dtype) from dy and pre, and dbias = its
+ *   column sums, summed before da is rounded (TT_LINEAR_COLSUM workspace), or
+ *   NULL. Then tt_linear_dgrad and tt_linear_wgrad of da.
+ * tt_linear_residual_fwd: y [m, n] = residual + row_scale[i] * drop(x w^T + bias),
+ *   each of residual, row_scale and bias NULL where there is none; drop as tt_dropout
+ *   with `threshold` and `key` (threshold 0: no dropout).
+ * tt_linear_residual_bwd: g = dy with the dropped elements cleared (written only
+ *   with dropout; without it g is dy itself), and dbias = the column sums of
+ *   row_scale * drop(dy) (TT_LINEAR_COLSUM workspace), or NULL.
+ * tt_linear_dgrad: with c = the inverse of the kept share (threshold as in the
+ *   forward, 0: c = 1): dx [m, k] = row_scale[i] * c * (g w), w [n, k]; and with a row
+ *   scale, where not NULL, xs = row_scale * x for the weight gradient, and dscale [m] =
+ *   c * (<x_i, (g w)_i> + <g_i, bias>). dx may be NULL. TT_LINEAR_DGRAD workspace,
+ *   needed for dscale.
+ * tt_linear_wgrad: dw [n, k] = c * g^T x. */
+enum { TT_LINEAR_ACT = 0, TT_LINEAR_GATED = 1, TT_LINEAR_RESIDUAL = 2, TT_LINEAR_DGRAD = 3,
+       TT_LINEAR_WGRAD = 4, TT_LINEAR_COLSUM = 5 };
+size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t k, int64_t n);
+int tt_linear_act_fwd(const void* x, const void* w, const void* bias, int bias_dtype, int dtype,
+                      int64_t m, int64_t k, int64_t n, int32_t activation, int32_t gated,
+                      float* pre, void* y, void* workspace, size_t workspace_bytes, void* stream);
+int tt_linear_act_bwd(const void* dy, const float* pre, int dtype, int64_t m, int64_t n,
+                      int32_t activation, int32_t gated, void* da, void* dbias, int bias_dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int tt_linear_residual_fwd(const void* x, const void* w, const void* bias, int bias_dtype,
+                           const void* residual, const void* row_scale, int scale_dtype, int dtype,
+                           int64_t m, int64_t k, int64_t n, int32_t threshold, const int64_t* key,
+                           void* y, void* workspace, size_t workspace_bytes, void* stream);
+int tt_linear_residual_bwd(const void* dy, const void* row_scale, int scale_dtype, int dtype,
+                           int64_t m, int64_t n, int32_t threshold, const int64_t* key, void* g,
+                           void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes,
+                           void* stream);
+int tt_linear_dgrad(const void* g, const void* w, const void* x, const void* row_scale,
+                    int scale_dtype, const void* bias, int bias_dtype, int dtype, int64_t m,
+                    int64_t k, int64_t n, int32_t threshold, void* dx, void* xs, void* dscale,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int tt_linear_wgrad(const void* g, const void* x, int dtype, int64_t m, int64_t k, int64_t n,
+                    int32_t threshold, void* dw, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* ---- Dropout from a counter-based generator ------------------------------
+ * y = x / (share kept) where an element is kept, else 0 (whatever it held); x and
+ * y [rows, cols] f32 / bf16 / f16. Element (r, c) is dropped when 16
+ * bits of Philox4x32-10, key = key[0], counter = (c / 8, r, key[1]), are below
+ * `threshold`: bits 16 (c % 2) .. + 15 of word (c % 8) / 2. So the share dropped is
+ * threshold / 65536 (0 none, 65536 all), and the backward is the same call on
+ * the gradient: no mask is stored. key: two int64 on the device. rows < 2^32. */
+int tt_dropout(const void* x, int dtype, int64_t rows, int64_t cols, int32_t threshold,
+               const int64_t* key, void* y, void* stream);
+
+/* The LoRA residual's three kernels with such a dropout on the rows of x (packed
+ * row, column): h = c (keep x) A, dx = keep c dh A^T rounded once, dA = c (keep x)^T
+ * dh, c the inverse of the kept share, in fp32 with the sums. Operands as in
+ * tt_lora_down / _up / _wgrad; threshold in [1, 65536]. */
+int tt_lora_down_dropout(const void* x, const float* a, int dtype, int64_t m, int64_t k, int32_t r,
+                         int32_t num_experts, const int64_t* counts, int32_t threshold,
+                         const int64_t* key, float* h, void* stream);
+int tt_lora_up_dropout(const float* dh, const float* a, int dtype, int64_t m, int64_t k, int32_t r,
+                       int32_t num_experts, const int64_t* counts, int32_t threshold,
+                       const int64_t* key, void* dx, void* stream);
+int tt_lora_wgrad_dropout(const void* x, const float* dh, int dtype, int64_t m, int64_t k,
+                          int32_t r, int32_t num_experts, const int64_t* counts, int32_t threshold,
+                          const int64_t* key, float* da, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,9 @@ reference checkout):
   ``src/torchturbo/models/modules/moe/utils.py:30-80,127-230``
 * ``native_providers/grouped_matmul_fp8.py`` and ``fp8.py`` —
   ``scripts/dequant/bailing.py:57-102``, ``scripts/dequant/dequantize.py:62-78``
+* ``native_providers/linear.py`` and ``dropout.py`` — the shared expert's products
+  (``src/torchturbo/models/modules/moe/moe_layer.py:175-182`` around the HF block's
+  linears) and dropout from a counter-based generator (no reference counterpart)
 * ``route_np.py`` — numpy restatement of the packed-row order defined by
   ``src/torchturbo/ops/moe.py:10-46`` (integer work, independent of torch)
 * ``layer.py`` — the composition of

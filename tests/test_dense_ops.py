@@ -1,0 +1,347 @@
+"""Dense products with an epilogue, counter-based dropout and the modules over them, on
+the CPU: the oracle's own pins, the refusals of the HIP providers and of the C entry
+points (checked before anything reaches a GPU), and the module logic with the oracle's
+providers."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle.native_providers import dropout as o_dropout
+from oracle.native_providers import linear as o_linear
+from torchturbo_amd import _lib as L
+from torchturbo_amd.dispatch import OpPolicy, ops
+from torchturbo_amd.moe import (CounterDropout, GroupedMLP, GroupedMLPLoRA, MoEConfig, MoELayer,
+                                MoESubmodules, ModuleSpec, SharedExpertMLP)
+from torchturbo_amd.providers.hip.dropout import HipDropout, drop_threshold
+from torchturbo_amd.providers.hip.linear import HipLinearAct, HipLinearResidual
+from torchturbo_amd.providers.hip.lora import HipLoRAResidual
+from torchturbo_amd.runtime import CpuRuntime
+
+
+# ---------------------------------------------------------------------------
+# The oracle
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("counter, key, words", [
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+     (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_philox_published_vectors(counter, key, words):
+    got = o_dropout.philox4x32([np.uint64(c) for c in counter], key)
+    assert tuple(int(w) for w in got) == words
+
+
+def test_oracle_mask_is_the_positions():
+    """A tensor's first rows and columns take the mask that the smaller tensor takes."""
+    key = torch.tensor([-5, 1 << 40])
+    big = o_dropout.factors(37, 53, 0.3, key)
+    assert torch.equal(big[:11, :9], o_dropout.factors(11, 9, 0.3, key))
+    assert abs((big == 0).double().mean().item() - 0.3) < 0.05
+    assert not torch.equal(big, o_dropout.factors(37, 53, 0.3, key + 1))
+
+
+def test_oracle_products_are_exact_on_integers():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(-4, 5, (5, 3, 12), generator=g).float()
+    w, b = (torch.randint(-4, 5, s, generator=g).float() for s in ((8, 12), (8,)))
+    r = torch.randint(-4, 5, (5, 3, 8), generator=g).float()
+    s = torch.tensor([0.0, 0.5, -2.0]).repeat(5, 1)
+    plain = torch.einsum("abk,nk->abn", x, w) + b
+    assert torch.equal(o_linear.linear_act(x, w, b), plain)
+    assert torch.equal(o_linear.linear_residual(x, w, b, r, s), r + s[..., None] * plain)
+    assert torch.equal(o_linear.linear_act(x, w, b, activation_func=F.silu, gated=True),
+                       F.silu(plain[..., :4]) * plain[..., 4:])
+
+
+@pytest.mark.parametrize("act, gated", [(None, False), (F.silu, True), (F.gelu, True),
+                                        (F.gelu, False)])
+def test_oracle_gradients_by_differences(act, gated):
+    g = torch.Generator().manual_seed(1)
+    x, w, b = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((3, 5), (8, 5), (8,)))
+    w2, b2 = (torch.randn(s, generator=g, dtype=torch.float64)
+              for s in ((6, 4 if gated else 8), (6,)))
+    r, s = (torch.randn(v, generator=g, dtype=torch.float64) for v in ((3, 6), (3, 1)))
+    key = torch.tensor([3, 4])
+    leaves = [t.requires_grad_() for t in (x, w, b, w2, b2, r, s)]
+
+    def both(x, w, b, w2, b2, r, s):
+        h = o_linear.linear_act(x, w, b, activation_func=act, gated=gated)
+        return o_linear.linear_residual(h, w2, b2, r, s, dropout_p=0.25, dropout_key=key)
+
+    assert torch.autograd.gradcheck(both, leaves)
+
+
+# ---------------------------------------------------------------------------
+# Refusals
+# ---------------------------------------------------------------------------
+def test_drop_threshold():
+    assert [drop_threshold(p) for p in (0, 1, 0.5, 1e-9, 1 - 1e-9, 0.1)] == \
+        [0, 65536, 32768, 1, 65535, 6554]
+    assert all(drop_threshold(p) == o_dropout.threshold_of(p)
+               for p in (0.0, 1.0, 0.05, 0.1, 0.3, 1e-7))
+    for p in (-0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError, match="dropout probability"):
+            drop_threshold(p)
+    with pytest.raises(ValueError, match="dropout probability"):
+        CounterDropout(1.5)
+
+
+KEY = torch.tensor([1, 2])
+
+
+@pytest.mark.parametrize("call, message", [
+    (lambda x, w: HipLinearAct()(x, w.half()), "x and weight must both be"),
+    (lambda x, w: HipLinearAct()(x.double(), w.double()), "x and weight must both be"),
+    (lambda x, w: HipLinearAct()(x[:, :5], w), "x has 5 features"),
+    (lambda x, w: HipLinearAct()(x, w[0]), r"expects x \[..., in\]"),
+    (lambda x, w: HipLinearAct()(x, w, torch.zeros(5)), r"the bias must be .* \[6\]"),
+    (lambda x, w: HipLinearAct()(x, w, torch.zeros(6, dtype=torch.int32)), "the bias must be"),
+    (lambda x, w: HipLinearAct()(x, w[:5], gated=True), "even number of rows"),
+    (lambda x, w: HipLinearAct()(x, w, activation_func=F.relu), "only supports"),
+    (lambda x, w: HipLinearAct()(x, w), "HIP kernels need device tensors"),
+    (lambda x, w: HipLinearResidual()(x, w, None, torch.zeros(4, 5)), "the residual must be"),
+    (lambda x, w: HipLinearResidual()(x, w, None, torch.zeros(4, 6).half()), "the residual must be"),
+    (lambda x, w: HipLinearResidual()(x, w, None, torch.zeros(1, 6)), "the residual must be"),
+    (lambda x, w: HipLinearResidual()(x, w, None, None, torch.zeros(4, 6)), "row_scale must be"),
+    (lambda x, w: HipLinearResidual()(x, w, None, None, torch.zeros(1)), "row_scale must be"),
+    (lambda x, w: HipLinearResidual()(x, w, dropout_p=0.5), "needs a key"),
+    (lambda x, w: HipLinearResidual()(x, w, dropout_p=0.5, dropout_key=KEY.int()), "needs a key"),
+    (lambda x, w: HipLinearResidual()(x, w, dropout_p=2.0), "dropout probability"),
+    (lambda x, w: HipLinearResidual()(x, w), "HIP kernels need device tensors"),
+    (lambda x, w: HipDropout()(x.double(), 0.5, KEY), "takes f32, bf16 or f16"),
+    (lambda x, w: HipDropout()(x[0, 0], 0.5, KEY), "at least one dimension"),
+    (lambda x, w: HipDropout()(x, 0.5, KEY[:1]), "needs a key"),
+    (lambda x, w: HipDropout()(x, 0.5, None), "needs a key"),
+    (lambda x, w: HipDropout()(x, 0.5, KEY), "HIP kernels need device tensors"),
+    (lambda x, w: HipLoRAResidual()(x, x, w, w, KEY, 1.0, dropout_p=-1), "dropout probability"),
+])
+def test_refusals_of_the_providers(call, message):
+    with pytest.raises(ValueError, match=message):
+        call(torch.zeros(4, 8), torch.zeros(6, 8))
+
+
+def null(name, **given):
+    """A call of a C entry point with null pointers and sizes that would be taken but for ``given``."""
+    sizes = {"m": 4, "k": 8, "n": 8, "dtype": L.TT_BF16, "act": 1, "gated": 1, "t": 0, "bias": None,
+             "bias_dt": L.TT_F32, "scale": None, "scale_dt": L.TT_F32, "key": None, "ds": None,
+             "xs": None}
+    s = {**sizes, **given}
+    args = {
+        "tt_linear_act_fwd": lambda: (None, None, s["bias"], s["bias_dt"], s["dtype"], s["m"],
+                                      s["k"], s["n"], s["act"], s["gated"], None, None, None, 0,
+                                      None),
+        "tt_linear_act_bwd": lambda: (None, None, s["dtype"], s["m"], s["n"], s["act"], s["gated"],
+                                      None, s["bias"], s["bias_dt"], None, 0, None),
+        "tt_linear_residual_fwd": lambda: (None, None, s["bias"], s["bias_dt"], None, s["scale"],
+                                           s["scale_dt"], s["dtype"], s["m"], s["k"], s["n"],
+                                           s["t"], s["key"], None, None, 0, None),
+        "tt_linear_residual_bwd": lambda: (None, s["scale"], s["scale_dt"], s["dtype"], s["m"],
+                                           s["n"], s["t"], s["key"], None, s["bias"],
+                                           s["bias_dt"], None, 0, None),
+        "tt_linear_dgrad": lambda: (None, None, None, s["scale"], s["scale_dt"], s["bias"],
+                                    s["bias_dt"], s["dtype"], s["m"], s["k"], s["n"], s["t"], None,
+                                    s["xs"], s["ds"], None, 0, None),
+        "tt_linear_wgrad": lambda: (None, None, s["dtype"], s["m"], s["k"], s["n"], s["t"], None,
+                                    None, 0, None),
+        "tt_dropout": lambda: (None, s["dtype"], s["m"], s["n"], s["t"], s["key"], None, None),
+        "tt_lora_down_dropout": lambda: (None, None, s["dtype"], s["m"], s["k"], 4, 2, None, s["t"],
+                                         s["key"], None, None),
+        "tt_lora_up_dropout": lambda: (None, None, s["dtype"], s["m"], s["k"], 4, 2, None, s["t"],
+                                       s["key"], None, None),
+        "tt_lora_wgrad_dropout": lambda: (None, None, s["dtype"], s["m"], s["k"], 4, 2, None,
+                                          s["t"], s["key"], None, None),
+    }[name]()
+    L.call(name, *args)
+
+
+P = ctypes.c_void_p(16)
+
+
+@pytest.mark.parametrize("name, given, message", [
+    ("tt_linear_act_fwd", {"dtype": L.TT_F64}, "must be f32, bf16 or f16"),
+    ("tt_linear_act_fwd", {"m": -1}, "bad sizes"),
+    ("tt_linear_act_fwd", {"n": 1 << 30}, "bad sizes"),
+    ("tt_linear_act_fwd", {"act": 3}, "unknown activation"),
+    ("tt_linear_act_fwd", {"bias": P, "bias_dt": L.TT_F8E4M3}, "the bias must be"),
+    ("tt_linear_act_bwd", {"act": -1}, "unknown activation"),
+    ("tt_linear_act_bwd", {"bias": P}, "workspace is too small"),
+    ("tt_linear_residual_fwd", {"t": 65537}, "threshold must be"),
+    ("tt_linear_residual_fwd", {"t": 5}, "dropout without a key"),
+    ("tt_linear_residual_fwd", {"scale": P, "scale_dt": L.TT_F64}, "the row scale must be"),
+    ("tt_linear_residual_bwd", {"t": 5, "key": P}, "a place for its gradient"),
+    ("tt_linear_residual_bwd", {"bias": P}, "workspace is too small"),
+    ("tt_linear_dgrad", {"xs": P}, "need a row scale"),
+    ("tt_linear_dgrad", {"ds": P}, "need a row scale"),
+    ("tt_linear_dgrad", {"scale": P}, "a row scale needs x"),
+    ("tt_linear_wgrad", {"t": -1}, "threshold must be"),
+    ("tt_dropout", {"dtype": L.TT_F64}, "must be f32, bf16 or f16"),
+    ("tt_dropout", {"m": 1 << 32}, "bad sizes"),
+    ("tt_dropout", {"t": 65537}, "threshold must be"),
+    ("tt_dropout", {"t": 5}, "null pointer"),
+    ("tt_lora_down_dropout", {"t": 0}, "threshold must be"),
+    ("tt_lora_up_dropout", {"t": 5}, "dropout without a key"),
+    ("tt_lora_wgrad_dropout", {"t": 5, "k": 9, "key": P}, "multiples of 8"),
+])
+def test_refusals_of_the_entry_points(name, given, message):
+    with pytest.raises(ValueError, match=message):
+        null(name, **given)
+
+
+def test_empty_calls_of_the_entry_points_launch_nothing():
+    null("tt_linear_act_fwd", m=0)
+    null("tt_linear_residual_fwd", n=0)
+    null("tt_linear_wgrad", k=0)
+    null("tt_linear_dgrad", m=0)
+    null("tt_dropout", n=0)
+    null("tt_lora_down_dropout", m=0, t=5, key=P)
+
+
+# ---------------------------------------------------------------------------
+# Modules
+# ---------------------------------------------------------------------------
+def shared_config(gated=True, act=F.silu, **more):
+    return MoEConfig(hidden_size=16, num_moe_experts=4, moe_ffn_hidden_size=8, moe_router_topk=2,
+                     gated_linear_unit=gated, activation_func=act,
+                     moe_shared_expert_intermediate_size=12, **more)
+
+
+@pytest.mark.parametrize("gated, act, bias", [(True, F.silu, False), (True, F.gelu, True),
+                                              (False, F.gelu, True)])
+def test_shared_expert_is_the_dense_mlp(process_ops, gated, act, bias):
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    torch.manual_seed(3)
+    mlp = SharedExpertMLP(shared_config(gated, act), bias=bias)
+    names = ["up_proj", "down_proj"] + (["gate_proj"] if gated else [])
+    hf = {}
+    for n in names:
+        rows, cols = (16, 12) if n == "down_proj" else (12, 16)
+        hf[n + ".weight"] = torch.randn(rows, cols)
+        if bias:
+            hf[n + ".bias"] = torch.randn(rows)
+    mlp.load_state_dict(hf)
+    x = torch.randn(2, 5, 16)
+
+    def lin(n, v):
+        return F.linear(v, hf[n + ".weight"], hf.get(n + ".bias"))
+
+    h = act(lin("gate_proj", x)) * lin("up_proj", x) if gated else act(lin("up_proj", x))
+    torch.testing.assert_close(mlp(x), lin("down_proj", h))
+    r, s = torch.randn(2, 5, 16), torch.rand(2, 5, 1)
+    torch.testing.assert_close(mlp(x, r, s), r + s * lin("down_proj", h))
+
+
+def test_shared_expert_arguments(process_ops):
+    with pytest.raises(ValueError, match="moe_shared_expert_intermediate_size"):
+        SharedExpertMLP(MoEConfig(hidden_size=8, activation_func=F.silu))
+    with pytest.raises(ValueError, match="silu or gelu"):
+        SharedExpertMLP(shared_config(act=F.relu))
+
+
+def test_shared_expert_dropout_follows_the_generator(process_ops):
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    torch.manual_seed(4)
+    mlp = SharedExpertMLP(shared_config(), dropout=0.4)
+    x, r = torch.randn(7, 16), torch.randn(7, 16)
+    torch.manual_seed(5)
+    a, b = mlp(x, r), mlp(x, r)
+    torch.manual_seed(5)
+    assert torch.equal(mlp(x, r), a) and not torch.equal(a, b)
+    assert 0 < (a == r).sum() < a.numel()  # dropped elements leave the residual
+    mlp.eval()
+    torch.testing.assert_close(mlp(x, r), r + mlp(x))
+
+
+class _Plain(torch.nn.Module):
+    """The same expert as its own module: the layer's earlier path."""
+
+    def __init__(self, mlp):
+        super().__init__()
+        self.mlp = mlp
+
+    def forward(self, x):
+        return self.mlp(x)
+
+
+@pytest.mark.parametrize("gate_width", [1, 16])
+def test_layer_adds_the_shared_expert(process_ops, gate_width):
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    torch.manual_seed(6)
+    cfg = shared_config()
+    layer = MoELayer(cfg, None, MoESubmodules(experts=ModuleSpec(module=GroupedMLP),
+                                              shared_experts=ModuleSpec(module=SharedExpertMLP)))
+    layer.shared_expert = SharedExpertMLP(cfg)
+    layer.shared_expert_gate = torch.nn.Linear(16, gate_width, bias=False)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.normal_(std=0.2)
+    x = torch.randn(3, 5, 16)
+    got, _ = layer(x)
+    grads = torch.autograd.grad(got.square().sum(), list(layer.parameters()))
+    one, two = layer.shared_expert, layer.shared_experts
+    layer.shared_expert, layer.shared_experts = _Plain(one), _Plain(two)
+    want, _ = layer(x)
+    torch.testing.assert_close(got, want)
+    for a, b in zip(grads, torch.autograd.grad(want.square().sum(), list(layer.parameters()))):
+        torch.testing.assert_close(a, b)
+
+
+def test_counter_dropout_module(process_ops):
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    drop = CounterDropout(0.25)
+    x = torch.randn(64, 40)
+    torch.manual_seed(1)
+    y, z = drop(x), drop(x)
+    torch.manual_seed(1)
+    assert torch.equal(drop(x), y) and not torch.equal(y, z)
+    kept = y != 0
+    torch.testing.assert_close(y[kept], x[kept] / 0.75, rtol=1e-5, atol=0)
+    drop.eval()
+    assert drop(x) is x
+    assert CounterDropout(0.0)(x) is x and "p=0.25" in repr(drop)
+
+
+def test_lora_counter_dropout_is_opt_in(process_ops):
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    cfg = MoEConfig(hidden_size=8, moe_ffn_hidden_size=6, gated_linear_unit=True,
+                    activation_func=F.silu)
+    torch.manual_seed(2)
+    base = GroupedMLP(2, False, cfg)
+    with torch.no_grad():
+        for p in base.parameters():
+            p.normal_(std=0.3)
+    plain = GroupedMLPLoRA(base, "default", r=2, lora_dropout=0.3)
+    assert type(plain.lora_dropout["default"]) is torch.nn.Dropout
+    lora = GroupedMLPLoRA(base, "default", r=2, lora_dropout=0.3, counter_dropout=True,
+                          init_lora_weights="gaussian")
+    assert type(lora.lora_dropout["default"]) is CounterDropout
+    with torch.no_grad():
+        for n, p in lora.named_parameters():
+            if "lora_B" in n:
+                p.normal_()
+    x, counts, probs = torch.randn(9, 8), torch.tensor([4, 5]), torch.rand(9)
+    torch.manual_seed(7)
+    got, _ = lora(x, counts, probs)
+    torch.manual_seed(7)
+    keys = [CounterDropout.draw_key("cpu") for _ in range(2)]
+
+    def residual(v, a, b, key):
+        d = ops.dropout(v, 0.3, key)
+        return ops.grouped_matmul(ops.grouped_matmul(d, a.weight, counts), b.weight,
+                                  counts) * lora.scaling["default"]
+
+    w1, w2 = base.weight1.view(2, 8, -1), base.weight2.view(2, 6, 8)
+    h = ops.grouped_matmul(x, w1, counts) + residual(x, lora.lora_A["default"],
+                                                     lora.lora_B["default"], keys[0])
+    act = base.activation_func_with_probs(h, probs)
+    want = ops.grouped_matmul(act, w2, counts) + residual(act, lora.lora_A2["default"],
+                                                          lora.lora_B2["default"], keys[1])
+    torch.testing.assert_close(got, want)
+    lora.eval()
+    assert torch.equal(lora(x, counts, probs)[0], lora(x, counts, probs)[0])

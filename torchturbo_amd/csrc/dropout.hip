@@ -1,0 +1,102 @@
+// Dropout with a counter-based mask (gfx950): y = keep x / (share kept), the
+// mask of element (row, col) as in philox.h, so nothing but the key is stored
+// for the backward, which is the same call on the gradient. A dropped element is
+// 0 whatever it held (infinities and NaN included).
+#include "philox.h"
+
+namespace {
+
+constexpr int DR_NT = 256;
+constexpr int DR_ROWS = 4;  // rows in flight per thread
+
+// Lanes along the groups of eight columns (L of a block's 256 threads, a power
+// of two), the others along rows; a thread keeps its group and walks rows.
+template <class TT, bool VEC>
+__global__ __launch_bounds__(DR_NT) void dropout_kernel(const typename TT::storage* __restrict__ x,
+                                                        typename TT::storage* __restrict__ y,
+                                                        int64_t rows, int64_t cols, int L,
+                                                        uint32_t threshold, float inv,
+                                                        const int64_t* __restrict__ key) {
+  typedef typename TT::storage St;
+  const DropKey dk = load_key(key);
+  const int64_t group = (int64_t)blockIdx.y * L + (threadIdx.x & (L - 1));
+  const int64_t c0 = 8 * group;
+  if (c0 >= cols) return;
+  const int64_t step = (int64_t)gridDim.x * (DR_NT / L);
+  const int64_t first = (int64_t)blockIdx.x * (DR_NT / L) + threadIdx.x / L;
+  for (int64_t r0 = first; r0 < rows; r0 += step * DR_ROWS) {
+    St v[DR_ROWS][8];
+#pragma unroll
+    for (int q = 0; q < DR_ROWS; ++q) {
+      const int64_t r = r0 + q * step;
+      if (r >= rows) break;
+      if constexpr (VEC) {
+        __builtin_memcpy(v[q], x + r * cols + c0, sizeof(v[q]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c0 + j < cols) v[q][j] = x[r * cols + c0 + j];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < DR_ROWS; ++q) {
+      const int64_t r = r0 + q * step;
+      if (r >= rows) break;
+      uint32_t w[4];
+      philox(dk, (uint32_t)group, (uint32_t)r, w);
+      St o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        o[j] = keeps(w, j, threshold) ? TT::from_f32(TT::to_f32(v[q][j]) * inv) : St(0);
+      if constexpr (VEC) {
+        __builtin_memcpy(y + r * cols + c0, o, sizeof(o));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c0 + j < cols) y[r * cols + c0 + j] = o[j];
+      }
+    }
+  }
+}
+
+template <class TT>
+int launch(const void* x, void* y, int64_t rows, int64_t cols, int32_t threshold,
+           const int64_t* key, hipStream_t s) {
+  typedef typename TT::storage St;
+  const int64_t groups = (cols + 7) / 8;
+  int L = 1;
+  while (L < DR_NT && L < groups) L *= 2;
+  const int64_t gy = (groups + L - 1) / L;
+  int64_t gx = (rows + (DR_NT / L) * DR_ROWS - 1) / ((DR_NT / L) * DR_ROWS);
+  TT_REQUIRE(gy <= 65535, "dropout: too many columns (%lld)", (long long)cols);
+  if (gx > 0x7fffffff) gx = 0x7fffffff;
+  const bool vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) |
+                                      reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  const dim3 grid((unsigned)gx, (unsigned)gy), block(DR_NT);
+  const float inv = keep_inverse(threshold);
+  if (vec)
+    hipLaunchKernelGGL((dropout_kernel<TT, true>), grid, block, 0, s, static_cast<const St*>(x),
+                       static_cast<St*>(y), rows, cols, L, (uint32_t)threshold, inv, key);
+  else
+    hipLaunchKernelGGL((dropout_kernel<TT, false>), grid, block, 0, s, static_cast<const St*>(x),
+                       static_cast<St*>(y), rows, cols, L, (uint32_t)threshold, inv, key);
+  return tt_check_launch("dropout");
+}
+
+}  // namespace
+
+extern "C" int tt_dropout(const void* x, int dtype, int64_t rows, int64_t cols, int32_t threshold,
+                          const int64_t* key, void* y, void* stream) {
+  TT_REQUIRE(rows >= 0 && cols >= 0 && rows < (1ll << 32), "dropout: bad sizes");
+  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "dropout: the threshold must be in [0, 65536]");
+  TT_REQUIRE(dtype == TT_F32 || dtype == TT_BF16 || dtype == TT_F16,
+             "dropout: x must be f32, bf16 or f16");
+  if (rows == 0 || cols == 0) return TT_OK;
+  TT_REQUIRE(x != nullptr && y != nullptr && key != nullptr, "dropout: null pointer");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TT_BF16: return launch<BF16T>(x, y, rows, cols, threshold, key, s);
+    case TT_F16: return launch<F16T>(x, y, rows, cols, threshold, key, s);
+    default: return launch<F32T>(x, y, rows, cols, threshold, key, s);
+  }
+}

@@ -1,0 +1,205 @@
+// What the kernels of the dense products share: the product's description and
+// what becomes of its sums (bias, activation, gate, dropout, row scale, residual).
+#pragma once
+
+#include <math.h>
+
+#include "philox.h"
+
+// What becomes of the fp32 sums v = sum over r of A(i, r) B(r, j):
+//   ACT    y = act(v + bias)
+//   GATED  y = act(v + bias) * (u + bias'), u the sums of the second J columns
+//   RES    y = residual + scale[i] * drop(v + bias)
+//   DGRAD  y = scale[i] * alpha v; xs = scale[i] * x; dots[i] = sum over j of x * alpha v
+//   PLAIN  y = alpha v
+enum { LIN_ACT = 0, LIN_GATED = 1, LIN_RES = 2, LIN_DGRAD = 3, LIN_PLAIN = 4 };
+// Activations.
+enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2 };
+// Columns that one partial dot product of DGRAD covers.
+constexpr int LIN_DOT = 64;
+
+// C [I, J] of A and B, both of the type of `out` (GATED: B has 2 J columns, the
+// gate's first). Which of A and B has the reduction contiguous in memory is the
+// kernel's template; lda and ldb are the distance of their rows, in elements.
+// Null pointers: that part is left out.
+struct LinArgs {
+  const void* a;
+  const void* b;
+  void* out;
+  int64_t I, J, R, lda, ldb;
+  const void* bias;
+  int bias_dt;
+  int act;
+  float* pre;  // ACT / GATED: v + bias, [I, J] or [I, 2 J] fp32
+  const void* res;
+  const void* scale;
+  int scale_dt;
+  uint32_t threshold;  // RES: 0 is no dropout
+  float alpha;         // RES: 1 / (share kept)
+  const int64_t* key;
+  const void* x;  // DGRAD
+  void* xs;
+  float* dots;  // [I, ceil(J / LIN_DOT)]
+  float* part;  // a split reduction's sums [splits, I, J or 2 J], instead of all of the above
+  int splits;
+  int64_t rsplit;  // reduction elements of a split
+};
+
+namespace {
+
+// The activation and its derivative. 16-bit tensors take the hardware's exp2 and
+// reciprocal (a few ulp of fp32, far below the rounding of what they end in).
+template <class TT>
+__device__ __forceinline__ float lin_sigmoid(float a) {
+  if constexpr (sizeof(typename TT::storage) == 4) return 1.0f / (1.0f + expf(-a));
+  else return __builtin_amdgcn_rcpf(1.0f + __expf(-a));
+}
+template <class TT>
+__device__ __forceinline__ float lin_act(int act, float a) {
+  if (act == ACT_SILU) return a * lin_sigmoid<TT>(a);
+  if (act == ACT_GELU) return 0.5f * a * (1.0f + erff(a * 0.70710678118654752f));
+  return a;
+}
+template <class TT>
+__device__ __forceinline__ void lin_act_grad(int act, float a, float& value, float& slope) {
+  if (act == ACT_SILU) {
+    const float s = lin_sigmoid<TT>(a);
+    value = a * s;
+    slope = s * (1.0f + a * (1.0f - s));
+  } else if (act == ACT_GELU) {
+    const float cdf = 0.5f * (1.0f + erff(a * 0.70710678118654752f));
+    value = a * cdf;
+    slope = cdf + a * 0.39894228040143268f * expf(-0.5f * a * a);
+  } else {
+    value = a;
+    slope = 1.0f;
+  }
+}
+
+// W consecutive elements at p[at], widened; n of them exist (VEC: all, aligned).
+template <class TT, int W, bool VEC>
+__device__ __forceinline__ void lin_load(const void* p, int64_t at, int n, float (&o)[W]) {
+  typedef typename TT::storage St;
+  const St* q = static_cast<const St*>(p) + at;
+  if constexpr (VEC) {
+    St v[W];
+    __builtin_memcpy(v, __builtin_assume_aligned(q, sizeof(St) * W < 16 ? sizeof(St) * W : 16), sizeof(v));
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = TT::to_f32(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = j < n ? TT::to_f32(q[j]) : 0.f;
+  }
+}
+template <class TT, int W, bool VEC>
+__device__ __forceinline__ void lin_store(void* p, int64_t at, int n, const float (&v)[W]) {
+  typedef typename TT::storage St;
+  St* q = static_cast<St*>(p) + at;
+  if constexpr (VEC) {
+    St o[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = TT::from_f32(v[j]);
+    __builtin_memcpy(__builtin_assume_aligned(q, sizeof(St) * W < 16 ? sizeof(St) * W : 16), o, sizeof(o));
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (j < n) q[j] = TT::from_f32(v[j]);
+  }
+}
+
+// W of a vector of `bias` (its own dtype) at column j.
+template <int W>
+__device__ __forceinline__ void lin_bias(const LinArgs& p, int64_t j, int n, float (&o)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) o[e] = e < n ? load_as_f32(p.bias, p.bias_dt, j + e) : 0.f;
+}
+
+// The sums v (GATED: gate v and up u) of row i, columns j .. j + W - 1 (n of
+// them exist) to what KIND makes of them. j is a multiple of W; W is 4 or 8.
+// Returns DGRAD's share of the row's dot product.
+template <int KIND, class TT, int W, bool VEC>
+__device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t j, int n,
+                                            float (&v)[W], float (&u)[W], const DropKey& dk) {
+  float dot = 0.f;
+  if constexpr (KIND == LIN_ACT || KIND == LIN_GATED) {
+    const int64_t width = KIND == LIN_GATED ? 2 * p.J : p.J;
+    if (p.bias != nullptr) {
+      float b[W];
+      lin_bias<W>(p, j, n, b);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] += b[e];
+      if constexpr (KIND == LIN_GATED) {
+        lin_bias<W>(p, p.J + j, n, b);
+#pragma unroll
+        for (int e = 0; e < W; ++e) u[e] += b[e];
+      }
+    }
+    if (p.pre != nullptr) {
+      lin_store<F32T, W, VEC>(p.pre, i * width + j, n, v);
+      if constexpr (KIND == LIN_GATED) lin_store<F32T, W, VEC>(p.pre, i * width + p.J + j, n, u);
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      v[e] = lin_act<TT>(p.act, v[e]);
+      if constexpr (KIND == LIN_GATED) v[e] *= u[e];
+    }
+  } else if constexpr (KIND == LIN_RES) {
+    if (p.bias != nullptr) {
+      float b[W];
+      lin_bias<W>(p, j, n, b);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] += b[e];
+    }
+    if (p.threshold != 0) {
+      uint32_t w[4];
+      philox(dk, (uint32_t)(j >> 3), (uint32_t)i, w);
+      const int at = W == 8 ? 0 : (int)(j & 4);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const bool keep = W == 8 ? keeps(w, e, p.threshold)
+                                 : (at ? keeps(w, 4 + (e & 3), p.threshold) : keeps(w, e & 3, p.threshold));
+        v[e] = keep ? v[e] * p.alpha : 0.f;
+      }
+    }
+    if (p.scale != nullptr) {
+      const float s = load_as_f32(p.scale, p.scale_dt, i);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] *= s;
+    }
+    if (p.res != nullptr) {
+      float r[W];
+      lin_load<TT, W, VEC>(p.res, i * p.J + j, n, r);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] += r[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] *= p.alpha;
+    if constexpr (KIND == LIN_DGRAD) {
+      if (p.scale != nullptr) {
+        const float s = load_as_f32(p.scale, p.scale_dt, i);
+        float x[W];
+        lin_load<TT, W, VEC>(p.x, i * p.J + j, n, x);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          dot += e < n ? x[e] * v[e] : 0.f;
+          v[e] *= s;
+          x[e] *= s;
+        }
+        if (p.xs != nullptr) lin_store<TT, W, VEC>(p.xs, i * p.J + j, n, x);
+      }
+      if (p.out == nullptr) return dot;
+    }
+  }
+  lin_store<TT, W, VEC>(p.out, i * p.J + j, n, v);
+  return dot;
+}
+
+}  // namespace
+
+// Operand layouts of a product: NT: A [I, R], B [J, R]. NN: A [I, R], B [R, J].
+// TN: A [R, I], B [R, J].
+enum { LAY_NT = 0, LAY_NN = 1, LAY_TN = 2 };
+
+// fp32 matrix instructions on any type, size and alignment (linear_any.hip).
+int tt_linear_any(int layout, int kind, int dtype, const LinArgs& a, hipStream_t s);

@@ -1,0 +1,554 @@
+// Dense products with bias, activation, gate, dropout, row scale and residual in
+// their epilogue, and their gradients: which kernel runs a product, the joining of
+// split reductions, and the passes over rows that the gradients need (gfx950).
+#include <algorithm>
+#include <initializer_list>
+
+#include "linear.h"
+
+namespace {
+
+inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
+
+constexpr int L_NT = 256;
+
+// ---------------------------------------------------------------------------
+// Joins the sums of a split reduction, in the order of the splits. A thread
+// takes eight columns; a row's groups of eight are padded to whole LIN_DOT runs
+// so that one run's lanes lie together.
+// ---------------------------------------------------------------------------
+template <int KIND, class TT, bool VEC>
+__global__ __launch_bounds__(L_NT) void linear_join_kernel(LinArgs p, int64_t groups) {
+  const int64_t idx = (int64_t)blockIdx.x * L_NT + threadIdx.x;
+  const int64_t i = idx / groups, j = 8 * (idx % groups);
+  const bool live = i < p.I && j < p.J;
+  const int n = !live ? 0 : p.J - j < 8 ? (int)(p.J - j) : 8;
+  const int64_t width = KIND == LIN_GATED ? 2 * p.J : p.J;
+  float v[8] = {}, u[8] = {};
+  if (live) {
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const int64_t at = ((int64_t)s * p.I + i) * width + j;
+      float t[8];
+      lin_load<F32T, 8, VEC>(p.part, at, n, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
+      if constexpr (KIND == LIN_GATED) {
+        lin_load<F32T, 8, VEC>(p.part, at + p.J, n, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] += t[e];
+      }
+    }
+  }
+  DropKey dk{};
+  if (KIND == LIN_RES && p.threshold != 0) dk = load_key(p.key);
+  float dot = 0.f;
+  if (live) dot = lin_finish<KIND, TT, 8, VEC>(p, i, j, n, v, u, dk);
+  if constexpr (KIND == LIN_DGRAD) {
+    if (p.dots != nullptr) {
+#pragma unroll
+      for (int off = 1; off < LIN_DOT / 8; off <<= 1) dot += __shfl_xor(dot, off, 64);
+      if (live && j % LIN_DOT == 0)
+        p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
+    }
+  }
+}
+
+bool vectors(const LinArgs& p) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) |
+                       reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.res) |
+                       reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.xs) |
+                       reinterpret_cast<uintptr_t>(p.pre);
+  return at % 16 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && p.J % 8 == 0;
+}
+
+template <int KIND, class TT>
+int join(const LinArgs& p, hipStream_t s) {
+  const int64_t run = LIN_DOT / 8, groups = ((p.J + 7) / 8 + run - 1) / run * run;
+  const int64_t blocks = (p.I * groups + L_NT - 1) / L_NT;
+  TT_REQUIRE(blocks < 0x7fffffff, "linear: grid too large");
+  if (vectors(p))
+    hipLaunchKernelGGL((linear_join_kernel<KIND, TT, true>), dim3((unsigned)blocks), dim3(L_NT), 0,
+                       s, p, groups);
+  else
+    hipLaunchKernelGGL((linear_join_kernel<KIND, TT, false>), dim3((unsigned)blocks), dim3(L_NT),
+                       0, s, p, groups);
+  return tt_check_launch("linear_join");
+}
+
+template <class TT>
+int join_kind(int kind, const LinArgs& p, hipStream_t s) {
+  switch (kind) {
+    case LIN_ACT: return join<LIN_ACT, TT>(p, s);
+    case LIN_GATED: return join<LIN_GATED, TT>(p, s);
+    case LIN_RES: return join<LIN_RES, TT>(p, s);
+    case LIN_DGRAD: return join<LIN_DGRAD, TT>(p, s);
+    default: return join<LIN_PLAIN, TT>(p, s);
+  }
+}
+
+// Splits of a reduction of R elements into whole runs of 64.
+struct Split {
+  int splits;
+  int64_t run;
+};
+Split split_of(int64_t R, int64_t wanted) {
+  const int64_t runs = (R + 63) / 64;
+  if (wanted > runs) wanted = runs;
+  if (wanted < 1) wanted = 1;
+  if (runs <= 1) return Split{1, 64};
+  const int64_t per = ((runs + wanted - 1) / wanted) * 64;
+  return Split{(int)((R + per - 1) / per), per};
+}
+
+// How many parts a product's reduction is split into on the kernel for any type:
+// enough for one block per CU, each at least 256 long.
+int64_t any_splits(int kind, int64_t I, int64_t J, int64_t R) {
+  const int64_t bo = kind == LIN_GATED ? 32 : 64;
+  const int64_t tiles = ((I + 63) / 64) * ((J + bo - 1) / bo);
+  int64_t want = 256 / (tiles > 0 ? tiles : 1);
+  if (want > R / 256) want = R / 256;
+  return want < 1 ? 1 : want > 32 ? 32 : want;
+}
+
+size_t part_bytes(int kind, int64_t I, int64_t J, int64_t splits) {
+  return splits <= 1 ? 0 : (size_t)splits * I * J * (kind == LIN_GATED ? 2 : 1) * 4;
+}
+size_t dots_bytes(int64_t I, int64_t J) {
+  return (((size_t)I * ((J + LIN_DOT - 1) / LIN_DOT) * 4) + 255) / 256 * 256;
+}
+
+int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_bytes,
+                hipStream_t s) {
+  Split sp = split_of(p.R, any_splits(kind, p.I, p.J, p.R));
+  if (part_bytes(kind, p.I, p.J, sp.splits) > ws_bytes) sp = split_of(p.R, 1);
+  p.splits = sp.splits;
+  p.rsplit = sp.run;
+  p.part = sp.splits > 1 ? static_cast<float*>(ws) : nullptr;
+  const int rc = tt_linear_any(layout, kind, dtype, p, s);
+  if (rc != TT_OK || p.part == nullptr) return rc;
+  switch (dtype) {
+    case TT_BF16: return join_kind<BF16T>(kind, p, s);
+    case TT_F16: return join_kind<F16T>(kind, p, s);
+    default: return join_kind<F32T>(kind, p, s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Passes over rows. A block takes 256 columns (32 lanes of eight) of a chunk of
+// rows, eight rows at a time; column sums are added in a fixed order: a thread's
+// rows, the block's eight threads of a column, then the chunks.
+// ---------------------------------------------------------------------------
+constexpr int P_COLS = 256, P_ROWS = 8;
+
+__device__ __forceinline__ void chunk_sums(const float (&sum)[8], float* part, int64_t width,
+                                           int64_t j, int64_t J, float* lds) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) lds[ty * P_COLS + 8 * tx + e] = sum[e];
+  __syncthreads();
+  const int c = threadIdx.x;
+  float t = 0.f;
+#pragma unroll
+  for (int y = 0; y < P_ROWS; ++y) t += lds[y * P_COLS + c];
+  const int64_t col = j - 8 * tx + c;
+  if (col < J) part[(int64_t)blockIdx.x * width + col] = t;
+}
+
+// da of y = act(a) (GATED: act(a_g) a_u) from dy and the fp32 a, rounded to the
+// tensor's type, and the column sums of the unrounded da.
+template <class TT, bool GATED, bool VEC>
+__global__ __launch_bounds__(L_NT) void linear_act_bwd_kernel(
+    const typename TT::storage* __restrict__ dy, const float* __restrict__ pre,
+    typename TT::storage* __restrict__ da, float* __restrict__ part, int64_t rows, int64_t J,
+    int64_t per, int act) {
+  __shared__ float lds[P_ROWS * P_COLS];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.y * P_COLS + 8 * tx, width = GATED ? 2 * J : J;
+  const int64_t r0 = (int64_t)blockIdx.x * per, r1 = r0 + per < rows ? r0 + per : rows;
+  const int n = j >= J ? 0 : J - j < 8 ? (int)(J - j) : 8;
+  float sum[8] = {}, sum_u[8] = {};
+  if (n > 0) {
+#pragma unroll 2
+    for (int64_t r = r0 + ty; r < r1; r += P_ROWS) {
+      float d[8], a[8], o[8];
+      lin_load<TT, 8, VEC>(dy, r * J + j, n, d);
+      lin_load<F32T, 8, VEC>(pre, r * width + j, n, a);
+      if constexpr (GATED) {
+        float u[8], ou[8];
+        lin_load<F32T, 8, VEC>(pre, r * width + J + j, n, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float value, slope;
+          lin_act_grad<TT>(act, a[e], value, slope);
+          o[e] = d[e] * u[e] * slope;
+          ou[e] = d[e] * value;
+          sum[e] += o[e];
+          sum_u[e] += ou[e];
+        }
+        lin_store<TT, 8, VEC>(da, r * width + J + j, n, ou);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float value, slope;
+          lin_act_grad<TT>(act, a[e], value, slope);
+          o[e] = d[e] * slope;
+          sum[e] += o[e];
+        }
+      }
+      lin_store<TT, 8, VEC>(da, r * width + j, n, o);
+    }
+  }
+  if (part == nullptr) return;
+  chunk_sums(sum, part, width, j, J, lds);
+  if constexpr (GATED) chunk_sums(sum_u, part + J, width, j, J, lds);
+}
+
+// g = dy with the dropped elements cleared (MASK), and the column sums of
+// scale[i] * g (scale may be null) where part is given.
+template <class TT, bool MASK, bool VEC>
+__global__ __launch_bounds__(L_NT) void linear_res_bwd_kernel(
+    const typename TT::storage* __restrict__ dy, const void* __restrict__ scale, int scale_dt,
+    uint32_t threshold, const int64_t* __restrict__ key, typename TT::storage* __restrict__ g,
+    float* __restrict__ part, int64_t rows, int64_t J, int64_t per) {
+  __shared__ float lds[P_ROWS * P_COLS];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.y * P_COLS + 8 * tx;
+  const int64_t r0 = (int64_t)blockIdx.x * per, r1 = r0 + per < rows ? r0 + per : rows;
+  const int n = j >= J ? 0 : J - j < 8 ? (int)(J - j) : 8;
+  DropKey dk{};
+  if constexpr (MASK) dk = load_key(key);
+  float sum[8] = {};
+  if (n > 0) {
+#pragma unroll 2
+    for (int64_t r = r0 + ty; r < r1; r += P_ROWS) {
+      float d[8];
+      lin_load<TT, 8, VEC>(dy, r * J + j, n, d);
+      if constexpr (MASK) {
+        uint32_t w[4];
+        philox(dk, (uint32_t)(j >> 3), (uint32_t)r, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = keeps(w, e, threshold) ? d[e] : 0.f;
+        lin_store<TT, 8, VEC>(g, r * J + j, n, d);
+      }
+      if (part != nullptr) {
+        const float s = scale != nullptr ? load_as_f32(scale, scale_dt, r) : 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += s * d[e];
+      }
+    }
+  }
+  if (part != nullptr) chunk_sums(sum, part, J, j, J, lds);
+}
+
+// out[j] = alpha * the chunks' sums of column j: 32 columns per block, eight
+// threads to each.
+__global__ __launch_bounds__(L_NT) void linear_colsum_kernel(const float* __restrict__ part,
+                                                             int64_t chunks, int64_t width,
+                                                             float alpha, void* __restrict__ out,
+                                                             int dt) {
+  __shared__ float lds[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + tx;
+  float t = 0.f;
+  if (j < width) {
+#pragma unroll 4
+    for (int64_t c = ty; c < chunks; c += 8) t += part[c * width + j];
+  }
+  lds[ty][tx] = t;
+  __syncthreads();
+  if (ty != 0 || j >= width) return;
+#pragma unroll
+  for (int y = 1; y < 8; ++y) t += lds[y][tx];
+  store_from_f32(out, dt, j, alpha * t);
+}
+
+// out[i] = sum over j of g[i, j] * bias[j], one wave per row.
+__global__ __launch_bounds__(L_NT) void linear_rowdot_kernel(const void* __restrict__ g, int dtype,
+                                                             const void* __restrict__ bias,
+                                                             int bias_dt, int64_t rows, int64_t J,
+                                                             float* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= rows) return;
+  float t = 0.f;
+  for (int64_t j = threadIdx.x & 63; j < J; j += 64)
+    t += load_as_f32(g, dtype, i * J + j) * load_as_f32(bias, bias_dt, j);
+  t = wave_sum(t);
+  if ((threadIdx.x & 63) == 0) out[i] = t;
+}
+
+// out[i] = the dots of row i, in order, + alpha * extra[i].
+__global__ __launch_bounds__(L_NT) void linear_rowsum_kernel(const float* __restrict__ dots, int nd,
+                                                             const float* __restrict__ extra,
+                                                             float alpha, int64_t rows,
+                                                             void* __restrict__ out, int dt) {
+  const int64_t i = (int64_t)blockIdx.x * L_NT + threadIdx.x;
+  if (i >= rows) return;
+  float t = 0.f;
+#pragma unroll 8
+  for (int d = 0; d < nd; ++d) t += dots[i * nd + d];
+  if (extra != nullptr) t += alpha * extra[i];
+  store_from_f32(out, dt, i, t);
+}
+
+// Chunks of rows of a pass over rows x J: about 1024 blocks, whole runs of
+// P_ROWS rows.
+int64_t chunk_rows(int64_t rows, int64_t J) {
+  const int64_t ct = (J + P_COLS - 1) / P_COLS;
+  int64_t chunks = 1024 / (ct > 0 ? ct : 1);
+  if (chunks < 1) chunks = 1;
+  int64_t per = (rows + chunks - 1) / chunks;
+  per = (per + P_ROWS - 1) / P_ROWS * P_ROWS;
+  return per > 0 ? per : P_ROWS;
+}
+
+int sizes_ok(int dtype, int64_t m, int64_t k, int64_t n) {
+  TT_REQUIRE(dtype == TT_F32 || dtype == TT_BF16 || dtype == TT_F16,
+             "linear: tensors must be f32, bf16 or f16");
+  TT_REQUIRE(m >= 0 && k >= 0 && n >= 0 && m < (1ll << 31) && k < (1ll << 31) && n < (1ll << 30),
+             "linear: bad sizes (%lld x %lld x %lld)", (long long)m, (long long)k, (long long)n);
+  return TT_OK;
+}
+int vector_ok(const char* what, const void* p, int dtype) {
+  TT_REQUIRE(p == nullptr || dtype == TT_F32 || dtype == TT_BF16 || dtype == TT_F16,
+             "linear: %s must be f32, bf16 or f16", what);
+  return TT_OK;
+}
+
+#define TT_TRY(call)            \
+  do {                          \
+    const int rc_ = (call);     \
+    if (rc_ != TT_OK) return rc_; \
+  } while (0)
+
+template <typename F>
+int typed(int dtype, F f) {
+  switch (dtype) {
+    case TT_BF16: return f(BF16T{});
+    case TT_F16: return f(F16T{});
+    default: return f(F32T{});
+  }
+}
+
+bool all_aligned(std::initializer_list<const void*> ps) {
+  uintptr_t at = 0;
+  for (const void* p : ps) at |= reinterpret_cast<uintptr_t>(p);
+  return at % 16 == 0;
+}
+
+}  // namespace
+
+extern "C" size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t k, int64_t n) {
+  if (m <= 0 || k < 0 || n < 0) return 0;
+  switch (op) {
+    case TT_LINEAR_ACT: return part_bytes(LIN_ACT, m, n, any_splits(LIN_ACT, m, n, k));
+    case TT_LINEAR_GATED: return part_bytes(LIN_GATED, m, n, any_splits(LIN_GATED, m, n, k));
+    case TT_LINEAR_RESIDUAL: return part_bytes(LIN_RES, m, n, any_splits(LIN_RES, m, n, k));
+    case TT_LINEAR_DGRAD:  // dot products, then the split sums, later the bias's part
+      return dots_bytes(m, k) +
+             std::max(part_bytes(LIN_DGRAD, m, k, any_splits(LIN_DGRAD, m, k, n)), (size_t)m * 4);
+    case TT_LINEAR_WGRAD: return part_bytes(LIN_PLAIN, n, k, any_splits(LIN_PLAIN, n, k, m));
+    case TT_LINEAR_COLSUM: {
+      const int64_t per = chunk_rows(m, n);
+      return (size_t)((m + per - 1) / per) * 2 * n * 4;  // gated: both halves
+    }
+    default: return 0;
+  }
+}
+
+extern "C" int tt_linear_act_fwd(const void* x, const void* w, const void* bias, int bias_dtype,
+                                 int dtype, int64_t m, int64_t k, int64_t n, int32_t act,
+                                 int32_t gated, float* pre, void* y, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  TT_TRY(sizes_ok(dtype, m, k, n));
+  TT_TRY(vector_ok("the bias", bias, bias_dtype));
+  TT_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, "linear: unknown activation %d", act);
+  if (m == 0 || n == 0) return TT_OK;
+  LinArgs p{};
+  p.a = x;
+  p.b = w;
+  p.out = y;
+  p.I = m;
+  p.J = n;
+  p.R = p.lda = p.ldb = k;
+  p.bias = bias;
+  p.bias_dt = bias_dtype;
+  p.act = act;
+  p.pre = pre;
+  return run_product(LAY_NT, gated ? LIN_GATED : LIN_ACT, dtype, p, workspace, workspace_bytes,
+                     S(stream));
+}
+
+extern "C" int tt_linear_act_bwd(const void* dy, const float* pre, int dtype, int64_t m, int64_t n,
+                                 int32_t act, int32_t gated, void* da, void* dbias, int bias_dtype,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  TT_TRY(sizes_ok(dtype, m, 0, n));
+  TT_TRY(vector_ok("the bias", dbias, bias_dtype));
+  TT_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, "linear: unknown activation %d", act);
+  if (n == 0) return TT_OK;
+  const int64_t width = gated ? 2 * n : n, per = chunk_rows(m, n), chunks = (m + per - 1) / per;
+  const int64_t tiles = (n + P_COLS - 1) / P_COLS;
+  TT_REQUIRE(tiles <= 65535, "linear: too many columns");
+  TT_REQUIRE(dbias == nullptr || workspace_bytes >= (size_t)chunks * width * 4,
+             "linear_act_bwd: the workspace is too small");
+  float* part = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
+  if (m > 0) {
+    const bool vec = n % 8 == 0 && all_aligned({dy, pre, da});
+    TT_TRY(typed(dtype, [&](auto tt) {
+      typedef decltype(tt) TT;
+      typedef typename TT::storage St;
+      const dim3 grid((unsigned)chunks, (unsigned)tiles), block(L_NT);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, block, 0, S(stream), static_cast<const St*>(dy), pre,
+                           static_cast<St*>(da), part, m, n, per, (int)act);
+        return tt_check_launch("linear_act_bwd");
+      };
+      if (gated)
+        return vec ? go(&linear_act_bwd_kernel<TT, true, true>)
+                   : go(&linear_act_bwd_kernel<TT, true, false>);
+      return vec ? go(&linear_act_bwd_kernel<TT, false, true>)
+                 : go(&linear_act_bwd_kernel<TT, false, false>);
+    }));
+  }
+  if (dbias == nullptr) return TT_OK;
+  hipLaunchKernelGGL(linear_colsum_kernel, dim3((unsigned)((width + 31) / 32)), dim3(L_NT), 0,
+                     S(stream), part, chunks, width, 1.0f, dbias, bias_dtype);
+  return tt_check_launch("linear_colsum");
+}
+
+extern "C" int tt_linear_residual_fwd(const void* x, const void* w, const void* bias,
+                                      int bias_dtype, const void* residual, const void* row_scale,
+                                      int scale_dtype, int dtype, int64_t m, int64_t k, int64_t n,
+                                      int32_t threshold, const int64_t* key, void* y,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  TT_TRY(sizes_ok(dtype, m, k, n));
+  TT_TRY(vector_ok("the bias", bias, bias_dtype));
+  TT_TRY(vector_ok("the row scale", row_scale, scale_dtype));
+  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
+  TT_REQUIRE(threshold == 0 || key != nullptr, "linear: dropout without a key");
+  if (m == 0 || n == 0) return TT_OK;
+  LinArgs p{};
+  p.a = x;
+  p.b = w;
+  p.out = y;
+  p.I = m;
+  p.J = n;
+  p.R = p.lda = p.ldb = k;
+  p.bias = bias;
+  p.bias_dt = bias_dtype;
+  p.res = residual;
+  p.scale = row_scale;
+  p.scale_dt = scale_dtype;
+  p.threshold = (uint32_t)threshold;
+  p.alpha = keep_inverse(threshold);
+  p.key = key;
+  return run_product(LAY_NT, LIN_RES, dtype, p, workspace, workspace_bytes, S(stream));
+}
+
+extern "C" int tt_linear_residual_bwd(const void* dy, const void* row_scale, int scale_dtype,
+                                      int dtype, int64_t m, int64_t n, int32_t threshold,
+                                      const int64_t* key, void* g, void* dbias, int bias_dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  TT_TRY(sizes_ok(dtype, m, 0, n));
+  TT_TRY(vector_ok("the bias", dbias, bias_dtype));
+  TT_TRY(vector_ok("the row scale", row_scale, scale_dtype));
+  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
+  TT_REQUIRE(threshold == 0 || (key != nullptr && g != nullptr),
+             "linear: dropout without a key or a place for its gradient");
+  if (n == 0) return TT_OK;
+  const int64_t per = chunk_rows(m, n), chunks = (m + per - 1) / per;
+  const int64_t tiles = (n + P_COLS - 1) / P_COLS;
+  TT_REQUIRE(tiles <= 65535, "linear: too many columns");
+  TT_REQUIRE(dbias == nullptr || workspace_bytes >= (size_t)chunks * n * 4,
+             "linear_residual_bwd: the workspace is too small");
+  float* part = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
+  if (m > 0 && (threshold != 0 || dbias != nullptr)) {
+    const bool vec = n % 8 == 0 && all_aligned({dy, threshold != 0 ? g : nullptr});
+    TT_TRY(typed(dtype, [&](auto tt) {
+      typedef decltype(tt) TT;
+      typedef typename TT::storage St;
+      const dim3 grid((unsigned)chunks, (unsigned)tiles), block(L_NT);
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, block, 0, S(stream), static_cast<const St*>(dy), row_scale,
+                           scale_dtype, (uint32_t)threshold, key, static_cast<St*>(g), part, m, n,
+                           per);
+        return tt_check_launch("linear_res_bwd");
+      };
+      if (threshold != 0)
+        return vec ? go(&linear_res_bwd_kernel<TT, true, true>)
+                   : go(&linear_res_bwd_kernel<TT, true, false>);
+      return vec ? go(&linear_res_bwd_kernel<TT, false, true>)
+                 : go(&linear_res_bwd_kernel<TT, false, false>);
+    }));
+  }
+  if (dbias == nullptr) return TT_OK;
+  const float alpha = keep_inverse(threshold);
+  hipLaunchKernelGGL(linear_colsum_kernel, dim3((unsigned)((n + 31) / 32)), dim3(L_NT), 0,
+                     S(stream), part, chunks, n, alpha, dbias, bias_dtype);
+  return tt_check_launch("linear_colsum");
+}
+
+extern "C" int tt_linear_dgrad(const void* g, const void* w, const void* x, const void* row_scale,
+                               int scale_dtype, const void* bias, int bias_dtype, int dtype,
+                               int64_t m, int64_t k, int64_t n, int32_t threshold, void* dx,
+                               void* xs, void* dscale, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  TT_TRY(sizes_ok(dtype, m, k, n));
+  TT_TRY(vector_ok("the bias", bias, bias_dtype));
+  TT_TRY(vector_ok("the row scale", row_scale, scale_dtype));
+  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
+  TT_REQUIRE(row_scale != nullptr || (xs == nullptr && dscale == nullptr),
+             "linear_dgrad: scaled rows and the scale's gradient need a row scale");
+  TT_REQUIRE(row_scale == nullptr || x != nullptr || k == 0, "linear_dgrad: a row scale needs x");
+  if (m == 0) return TT_OK;
+  const size_t db = dscale != nullptr ? dots_bytes(m, k) : 0;
+  const int64_t nd = (k + LIN_DOT - 1) / LIN_DOT;
+  // The bias's part of the scale's gradient goes where the split sums were.
+  const size_t need = db + (dscale != nullptr && bias != nullptr ? (size_t)m * 4 : 0);
+  TT_REQUIRE(workspace_bytes >= need, "linear_dgrad: the workspace is too small");
+  char* const rest = static_cast<char*>(workspace) + db;
+  LinArgs p{};
+  p.a = g;
+  p.b = w;
+  p.out = dx;
+  p.I = m;
+  p.J = p.ldb = k;
+  p.R = p.lda = n;
+  p.scale = row_scale;
+  p.scale_dt = scale_dtype;
+  p.alpha = keep_inverse(threshold);
+  p.x = x;
+  p.xs = xs;
+  p.dots = dscale != nullptr ? static_cast<float*>(workspace) : nullptr;
+  if (k > 0)
+    TT_TRY(run_product(LAY_NN, LIN_DGRAD, dtype, p, rest, workspace_bytes - db, S(stream)));
+  if (dscale == nullptr) return TT_OK;
+  float* extra = nullptr;
+  if (bias != nullptr) {
+    extra = reinterpret_cast<float*>(rest);
+    hipLaunchKernelGGL(linear_rowdot_kernel, dim3((unsigned)((m + 3) / 4)), dim3(L_NT), 0,
+                       S(stream), g, dtype, bias, bias_dtype, m, n, extra);
+    TT_TRY(tt_check_launch("linear_rowdot"));
+  }
+  hipLaunchKernelGGL(linear_rowsum_kernel, dim3((unsigned)((m + L_NT - 1) / L_NT)), dim3(L_NT), 0,
+                     S(stream), p.dots, (int)nd, extra, p.alpha, m, dscale, scale_dtype);
+  return tt_check_launch("linear_rowsum");
+}
+
+extern "C" int tt_linear_wgrad(const void* g, const void* x, int dtype, int64_t m, int64_t k,
+                               int64_t n, int32_t threshold, void* dw, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  TT_TRY(sizes_ok(dtype, m, k, n));
+  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
+  if (n == 0 || k == 0) return TT_OK;
+  LinArgs p{};
+  p.a = g;
+  p.b = x;
+  p.out = dw;
+  p.I = p.lda = n;
+  p.J = p.ldb = k;
+  p.R = m;
+  p.alpha = keep_inverse(threshold);
+  return run_product(LAY_TN, LIN_PLAIN, dtype, p, workspace, workspace_bytes, S(stream));
+}

@@ -20,10 +20,20 @@
 // 4098 -> 1843 us, r 64 5017 -> 2980. (Sums split over the waves of a block
 // took 354 us, but in an order of their own: other last bits.)
 #include "gemm.h"
+#include "philox.h"
 
 #include <type_traits>
 
 namespace {
+
+// Dropout on the rows of x (DROP kernels): an element is kept or cleared by its
+// packed row and column (philox.h), and the inverse of the kept share multiplies
+// the fp32 sums, so that clearing is exact and nothing is rounded on its account.
+struct Drop {
+  const int64_t* key;
+  uint32_t threshold;
+  float inv;
+};
 
 struct BF { static constexpr int code = TT_BF16; };
 struct HF { static constexpr int code = TT_F16; };
@@ -104,12 +114,14 @@ __device__ __forceinline__ float widen1(uint32_t w, bool odd, float s) {
 // slot c ^ ((r >> 1) & 7); then W_e's 64 x r elements as they lie in memory,
 // or (WT) 256 bytes per row j, chunk c in slot c ^ (j % 16).
 // ---------------------------------------------------------------------------
-template <class TT, int RT, bool WT, bool SCALE, int WC>
+template <class TT, int RT, bool WT, bool SCALE, int WC, bool DROP>
 __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __restrict__ in,
                                                           const float* __restrict__ W,
                                                           float* __restrict__ out, int C, int r,
                                                           float s, int E,
-                                                          const int64_t* __restrict__ counts) {
+                                                          const int64_t* __restrict__ counts,
+                                                          Drop drop) {
+  static_assert(!(DROP && (WT || SCALE)), "dropout is on the forward's rows");
   constexpr int BM = 64 / WC, BK = 64, S = RT == 1 ? 4 : RT == 2 ? 3 : 2;
   constexpr int T_X = BM * BK * 2, T_W = 16 * RT * BK * 4, STAGE = T_X + T_W;
   constexpr int LX = BM / 32, LD = LX + RT;  // loads per wave and k-tile
@@ -162,6 +174,8 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
   const int wr = wave / WC, wc = wave % WC;  // the wave's rows and columns
   const int row = 16 * wr + l16;
   f32x4 acc[CT] = {};
+  DropKey dk{};
+  if constexpr (DROP) dk = load_key(drop.key);
 #pragma unroll
   for (int i = 0; i < S - 1; ++i)
     if (i < nkt) issue(i, i);
@@ -193,6 +207,25 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
         }
     };
     if (16 * wr < rows) {
+      // DROP: lanes l and l ^ 32 read the same eight elements of each 16 (and
+      // multiply four of them each); each makes two of the k-tile's four masks,
+      // one bit per element, and hands them to the other.
+      uint32_t kept = 0;
+      if constexpr (DROP) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[4];
+          philox(dk, (uint32_t)(kt * (BK / 8) + 2 * (2 * (g >> 1) + i) + (g & 1)),
+                 (uint32_t)(row0 + row), w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            mine |= (keeps(w, e, drop.threshold) ? 1u : 0u) << (8 * i + e);
+        }
+        const uint32_t theirs = (uint32_t)__shfl_xor((int)mine, 32, 64);
+        kept = odd ? theirs | (mine << 16) : mine | (theirs << 16);
+        kept >>= odd ? 1 : 0;  // bit 8 b + 2 q: the element this lane multiplies
+      }
       read(0);
 #pragma unroll
       for (int b = 0; b < BK / 16; ++b) {
@@ -201,7 +234,8 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
         const uint32_t x[4] = {xv[b & 1].x, xv[b & 1].y, xv[b & 1].z, xv[b & 1].w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float a = widen1<TT, SCALE>(x[q], odd, s);
+          float a = widen1<TT, SCALE>(x[q], odd, s);
+          if constexpr (DROP) a = (kept >> (8 * b + 2 * q)) & 1u ? a : 0.f;
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt) acc[jt] = mfma16(a, wv[b & 1][q][jt], acc[jt]);
         }
@@ -216,7 +250,7 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int m = 16 * wr + 4 * g + e, j = 16 * (CT * wc + jt) + l16;
-      if (m < rows && j < r) out[(row0 + m) * r + j] = acc[jt][e];
+      if (m < rows && j < r) out[(row0 + m) * r + j] = DROP ? acc[jt][e] * drop.inv : acc[jt][e];
     }
 }
 
@@ -228,11 +262,12 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
 // 64 w .. + 63 for all rows, and the rounded products pass through LDS so that
 // base and y move as whole 128-byte row segments.
 // ---------------------------------------------------------------------------
-template <class TT, int RT, bool WT, bool BASE>
+template <class TT, int RT, bool WT, bool BASE, bool DROP>
 __global__ __launch_bounds__(LR_NT, RT == 2 && WT ? 3 : 1) void lora_up_kernel(
     const float* __restrict__ h, const float* __restrict__ W, const uint16_t* __restrict__ base,
     uint16_t* __restrict__ y, int N, int r, float s, int E, const int64_t* __restrict__ counts,
-    int tiles_n) {
+    int tiles_n, Drop drop) {
+  static_assert(!(DROP && BASE), "the gradient of the dropped rows has no base");
   constexpr int BM = 64, BN = 256, MI = BM / 16, R = 16 * RT;
   constexpr int WS = BN + 16;  // row stride of W in LDS: four rows on distinct banks
   constexpr int LDS = R * WS * 4 > BM * BN * 2 ? R * WS * 4 : BM * BN * 2;
@@ -326,7 +361,8 @@ __global__ __launch_bounds__(LR_NT, RT == 2 && WT ? 3 : 1) void lora_up_kernel(
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt) {
       const int m = 16 * mi + l16, ch = 2 * nt + (g >> 1);
-      const f32x4 a = acc[nt][mi];
+      f32x4 a = acc[nt][mi];
+      if constexpr (DROP) a *= drop.inv;
       uint2 v;
       v.x = pack2<TT>(a[0], a[1]);
       v.y = pack2<TT>(a[2], a[3]);
@@ -334,12 +370,20 @@ __global__ __launch_bounds__(LR_NT, RT == 2 && WT ? 3 : 1) void lora_up_kernel(
     }
   __syncthreads();
   if (n >= N) return;
+  DropKey dk{};
+  if constexpr (DROP) dk = load_key(drop.key);
 #pragma unroll
   for (int p = 0; p < BM / 8; ++p) {
     const int m = 8 * p + (lane >> 3);
     if (m >= rows) continue;
     uint4 v = *reinterpret_cast<const uint4*>(stg + m * 128 + ((c ^ (m & 7)) << 4));
     const int64_t at = (row0 + m) * N + n;
+    if constexpr (DROP) {
+      uint32_t w[4];
+      philox(dk, (uint32_t)(n >> 3), (uint32_t)(row0 + m), w);
+      v = uint4{keep_pair(v.x, w[0], drop.threshold), keep_pair(v.y, w[1], drop.threshold),
+                keep_pair(v.z, w[2], drop.threshold), keep_pair(v.w, w[3], drop.threshold)};
+    }
     if constexpr (BASE) {
       float d[8], b[8];
       widen8<TT, true>(v, s, d);
@@ -351,6 +395,23 @@ __global__ __launch_bounds__(LR_NT, RT == 2 && WT ? 3 : 1) void lora_up_kernel(
   }
 }
 
+// w[q] of lane i of a quad becomes w[i] of its lane q.
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4], int i) {
+#pragma unroll
+  for (int d = 1; d <= 2; d *= 2) {
+    const bool up = (i & d) != 0;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      if (a & d) continue;
+      const uint32_t send = up ? w[a] : w[a + d];
+      const uint32_t got = (uint32_t)(d == 1 ? __builtin_amdgcn_mov_dpp((int)send, 0xB1, 0xf, 0xf, true)
+                                             : __builtin_amdgcn_mov_dpp((int)send, 0x4E, 0xf, 0xf, true));
+      if (up) w[a] = got;
+      else w[a + d] = got;
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // G_e[c, j] = sum over e's rows m of in[m, c] v[m, j], in [M, C] 16-bit (scaled
 // by s and rounded first with SCALE), v fp32 [M, r]; written [C, r], or [r, C]
@@ -359,12 +420,14 @@ __global__ __launch_bounds__(LR_NT, RT == 2 && WT ? 3 : 1) void lora_up_kernel(
 // + 1 of the four rows of a step, and MFMA i multiplies column 2 (l % 16) + i,
 // so that no operand is transposed. An expert without rows gets zeros.
 // ---------------------------------------------------------------------------
-template <class TT, int RT, bool GT, bool SCALE>
+template <class TT, int RT, bool GT, bool SCALE, bool DROP>
 __global__ __launch_bounds__(LR_NT) void lora_wgrad_kernel(const uint16_t* __restrict__ in,
                                                            const float* __restrict__ v,
                                                            float* __restrict__ out, int C, int r,
                                                            float s,
-                                                           const int64_t* __restrict__ counts) {
+                                                           const int64_t* __restrict__ counts,
+                                                           Drop drop) {
+  static_assert(!(DROP && (GT || SCALE)), "dropout is on the rows of x");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
@@ -396,11 +459,22 @@ __global__ __launch_bounds__(LR_NT) void lora_wgrad_kernel(const uint16_t* __res
         vv[buf][q][jt] = vsrc[at * r + (16 * jt + l16 < r ? 16 * jt + l16 : 0)];
     }
   };
+  DropKey dk{};
+  if constexpr (DROP) dk = load_key(drop.key);
   auto multiply = [&](int64_t m0, int buf) {
+    uint32_t w[4];
+    if constexpr (DROP) {
+      // The four lanes of a group of eight columns make one row's words each,
+      // and a 4x4 transpose over them gives each lane its word of every row.
+      const int i = lane & 3;
+      philox(dk, (uint32_t)(c0 >> 3), (uint32_t)(row0 + m0 + first + 2 * i), w);
+      quad_transpose(w, i);
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool ok = m0 + first + 2 * q < rows;
-      const uint32_t xq = ok && live ? x[buf][q] : 0;
+      uint32_t xq = ok && live ? x[buf][q] : 0;
+      if constexpr (DROP) xq = keep_pair(xq, w[q], drop.threshold);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float a = widen1<TT, SCALE>(xq, i == 1, s);
@@ -423,6 +497,13 @@ __global__ __launch_bounds__(LR_NT) void lora_wgrad_kernel(const uint16_t* __res
     multiply(m0 + 16, 1);
   }
   float* const o = out + (int64_t)e * C * r;
+  if constexpr (DROP) {
+#pragma unroll
+    for (int jt = 0; jt < RT; ++jt) {
+      acc[jt][0] *= drop.inv;
+      acc[jt][1] *= drop.inv;
+    }
+  }
 #pragma unroll
   for (int jt = 0; jt < RT; ++jt)
 #pragma unroll
@@ -453,15 +534,16 @@ struct LoraArgs {
   float s;
   int E;
   const int64_t* counts;
+  Drop drop;
 };
 
 int64_t row_blocks(int64_t M, int E, int bm = 64) { return M / bm + (M < E ? M : E); }
 
-template <class TT, int RT, bool WT, bool SCALE, int WC>
+template <class TT, int RT, bool WT, bool SCALE, int WC, bool DROP>
 int launch_down_wc(const LoraArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((lora_down_kernel<TT, RT, WT, SCALE, WC>),
+  hipLaunchKernelGGL((lora_down_kernel<TT, RT, WT, SCALE, WC, DROP>),
                      dim3((unsigned)row_blocks(a.M, a.E, 64 / WC)), dim3(LR_NT), 0, s, a.in, a.w,
-                     static_cast<float*>(a.out), a.C, a.r, a.s, a.E, a.counts);
+                     static_cast<float*>(a.out), a.C, a.r, a.s, a.E, a.counts, a.drop);
   return tt_check_launch("lora_down");
 }
 // Ranks above 32 in blocks of 32 rows, two waves to the columns, ranks above 16
@@ -470,29 +552,30 @@ int launch_down_wc(const LoraArgs& a, hipStream_t s) {
 // 128 of 130 108.6 + 119.5 / 85.4 + 97.9, of 256 149.4 + 162.8 / 136.9 + 155.0; r
 // 32, 32 of 55 43.9 + 47.3 / 29.2 + 34.3, 128 of 130 (388 blocks) 65.4 + 70.4 /
 // 52.1 + 65.1, of 200 (528) 65.6 + 71.0 / 65.7 + 80.6.
-template <class TT, int RT, bool WT, bool SCALE>
+template <class TT, int RT, bool WT, bool SCALE, bool DROP>
 int launch_down(const LoraArgs& a, hipStream_t s) {
   if constexpr (RT == 4) {
-    return launch_down_wc<TT, RT, WT, SCALE, 2>(a, s);
+    return launch_down_wc<TT, RT, WT, SCALE, 2, DROP>(a, s);
   } else {
     if constexpr (RT == 2)
-      if (row_blocks(a.M, a.E) <= LD_BLOCKS) return launch_down_wc<TT, RT, WT, SCALE, 2>(a, s);
-    return launch_down_wc<TT, RT, WT, SCALE, 1>(a, s);
+      if (row_blocks(a.M, a.E) <= LD_BLOCKS)
+        return launch_down_wc<TT, RT, WT, SCALE, 2, DROP>(a, s);
+    return launch_down_wc<TT, RT, WT, SCALE, 1, DROP>(a, s);
   }
 }
-template <class TT, int RT, bool WT, bool BASE>
+template <class TT, int RT, bool WT, bool BASE, bool DROP>
 int launch_up(const LoraArgs& a, const float* h, hipStream_t s) {
   const int tn = (a.C + 255) / 256;
-  hipLaunchKernelGGL((lora_up_kernel<TT, RT, WT, BASE>),
+  hipLaunchKernelGGL((lora_up_kernel<TT, RT, WT, BASE, DROP>),
                      dim3((unsigned)(row_blocks(a.M, a.E) * tn)), dim3(LR_NT), 0, s, h, a.w, a.base,
-                     static_cast<uint16_t*>(a.out), a.C, a.r, a.s, a.E, a.counts, tn);
+                     static_cast<uint16_t*>(a.out), a.C, a.r, a.s, a.E, a.counts, tn, a.drop);
   return tt_check_launch("lora_up");
 }
-template <class TT, int RT, bool GT, bool SCALE>
+template <class TT, int RT, bool GT, bool SCALE, bool DROP>
 int launch_wgrad(const LoraArgs& a, const float* v, hipStream_t s) {
-  hipLaunchKernelGGL((lora_wgrad_kernel<TT, RT, GT, SCALE>),
+  hipLaunchKernelGGL((lora_wgrad_kernel<TT, RT, GT, SCALE, DROP>),
                      dim3((unsigned)((a.C + 127) / 128), (unsigned)a.E), dim3(LR_NT), 0, s, a.in, v,
-                     static_cast<float*>(a.out), a.C, a.r, a.s, a.counts);
+                     static_cast<float*>(a.out), a.C, a.r, a.s, a.counts, a.drop);
   return tt_check_launch("lora_wgrad");
 }
 
@@ -520,6 +603,14 @@ int lora_checks(int dtype, int64_t m, int64_t c, int r, int E, const void* p0, c
   TT_REQUIRE(row_blocks(m, E) * ((c + 255) / 256) < 0x7fffffff, "lora: grid too large");
   return TT_OK;
 }
+int drop_checks(int32_t threshold, const int64_t* key) {
+  TT_REQUIRE(threshold >= 1 && threshold <= 65536, "lora: the threshold must be in [1, 65536]");
+  TT_REQUIRE(key != nullptr, "lora: dropout without a key");
+  return TT_OK;
+}
+Drop drop_of(int32_t threshold, const int64_t* key) {
+  return Drop{key, (uint32_t)threshold, keep_inverse(threshold)};
+}
 
 }  // namespace
 
@@ -530,12 +621,27 @@ extern "C" int tt_lora_down(const void* in, const float* w, int dtype, int64_t m
   if (rc != TT_OK) return rc;
   if (m == 0) return TT_OK;
   const LoraArgs a{static_cast<const uint16_t*>(in), w, nullptr, out, m, (int)c, r, scale,
-                   num_experts, counts};
+                   num_experts, counts, Drop{}};
   return typed(dtype, r, [&](auto tt, auto rt) {
     typedef decltype(tt) TT;
     constexpr int RT = decltype(rt)::value;
-    return transposed ? launch_down<TT, RT, true, true>(a, S(stream))
-                      : launch_down<TT, RT, false, false>(a, S(stream));
+    return transposed ? launch_down<TT, RT, true, true, false>(a, S(stream))
+                      : launch_down<TT, RT, false, false, false>(a, S(stream));
+  });
+}
+
+extern "C" int tt_lora_down_dropout(const void* in, const float* w, int dtype, int64_t m, int64_t c,
+                                    int32_t r, int32_t num_experts, const int64_t* counts,
+                                    int32_t threshold, const int64_t* key, float* out,
+                                    void* stream) {
+  int rc = lora_checks(dtype, m, c, r, num_experts, in, w, nullptr);
+  if (rc == TT_OK) rc = drop_checks(threshold, key);
+  if (rc != TT_OK) return rc;
+  if (m == 0) return TT_OK;
+  const LoraArgs a{static_cast<const uint16_t*>(in), w, nullptr, out, m, (int)c, r, 1.0f,
+                   num_experts, counts, drop_of(threshold, key)};
+  return typed(dtype, r, [&](auto tt, auto rt) {
+    return launch_down<decltype(tt), decltype(rt)::value, false, false, true>(a, S(stream));
   });
 }
 
@@ -544,16 +650,30 @@ extern "C" int tt_lora_up(const float* h, const float* w, const void* base, int 
                           int32_t num_experts, const int64_t* counts, void* out, void* stream) {
   const int rc = lora_checks(dtype, m, c, r, num_experts, base, w, out);
   if (rc != TT_OK) return rc;
+  if (m == 0 || c == 0) return TT_OK;
   TT_REQUIRE((base == nullptr) == (transposed != 0),
              "lora: the base is added in the forward form only");
-  if (m == 0 || c == 0) return TT_OK;
   const LoraArgs a{nullptr, w, static_cast<const uint16_t*>(base), out, m, (int)c, r, scale,
-                   num_experts, counts};
+                   num_experts, counts, Drop{}};
   return typed(dtype, r, [&](auto tt, auto rt) {
     typedef decltype(tt) TT;
     constexpr int RT = decltype(rt)::value;
-    return transposed ? launch_up<TT, RT, true, false>(a, h, S(stream))
-                      : launch_up<TT, RT, false, true>(a, h, S(stream));
+    return transposed ? launch_up<TT, RT, true, false, false>(a, h, S(stream))
+                      : launch_up<TT, RT, false, true, false>(a, h, S(stream));
+  });
+}
+
+extern "C" int tt_lora_up_dropout(const float* h, const float* w, int dtype, int64_t m, int64_t c,
+                                  int32_t r, int32_t num_experts, const int64_t* counts,
+                                  int32_t threshold, const int64_t* key, void* out, void* stream) {
+  int rc = lora_checks(dtype, m, c, r, num_experts, w, out, nullptr);
+  if (rc == TT_OK) rc = drop_checks(threshold, key);
+  if (rc != TT_OK) return rc;
+  if (m == 0 || c == 0) return TT_OK;
+  const LoraArgs a{nullptr, w, nullptr, out, m, (int)c, r, 1.0f, num_experts, counts,
+                   drop_of(threshold, key)};
+  return typed(dtype, r, [&](auto tt, auto rt) {
+    return launch_up<decltype(tt), decltype(rt)::value, true, false, true>(a, h, S(stream));
   });
 }
 
@@ -564,11 +684,26 @@ extern "C" int tt_lora_wgrad(const void* in, const float* v, int dtype, int64_t 
   if (rc != TT_OK) return rc;
   if (c == 0) return TT_OK;
   const LoraArgs a{static_cast<const uint16_t*>(in), nullptr, nullptr, out, m, (int)c, r, scale,
-                   num_experts, counts};
+                   num_experts, counts, Drop{}};
   return typed(dtype, r, [&](auto tt, auto rt) {
     typedef decltype(tt) TT;
     constexpr int RT = decltype(rt)::value;
-    return transposed ? launch_wgrad<TT, RT, true, true>(a, v, S(stream))
-                      : launch_wgrad<TT, RT, false, false>(a, v, S(stream));
+    return transposed ? launch_wgrad<TT, RT, true, true, false>(a, v, S(stream))
+                      : launch_wgrad<TT, RT, false, false, false>(a, v, S(stream));
+  });
+}
+
+extern "C" int tt_lora_wgrad_dropout(const void* in, const float* v, int dtype, int64_t m,
+                                     int64_t c, int32_t r, int32_t num_experts,
+                                     const int64_t* counts, int32_t threshold, const int64_t* key,
+                                     float* out, void* stream) {
+  int rc = lora_checks(dtype, m, c, r, num_experts, in, out, nullptr);
+  if (rc == TT_OK) rc = drop_checks(threshold, key);
+  if (rc != TT_OK) return rc;
+  if (c == 0) return TT_OK;
+  const LoraArgs a{static_cast<const uint16_t*>(in), nullptr, nullptr, out, m, (int)c, r, 1.0f,
+                   num_experts, counts, drop_of(threshold, key)};
+  return typed(dtype, r, [&](auto tt, auto rt) {
+    return launch_wgrad<decltype(tt), decltype(rt)::value, false, false, true>(a, v, S(stream));
   });
 }

@@ -239,6 +239,25 @@ class OpDispatcher:
     def swiglu(self, x, *, impl: str | None = None):
         return self._dispatch("swiglu", x, impl=impl)
 
+    def linear_act(self, x, weight, bias=None, *, activation_func=None, gated: bool = False,
+                   impl: str | None = None):
+        """``act(x @ weight.T + bias)``; gated: ``act`` of the first half of the features
+        times the second half. No reference counterpart as one op."""
+        return self._dispatch("linear_act", x, weight, bias, activation_func=activation_func,
+                              gated=gated, impl=impl)
+
+    def linear_residual(self, x, weight, bias=None, residual=None, row_scale=None, *,
+                        dropout_p: float = 0.0, dropout_key=None, impl: str | None = None):
+        """``residual + row_scale * dropout(x @ weight.T + bias)``. No reference counterpart
+        as one op."""
+        return self._dispatch("linear_residual", x, weight, bias, residual, row_scale,
+                              dropout_p=dropout_p, dropout_key=dropout_key, impl=impl)
+
+    def dropout(self, x, p: float, key, *, impl: str | None = None):
+        """Dropout whose mask follows from ``key`` (int64 ``[2]`` on the device) and the
+        position of an element. No reference counterpart."""
+        return self._dispatch("dropout", x, p, key, impl=impl)
+
     def moe_permutation(
         self,
         tokens: torch.Tensor,

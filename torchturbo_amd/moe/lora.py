@@ -10,7 +10,9 @@ Mirrors ``src/torchturbo/engine/peft/lora.py:54-725``:
   fc2 outputs (additive residual, no ``[E, in, out]`` delta is formed; on the
   GPU the ``lora_residual`` op, without fp32 copies of the rows), with
   the reference's adapter management: ranks, ``lora_alpha`` scaling (plain or
-  rank-stabilised), dropout, Kaiming-uniform or Gaussian initialisation, active
+  rank-stabilised), dropout (``torch.nn.Dropout``, or with ``counter_dropout=True`` a
+  :class:`CounterDropout`, which the ``lora_residual`` op takes into its products),
+  Kaiming-uniform or Gaussian initialisation, active
   adapter selection, merge / unmerge into the base weights and the conversion
   of legacy 2-D LoRA checkpoints (``lora.py:245-319``).
 
@@ -28,6 +30,7 @@ import torch
 import torch.nn as nn
 
 from ..dispatch import op_resolves, ops
+from .dropout import CounterDropout
 from .experts import GroupedMLP
 
 try:  # PEFT integration is optional (the reference requires it)
@@ -73,7 +76,8 @@ class GroupedMLPLoRA(nn.Module, _TunerBase):
     def __init__(self, base_layer: GroupedMLP, adapter_name: str, r: int = 0,
                  lora_alpha: int = 1, lora_dropout: float = 0.0,
                  init_lora_weights: Union[bool, str] = True, use_rslora: bool = False,
-                 use_dora: bool = False, lora_bias: bool = False, **kwargs) -> None:
+                 use_dora: bool = False, lora_bias: bool = False,
+                 counter_dropout: bool = False, **kwargs) -> None:
         nn.Module.__init__(self)
         if use_dora:
             raise ValueError("GroupedMLPLoRA does not support DoRA (use_dora=True).")
@@ -108,6 +112,7 @@ class GroupedMLPLoRA(nn.Module, _TunerBase):
         self.ephemeral_gpu_offload = False
         self.cast_input_dtype_enabled = True
         self.kwargs = kwargs
+        self.counter_dropout = bool(counter_dropout)
         self._active_adapter = adapter_name
         self.update_layer(adapter_name, r, lora_alpha=lora_alpha, lora_dropout=lora_dropout,
                           init_lora_weights=init_lora_weights, use_rslora=use_rslora,
@@ -193,7 +198,8 @@ class GroupedMLPLoRA(nn.Module, _TunerBase):
             raise ValueError("GroupedMLPLoRA does not support lora_bias=True.")
         self.r[adapter_name] = r
         self.lora_alpha[adapter_name] = lora_alpha
-        self.lora_dropout[adapter_name] = nn.Dropout(p=lora_dropout) if lora_dropout > 0.0 \
+        dropout = CounterDropout if self.counter_dropout else nn.Dropout
+        self.lora_dropout[adapter_name] = dropout(p=lora_dropout) if lora_dropout > 0.0 \
             else nn.Identity()
         n = self.num_local_experts
         # fp32 adapters whatever the base dtype (lora.py:426-440).
@@ -265,12 +271,22 @@ class GroupedMLPLoRA(nn.Module, _TunerBase):
     # -- forward --------------------------------------------------------------
     def _add_residual(self, base, x, counts, name, a_group, b_group):
         """``base`` plus adapter ``name``'s residual of ``x``."""
-        a, b = a_group[name], b_group[name]
-        xd, scale = self.lora_dropout[name](x), self.scaling[name]
+        a, b, drop = a_group[name], b_group[name], self.lora_dropout[name]
+        scale = self.scaling[name]
         # In place of the HIP grouped product only: another one chosen for it is called.
-        if (x.is_cuda and op_resolves("lora_residual")
-                and ops.selected_impl_name("grouped_matmul") == "hip_grouped_matmul"):
-            y = ops.lora_residual(base, xd, a.weight, b.weight, counts, scale)
+        fused = (x.is_cuda and op_resolves("lora_residual")
+                 and ops.selected_impl_name("grouped_matmul") == "hip_grouped_matmul")
+        if (fused and type(drop) is CounterDropout and drop.active
+                and ops.selected_impl_name("dropout") == "hip_dropout"):
+            key = drop.draw_key(x.device)
+            y = ops.lora_residual(base, x, a.weight, b.weight, counts, scale, dropout_p=drop.p,
+                                  dropout_key=key)
+            if y is not None:
+                return y
+            xd = ops.dropout(x, drop.p, key)
+        else:
+            xd = drop(x)
+            y = ops.lora_residual(base, xd, a.weight, b.weight, counts, scale) if fused else None
             if y is not None:
                 return y
         xd = xd.to(a.weight.dtype)

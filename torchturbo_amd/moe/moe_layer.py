@@ -21,6 +21,7 @@ from .experts import Fp8GroupedMLP, GroupedMLP
 from .module import ModuleSpec, build_module
 from .moe_config import MoEConfig
 from .router import TopKRouter
+from .shared_experts import SharedExpertMLP
 from .token_dispatcher import MoEAlltoAllTokenDispatcher
 
 
@@ -167,10 +168,18 @@ class MoELayer(BaseMoELayer):
                 output = self._dispatched_experts(hidden_states, probs, routing_map,
                                                   expert_indices)
         if self.shared_expert is not None:
-            shared = self.shared_expert(hidden_states)
-            output = output + F.sigmoid(self.shared_expert_gate(hidden_states)) * shared
+            gate = F.sigmoid(self.shared_expert_gate(hidden_states))
+            if (type(self.shared_expert) is SharedExpertMLP
+                    and gate.shape == (*hidden_states.shape[:-1], 1)):
+                # The token's gate and the sum in the expert's last product.
+                output = self.shared_expert(hidden_states, output, gate)
+            else:
+                output = output + gate * self.shared_expert(hidden_states)
         if self.shared_experts is not None:
-            output = output + self.shared_experts(hidden_states)
+            if type(self.shared_experts) is SharedExpertMLP:
+                output = self.shared_experts(hidden_states, output)
+            else:
+                output = output + self.shared_experts(hidden_states)
         return output
 
     def _dispatched_experts(self, hidden_states, probs, routing_map, expert_indices):
