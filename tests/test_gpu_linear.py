@@ -192,6 +192,18 @@ def test_linear_residual(hip_ops, T, K, N, dtype, bias, res, scale, p):
     check_residual(hip_ops, x, w, b, r, s, p, key)
 
 
+# Enough tiles of 256 for the largest kernels: in the forward, in the gradient of x and
+# in the gradient of the weight.
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T, K, N", [(3850, 136, 3400), (3850, 3400, 136), (140, 3400, 3848)])
+def test_largest_tiles(hip_ops, T, K, N, dtype):
+    x, w, b = make((T, K), 1, dtype), make((N, K), 2, dtype, K ** -0.5), make((N,), 3, dtype, 0.3)
+    check_act(hip_ops, x, w, b, F.gelu, False)
+    check_act(hip_ops, x, make((N + N % 16, K), 4, dtype, K ** -0.5), None, F.silu, True)
+    key = torch.tensor([K, N], device=DEV)
+    check_residual(hip_ops, x, w, b, make((T, N), 5, dtype), make((T, 1), 6, dtype), 0.2, key)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_empty_sizes(hip_ops, dtype):
     for T, K, N in ((0, 16, 8), (4, 0, 8), (4, 16, 0), (0, 0, 0)):

@@ -202,4 +202,7 @@ __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t
 enum { LAY_NT = 0, LAY_NN = 1, LAY_TN = 2 };
 
 // fp32 matrix instructions on any type, size and alignment (linear_any.hip).
-int tt_linear_any(int layout, int kind, int dtype, const LinArgs& a, hipStream_t s);
+int tt_linear_any(int kind, int dtype, const LinArgs& a, hipStream_t s);
+// 16-bit matrix instructions on tiles of `tile` (128 or 256) rows and columns, for
+// aligned rows of whole 16-byte vectors (linear_tile.hip).
+int tt_linear_tile(int kind, int tile, int dtype, const LinArgs& a, hipStream_t s);

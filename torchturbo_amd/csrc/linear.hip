@@ -101,14 +101,24 @@ Split split_of(int64_t R, int64_t wanted) {
   return Split{(int)((R + per - 1) / per), per};
 }
 
-// How many parts a product's reduction is split into on the kernel for any type:
-// enough for one block per CU, each at least 256 long.
-int64_t any_splits(int kind, int64_t I, int64_t J, int64_t R) {
-  const int64_t bo = kind == LIN_GATED ? 32 : 64;
-  const int64_t tiles = ((I + 63) / 64) * ((J + bo - 1) / bo);
-  int64_t want = 256 / (tiles > 0 ? tiles : 1);
-  if (want > R / 256) want = R / 256;
-  return want < 1 ? 1 : want > 32 ? 32 : want;
+// The kernel that runs a product (0: any type, else the tile of linear_tile.hip)
+// and how many parts its reduction is split into.
+struct Plan {
+  int tile;
+  Split split;
+};
+
+Plan plan_of(int kind, int64_t I, int64_t J, int64_t R, bool fast) {
+  const int64_t half = kind == LIN_GATED ? 2 : 1;
+  auto tiles = [&](int64_t t) { return ((I + t - 1) / t) * ((half * J + t - 1) / t); };
+  if (!fast) {
+    // Enough blocks for the CUs, each reduction at least 256 long.
+    const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64), 1), R / 256);
+    return Plan{0, split_of(R, std::min<int64_t>(want, 32))};
+  }
+  if (tiles(256) >= 192) return Plan{256, split_of(R, 1)};
+  const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(tiles(128), 1), R / 256);
+  return Plan{128, split_of(R, std::min<int64_t>(want, 32))};
 }
 
 size_t part_bytes(int kind, int64_t I, int64_t J, int64_t splits) {
@@ -118,14 +128,29 @@ size_t dots_bytes(int64_t I, int64_t J) {
   return (((size_t)I * ((J + LIN_DOT - 1) / LIN_DOT) * 4) + 255) / 256 * 256;
 }
 
+// Whether the sizes of a product fit the 16-bit tiles: rows of whole 16-byte
+// vectors, and tiles within reach of a 32-bit offset (a gated tile's columns lie
+// half the weight apart).
+bool fast_sizes(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R) {
+  if (dtype != TT_BF16 && dtype != TT_F16) return false;
+  const bool a_ok = layout == LAY_TN ? I % 8 == 0 : R % 8 == 0;
+  const bool b_ok = layout == LAY_NT ? R % 8 == 0 : J % 8 == 0;
+  if (!a_ok || !b_ok || J % 8 != 0 || R == 0) return false;
+  const int64_t row = 2 * std::max(std::max(I, J), R);
+  return row * 256 < (1ll << 31) && (kind != LIN_GATED || (J + 256) * R * 2 < (1ll << 31));
+}
+
 int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_bytes,
                 hipStream_t s) {
-  Split sp = split_of(p.R, any_splits(kind, p.I, p.J, p.R));
-  if (part_bytes(kind, p.I, p.J, sp.splits) > ws_bytes) sp = split_of(p.R, 1);
+  const bool fast = vectors(p) && fast_sizes(layout, kind, dtype, p.I, p.J, p.R);
+  Plan pl = plan_of(kind, p.I, p.J, p.R, fast);
+  if (part_bytes(kind, p.I, p.J, pl.split.splits) > ws_bytes) pl.split = split_of(p.R, 1);
+  const Split sp = pl.split;
   p.splits = sp.splits;
   p.rsplit = sp.run;
   p.part = sp.splits > 1 ? static_cast<float*>(ws) : nullptr;
-  const int rc = tt_linear_any(layout, kind, dtype, p, s);
+  const int rc = pl.tile != 0 ? tt_linear_tile(kind, pl.tile, dtype, p, s)
+                              : tt_linear_any(kind, dtype, p, s);
   if (rc != TT_OK || p.part == nullptr) return rc;
   switch (dtype) {
     case TT_BF16: return join_kind<BF16T>(kind, p, s);
@@ -341,14 +366,20 @@ bool all_aligned(std::initializer_list<const void*> ps) {
 
 extern "C" size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t k, int64_t n) {
   if (m <= 0 || k < 0 || n < 0) return 0;
+  // The larger of the two plans: which one runs also depends on the addresses.
+  auto parts = [&](int layout, int kind, int64_t I, int64_t J, int64_t R) {
+    const int64_t any = plan_of(kind, I, J, R, false).split.splits;
+    const int64_t fast = fast_sizes(layout, kind, dtype, I, J, R)
+                             ? plan_of(kind, I, J, R, true).split.splits : 1;
+    return part_bytes(kind, I, J, std::max(any, fast));
+  };
   switch (op) {
-    case TT_LINEAR_ACT: return part_bytes(LIN_ACT, m, n, any_splits(LIN_ACT, m, n, k));
-    case TT_LINEAR_GATED: return part_bytes(LIN_GATED, m, n, any_splits(LIN_GATED, m, n, k));
-    case TT_LINEAR_RESIDUAL: return part_bytes(LIN_RES, m, n, any_splits(LIN_RES, m, n, k));
+    case TT_LINEAR_ACT: return parts(LAY_NT, LIN_ACT, m, n, k);
+    case TT_LINEAR_GATED: return parts(LAY_NT, LIN_GATED, m, n, k);
+    case TT_LINEAR_RESIDUAL: return parts(LAY_NT, LIN_RES, m, n, k);
     case TT_LINEAR_DGRAD:  // dot products, then the split sums, later the bias's part
-      return dots_bytes(m, k) +
-             std::max(part_bytes(LIN_DGRAD, m, k, any_splits(LIN_DGRAD, m, k, n)), (size_t)m * 4);
-    case TT_LINEAR_WGRAD: return part_bytes(LIN_PLAIN, n, k, any_splits(LIN_PLAIN, n, k, m));
+      return dots_bytes(m, k) + std::max(parts(LAY_NN, LIN_DGRAD, m, k, n), (size_t)m * 4);
+    case TT_LINEAR_WGRAD: return parts(LAY_TN, LIN_PLAIN, n, k, m);
     case TT_LINEAR_COLSUM: {
       const int64_t per = chunk_rows(m, n);
       return (size_t)((m + per - 1) / per) * 2 * n * 4;  // gated: both halves

@@ -175,9 +175,6 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
         } else {
           dot += lin_finish<KIND, TT, 4, false>(p, i, j, left, v, u, dk);
         }
-        if constexpr (KIND == LIN_DGRAD) {
-          // The last block of a LIN_DOT-wide run: the two lanes of the row add up.
-        }
       }
     if constexpr (KIND == LIN_DGRAD) {
       static_assert(LIN_DOT == 64, "see below");
@@ -235,14 +232,12 @@ int typed(int dtype, const LinArgs& p, hipStream_t s) {
 
 }  // namespace
 
-int tt_linear_any(int layout, int kind, int dtype, const LinArgs& p, hipStream_t s) {
+int tt_linear_any(int kind, int dtype, const LinArgs& p, hipStream_t s) {
   switch (kind) {
     case LIN_ACT: return typed<LAY_NT, LIN_ACT>(dtype, p, s);
     case LIN_GATED: return typed<LAY_NT, LIN_GATED>(dtype, p, s);
     case LIN_RES: return typed<LAY_NT, LIN_RES>(dtype, p, s);
     case LIN_DGRAD: return typed<LAY_NN, LIN_DGRAD>(dtype, p, s);
-    default:
-      return layout == LAY_NN ? typed<LAY_NN, LIN_PLAIN>(dtype, p, s)
-                              : typed<LAY_TN, LIN_PLAIN>(dtype, p, s);
+    default: return typed<LAY_TN, LIN_PLAIN>(dtype, p, s);
   }
 }
