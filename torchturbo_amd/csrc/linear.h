@@ -9,10 +9,11 @@
 // What becomes of the fp32 sums v = sum over r of A(i, r) B(r, j):
 //   ACT    y = act(v + bias)
 //   GATED  y = act(v + bias) * (u + bias'), u the sums of the second J columns
-//   RES    y = residual + scale[i] * drop(v + bias)
+//   RES    y = residual + scale[i] * (v + bias)
+//   DROP   y = residual + scale[i] * drop(v + bias)
 //   DGRAD  y = scale[i] * alpha v; xs = scale[i] * x; dots[i] = sum over j of x * alpha v
 //   PLAIN  y = alpha v
-enum { LIN_ACT = 0, LIN_GATED = 1, LIN_RES = 2, LIN_DGRAD = 3, LIN_PLAIN = 4 };
+enum { LIN_ACT = 0, LIN_GATED = 1, LIN_RES = 2, LIN_DROP = 3, LIN_DGRAD = 4, LIN_PLAIN = 5 };
 // Activations.
 enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2 };
 // Columns that one partial dot product of DGRAD covers.
@@ -34,8 +35,8 @@ struct LinArgs {
   const void* res;
   const void* scale;
   int scale_dt;
-  uint32_t threshold;  // RES: 0 is no dropout
-  float alpha;         // RES: 1 / (share kept)
+  uint32_t threshold;  // DROP
+  float alpha;         // DROP, DGRAD, PLAIN: 1 / (share kept)
   const int64_t* key;
   const void* x;  // DGRAD
   void* xs;
@@ -107,11 +108,64 @@ __device__ __forceinline__ void lin_store(void* p, int64_t at, int n, const floa
   }
 }
 
-// W of a vector of `bias` (its own dtype) at column j.
-template <int W>
-__device__ __forceinline__ void lin_bias(const LinArgs& p, int64_t j, int n, float (&o)[W]) {
+// What a result needs besides its sums: of its columns (the same for every row),
+// and of its row; fetched ahead of the sums' arrival where a kernel can.
+template <int KIND, int W>
+struct LinCols {
+  float b[W], bu[KIND == LIN_GATED ? W : 1];
+};
+template <class TT, int W>
+struct LinRow {
+  typename TT::storage v[W];  // RES: the residual, DGRAD: x
+  float s;                    // the row's scale
+};
+
+// Columns j .. j + W - 1, n of them exist.
+template <int KIND, int W>
+__device__ __forceinline__ LinCols<KIND, W> lin_cols(const LinArgs& p, int64_t j, int n) {
+  LinCols<KIND, W> c;
 #pragma unroll
-  for (int e = 0; e < W; ++e) o[e] = e < n ? load_as_f32(p.bias, p.bias_dt, j + e) : 0.f;
+  for (int e = 0; e < W; ++e) c.b[e] = 0.f;
+  if constexpr (KIND == LIN_GATED) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) c.bu[e] = 0.f;
+  }
+  if (KIND <= LIN_DROP && p.bias != nullptr) {
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (e < n) c.b[e] = load_as_f32(p.bias, p.bias_dt, j + e);
+    if constexpr (KIND == LIN_GATED) {
+#pragma unroll
+      for (int e = 0; e < W; ++e)
+        if (e < n) c.bu[e] = load_as_f32(p.bias, p.bias_dt, p.J + j + e);
+    }
+  }
+  return c;
+}
+
+template <int KIND, class TT, int W, bool VEC>
+__device__ __forceinline__ LinRow<TT, W> lin_row(const LinArgs& p, int64_t i, int64_t j, int n) {
+  typedef typename TT::storage St;
+  LinRow<TT, W> r;
+  r.s = 1.f;
+#pragma unroll
+  for (int e = 0; e < W; ++e) r.v[e] = St(0);
+  if constexpr (KIND == LIN_RES || KIND == LIN_DROP || KIND == LIN_DGRAD) {
+    const void* src = KIND == LIN_DGRAD ? (p.scale != nullptr ? p.x : nullptr) : p.res;
+    if (p.scale != nullptr) r.s = load_as_f32(p.scale, p.scale_dt, i);
+    if (src != nullptr) {
+      const St* q = static_cast<const St*>(src) + i * p.J + j;
+      if constexpr (VEC) {
+        __builtin_memcpy(r.v, __builtin_assume_aligned(q, sizeof(St) * W < 16 ? sizeof(St) * W : 16),
+                         sizeof(r.v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (e < n) r.v[e] = q[e];
+      }
+    }
+  }
+  return r;
 }
 
 // The sums v (GATED: gate v and up u) of row i, columns j .. j + W - 1 (n of
@@ -119,20 +173,15 @@ __device__ __forceinline__ void lin_bias(const LinArgs& p, int64_t j, int n, flo
 // Returns DGRAD's share of the row's dot product.
 template <int KIND, class TT, int W, bool VEC>
 __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t j, int n,
-                                            float (&v)[W], float (&u)[W], const DropKey& dk) {
+                                            float (&v)[W], float (&u)[W], const DropKey& dk,
+                                            const LinCols<KIND, W>& col, const LinRow<TT, W>& row) {
   float dot = 0.f;
   if constexpr (KIND == LIN_ACT || KIND == LIN_GATED) {
     const int64_t width = KIND == LIN_GATED ? 2 * p.J : p.J;
-    if (p.bias != nullptr) {
-      float b[W];
-      lin_bias<W>(p, j, n, b);
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[e] += b[e];
-      if constexpr (KIND == LIN_GATED) {
-        lin_bias<W>(p, p.J + j, n, b);
-#pragma unroll
-        for (int e = 0; e < W; ++e) u[e] += b[e];
-      }
+    for (int e = 0; e < W; ++e) {
+      v[e] += col.b[e];
+      if constexpr (KIND == LIN_GATED) u[e] += col.bu[e];
     }
     if (p.pre != nullptr) {
       lin_store<F32T, W, VEC>(p.pre, i * width + j, n, v);
@@ -143,48 +192,32 @@ __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t
       v[e] = lin_act<TT>(p.act, v[e]);
       if constexpr (KIND == LIN_GATED) v[e] *= u[e];
     }
-  } else if constexpr (KIND == LIN_RES) {
-    if (p.bias != nullptr) {
-      float b[W];
-      lin_bias<W>(p, j, n, b);
+  } else if constexpr (KIND == LIN_RES || KIND == LIN_DROP) {
+    uint32_t w[4] = {};
+    if constexpr (KIND == LIN_DROP) philox(dk, (uint32_t)(j >> 3), (uint32_t)i, w);
+    const bool upper = W == 4 && (j & 4) != 0;  // the upper four of the group
 #pragma unroll
-      for (int e = 0; e < W; ++e) v[e] += b[e];
-    }
-    if (p.threshold != 0) {
-      uint32_t w[4];
-      philox(dk, (uint32_t)(j >> 3), (uint32_t)i, w);
-      const int at = W == 8 ? 0 : (int)(j & 4);
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const bool keep = W == 8 ? keeps(w, e, p.threshold)
-                                 : (at ? keeps(w, 4 + (e & 3), p.threshold) : keeps(w, e & 3, p.threshold));
-        v[e] = keep ? v[e] * p.alpha : 0.f;
+    for (int e = 0; e < W; ++e) {
+      float t = v[e] + col.b[e];
+      if constexpr (KIND == LIN_DROP) {
+        const bool keep = upper ? keeps(w, 4 + (e & 3), p.threshold) : keeps(w, e, p.threshold);
+        t = keep ? t * p.alpha : 0.f;
       }
-    }
-    if (p.scale != nullptr) {
-      const float s = load_as_f32(p.scale, p.scale_dt, i);
-#pragma unroll
-      for (int e = 0; e < W; ++e) v[e] *= s;
-    }
-    if (p.res != nullptr) {
-      float r[W];
-      lin_load<TT, W, VEC>(p.res, i * p.J + j, n, r);
-#pragma unroll
-      for (int e = 0; e < W; ++e) v[e] += r[e];
+      if (p.scale != nullptr) t *= row.s;
+      v[e] = p.res != nullptr ? t + TT::to_f32(row.v[e]) : t;
     }
   } else {
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] *= p.alpha;
     if constexpr (KIND == LIN_DGRAD) {
       if (p.scale != nullptr) {
-        const float s = load_as_f32(p.scale, p.scale_dt, i);
         float x[W];
-        lin_load<TT, W, VEC>(p.x, i * p.J + j, n, x);
 #pragma unroll
         for (int e = 0; e < W; ++e) {
+          x[e] = TT::to_f32(row.v[e]);
           dot += e < n ? x[e] * v[e] : 0.f;
-          v[e] *= s;
-          x[e] *= s;
+          v[e] *= row.s;
+          x[e] *= row.s;
         }
         if (p.xs != nullptr) lin_store<TT, W, VEC>(p.xs, i * p.J + j, n, x);
       }

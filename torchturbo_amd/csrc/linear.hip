@@ -24,8 +24,11 @@ __global__ __launch_bounds__(L_NT) void linear_join_kernel(LinArgs p, int64_t gr
   const bool live = i < p.I && j < p.J;
   const int n = !live ? 0 : p.J - j < 8 ? (int)(p.J - j) : 8;
   const int64_t width = KIND == LIN_GATED ? 2 * p.J : p.J;
+  const LinCols<KIND, 8> cols = lin_cols<KIND, 8>(p, j, n);
+  LinRow<TT, 8> row{};
   float v[8] = {}, u[8] = {};
   if (live) {
+    row = lin_row<KIND, TT, 8, VEC>(p, i, j, n);
 #pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
       const int64_t at = ((int64_t)s * p.I + i) * width + j;
@@ -41,9 +44,9 @@ __global__ __launch_bounds__(L_NT) void linear_join_kernel(LinArgs p, int64_t gr
     }
   }
   DropKey dk{};
-  if (KIND == LIN_RES && p.threshold != 0) dk = load_key(p.key);
+  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
   float dot = 0.f;
-  if (live) dot = lin_finish<KIND, TT, 8, VEC>(p, i, j, n, v, u, dk);
+  if (live) dot = lin_finish<KIND, TT, 8, VEC>(p, i, j, n, v, u, dk, cols, row);
   if constexpr (KIND == LIN_DGRAD) {
     if (p.dots != nullptr) {
 #pragma unroll
@@ -82,6 +85,7 @@ int join_kind(int kind, const LinArgs& p, hipStream_t s) {
     case LIN_ACT: return join<LIN_ACT, TT>(p, s);
     case LIN_GATED: return join<LIN_GATED, TT>(p, s);
     case LIN_RES: return join<LIN_RES, TT>(p, s);
+    case LIN_DROP: return join<LIN_DROP, TT>(p, s);
     case LIN_DGRAD: return join<LIN_DGRAD, TT>(p, s);
     default: return join<LIN_PLAIN, TT>(p, s);
   }
@@ -108,17 +112,25 @@ struct Plan {
   Split split;
 };
 
-Plan plan_of(int kind, int64_t I, int64_t J, int64_t R, bool fast) {
+// The part of an MN-major operand that a block of the 16-bit tiles walks has to
+// stay within 32-bit offsets.
+int64_t least_splits(int layout, int64_t I, int64_t J, int64_t R) {
+  const int64_t ld = layout == LAY_TN ? std::max(I, J) : layout == LAY_NN ? J : 0;
+  return std::max<int64_t>((R * ld * 2 + (1ll << 31) - 1) >> 31, 1);
+}
+
+Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, bool fast) {
   const int64_t half = kind == LIN_GATED ? 2 : 1;
+  const int64_t least = least_splits(layout, I, J, R);
   auto tiles = [&](int64_t t) { return ((I + t - 1) / t) * ((half * J + t - 1) / t); };
   if (!fast) {
     // Enough blocks for the CUs, each reduction at least 256 long.
     const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64), 1), R / 256);
     return Plan{0, split_of(R, std::min<int64_t>(want, 32))};
   }
-  if (tiles(256) >= 192) return Plan{256, split_of(R, 1)};
+  if (tiles(256) >= 192) return Plan{256, split_of(R, least)};
   const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(tiles(128), 1), R / 256);
-  return Plan{128, split_of(R, std::min<int64_t>(want, 32))};
+  return Plan{128, split_of(R, std::max(least, std::min<int64_t>(want, 32)))};
 }
 
 size_t part_bytes(int kind, int64_t I, int64_t J, int64_t splits) {
@@ -143,8 +155,12 @@ bool fast_sizes(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R
 int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_bytes,
                 hipStream_t s) {
   const bool fast = vectors(p) && fast_sizes(layout, kind, dtype, p.I, p.J, p.R);
-  Plan pl = plan_of(kind, p.I, p.J, p.R, fast);
-  if (part_bytes(kind, p.I, p.J, pl.split.splits) > ws_bytes) pl.split = split_of(p.R, 1);
+  Plan pl = plan_of(layout, kind, p.I, p.J, p.R, fast);
+  if (part_bytes(kind, p.I, p.J, pl.split.splits) > ws_bytes) {
+    // Without room for the parts: a whole reduction, on the kernel for any size where
+    // the tiles cannot walk it.
+    pl = Plan{fast && least_splits(layout, p.I, p.J, p.R) == 1 ? pl.tile : 0, split_of(p.R, 1)};
+  }
   const Split sp = pl.split;
   p.splits = sp.splits;
   p.rsplit = sp.run;
@@ -368,9 +384,9 @@ extern "C" size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t 
   if (m <= 0 || k < 0 || n < 0) return 0;
   // The larger of the two plans: which one runs also depends on the addresses.
   auto parts = [&](int layout, int kind, int64_t I, int64_t J, int64_t R) {
-    const int64_t any = plan_of(kind, I, J, R, false).split.splits;
+    const int64_t any = plan_of(layout, kind, I, J, R, false).split.splits;
     const int64_t fast = fast_sizes(layout, kind, dtype, I, J, R)
-                             ? plan_of(kind, I, J, R, true).split.splits : 1;
+                             ? plan_of(layout, kind, I, J, R, true).split.splits : 1;
     return part_bytes(kind, I, J, std::max(any, fast));
   };
   switch (op) {
@@ -474,7 +490,8 @@ extern "C" int tt_linear_residual_fwd(const void* x, const void* w, const void* 
   p.threshold = (uint32_t)threshold;
   p.alpha = keep_inverse(threshold);
   p.key = key;
-  return run_product(LAY_NT, LIN_RES, dtype, p, workspace, workspace_bytes, S(stream));
+  return run_product(LAY_NT, threshold != 0 ? LIN_DROP : LIN_RES, dtype, p, workspace,
+                     workspace_bytes, S(stream));
 }
 
 extern "C" int tt_linear_residual_bwd(const void* dy, const void* row_scale, int scale_dtype,

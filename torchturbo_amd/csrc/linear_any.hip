@@ -141,7 +141,7 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
   }
   // Lane l holds row 32 m + l % 32, columns 32 n + 8 g + 4 (l / 32) + 0..3 of the wave's.
   DropKey dk{};
-  if (KIND == LIN_RES && p.threshold != 0) dk = load_key(p.key);
+  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
   const int64_t width = GATED ? 2 * p.J : p.J;
 #pragma unroll
   for (int m = 0; m < F; ++m) {
@@ -171,9 +171,11 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
             if (GATED) o[p.J + e] = u[e];
           }
         } else if (vec && p.J % 4 == 0) {
-          dot += lin_finish<KIND, TT, 4, true>(p, i, j, left, v, u, dk);
+          dot += lin_finish<KIND, TT, 4, true>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
+                                             lin_row<KIND, TT, 4, true>(p, i, j, left));
         } else {
-          dot += lin_finish<KIND, TT, 4, false>(p, i, j, left, v, u, dk);
+          dot += lin_finish<KIND, TT, 4, false>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
+                                             lin_row<KIND, TT, 4, false>(p, i, j, left));
         }
       }
     if constexpr (KIND == LIN_DGRAD) {
@@ -237,6 +239,7 @@ int tt_linear_any(int kind, int dtype, const LinArgs& p, hipStream_t s) {
     case LIN_ACT: return typed<LAY_NT, LIN_ACT>(dtype, p, s);
     case LIN_GATED: return typed<LAY_NT, LIN_GATED>(dtype, p, s);
     case LIN_RES: return typed<LAY_NT, LIN_RES>(dtype, p, s);
+    case LIN_DROP: return typed<LAY_NT, LIN_DROP>(dtype, p, s);
     case LIN_DGRAD: return typed<LAY_NN, LIN_DGRAD>(dtype, p, s);
     default: return typed<LAY_TN, LIN_PLAIN>(dtype, p, s);
   }

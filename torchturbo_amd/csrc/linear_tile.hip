@@ -14,28 +14,44 @@
 #include "gemm.h"
 #include "linear.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int T_NT = 256, T_BK = 64;
 
-// A buffer resource that walks along an operand, 64 bits wide: k-tiles of
-// operands of any size.
+// A buffer resource that walks along an operand a k-tile at a time, in scalar
+// registers. MN-major: it ends with the reduction's rows, so it is empty past them (the
+// part of a reduction that a block walks is under 4 GiB). K-major: a row's end is
+// masked by the loads, the resource keeps ending with the operand's last row.
 struct Walk {
-  uint64_t base;
-  int64_t left;
-  __device__ __forceinline__ i32x4 rsrc() const {
-    i32x4 r;
-    r.x = (int)(uint32_t)base;
-    r.y = (int)((uint32_t)(base >> 32) & 0xFFFFu);
-    r.z = (int)(left <= 0 ? 0u : left < (int64_t)DM_OOB ? (uint32_t)left : DM_OOB);
-    r.w = 0x00020000;
-    return r;
-  }
-  __device__ __forceinline__ void advance(int64_t by) {
-    base += (uint64_t)by;
-    left -= by;
+  i32x4 r;
+  __device__ __forceinline__ void start(const void* base, int64_t left) { r = make_rsrc(base, left); }
+  template <bool KM>
+  __device__ __forceinline__ void advance(uint32_t by, bool more) {
+    const uint32_t lo = (uint32_t)r.x + by;
+    r.y += lo < by ? 1 : 0;  // a stride of 0 above the address
+    r.x = (int)lo;
+    if constexpr (KM) {
+      r.z = more ? r.z : 0;
+    } else {
+      // max(records - by, 0) in scalar instructions (the compiler's is a vector one).
+      uint32_t n;
+      asm("s_sub_u32 %0, %1, %2\n\ts_cselect_b32 %0, 0, %0" : "=s"(n) : "s"(r.z), "s"(by) : "scc");
+      r.z = (int)n;
+    }
   }
 };
+
+// 16 bytes per lane into LDS at base + at + 16 lane (gemm.h's dma16 with the
+// address formed in M0).
+template <int AT>
+__device__ __forceinline__ void dma16_at(uint32_t voff, const i32x4& rsrc, uint32_t base) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(base), "v"(voff), "s"(rsrc), "i"(AT)
+               : "memory", "scc");
+}
 
 // Fragment offset of MN-major tiles with RB bytes per k-row: columns c0 .. c0 + 31;
 // the second read is at + 4 RB and k-step s adds 16 RB.
@@ -95,12 +111,21 @@ struct Operand {
       for (int m = 0; m < FR; ++m) frag[m] = frag_mn<RB>((BR / 2) * half + 32 * m, lane);
     }
   }
-  // Load q of a k-tile of which `valid` reduction elements exist.
-  template <bool KMASK>
-  __device__ __forceinline__ void load(int q, const i32x4& rs, uint32_t lds, int wave, int valid) const {
-    uint32_t o = off[q];
-    if constexpr (KM && KMASK) o = kof[q & 1] >= valid ? DM_OOB : o;
-    dma16(o, rs, lds + (uint32_t)(LOADS * wave + q) * 1024u);
+  // Load Q of a k-tile of which `valid` reduction elements exist, into the operand's
+  // stage; `lds` is the wave's first byte of it.
+  template <bool KMASK, int Q>
+  __device__ __forceinline__ void load(const i32x4& rs, uint32_t lds, int valid) const {
+    uint32_t o = off[Q];
+    if constexpr (KM && KMASK) o = kof[Q & 1] >= valid ? DM_OOB : o;
+    dma16_at<Q * 1024>(o, rs, lds);
+  }
+  // Loads FROM .. TO - 1.
+  template <bool KMASK, int FROM, int TO>
+  __device__ __forceinline__ void loads(const i32x4& rs, uint32_t lds, int valid) const {
+    if constexpr (FROM < TO) {
+      load<KMASK, FROM>(rs, lds, valid);
+      loads<KMASK, FROM + 1, TO>(rs, lds, valid);
+    }
   }
   __device__ __forceinline__ uint4 read(lds_char* tile, int m, int s) const {
     if constexpr (KM) return read_k(tile, frag[s] + m * 4096);
@@ -115,76 +140,215 @@ struct TypeOf<TT_BF16> { typedef BF16T type; };
 template <>
 struct TypeOf<TT_F16> { typedef F16T type; };
 
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((address_space(3))) f32x4_t lds_f32x4;
+
+// Eight 16-bit values of four dwords, and back (hardware round to nearest even).
+template <int ET>
+__device__ __forceinline__ void unpack8(const u32x4& w, float (&o)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (ET == TT_BF16) {
+      o[2 * e] = __uint_as_float(w[e] << 16);
+      o[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    } else {
+      o[2 * e] = f16_to_f32((uint16_t)(w[e] & 0xffffu));
+      o[2 * e + 1] = f16_to_f32((uint16_t)(w[e] >> 16));
+    }
+  }
+}
+template <int ET>
+__device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
+  const uint2 lo = pack4<ET>(v[0], v[1], v[2], v[3]), hi = pack4<ET>(v[4], v[5], v[6], v[7]);
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// Sum over the eight lanes of a group of eight.
+__device__ __forceinline__ float sum8(float v) {
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true));   // ^ 1
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true));   // ^ 2
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true));  // ^ 7
+  return v;
+}
+
+// The wave's rows [i0, I) of a matrix of `ld` elements of `size` bytes per row, from column
+// j0 on: rows past I read as zeros, and stores to them are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* m, int64_t i0, int64_t I,
+                                                            int64_t ld, int64_t j0, int size) {
+  const int64_t at = (i0 * ld + j0) * size, left = m == nullptr ? 0 : I * ld * size - at;
+  return __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(m)) + at, (short)0,
+      (int)(left <= 0 ? 0u : left < (int64_t)DM_OOB ? (uint32_t)left : DM_OOB), 0x00020000);
+}
+
 // The sums of a wave's (32 FM) x (32 FN) part of the tile to what KIND makes of
-// them, 32 rows at a time through the wave's own LDS (rows of 128 FN bytes,
-// 16-byte chunk c of row r in slot c ^ r), so that a lane gets eight consecutive
-// columns, with GATED their ups too.
+// them (linear.h), 32 rows at a time through the wave's own LDS, so that a lane gets
+// eight consecutive columns, with GATED their ups too. Rows of 128 FN bytes; chunk
+// c of row r in slot ((c / 2) ^ r) + (c % 2) CH / 2, which neither the writes (four
+// columns of 32 rows) nor the reads (a row's chunks) of eight lanes meet in a bank.
+// One wave per SIMD has nothing to hide instructions behind, so memory is reached
+// through resources with 32-bit offsets, conversions are the hardware's, and what a
+// row needs is fetched 32 rows ahead: 4096 x 4096 x 512 with a residual 48 -> XX us,
+// the gradient's form 73 -> XX.
 template <int KIND, int ET, int FM, int FN>
 __device__ __forceinline__ void tile_finish(const LinArgs& p, const f32x16 (&acc)[FM][FN],
                                             lds_char* region, int64_t i0, int64_t j0, int lane) {
   typedef typename TypeOf<ET>::type TT;
   constexpr bool GATED = KIND == LIN_GATED;
-  constexpr int W = 32 * FN, CH = W / 4, MASK = CH - 1;  // columns and 16-byte chunks of a row
-  constexpr int NG = (GATED ? W / 2 : W) / 8;            // groups of eight outputs of a row
-  constexpr int RP = 64 / NG;                            // rows per pass
-  typedef __attribute__((ext_vector_type(4))) float f32x4_t;
-  typedef __attribute__((address_space(3))) f32x4_t lds_f32x4;
+  constexpr int W = 32 * FN, CH = W / 4;       // columns and 16-byte chunks of a row
+  constexpr int NG = (GATED ? W / 2 : W) / 8;  // groups of eight outputs of a row
+  constexpr int RP = 64 / NG, NP = 32 / RP;    // rows per pass, passes per 32 rows
+  constexpr bool SRC = KIND == LIN_RES || KIND == LIN_DROP || KIND == LIN_DGRAD;
+  constexpr int BUF = KIND == LIN_DROP ? 1 : 2;  // random words take the registers of one
   const int r_l = lane & 31, h = lane >> 5;
   const int gi = lane % NG, rr = lane / NG;
   const int64_t j = j0 + 8 * gi, width = GATED ? 2 * p.J : p.J;
+  const bool col_ok = j < p.J;
   DropKey dk{};
-  if (KIND == LIN_RES && p.threshold != 0) dk = load_key(p.key);
+  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
+  const LinCols<KIND, 8> cols = lin_cols<KIND, 8>(p, j, col_ok ? 8 : 0);
+  // Scale of rows lane and lane + 64 of the wave's.
+  const bool scaled = SRC && p.scale != nullptr && p.part == nullptr;
+  float sc[2] = {1.f, 1.f};
+  if (scaled) {
+#pragma unroll
+    for (int q = 0; q < (FM + 1) / 2; ++q) {
+      const int64_t i = i0 + 64 * q + lane;
+      if (i < p.I) sc[q] = load_as_f32(p.scale, p.scale_dt, i);
+    }
+  }
+  // Byte offsets of the lane's group in 16-bit rows and in fp32 ones (columns that
+  // do not exist get one past any resource).
+  const uint32_t off16 = (uint32_t)((rr * p.J + 8 * gi) * 2);
+  const uint32_t off32 = (uint32_t)((rr * width + 8 * gi) * 4);
+  const uint32_t row16 = (uint32_t)(p.J * 2), row32 = (uint32_t)(width * 4);
+  const __amdgpu_buffer_rsrc_t out = rows_rsrc(p.out, i0, p.I, p.J, j0, 2);
+  const void* src = KIND == LIN_DGRAD ? (scaled ? p.x : nullptr) : SRC ? p.res : nullptr;
+  const __amdgpu_buffer_rsrc_t in = rows_rsrc(src, i0, p.I, p.J, j0, 2);
+  const __amdgpu_buffer_rsrc_t xs = rows_rsrc(KIND == LIN_DGRAD ? p.xs : nullptr, i0, p.I, p.J, j0, 2);
+  float* const wide = p.part != nullptr ? p.part + (int64_t)blockIdx.y * p.I * width : p.pre;
+  const __amdgpu_buffer_rsrc_t w0 = rows_rsrc(wide, i0, p.I, width, j0, 4);
+  const __amdgpu_buffer_rsrc_t w1 = rows_rsrc(GATED ? wide : nullptr, i0, p.I, width, p.J + j0, 4);
+  const bool keep_sums = wide != nullptr, whole = p.part == nullptr;
+  const int nd = (int)((p.J + LIN_DOT - 1) / LIN_DOT);
+
+  auto put32 = [&](const __amdgpu_buffer_rsrc_t& rs, const float (&v)[8], uint32_t off) {
+    const f32x4_t lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rs,
+                                           (int)(col_ok ? off : DM_OOB), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rs,
+                                           (int)(col_ok ? off + 16 : DM_OOB), 0, 0);
+  };
+  u32x4 rows[BUF][SRC ? NP : 1] = {};
+  const bool fetched = SRC && src != nullptr && whole;
+  auto fetch = [&](int mi) {
+#pragma unroll
+    for (int ps = 0; ps < NP; ++ps)
+      rows[mi % BUF][ps] = __builtin_amdgcn_raw_buffer_load_b128(
+          in, (int)(col_ok ? off16 + (uint32_t)(32 * mi + ps * RP) * row16 : DM_OOB), 0, 0);
+  };
+  auto pass = [&](int mi, int ps, const u32x4& row) {
+    const int r = ps * RP + rr;
+    auto chunk = [&](int c) {
+      return *reinterpret_cast<const lds_f32x4*>(
+          region + r * (W * 4) + ((((c >> 1) ^ (r & (CH / 2 - 1))) + (c & 1) * (CH / 2)) << 4));
+    };
+    float v[8], u[8];
+    const f32x4_t a = chunk(2 * gi), b = chunk(2 * gi + 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[4 + e] = b[e];
+    }
+    if constexpr (GATED) {
+      const f32x4_t c = chunk(CH / 2 + 2 * gi), d = chunk(CH / 2 + 2 * gi + 1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u[e] = c[e];
+        u[4 + e] = d[e];
+      }
+    }
+    const int q = 32 * mi + ps * RP;  // the pass's first row in the wave's
+    const uint32_t at16 = off16 + (uint32_t)q * row16, at32 = off32 + (uint32_t)q * row32;
+    if (!whole) {  // a split's sums
+      put32(w0, v, at32);
+      if constexpr (GATED) put32(w1, u, at32);
+      return;
+    }
+    float s = 1.f;
+    if (scaled) s = __shfl(sc[FM > 2 ? mi / 2 : 0], 32 * (mi & 1) + ps * RP + rr, 64);
+    if constexpr (KIND == LIN_ACT || KIND == LIN_GATED) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] += cols.b[e];
+        if constexpr (GATED) u[e] += cols.bu[e];
+      }
+      if (keep_sums) {
+        put32(w0, v, at32);
+        if constexpr (GATED) put32(w1, u, at32);
+      }
+      auto activate = [&](int act) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = lin_act<TT>(act, v[e]);
+      };
+      if (p.act == ACT_SILU) activate(ACT_SILU);
+      else if (p.act == ACT_GELU) activate(ACT_GELU);
+      if constexpr (GATED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= u[e];
+      }
+    } else if constexpr (KIND == LIN_RES || KIND == LIN_DROP) {
+      uint32_t w[4] = {};
+      if constexpr (KIND == LIN_DROP)
+        philox(dk, (uint32_t)(j >> 3), (uint32_t)(i0 + q + rr), w);
+      float x[8];
+      unpack8<ET>(row, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float t = v[e] + cols.b[e];
+        if constexpr (KIND == LIN_DROP) t = keeps(w, e, p.threshold) ? t * p.alpha : 0.f;
+        v[e] = x[e] + s * t;  // x is zero where there is no residual
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= p.alpha;
+      if (KIND == LIN_DGRAD && scaled) {
+        float x[8], dot = 0.f;
+        unpack8<ET>(row, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          dot += x[e] * v[e];
+          v[e] *= s;
+          x[e] *= s;
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(pack8<ET>(x), xs, (int)(col_ok ? at16 : DM_OOB), 0, 0);
+        if (p.dots != nullptr) {
+          dot = sum8(dot);
+          const int64_t i = i0 + q + rr;
+          if ((lane & 7) == 0 && i < p.I && col_ok) p.dots[i * nd + j / LIN_DOT] = dot;
+        }
+      }
+    }
+    __builtin_amdgcn_raw_buffer_store_b128(pack8<ET>(v), out, (int)(col_ok ? at16 : DM_OOB), 0, 0);
+  };
+  if (fetched && BUF == 2) fetch(0);
 #pragma unroll
   for (int mi = 0; mi < FM; ++mi) {
+    if (fetched && mi + BUF - 1 < FM) fetch(mi + BUF - 1);
 #pragma unroll
     for (int ni = 0; ni < FN; ++ni)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 8 * ni + 2 * g + h;
-        *reinterpret_cast<lds_f32x4*>(region + r_l * (W * 4) + ((c ^ (r_l & MASK)) << 4)) =
+      for (int g = 0; g < 4; ++g)  // chunk 8 ni + 2 g + h
+        *reinterpret_cast<lds_f32x4*>(
+            region + r_l * (W * 4) + ((((4 * ni + g) ^ (r_l & (CH / 2 - 1))) + h * (CH / 2)) << 4)) =
             f32x4_t{acc[mi][ni][4 * g], acc[mi][ni][4 * g + 1], acc[mi][ni][4 * g + 2],
                     acc[mi][ni][4 * g + 3]};
-      }
-#pragma unroll 1
-    for (int ps = 0; ps < 32 / RP; ++ps) {
-      const int r = ps * RP + rr;
-      const int64_t i = i0 + 32 * mi + r;
-      auto chunk = [&](int c) {
-        return *reinterpret_cast<const lds_f32x4*>(region + r * (W * 4) + ((c ^ (r & MASK)) << 4));
-      };
-      float v[8], u[8] = {};
-      const f32x4_t a = chunk(2 * gi), b = chunk(2 * gi + 1);
+    if constexpr (SRC) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-      }
-      if constexpr (GATED) {
-        const f32x4_t c = chunk(CH / 2 + 2 * gi), d = chunk(CH / 2 + 2 * gi + 1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          u[e] = c[e];
-          u[4 + e] = d[e];
-        }
-      }
-      float dot = 0.f;
-      if (i < p.I && j < p.J) {
-        if (p.part != nullptr) {
-          const int64_t at = ((int64_t)blockIdx.y * p.I + i) * width + j;
-          lin_store<F32T, 8, true>(p.part, at, 8, v);
-          if constexpr (GATED) lin_store<F32T, 8, true>(p.part, at + p.J, 8, u);
-        } else {
-          dot = lin_finish<KIND, TT, 8, true>(p, i, j, 8, v, u, dk);
-        }
-      }
-      if constexpr (KIND == LIN_DGRAD) {
-        if (p.dots != nullptr && p.part == nullptr) {
-#pragma unroll
-          for (int off = 1; off < LIN_DOT / 8; off <<= 1) dot += __shfl_xor(dot, off, 64);
-          if (i < p.I && j < p.J && j % LIN_DOT == 0)
-            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
-        }
-      }
+      for (int ps = 0; ps < NP; ++ps) pass(mi, ps, rows[mi % BUF][ps]);
+    } else {
+#pragma unroll 2
+      for (int ps = 0; ps < NP; ++ps) pass(mi, ps, rows[0][0]);
     }
   }
 }
@@ -210,7 +374,7 @@ struct Tile {
   OpA a;
   OpB b;
   Walk wa, wb;
-  int64_t sa, sb;  // bytes of a k-tile step
+  uint32_t sa, sb;  // bytes of a k-tile step
   int64_t i0, j0;
   int nkt, kn;  // k-tiles and reduction elements of this block
 
@@ -228,16 +392,18 @@ struct Tile {
     // First byte of the tile's part of the operand, and the bytes from there to
     // the operand's end (of this split's reduction rows where they are MN-major).
     const int64_t oa = A_K ? (i0 * p.lda + r0) * 2 : (r0 * p.lda + i0) * 2;
-    wa = Walk{reinterpret_cast<uint64_t>(pa) + (uint64_t)oa,
-              (A_K ? p.I * p.lda * 2 : (r0 + n) * p.lda * 2) - oa};
-    sa = A_K ? T_BK * 2 : T_BK * p.lda * 2;
+    wa.start(pa + oa, (A_K ? p.I * p.lda * 2 : (r0 + n) * p.lda * 2) - oa);
+    sa = A_K ? T_BK * 2 : (uint32_t)(T_BK * p.lda * 2);
     const int64_t ob = B_K ? (j0 * p.ldb + r0) * 2 : (r0 * p.ldb + j0) * 2;
-    wb = Walk{reinterpret_cast<uint64_t>(pb) + (uint64_t)ob,
-              (B_K ? (GATED ? 2 : 1) * p.J * p.ldb * 2 : (r0 + n) * p.ldb * 2) - ob};
-    sb = B_K ? T_BK * 2 : T_BK * p.ldb * 2;
+    wb.start(pb + ob, (B_K ? (GATED ? 2 : 1) * p.J * p.ldb * 2 : (r0 + n) * p.ldb * 2) - ob);
+    sb = B_K ? T_BK * 2 : (uint32_t)(T_BK * p.ldb * 2);
+    if (nkt == 0) wa.r.z = wb.r.z = 0;
     a.setup(wave, lane, wave >> 1, p.lda, 0);
     b.setup(wave, lane, wave & 1, p.ldb, p.J);
   }
+  // The resources of the k-tile after the one they stand at, kt.
+  __device__ __forceinline__ void next_a(int kt) { wa.template advance<A_K>(sa, kt + 1 < nkt); }
+  __device__ __forceinline__ void next_b(int kt) { wb.template advance<B_K>(sb, kt + 1 < nkt); }
 };
 
 // 256 x 256 tiles, 128 x 128 per wave (256 accumulators, one wave per SIMD), two
@@ -249,81 +415,106 @@ struct Tile {
 template <int LAYOUT, int KIND, int ET, bool KMASK>
 __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, 256, 256> TL;
-  constexpr int FM = 4, FN = 4, NM = FM * FN, NF = FM + FN;
+  constexpr int FM = 4, FN = 4, NM = FM * FN;
   constexpr int LA = TL::OpA::LOADS, LB = TL::OpB::LOADS;
-  __shared__ __align__(16) char lds_raw[2 * TL::STAGE];
+  static_assert(LA == 8 && LB == 8, "four loads per k-step");
+  constexpr uint32_t BA = TL::OpA::BYTES, BB = TL::OpB::BYTES;
+  __shared__ __align__(16) char lds_raw[2 * BA + 3 * BB];  // two k-tiles of A, then three of B
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   TL t;
   t.setup(p, ti, tj, wave, lane);
   lds_char* const lds = (lds_char*)lds_raw;
   const uint32_t lds0 = lds_addr_of(lds);
-  auto load_a = [&](int q, const i32x4& rs, int kt) {
-    t.a.template load<KMASK>(q, rs, lds0 + (uint32_t)(kt & 1) * TL::STAGE, wave, t.kn - kt * T_BK);
-  };
-  auto load_b = [&](int q, const i32x4& rs, int kt) {
-    t.b.template load<KMASK>(q, rs, lds0 + (uint32_t)(kt & 1) * TL::STAGE + TL::OpA::BYTES, wave,
-                             t.kn - kt * T_BK);
-  };
-  // Resource of k-tile kt of a walk that stands there; none past the last.
-  auto at = [&](const Walk& w, int kt) {
-    i32x4 r = w.rsrc();
-    if (kt >= t.nkt) r.z = 0;
-    return r;
-  };
-  uint4 a0[FM], b0[FN], a1[FM], b1[FN];
-  auto frag = [&](lds_char* stg, int s, int i, uint4 (&fa)[FM], uint4 (&fb)[FN]) {
-    if (i < FM) fa[i] = t.a.read(stg, i, s);
-    else fb[i - FM] = t.b.read(stg + TL::OpA::BYTES, i - FM, s);
-  };
+  const uint32_t wa0 = lds0 + (uint32_t)(LA * wave) * 1024u;           // the wave's part of A's stages
+  const uint32_t wb0 = lds0 + 2 * BA + (uint32_t)(LB * wave) * 1024u;  // and of B's
+  // Fragments of the four k-steps of a k-tile (at most about half of them live).
+  uint4 fa[4][FM], fb[4][FN];
+  auto read_a = [&](lds_char* sa, int s, int i) { fa[s][i] = t.a.read(sa, i, s); };
+  auto read_b = [&](lds_char* sb, int s, int i) { fb[s][i] = t.b.read(sb, i, s); };
   f32x16 acc[FM][FN] = {};
   {
-    const i32x4 ra = at(t.wa, 0), rb = at(t.wb, 0);
-#pragma unroll
-    for (int q = 0; q < LA; ++q) load_a(q, ra, 0);
-#pragma unroll
-    for (int q = 0; q < LB; ++q) load_b(q, rb, 0);
-    t.wa.advance(t.sa);
-    t.wb.advance(t.sb);
-    const i32x4 r1 = at(t.wa, 1);
-#pragma unroll
-    for (int q = 0; q < LA; ++q) load_a(q, r1, 1);
-    t.wa.advance(t.sa);
-    TT_WAIT_VMCNT(LA);
+    t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0, t.kn);
+    t.b.template loads<KMASK, 0, LB>(t.wb.r, wb0, t.kn);
+    t.next_a(0);
+    t.next_b(0);
+    t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0 + BA, t.kn - T_BK);
+    t.b.template loads<KMASK, 0, LB>(t.wb.r, wb0 + BB, t.kn - T_BK);
+    t.next_a(1);
+    t.next_b(1);
+    TT_WAIT_VMCNT(LA + LB);
     TT_LDS_BARRIER();
 #pragma unroll
-    for (int i = 0; i < NF; ++i) frag(lds, 0, i, a0, b0);
+    for (int i = 0; i < FM; ++i) read_a(lds, 0, i);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) read_b(lds + 2 * BA, 0, i);
   }
+  int slot = 0;  // of B's k-tile kt
   for (int kt = 0; kt < t.nkt; ++kt) {
-    lds_char* const cur = lds + (kt & 1) * TL::STAGE;
-    lds_char* const nxt = lds + ((kt + 1) & 1) * TL::STAGE;
-    const i32x4 rb = at(t.wb, kt + 1), ra = at(t.wa, kt + 2);
-#pragma unroll
-    for (int s = 0; s < 3; ++s) {
-#pragma unroll
-      for (int i = 0; i < NM; ++i) {
-        f32x16& c = acc[i / FN][i % FN];
-        c = (s & 1) ? Mma<ET>::run(b1[i % FN], a1[i / FN], c) : Mma<ET>::run(b0[i % FN], a0[i / FN], c);
-        if (i < NF) {
-          if (s & 1) frag(cur, s + 1, i, a0, b0);
-          else frag(cur, s + 1, i, a1, b1);
-        }
-        if (s == 0 && (i & 1)) load_b(i / 2, rb, kt + 1);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    TT_WAIT_VMCNT(0);
-    TT_LDS_BARRIER();
-#pragma unroll
-    for (int i = 0; i < NM; ++i) {
+    const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
+    lds_char* const ca = lds + (uint32_t)(kt & 1) * BA;
+    lds_char* const na = lds + (uint32_t)((kt + 1) & 1) * BA;
+    lds_char* const cb = lds + 2 * BA + (uint32_t)slot * BB;
+    lds_char* const nb = lds + 2 * BA + (uint32_t)slot1 * BB;
+    const uint32_t to_a = wa0 + (uint32_t)(kt & 1) * BA, to_b = wb0 + (uint32_t)slot2 * BB;
+    const int valid = t.kn - (kt + 2) * T_BK;
+    // Product i of k-step s. The empty asm keeps it in its slot: products have no side
+    // effects, and the compiler otherwise moves half of them behind the barriers.
+    auto mul = [&](int s, int i) {
       f32x16& c = acc[i / FN][i % FN];
-      c = Mma<ET>::run(b1[i % FN], a1[i / FN], c);
-      if (i < NF) frag(nxt, 0, i, a0, b0);
-      if (i & 1) load_a(i / 2, ra, kt + 2);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    t.wa.advance(t.sa);
-    t.wb.advance(t.sb);
+      c = Mma<ET>::run(fb[s][i % FN], fa[s][i / FN], c);
+      asm volatile("" : "+a"(c));
+    };
+    // k-step s: its products, in slot i what `read` reads, and every fourth one a load
+    // Q0 .. Q0 + 3 of A or B.
+    auto k_step = [&](auto s_c, auto is_a, auto q0_c, auto read) {
+      constexpr int s = decltype(s_c)::value, Q0 = decltype(q0_c)::value;
+      constexpr bool IS_A = decltype(is_a)::value;
+      auto four = [&](auto g_c) {
+        constexpr int g = decltype(g_c)::value;
+#pragma unroll
+        for (int i = 4 * g; i < 4 * g + 4; ++i) {
+          mul(s, i);
+          read(i);
+          if (i == 4 * g + 3) {
+            if constexpr (IS_A) t.a.template load<KMASK, Q0 + g>(t.wa.r, to_a, valid);
+            else t.b.template load<KMASK, Q0 + g>(t.wb.r, to_b, valid);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      four(std::integral_constant<int, 0>{});
+      four(std::integral_constant<int, 1>{});
+      four(std::integral_constant<int, 2>{});
+      four(std::integral_constant<int, 3>{});
+    };
+    constexpr std::integral_constant<int, 0> C0{};
+    constexpr std::integral_constant<int, 1> C1{};
+    constexpr std::integral_constant<int, 2> C2{};
+    constexpr std::integral_constant<int, 3> C3{};
+    constexpr std::integral_constant<int, 4> C4{};
+    k_step(C0, std::false_type{}, C0, [&](int i) {
+      if (i < 4) read_b(cb, 1, i);
+      else if (i < 8) read_a(ca, 1, i - 4);
+      else if (i < 12) read_a(ca, 2, i - 8);
+    });
+    k_step(C1, std::false_type{}, C4, [&](int i) {
+      if (i < 4) read_a(ca, 3, i);
+      else if (i < 8) read_b(cb, 2, i - 4);
+    });
+    t.next_b(kt + 2);
+    TT_LDS_BARRIER();  // every wave has read A's k-tile: its stage is free
+    k_step(C2, std::true_type{}, C0, [&](int i) {
+      if (i < 4) read_b(cb, 3, i);
+    });
+    TT_WAIT_VMCNT(LA / 2 + LB);  // k-tile kt + 1 has landed
+    TT_LDS_BARRIER();
+    k_step(C3, std::true_type{}, C4, [&](int i) {
+      if (i < 4) read_b(nb, 0, i);
+      else if (i < 8) read_a(na, 0, i - 4);
+    });
+    t.next_a(kt + 2);
+    slot = slot1;
   }
   TT_WAIT_VMCNT(0);
   __syncthreads();  // every wave is past its fragment reads, and every load has landed
@@ -346,15 +537,13 @@ __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int
   lds_char* const lds = (lds_char*)lds_raw;
   const uint32_t lds0 = lds_addr_of(lds);
   auto issue = [&](int kt, int slot) {
-    const i32x4 ra = t.wa.rsrc(), rb = t.wb.rsrc();
     const uint32_t at = lds0 + (uint32_t)slot * TL::STAGE;
     const int valid = t.kn - kt * T_BK;
-#pragma unroll
-    for (int q = 0; q < LA; ++q) t.a.template load<KMASK>(q, ra, at, wave, valid);
-#pragma unroll
-    for (int q = 0; q < LB; ++q) t.b.template load<KMASK>(q, rb, at + TL::OpA::BYTES, wave, valid);
-    t.wa.advance(t.sa);
-    t.wb.advance(t.sb);
+    t.a.template loads<KMASK, 0, LA>(t.wa.r, at + (uint32_t)(LA * wave) * 1024u, valid);
+    t.b.template loads<KMASK, 0, LB>(t.wb.r, at + TL::OpA::BYTES + (uint32_t)(LB * wave) * 1024u,
+                                     valid);
+    t.next_a(kt);
+    t.next_b(kt);
   };
   f32x16 acc[FM][FN] = {};
 #pragma unroll
@@ -426,6 +615,7 @@ int tt_linear_tile(int kind, int tile, int dtype, const LinArgs& p, hipStream_t 
     case LIN_ACT: return typed<LAY_NT, LIN_ACT>(tile, dtype, p, s);
     case LIN_GATED: return typed<LAY_NT, LIN_GATED>(tile, dtype, p, s);
     case LIN_RES: return typed<LAY_NT, LIN_RES>(tile, dtype, p, s);
+    case LIN_DROP: return typed<LAY_NT, LIN_DROP>(tile, dtype, p, s);
     case LIN_DGRAD: return typed<LAY_NN, LIN_DGRAD>(tile, dtype, p, s);
     default: return typed<LAY_TN, LIN_PLAIN>(tile, dtype, p, s);
   }
