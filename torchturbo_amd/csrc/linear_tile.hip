@@ -62,6 +62,14 @@ __device__ __forceinline__ uint32_t frag_mn(int c0, int lane) {
   const int kr = 8 * (g >> 1) + (i >> 2);
   return (uint32_t)(kr * RB + (((col >> 3) ^ (4 * (kr & 3))) << 4) + (col & 7) * 2);
 }
+// The same for 16 columns of a 32-deep k-step (which adds 32 RB): lane l gets column
+// c0 + l % 16, k-rows 8 (l / 16) .. + 7.
+template <int RB>
+__device__ __forceinline__ uint32_t frag_mn16(int c0, int lane) {
+  const int g = lane >> 4, i = lane & 15;
+  const int col = c0 + 4 * (i & 3), kr = 8 * g + (i >> 2);
+  return (uint32_t)(kr * RB + (((col >> 3) ^ (4 * (kr & 3))) << 4) + (col & 7) * 2);
+}
 template <int RB>
 __device__ __forceinline__ uint4 read_mn(lds_char* tile, uint32_t off) {
   const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + off));
@@ -73,15 +81,17 @@ __device__ __forceinline__ uint4 read_mn(lds_char* tile, uint32_t off) {
 // One operand of a tile of BR rows (columns): its loads and its fragments.
 // GATE (K-major only): the tile's rows are, per wave column, BR / 4 rows of the
 // first half of the operand (from row 0 of the resource) and as many of the second.
-template <bool KM, int BR, bool GATE>
+// BS: rows of a fragment, 32 (16-deep k-steps) or 16 (32-deep ones).
+template <bool KM, int BR, bool GATE, int BS>
 struct Operand {
   static constexpr int BYTES = BR * T_BK * 2;
   static constexpr int LOADS = BR / 32;    // per wave and k-tile, 1 KiB each
   static constexpr int FR = BR / 64;       // 32-row blocks of a wave
   static constexpr int RB = BR * 2;        // bytes of a k-row (MN-major)
+  static constexpr int KS = BS / 8;        // k-steps of a k-tile
   uint32_t off[LOADS];
   int kof[2];
-  uint32_t frag[KM ? 4 : FR];
+  uint32_t frag[KM ? KS : FR];
 
   __device__ __forceinline__ void setup(int wave, int lane, int half, int64_t ld, int64_t rows2) {
 #pragma unroll
@@ -105,10 +115,19 @@ struct Operand {
     }
     if constexpr (KM) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) frag[s] = fragk64((BR / 2) * half, s, lane);
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (BS == 32) {
+          frag[s] = fragk64((BR / 2) * half, s, lane);
+        } else {  // row lane % 16, chunk 4 s + lane / 16
+          const int r = (BR / 2) * half + (lane & 15), c = 4 * s + (lane >> 4);
+          frag[s] = (uint32_t)(r * 128 + ((c ^ ((r >> 1) & 7)) << 4));
+        }
+      }
     } else {
 #pragma unroll
-      for (int m = 0; m < FR; ++m) frag[m] = frag_mn<RB>((BR / 2) * half + 32 * m, lane);
+      for (int m = 0; m < FR; ++m)
+        frag[m] = BS == 32 ? frag_mn<RB>((BR / 2) * half + 32 * m, lane)
+                           : frag_mn16<RB>((BR / 2) * half + 32 * m, lane);
     }
   }
   // Load Q of a k-tile of which `valid` reduction elements exist, into the operand's
@@ -127,9 +146,11 @@ struct Operand {
       loads<KMASK, FROM + 1, TO>(rs, lds, valid);
     }
   }
+  // Fragment m (BS rows) of k-step s.
   __device__ __forceinline__ uint4 read(lds_char* tile, int m, int s) const {
-    if constexpr (KM) return read_k(tile, frag[s] + m * 4096);
-    else return read_mn<RB>(tile, frag[m] + s * 16 * RB);
+    if constexpr (KM) return read_k(tile, frag[s] + m * (BS * 128));
+    else if constexpr (BS == 32) return read_mn<RB>(tile, frag[m] + s * 16 * RB);
+    else return read_mn<RB>(tile, frag[m / 2] + (m & 1) * 32 + s * 32 * RB);
   }
 };
 
@@ -190,9 +211,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* m, int64
 // through resources with 32-bit offsets, conversions are the hardware's, and what a
 // row needs is fetched 32 rows ahead: 4096 x 4096 x 512 with a residual 48 -> XX us,
 // the gradient's form 73 -> XX.
-template <int KIND, int ET, int FM, int FN>
-__device__ __forceinline__ void tile_finish(const LinArgs& p, const f32x16 (&acc)[FM][FN],
-                                            lds_char* region, int64_t i0, int64_t j0, int lane) {
+// stage(mi, put): calls put(row, chunk, four sums) for the lane's part of the 32 rows mi.
+template <int KIND, int ET, int FM, int FN, typename F>
+__device__ __forceinline__ void tile_finish(const LinArgs& p, F stage, lds_char* region, int64_t i0,
+                                            int64_t j0, int lane) {
   typedef typename TypeOf<ET>::type TT;
   constexpr bool GATED = KIND == LIN_GATED;
   constexpr int W = 32 * FN, CH = W / 4;       // columns and 16-byte chunks of a row
@@ -200,7 +222,6 @@ __device__ __forceinline__ void tile_finish(const LinArgs& p, const f32x16 (&acc
   constexpr int RP = 64 / NG, NP = 32 / RP;    // rows per pass, passes per 32 rows
   constexpr bool SRC = KIND == LIN_RES || KIND == LIN_DROP || KIND == LIN_DGRAD;
   constexpr int BUF = KIND == LIN_DROP ? 1 : 2;  // random words take the registers of one
-  const int r_l = lane & 31, h = lane >> 5;
   const int gi = lane % NG, rr = lane / NG;
   const int64_t j = j0 + 8 * gi, width = GATED ? 2 * p.J : p.J;
   const bool col_ok = j < p.J;
@@ -335,14 +356,10 @@ __device__ __forceinline__ void tile_finish(const LinArgs& p, const f32x16 (&acc
 #pragma unroll
   for (int mi = 0; mi < FM; ++mi) {
     if (fetched && mi + BUF - 1 < FM) fetch(mi + BUF - 1);
-#pragma unroll
-    for (int ni = 0; ni < FN; ++ni)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)  // chunk 8 ni + 2 g + h
-        *reinterpret_cast<lds_f32x4*>(
-            region + r_l * (W * 4) + ((((4 * ni + g) ^ (r_l & (CH / 2 - 1))) + h * (CH / 2)) << 4)) =
-            f32x4_t{acc[mi][ni][4 * g], acc[mi][ni][4 * g + 1], acc[mi][ni][4 * g + 2],
-                    acc[mi][ni][4 * g + 3]};
+    stage(mi, [&](int r, int c, const f32x4_t& v) {
+      *reinterpret_cast<lds_f32x4*>(
+          region + r * (W * 4) + ((((c >> 1) ^ (r & (CH / 2 - 1))) + (c & 1) * (CH / 2)) << 4)) = v;
+    });
     if constexpr (SRC) {
 #pragma unroll
       for (int ps = 0; ps < NP; ++ps) pass(mi, ps, rows[mi % BUF][ps]);
@@ -364,11 +381,11 @@ __device__ __forceinline__ void tile_of(int ti, int tj, int& i, int& j) {
   j = in / rows;
 }
 
-template <int LAYOUT, int KIND, int BM, int BN>
+template <int LAYOUT, int KIND, int BM, int BN, int BS>
 struct Tile {
   static constexpr bool A_K = LAYOUT != LAY_TN, B_K = LAYOUT == LAY_NT, GATED = KIND == LIN_GATED;
-  typedef Operand<A_K, BM, false> OpA;
-  typedef Operand<B_K, BN, GATED> OpB;
+  typedef Operand<A_K, BM, false, BS> OpA;
+  typedef Operand<B_K, BN, GATED, BS> OpB;
   static constexpr int STAGE = OpA::BYTES + OpB::BYTES;
   static constexpr int BO = GATED ? BN / 2 : BN;  // output columns
   OpA a;
@@ -406,18 +423,33 @@ struct Tile {
   __device__ __forceinline__ void next_b(int kt) { wb.template advance<B_K>(sb, kt + 1 < nkt); }
 };
 
-// 256 x 256 tiles, 128 x 128 per wave (256 accumulators, one wave per SIMD), two
-// 64 KiB stages. k-steps 0-2 of a k-tile multiply while they read the next
-// k-step's fragments, k-step 0 with the loads of B's next k-tile into the other
-// stage between its products; then one barrier, and k-step 3 multiplies while it
-// reads the first fragments of the next k-tile and loads A's k-tile after that
-// into this stage.
+// c += a b in the accumulation registers, in its place among the other volatile
+// assembly: as a builtin a product has no side effects, and the compiler moved half of
+// a k-tile's products behind its barriers, and copied accumulators that it held fixed to
+// places (160 moves per k-tile). Nothing but these products touches c before mma_done.
+template <int ET>
+__device__ __forceinline__ void mma16(f32x4_t& c, const uint4& a, const uint4& b) {
+  const u32x4 va = __builtin_bit_cast(u32x4, a), vb = __builtin_bit_cast(u32x4, b);
+  if constexpr (ET == TT_BF16)
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(va), "v"(vb));
+  else
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(va), "v"(vb));
+}
+// The last product's results may be read: the compiler's padding between a product
+// and the use of its result does not see assembly.
+__device__ __forceinline__ void mma_done() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
+
+// 256 x 256 tiles, 128 x 128 per wave (256 accumulators, one wave per SIMD), in
+// 16x16x32 products. Two k-tiles of A and three of B in LDS. k-step 0 multiplies,
+// reads the fragments of k-step 1 and loads B's k-tile kt + 2; then every wave has
+// read k-tile kt, and k-step 1 loads A's k-tile kt + 2 into its place, and after a
+// second barrier, which publishes k-tile kt + 1, reads that one's first fragments.
 template <int LAYOUT, int KIND, int ET, bool KMASK>
 __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int tj) {
-  typedef Tile<LAYOUT, KIND, 256, 256> TL;
-  constexpr int FM = 4, FN = 4, NM = FM * FN;
+  typedef Tile<LAYOUT, KIND, 256, 256, 16> TL;
+  constexpr int FM = 8, FN = 8;
   constexpr int LA = TL::OpA::LOADS, LB = TL::OpB::LOADS;
-  static_assert(LA == 8 && LB == 8, "four loads per k-step");
+  static_assert(LA == 8 && LB == 8, "one load per eight or four products");
   constexpr uint32_t BA = TL::OpA::BYTES, BB = TL::OpB::BYTES;
   __shared__ __align__(16) char lds_raw[2 * BA + 3 * BB];  // two k-tiles of A, then three of B
   const int lane = threadIdx.x & 63;
@@ -428,27 +460,22 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
   const uint32_t lds0 = lds_addr_of(lds);
   const uint32_t wa0 = lds0 + (uint32_t)(LA * wave) * 1024u;           // the wave's part of A's stages
   const uint32_t wb0 = lds0 + 2 * BA + (uint32_t)(LB * wave) * 1024u;  // and of B's
-  // Fragments of the four k-steps of a k-tile (at most about half of them live).
-  uint4 fa[4][FM], fb[4][FN];
-  auto read_a = [&](lds_char* sa, int s, int i) { fa[s][i] = t.a.read(sa, i, s); };
-  auto read_b = [&](lds_char* sb, int s, int i) { fb[s][i] = t.b.read(sb, i, s); };
-  f32x16 acc[FM][FN] = {};
-  {
-    t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0, t.kn);
-    t.b.template loads<KMASK, 0, LB>(t.wb.r, wb0, t.kn);
-    t.next_a(0);
-    t.next_b(0);
-    t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0 + BA, t.kn - T_BK);
-    t.b.template loads<KMASK, 0, LB>(t.wb.r, wb0 + BB, t.kn - T_BK);
-    t.next_a(1);
-    t.next_b(1);
-    TT_WAIT_VMCNT(LA + LB);
-    TT_LDS_BARRIER();
+  uint4 fa[2][FM], fb[2][FN];
+  f32x4_t acc[FM][FN] = {};
+  t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0, t.kn);
+  t.b.template loads<KMASK, 0, LB>(t.wb.r, wb0, t.kn);
+  t.next_a(0);
+  t.next_b(0);
+  t.b.template loads<KMASK, 0, LB>(t.wb.r, wb0 + BB, t.kn - T_BK);
+  t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0 + BA, t.kn - T_BK);
+  t.next_a(1);
+  t.next_b(1);
+  TT_WAIT_VMCNT(LA + LB);
+  TT_LDS_BARRIER();
 #pragma unroll
-    for (int i = 0; i < FM; ++i) read_a(lds, 0, i);
+  for (int i = 0; i < FM; ++i) fa[0][i] = t.a.read(lds, i, 0);
 #pragma unroll
-    for (int i = 0; i < FN; ++i) read_b(lds + 2 * BA, 0, i);
-  }
+  for (int i = 0; i < FN; ++i) fb[0][i] = t.b.read(lds + 2 * BA, i, 0);
   int slot = 0;  // of B's k-tile kt
   for (int kt = 0; kt < t.nkt; ++kt) {
     const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
@@ -458,75 +485,84 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
     lds_char* const nb = lds + 2 * BA + (uint32_t)slot1 * BB;
     const uint32_t to_a = wa0 + (uint32_t)(kt & 1) * BA, to_b = wb0 + (uint32_t)slot2 * BB;
     const int valid = t.kn - (kt + 2) * T_BK;
-    // Product i of k-step s. The empty asm keeps it in its slot: products have no side
-    // effects, and the compiler otherwise moves half of them behind the barriers.
-    auto mul = [&](int s, int i) {
-      f32x16& c = acc[i / FN][i % FN];
-      c = Mma<ET>::run(fb[s][i % FN], fa[s][i / FN], c);
-      asm volatile("" : "+a"(c));
+    // Products of row m and columns n, n + 1 of k-step s.
+    auto mul = [&](int s, int m, int n) {
+      mma16<ET>(acc[m][n], fb[s][n], fa[s][m]);
+      mma16<ET>(acc[m][n + 1], fb[s][n + 1], fa[s][m]);
     };
-    // k-step s: its products, in slot i what `read` reads, and every fourth one a load
-    // Q0 .. Q0 + 3 of A or B.
-    auto k_step = [&](auto s_c, auto is_a, auto q0_c, auto read) {
-      constexpr int s = decltype(s_c)::value, Q0 = decltype(q0_c)::value;
-      constexpr bool IS_A = decltype(is_a)::value;
-      auto four = [&](auto g_c) {
-        constexpr int g = decltype(g_c)::value;
+    // k-step 0: row m of the products.
+    auto first = [&](auto m_c) {
+      constexpr int m = decltype(m_c)::value;
 #pragma unroll
-        for (int i = 4 * g; i < 4 * g + 4; ++i) {
-          mul(s, i);
-          read(i);
-          if (i == 4 * g + 3) {
-            if constexpr (IS_A) t.a.template load<KMASK, Q0 + g>(t.wa.r, to_a, valid);
-            else t.b.template load<KMASK, Q0 + g>(t.wb.r, to_b, valid);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      };
-      four(std::integral_constant<int, 0>{});
-      four(std::integral_constant<int, 1>{});
-      four(std::integral_constant<int, 2>{});
-      four(std::integral_constant<int, 3>{});
+      for (int n = 0; n < FN; n += 2) {
+        mul(0, m, n);
+        if (n == 0) fb[1][m] = t.b.read(cb, m, 1);
+        if (n == 4) fa[1][m] = t.a.read(ca, m, 1);
+        if (n == 6) t.b.template load<KMASK, m>(t.wb.r, to_b, valid);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
-    constexpr std::integral_constant<int, 0> C0{};
-    constexpr std::integral_constant<int, 1> C1{};
-    constexpr std::integral_constant<int, 2> C2{};
-    constexpr std::integral_constant<int, 3> C3{};
-    constexpr std::integral_constant<int, 4> C4{};
-    k_step(C0, std::false_type{}, C0, [&](int i) {
-      if (i < 4) read_b(cb, 1, i);
-      else if (i < 8) read_a(ca, 1, i - 4);
-      else if (i < 12) read_a(ca, 2, i - 8);
-    });
-    k_step(C1, std::false_type{}, C4, [&](int i) {
-      if (i < 4) read_a(ca, 3, i);
-      else if (i < 8) read_b(cb, 2, i - 4);
-    });
+    first(std::integral_constant<int, 0>{});
+    first(std::integral_constant<int, 1>{});
+    first(std::integral_constant<int, 2>{});
+    first(std::integral_constant<int, 3>{});
+    first(std::integral_constant<int, 4>{});
+    first(std::integral_constant<int, 5>{});
+    first(std::integral_constant<int, 6>{});
+    first(std::integral_constant<int, 7>{});
     t.next_b(kt + 2);
-    TT_LDS_BARRIER();  // every wave has read A's k-tile: its stage is free
-    k_step(C2, std::true_type{}, C0, [&](int i) {
-      if (i < 4) read_b(cb, 3, i);
-    });
-    TT_WAIT_VMCNT(LA / 2 + LB);  // k-tile kt + 1 has landed
-    TT_LDS_BARRIER();
-    k_step(C3, std::true_type{}, C4, [&](int i) {
-      if (i < 4) read_b(nb, 0, i);
-      else if (i < 8) read_a(na, 0, i - 4);
-    });
+    TT_LDS_BARRIER();  // every wave has read k-tile kt
+    // Rows 0-2 of k-step 1, with A's loads.
+    auto load_a = [&](auto m_c) {
+      constexpr int m = decltype(m_c)::value;
+#pragma unroll
+      for (int n = 0; n < FN; n += 2) {
+        mul(1, m, n);
+        if (n == 2) t.a.template load<KMASK, 2 * m>(t.wa.r, to_a, valid);
+        if (n == 6) t.a.template load<KMASK, 2 * m + 1>(t.wa.r, to_a, valid);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    load_a(std::integral_constant<int, 0>{});
+    load_a(std::integral_constant<int, 1>{});
+    load_a(std::integral_constant<int, 2>{});
+    load_a(std::integral_constant<int, 3>{});
     t.next_a(kt + 2);
+    TT_WAIT_VMCNT(LA + LB);  // k-tile kt + 1 has landed
+    TT_LDS_BARRIER();
+#pragma unroll
+    for (int m = 4; m < 8; ++m)
+#pragma unroll
+      for (int n = 0; n < FN; n += 2) {
+        mul(1, m, n);
+        const int i = 4 * (m - 4) + n / 2;
+        if (i < 8) fb[0][i] = t.b.read(nb, i, 0);
+        else fa[0][i - 8] = t.a.read(na, i - 8, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     slot = slot1;
   }
+  mma_done();
   TT_WAIT_VMCNT(0);
   __syncthreads();  // every wave is past its fragment reads, and every load has landed
-  tile_finish<KIND, ET, FM, FN>(p, acc, lds + wave * (32 * 128 * 4), t.i0 + (wave >> 1) * 128,
-                                t.j0 + (wave & 1) * (TL::BO / 2), lane);
+  // Lane l holds row 16 m + l % 16, columns 16 n + 4 (l / 16) + 0..3.
+  auto stage = [&](auto mi, auto put) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < FN; ++n)
+        put(16 * m + (lane & 15), 4 * n + (lane >> 4), acc[2 * mi + m][n]);
+  };
+  tile_finish<KIND, ET, FM / 2, FN / 2>(p, stage, lds + wave * (32 * 128 * 4),
+                                        t.i0 + (wave >> 1) * 128,
+                                        t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
 
 // 128 x 128 tiles, 64 x 64 per wave, a ring of S 32 KiB stages with one barrier
 // per k-tile, which publishes k-tile kt and frees the stage of kt - 1.
 template <int LAYOUT, int KIND, int ET, bool KMASK, int S>
 __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int tj) {
-  typedef Tile<LAYOUT, KIND, 128, 128> TL;
+  typedef Tile<LAYOUT, KIND, 128, 128, 32> TL;
   constexpr int FM = 2, FN = 2;
   constexpr int LA = TL::OpA::LOADS, LB = TL::OpB::LOADS, LD = LA + LB;
   __shared__ __align__(16) char lds_raw[S * TL::STAGE];
@@ -579,7 +615,17 @@ __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int
   }
   TT_WAIT_VMCNT(0);
   __syncthreads();
-  tile_finish<KIND, ET, FM, FN>(p, acc, lds + wave * (32 * 64 * 4), t.i0 + (wave >> 1) * 64,
+  // Lane l holds row 32 mi + l % 32, columns 32 ni + 8 g + 4 (l / 32) + 0..3.
+  auto stage = [&](auto mi, auto put) {
+#pragma unroll
+    for (int ni = 0; ni < FN; ++ni)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        put(lane & 31, 8 * ni + 2 * g + (lane >> 5),
+            f32x4_t{acc[mi][ni][4 * g], acc[mi][ni][4 * g + 1], acc[mi][ni][4 * g + 2],
+                    acc[mi][ni][4 * g + 3]});
+  };
+  tile_finish<KIND, ET, FM, FN>(p, stage, lds + wave * (32 * 64 * 4), t.i0 + (wave >> 1) * 64,
                                 t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
 
