@@ -239,3 +239,5 @@ int tt_linear_any(int kind, int dtype, const LinArgs& a, hipStream_t s);
 // 16-bit matrix instructions on tiles of `tile` (128 or 256) rows and columns, for
 // aligned rows of whole 16-byte vectors (linear_tile.hip).
 int tt_linear_tile(int kind, int tile, int dtype, const LinArgs& a, hipStream_t s);
+// The same for at most 64 rows of x and NT operands under 2 GiB (linear_thin.hip).
+int tt_linear_thin(int kind, int dtype, const LinArgs& a, hipStream_t s);

@@ -105,8 +105,8 @@ Split split_of(int64_t R, int64_t wanted) {
   return Split{(int)((R + per - 1) / per), per};
 }
 
-// The kernel that runs a product (0: any type, else the tile of linear_tile.hip)
-// and how many parts its reduction is split into.
+// The kernel that runs a product (0: any type, 64: few rows, 128 and 256: the tile of
+// linear_tile.hip) and how many parts its reduction is split into.
 struct Plan {
   int tile;
   Split split;
@@ -128,6 +128,7 @@ Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, bool fast) {
     const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64), 1), R / 256);
     return Plan{0, split_of(R, std::min<int64_t>(want, 32))};
   }
+  if (layout == LAY_NT && I <= 64 && half * J * R * 2 < (1ll << 32)) return Plan{64, split_of(R, 1)};
   if (tiles(256) >= 192) return Plan{256, split_of(R, least)};
   const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(tiles(128), 1), R / 256);
   return Plan{128, split_of(R, std::max(least, std::min<int64_t>(want, 32)))};
@@ -165,8 +166,9 @@ int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_
   p.splits = sp.splits;
   p.rsplit = sp.run;
   p.part = sp.splits > 1 ? static_cast<float*>(ws) : nullptr;
-  const int rc = pl.tile != 0 ? tt_linear_tile(kind, pl.tile, dtype, p, s)
-                              : tt_linear_any(kind, dtype, p, s);
+  const int rc = pl.tile == 0    ? tt_linear_any(kind, dtype, p, s)
+                 : pl.tile == 64 ? tt_linear_thin(kind, dtype, p, s)
+                                 : tt_linear_tile(kind, pl.tile, dtype, p, s);
   if (rc != TT_OK || p.part == nullptr) return rc;
   switch (dtype) {
     case TT_BF16: return join_kind<BF16T>(kind, p, s);
