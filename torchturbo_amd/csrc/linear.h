@@ -16,8 +16,8 @@
 enum { LIN_ACT = 0, LIN_GATED = 1, LIN_RES = 2, LIN_DROP = 3, LIN_DGRAD = 4, LIN_PLAIN = 5 };
 // Activations.
 enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2 };
-// Columns that one partial dot product of DGRAD covers.
-constexpr int LIN_DOT = 64;
+// Columns that one partial dot product of DGRAD covers: the least that a wave has.
+constexpr int LIN_DOT = 32;
 
 // C [I, J] of A and B, both of the type of `out` (GATED: B has 2 J columns, the
 // gate's first). Which of A and B has the reduction contiguous in memory is the

@@ -105,8 +105,8 @@ Split split_of(int64_t R, int64_t wanted) {
   return Split{(int)((R + per - 1) / per), per};
 }
 
-// The kernel that runs a product (0: any type, 64: few rows, 128 and 256: the tile of
-// linear_tile.hip) and how many parts its reduction is split into.
+// The kernel that runs a product (0: any type, 16: few rows, 64, 128 and 256: the tile
+// of linear_tile.hip) and how many parts its reduction is split into.
 struct Plan {
   int tile;
   Split split;
@@ -119,19 +119,64 @@ int64_t least_splits(int layout, int64_t I, int64_t J, int64_t R) {
   return std::max<int64_t>((R * ld * 2 + (1ll << 31) - 1) >> 31, 1);
 }
 
+// Microseconds of a product of `tiles` tiles in `splits` parts of nkt 64-deep k-tiles. A
+// k-tile of a 64-wide tile takes 0.30 us where a CU has one block and 0.5 with two,
+// of a 128-wide one 0.62 and 1.0, of a 256-wide one (one block per CU) 0.85 on a few
+// CUs and 1.2 on all (the part is then at its power limit); the rest are starts and
+// epilogues. Measured / this estimate: 1000 x 704 -> 1024 (352 tiles of 64) 6.5 / 7.2,
+// 2048 x 768 -> 2048 (1024 of 64) 15.8 / 15.8, in 256 tiles of 128 13.0 / 11.6, 512 x
+// 2048 -> 7168 (224 of 128) 24.7 / 24.0, 1000 rows (448 of 128) 34.2 / 34.6, 2048 rows
+// (224 of 256) 54 / 57; 24 x 7168 -> 4096 in four parts (256 blocks of 64) 15.6 / 15.0.
+double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sums) {
+  const int64_t blocks = tiles * splits, full = blocks / 512, rest = blocks % 512;
+  double us;
+  if (tile == 256) {
+    const double fill = std::min(1.0, (double)blocks / 256);
+    us = 8 + (double)((blocks + 255) / 256) * (12 + (double)nkt * (0.85 + 0.35 * fill));
+  } else {
+    const double one = tile == 64 ? 0.30 : 0.62, two = tile == 64 ? 0.5 : 1.0;
+    us = (tile == 64 ? 2.8 : 4.2) + (double)full * (tile == 64 ? 0.5 : 1.5) +
+         (double)nkt * ((double)full * two + (rest == 0 ? 0 : rest <= 256 ? one : two));
+  }
+  // The parts are written and read again by a second launch.
+  return splits == 1 ? us : us + 3 + (double)(splits * sums) * 8 / 6.5e6;
+}
+
+// The same of the kernel of few rows: the weight at 4.6 TB/s and, for each block of its
+// columns, all of x at 9 TB/s, with fewer than 256 blocks accordingly slower. Measured /
+// this estimate: 1 x 7168 -> 2 x 2048 13.8 / 14.7, 24 x 2048 -> 7168 12.8 / 12.8, 24 x
+// 2048 -> 2 x 768 8.1 / 8.0, 64 x 7168 -> 2 x 2048 40.9 / 40.3.
+double rows_us(int64_t blocks, int64_t I, int64_t J, int64_t R) {
+  const double work = (double)(J * R) * 2 / 4.6e6 + (double)(blocks * I * R) * 2 / 9e6;
+  return 1.5 + work * std::max(1.0, 256.0 / (double)blocks);
+}
+
 Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, bool fast) {
-  const int64_t half = kind == LIN_GATED ? 2 : 1;
-  const int64_t least = least_splits(layout, I, J, R);
-  auto tiles = [&](int64_t t) { return ((I + t - 1) / t) * ((half * J + t - 1) / t); };
+  const int64_t half = kind == LIN_GATED ? 2 : 1, width = half * J;
+  auto tiles = [&](int64_t t) { return ((I + t - 1) / t) * ((width + t - 1) / t); };
   if (!fast) {
     // Enough blocks for the CUs, each reduction at least 256 long.
     const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64), 1), R / 256);
     return Plan{0, split_of(R, std::min<int64_t>(want, 32))};
   }
-  if (layout == LAY_NT && I <= 64 && half * J * R * 2 < (1ll << 32)) return Plan{64, split_of(R, 1)};
-  if (tiles(256) >= 192) return Plan{256, split_of(R, least)};
-  const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(tiles(128), 1), R / 256);
-  return Plan{128, split_of(R, std::max(least, std::min<int64_t>(want, 32)))};
+  const int64_t least = least_splits(layout, I, J, R);
+  Plan best{256, split_of(R, least)};
+  double best_us = 1e30;
+  if (layout == LAY_NT && I <= 64 && width * R * 2 < (1ll << 32)) {
+    best = Plan{16, split_of(R, 1)};
+    best_us = rows_us((width + 15) / 16, I, width, R);
+  }
+  for (int tile : {64, 128, 256})
+    for (int64_t want = least; want <= std::max<int64_t>(least, 16); want *= 2) {
+      const Split sp = split_of(R, want);
+      if (sp.splits > least && sp.run < 256) break;
+      const double us = tile_us(tile, tiles(tile), sp.splits, sp.run / 64, I * width);
+      if (us < best_us) {
+        best_us = us;
+        best = Plan{tile, sp};
+      }
+    }
+  return best;
 }
 
 size_t part_bytes(int kind, int64_t I, int64_t J, int64_t splits) {
@@ -167,7 +212,7 @@ int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_
   p.rsplit = sp.run;
   p.part = sp.splits > 1 ? static_cast<float*>(ws) : nullptr;
   const int rc = pl.tile == 0    ? tt_linear_any(kind, dtype, p, s)
-                 : pl.tile == 64 ? tt_linear_thin(kind, dtype, p, s)
+                 : pl.tile == 16 ? tt_linear_thin(kind, dtype, p, s)
                                  : tt_linear_tile(kind, pl.tile, dtype, p, s);
   if (rc != TT_OK || p.part == nullptr) return rc;
   switch (dtype) {

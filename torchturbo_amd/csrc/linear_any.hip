@@ -147,7 +147,7 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
   for (int m = 0; m < F; ++m) {
     const int64_t i = i0 + wr + 32 * m + l32;
     const bool live = i < p.I;
-    float dot = 0.f;
+    float dots[F] = {};  // of each 32 columns
 #pragma unroll
     for (int n = 0; n < (GATED ? (F + 1) / 2 : F); ++n)
 #pragma unroll
@@ -171,27 +171,22 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
             if (GATED) o[p.J + e] = u[e];
           }
         } else if (vec && p.J % 4 == 0) {
-          dot += lin_finish<KIND, TT, 4, true>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
+          dots[n] += lin_finish<KIND, TT, 4, true>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
                                              lin_row<KIND, TT, 4, true>(p, i, j, left));
         } else {
-          dot += lin_finish<KIND, TT, 4, false>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
+          dots[n] += lin_finish<KIND, TT, 4, false>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
                                              lin_row<KIND, TT, 4, false>(p, i, j, left));
         }
       }
     if constexpr (KIND == LIN_DGRAD) {
-      static_assert(LIN_DOT == 64, "see below");
+      static_assert(LIN_DOT == 32, "a block's columns");
       if (p.dots != nullptr && p.part == nullptr) {
-        dot += __shfl_xor(dot, 32, 64);
-        // A wave's 32 or 64 columns; two waves share a run when they have 32 each.
-        if constexpr (F == 2) {
-          if (live && h == 0 && j0 + wc < p.J)
-            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + (j0 + wc) / LIN_DOT] = dot;
-        } else {
-          __shared__ float other[2][32];
-          if ((wave & 1) == 1 && h == 0) other[wave >> 1][l32] = dot;
-          __syncthreads();
-          if ((wave & 1) == 0 && live && h == 0 && j0 < p.J)
-            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j0 / LIN_DOT] = dot + other[wave >> 1][l32];
+#pragma unroll
+        for (int n = 0; n < F; ++n) {
+          const float dot = dots[n] + __shfl_xor(dots[n], 32, 64);
+          const int64_t j = j0 + wc + 32 * n;
+          if (live && h == 0 && j < p.J)
+            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
         }
       }
     }

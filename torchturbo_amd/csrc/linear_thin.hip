@@ -135,7 +135,7 @@ int launch(const LinArgs& p, hipStream_t s) {
 
 template <int KIND, class TT>
 int rows(const LinArgs& p, hipStream_t s) {
-  if (p.I <= 16) return launch<KIND, TT, 1, 1, 8>(p, s);
+  if (p.I <= 16) return launch<KIND, TT, 1, 1, 4>(p, s);
   if (p.I <= 32) return launch<KIND, TT, 2, 1, 4>(p, s);
   return launch<KIND, TT, 4, 1, 4>(p, s);
 }

@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t frag_mn(int c0, int lane) {
   const int g = lane >> 4, i = lane & 15;
   const int col = c0 + 16 * (g & 1) + 4 * (i & 3);
   const int kr = 8 * (g >> 1) + (i >> 2);
-  return (uint32_t)(kr * RB + (((col >> 3) ^ (4 * (kr & 3))) << 4) + (col & 7) * 2);
+  return (uint32_t)(kr * RB + (((col >> 3) ^ (4 * (kr & 3) & (RB / 16 - 1))) << 4) + (col & 7) * 2);
 }
 // The same for 16 columns of a 32-deep k-step (which adds 32 RB): lane l gets column
 // c0 + l % 16, k-rows 8 (l / 16) .. + 7.
@@ -68,7 +68,7 @@ template <int RB>
 __device__ __forceinline__ uint32_t frag_mn16(int c0, int lane) {
   const int g = lane >> 4, i = lane & 15;
   const int col = c0 + 4 * (i & 3), kr = 8 * g + (i >> 2);
-  return (uint32_t)(kr * RB + (((col >> 3) ^ (4 * (kr & 3))) << 4) + (col & 7) * 2);
+  return (uint32_t)(kr * RB + (((col >> 3) ^ (4 * (kr & 3) & (RB / 16 - 1))) << 4) + (col & 7) * 2);
 }
 template <int RB>
 __device__ __forceinline__ uint4 read_mn(lds_char* tile, uint32_t off) {
@@ -109,7 +109,7 @@ struct Operand {
       } else {
         constexpr int LPR = RB / 16;  // lanes per k-row
         const int kr = 16 * wave + (64 / LPR) * q + lane / LPR;
-        const int c = (lane % LPR) ^ (4 * (kr & 3));
+        const int c = (lane % LPR) ^ (4 * (kr & 3) & (LPR - 1));
         off[q] = (uint32_t)((kr * ld + 8 * c) * 2);
       }
     }
@@ -184,11 +184,10 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
   return u32x4{lo.x, lo.y, hi.x, hi.y};
 }
 
-// Sum over the eight lanes of a group of eight.
-__device__ __forceinline__ float sum8(float v) {
-  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true));   // ^ 1
-  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true));   // ^ 2
-  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true));  // ^ 7
+// Sum over the four lanes of a quad.
+__device__ __forceinline__ float sum4(float v) {
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true));  // ^ 1
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true));  // ^ 2
   return v;
 }
 
@@ -344,9 +343,10 @@ __device__ __forceinline__ void tile_finish(const LinArgs& p, F stage, lds_char*
         }
         __builtin_amdgcn_raw_buffer_store_b128(pack8<ET>(x), xs, (int)(col_ok ? at16 : DM_OOB), 0, 0);
         if (p.dots != nullptr) {
-          dot = sum8(dot);
+          static_assert(LIN_DOT == 32, "four lanes of eight columns");
+          dot = sum4(dot);
           const int64_t i = i0 + q + rr;
-          if ((lane & 7) == 0 && i < p.I && col_ok) p.dots[i * nd + j / LIN_DOT] = dot;
+          if ((lane & 3) == 0 && i < p.I && col_ok) p.dots[i * nd + j / LIN_DOT] = dot;
         }
       }
     }
@@ -558,12 +558,12 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
                                         t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
 
-// 128 x 128 tiles, 64 x 64 per wave, a ring of S 32 KiB stages with one barrier
-// per k-tile, which publishes k-tile kt and frees the stage of kt - 1.
-template <int LAYOUT, int KIND, int ET, bool KMASK, int S>
+// BT x BT tiles (64 or 128), a quarter per wave, a ring of S stages (16 or 32 KiB) with
+// one barrier per k-tile, which publishes k-tile kt and frees the stage of kt - 1.
+template <int LAYOUT, int KIND, int ET, bool KMASK, int BT, int S>
 __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int tj) {
-  typedef Tile<LAYOUT, KIND, 128, 128, 32> TL;
-  constexpr int FM = 2, FN = 2;
+  typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;
+  constexpr int FM = BT / 64, FN = BT / 64;
   constexpr int LA = TL::OpA::LOADS, LB = TL::OpB::LOADS, LD = LA + LB;
   __shared__ __align__(16) char lds_raw[S * TL::STAGE];
   const int lane = threadIdx.x & 63;
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int
             f32x4_t{acc[mi][ni][4 * g], acc[mi][ni][4 * g + 1], acc[mi][ni][4 * g + 2],
                     acc[mi][ni][4 * g + 3]});
   };
-  tile_finish<KIND, ET, FM, FN>(p, stage, lds + wave * (32 * 64 * 4), t.i0 + (wave >> 1) * 64,
+  tile_finish<KIND, ET, FM, FN>(p, stage, lds + wave * (32 * (BT / 2) * 4), t.i0 + (wave >> 1) * (BT / 2),
                                 t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
 
@@ -638,8 +638,14 @@ int launch(int tile, const LinArgs& p, hipStream_t s) {
   if (tile == 256)
     hipLaunchKernelGGL((linear_big_kernel<LAYOUT, KIND, ET, KMASK>), grid, block, 0, s, p, (int)ti,
                        (int)tj);
+  else if (tile == 64)
+    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 64, 4>), grid, block, 0, s, p,
+                       (int)ti, (int)tj);
+  else if (ti * tj * p.splits <= 256)
+    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 4>), grid, block, 0, s, p,
+                       (int)ti, (int)tj);
   else
-    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 2>), grid, block, 0, s, p,
+    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 2>), grid, block, 0, s, p,
                        (int)ti, (int)tj);
   return tt_check_launch("linear");
 }
