@@ -419,51 +419,44 @@ int tt_moe_experts_fwd(const void* x, int dtype, int64_t num_tokens, int64_t hid
  * 16 run on the 16-bit matrix instructions, all others on the fp32 ones.
  * activation: 0 none, 1 SiLU, 2 GELU (erf form).
  *
- * tt_linear_workspace: bytes of scratch for an op of these sizes (0: none). With
- * less, TT_LINEAR_ACT / _GATED / _RESIDUAL / _WGRAD do not split their reductions.
+ * tt_linear_workspace: bytes of scratch of a forward of these sizes (0: none). With
+ * less, it does not split its reduction. The backward's scratch has a query of its own
+ * and is needed in full.
  *
  * tt_linear_act_fwd: a = x w^T + bias; y [m, n] = act(a), w [n, k]; gated: y =
  *   act(a[:, :n]) * a[:, n:], w [2n, k], the gate's rows first. pre (or NULL): a in
- *   fp32, [m, n] or [m, 2n], for the backward.
- * tt_linear_act_bwd: da [m, n or 2n] (dtype) from dy and pre, and dbias = its
- *   column sums, summed before da is rounded (TT_LINEAR_COLSUM workspace), or
- *   NULL. Then tt_linear_dgrad and tt_linear_wgrad of da.
+ *   fp32, [m, n] or [m, 2n], for the backward (not needed for activation 0 without gate).
+ * tt_linear_act_bwd: with da = the gradient of a, rounded to dtype: dx [m, k] = da w,
+ *   dw = da^T x, dbias = the column sums of the unrounded da; each skipped when NULL.
  * tt_linear_residual_fwd: y [m, n] = residual + row_scale[i] * drop(x w^T + bias),
  *   each of residual, row_scale and bias NULL where there is none; drop as tt_dropout
  *   with `threshold` and `key` (threshold 0: no dropout).
- * tt_linear_residual_bwd: g = dy with the dropped elements cleared (written only
- *   with dropout; without it g is dy itself), and dbias = the column sums of
- *   row_scale * drop(dy) (TT_LINEAR_COLSUM workspace), or NULL.
- * tt_linear_dgrad: with c = the inverse of the kept share (threshold as in the
- *   forward, 0: c = 1): dx [m, k] = row_scale[i] * c * (g w), w [n, k]; and with a row
- *   scale, where not NULL, xs = row_scale * x for the weight gradient, and dscale [m] =
- *   c * (<x_i, (g w)_i> + <g_i, bias>). dx may be NULL. TT_LINEAR_DGRAD workspace,
- *   needed for dscale.
- * tt_linear_wgrad: dw [n, k] = c * g^T x. */
-enum { TT_LINEAR_ACT = 0, TT_LINEAR_GATED = 1, TT_LINEAR_RESIDUAL = 2, TT_LINEAR_DGRAD = 3,
-       TT_LINEAR_WGRAD = 4, TT_LINEAR_COLSUM = 5 };
+ * tt_linear_residual_bwd: with g = drop(dy): dx = row_scale[i] * (g w), dw = g^T
+ *   (row_scale x), the scaled rows rounded to dtype, dbias = the column sums of
+ *   row_scale g, dscale [m] = <x_i, (g w)_i> + <g_i, bias>; each skipped when NULL.
+ *   bias is read for dscale only; bias_dtype is dbias's as well. */
+enum { TT_LINEAR_ACT = 0, TT_LINEAR_GATED = 1, TT_LINEAR_RESIDUAL = 2 };
 size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t k, int64_t n);
 int tt_linear_act_fwd(const void* x, const void* w, const void* bias, int bias_dtype, int dtype,
                       int64_t m, int64_t k, int64_t n, int32_t activation, int32_t gated,
                       float* pre, void* y, void* workspace, size_t workspace_bytes, void* stream);
-int tt_linear_act_bwd(const void* dy, const float* pre, int dtype, int64_t m, int64_t n,
-                      int32_t activation, int32_t gated, void* da, void* dbias, int bias_dtype,
-                      void* workspace, size_t workspace_bytes, void* stream);
+size_t tt_linear_act_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t n, int32_t activation,
+                                   int32_t gated);
+int tt_linear_act_bwd(const void* dy, const void* x, const void* w, const float* pre, int dtype,
+                      int64_t m, int64_t k, int64_t n, int32_t activation, int32_t gated, void* dx,
+                      void* dw, void* dbias, int bias_dtype, void* workspace,
+                      size_t workspace_bytes, void* stream);
 int tt_linear_residual_fwd(const void* x, const void* w, const void* bias, int bias_dtype,
                            const void* residual, const void* row_scale, int scale_dtype, int dtype,
                            int64_t m, int64_t k, int64_t n, int32_t threshold, const int64_t* key,
                            void* y, void* workspace, size_t workspace_bytes, void* stream);
-int tt_linear_residual_bwd(const void* dy, const void* row_scale, int scale_dtype, int dtype,
-                           int64_t m, int64_t n, int32_t threshold, const int64_t* key, void* g,
-                           void* dbias, int bias_dtype, void* workspace, size_t workspace_bytes,
-                           void* stream);
-int tt_linear_dgrad(const void* g, const void* w, const void* x, const void* row_scale,
-                    int scale_dtype, const void* bias, int bias_dtype, int dtype, int64_t m,
-                    int64_t k, int64_t n, int32_t threshold, void* dx, void* xs, void* dscale,
-                    void* workspace, size_t workspace_bytes, void* stream);
-int tt_linear_wgrad(const void* g, const void* x, int dtype, int64_t m, int64_t k, int64_t n,
-                    int32_t threshold, void* dw, void* workspace, size_t workspace_bytes,
-                    void* stream);
+size_t tt_linear_residual_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t n, int32_t scaled,
+                                        int32_t dropped);
+int tt_linear_residual_bwd(const void* dy, const void* x, const void* w, const void* bias,
+                           int bias_dtype, const void* row_scale, int scale_dtype, int dtype,
+                           int64_t m, int64_t k, int64_t n, int32_t threshold, const int64_t* key,
+                           void* dx, void* dw, void* dbias, void* dscale, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 /* ---- Dropout from a counter-based generator ------------------------------
  * y = x / (share kept) where an element is kept, else 0 (whatever it held); x and

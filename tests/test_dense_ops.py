@@ -131,25 +131,22 @@ def null(name, **given):
     """A call of a C entry point with null pointers and sizes that would be taken but for ``given``."""
     sizes = {"m": 4, "k": 8, "n": 8, "dtype": L.TT_BF16, "act": 1, "gated": 1, "t": 0, "bias": None,
              "bias_dt": L.TT_F32, "scale": None, "scale_dt": L.TT_F32, "key": None, "ds": None,
-             "xs": None}
+             "bytes": 1 << 40}
     s = {**sizes, **given}
     args = {
         "tt_linear_act_fwd": lambda: (None, None, s["bias"], s["bias_dt"], s["dtype"], s["m"],
                                       s["k"], s["n"], s["act"], s["gated"], None, None, None, 0,
                                       None),
-        "tt_linear_act_bwd": lambda: (None, None, s["dtype"], s["m"], s["n"], s["act"], s["gated"],
-                                      None, s["bias"], s["bias_dt"], None, 0, None),
+        "tt_linear_act_bwd": lambda: (None, None, None, None, s["dtype"], s["m"], s["k"], s["n"],
+                                      s["act"], s["gated"], None, None, s["bias"], s["bias_dt"],
+                                      None, s["bytes"], None),
         "tt_linear_residual_fwd": lambda: (None, None, s["bias"], s["bias_dt"], None, s["scale"],
                                            s["scale_dt"], s["dtype"], s["m"], s["k"], s["n"],
                                            s["t"], s["key"], None, None, 0, None),
-        "tt_linear_residual_bwd": lambda: (None, s["scale"], s["scale_dt"], s["dtype"], s["m"],
-                                           s["n"], s["t"], s["key"], None, s["bias"],
-                                           s["bias_dt"], None, 0, None),
-        "tt_linear_dgrad": lambda: (None, None, None, s["scale"], s["scale_dt"], s["bias"],
-                                    s["bias_dt"], s["dtype"], s["m"], s["k"], s["n"], s["t"], None,
-                                    s["xs"], s["ds"], None, 0, None),
-        "tt_linear_wgrad": lambda: (None, None, s["dtype"], s["m"], s["k"], s["n"], s["t"], None,
-                                    None, 0, None),
+        "tt_linear_residual_bwd": lambda: (None, None, None, s["bias"], s["bias_dt"], s["scale"],
+                                           s["scale_dt"], s["dtype"], s["m"], s["k"], s["n"],
+                                           s["t"], s["key"], None, None, None, s["ds"], None,
+                                           s["bytes"], None),
         "tt_dropout": lambda: (None, s["dtype"], s["m"], s["n"], s["t"], s["key"], None, None),
         "tt_lora_down_dropout": lambda: (None, None, s["dtype"], s["m"], s["k"], 4, 2, None, s["t"],
                                          s["key"], None, None),
@@ -171,16 +168,15 @@ P = ctypes.c_void_p(16)
     ("tt_linear_act_fwd", {"act": 3}, "unknown activation"),
     ("tt_linear_act_fwd", {"bias": P, "bias_dt": L.TT_F8E4M3}, "the bias must be"),
     ("tt_linear_act_bwd", {"act": -1}, "unknown activation"),
-    ("tt_linear_act_bwd", {"bias": P}, "workspace is too small"),
+    ("tt_linear_act_bwd", {"bias": P, "bias_dt": L.TT_F64}, "the bias must be"),
+    ("tt_linear_act_bwd", {"bytes": 100}, "workspace is too small"),
     ("tt_linear_residual_fwd", {"t": 65537}, "threshold must be"),
     ("tt_linear_residual_fwd", {"t": 5}, "dropout without a key"),
     ("tt_linear_residual_fwd", {"scale": P, "scale_dt": L.TT_F64}, "the row scale must be"),
-    ("tt_linear_residual_bwd", {"t": 5, "key": P}, "a place for its gradient"),
-    ("tt_linear_residual_bwd", {"bias": P}, "workspace is too small"),
-    ("tt_linear_dgrad", {"xs": P}, "need a row scale"),
-    ("tt_linear_dgrad", {"ds": P}, "need a row scale"),
-    ("tt_linear_dgrad", {"scale": P}, "a row scale needs x"),
-    ("tt_linear_wgrad", {"t": -1}, "threshold must be"),
+    ("tt_linear_residual_bwd", {"t": 5}, "dropout without a key"),
+    ("tt_linear_residual_bwd", {"t": -1}, "threshold must be"),
+    ("tt_linear_residual_bwd", {"t": 5, "key": P, "bytes": 100}, "workspace is too small"),
+    ("tt_linear_residual_bwd", {"ds": P}, "needs a row scale"),
     ("tt_dropout", {"dtype": L.TT_F64}, "must be f32, bf16 or f16"),
     ("tt_dropout", {"m": 1 << 32}, "bad sizes"),
     ("tt_dropout", {"t": 65537}, "threshold must be"),
@@ -197,8 +193,8 @@ def test_refusals_of_the_entry_points(name, given, message):
 def test_empty_calls_of_the_entry_points_launch_nothing():
     null("tt_linear_act_fwd", m=0)
     null("tt_linear_residual_fwd", n=0)
-    null("tt_linear_wgrad", k=0)
-    null("tt_linear_dgrad", m=0)
+    null("tt_linear_act_bwd", n=0)  # nor here, with no gradient asked for
+    null("tt_linear_residual_bwd")
     null("tt_dropout", n=0)
     null("tt_lora_down_dropout", m=0, t=5, key=P)
 

@@ -78,20 +78,22 @@ _PROTOS: dict[str, list] = {
     "tt_lora_wgrad_dropout": [P, P, c_int, I64, I64, I32, I32, P, I32, P, P, P],
     "tt_linear_workspace": [I32, c_int, I64, I64, I64],
     "tt_linear_act_fwd": [P, P, P, c_int, c_int, I64, I64, I64, I32, I32, P, P, P, c_size_t, P],
-    "tt_linear_act_bwd": [P, P, c_int, I64, I64, I32, I32, P, P, c_int, P, c_size_t, P],
+    "tt_linear_act_bwd_workspace": [c_int, I64, I64, I64, I32, I32],
+    "tt_linear_act_bwd": [P, P, P, P, c_int, I64, I64, I64, I32, I32, P, P, P, c_int, P, c_size_t,
+                          P],
     "tt_linear_residual_fwd": [P, P, P, c_int, P, P, c_int, c_int, I64, I64, I64, I32, P, P, P,
                                c_size_t, P],
-    "tt_linear_residual_bwd": [P, P, c_int, c_int, I64, I64, I32, P, P, P, c_int, P, c_size_t, P],
-    "tt_linear_dgrad": [P, P, P, P, c_int, P, c_int, c_int, I64, I64, I64, I32, P, P, P, P,
-                        c_size_t, P],
-    "tt_linear_wgrad": [P, P, c_int, I64, I64, I64, I32, P, P, c_size_t, P],
+    "tt_linear_residual_bwd_workspace": [c_int, I64, I64, I64, I32, I32],
+    "tt_linear_residual_bwd": [P, P, P, P, c_int, P, c_int, c_int, I64, I64, I64, I32, P, P, P, P,
+                               P, P, c_size_t, P],
     "tt_dropout": [P, c_int, I64, I64, I32, P, P, P],
     "tt_fp8_quantize_blocks": [P, c_int, I64, I64, I64, P, P, c_int, P],
 }
 _RESTYPES = {"tt_last_error": ctypes.c_char_p, "tt_route_index_workspace": c_size_t,
              "tt_route_index_rejected_offset": c_size_t, "tt_router_loss_workspace": c_size_t,
              "tt_moe_experts_workspace": c_size_t, "tt_router_gate_bwd_workspace": c_size_t,
-             "tt_linear_workspace": c_size_t}
+             "tt_linear_workspace": c_size_t, "tt_linear_act_bwd_workspace": c_size_t,
+             "tt_linear_residual_bwd_workspace": c_size_t}
 ABI_VERSION = 1
 
 _LIB: ctypes.CDLL | None = None

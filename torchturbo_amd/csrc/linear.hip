@@ -127,7 +127,8 @@ int64_t least_splits(int layout, int64_t I, int64_t J, int64_t R) {
 // 2048 x 768 -> 2048 (1024 of 64) 15.8 / 15.8, in 256 tiles of 128 13.0 / 11.6, 512 x
 // 2048 -> 7168 (224 of 128) 24.7 / 24.0, 1000 rows (448 of 128) 34.2 / 34.6, 2048 rows
 // (224 of 256) 54 / 57; 24 x 7168 -> 4096 in four parts (256 blocks of 64) 15.6 / 15.0.
-double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sums) {
+// No plan is faster than its operands' bytes at 4.6 TB/s.
+double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sums, int64_t bytes) {
   const int64_t blocks = tiles * splits, full = blocks / 512, rest = blocks % 512;
   double us;
   if (tile == 256) {
@@ -138,6 +139,7 @@ double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sum
     us = (tile == 64 ? 2.8 : 4.2) + (double)full * (tile == 64 ? 0.5 : 1.5) +
          (double)nkt * ((double)full * two + (rest == 0 ? 0 : rest <= 256 ? one : two));
   }
+  us = std::max(us, 2.8 + (double)bytes / 4.6e6);
   // The parts are written and read again by a second launch.
   return splits == 1 ? us : us + 3 + (double)(splits * sums) * 8 / 6.5e6;
 }
@@ -170,7 +172,8 @@ Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, bool fast) {
     for (int64_t want = least; want <= std::max<int64_t>(least, 16); want *= 2) {
       const Split sp = split_of(R, want);
       if (sp.splits > least && sp.run < 256) break;
-      const double us = tile_us(tile, tiles(tile), sp.splits, sp.run / 64, I * width);
+      const double us = tile_us(tile, tiles(tile), sp.splits, sp.run / 64, I * width,
+                                (I + width) * R * 2);
       if (us < best_us) {
         best_us = us;
         best = Plan{tile, sp};
@@ -425,28 +428,88 @@ bool all_aligned(std::initializer_list<const void*> ps) {
   return at % 16 == 0;
 }
 
+// Bytes of the parts of a product, for the larger of its two plans: which one runs also
+// depends on the addresses.
+size_t parts_of(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R) {
+  const int64_t any = plan_of(layout, kind, I, J, R, false).split.splits;
+  const int64_t fast = fast_sizes(layout, kind, dtype, I, J, R)
+                           ? plan_of(layout, kind, I, J, R, true).split.splits : 1;
+  return part_bytes(kind, I, J, std::max(any, fast));
+}
+size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// dx = row_scale (alpha g w) and what goes with it (linear.h's DGRAD).
+int data_gradient(const void* g, const void* w, const void* x, const void* scale, int scale_dt,
+                  int dtype, int64_t m, int64_t k, int64_t n, float alpha, void* dx, void* xs,
+                  float* dots, void* ws, size_t ws_bytes, hipStream_t s) {
+  LinArgs p{};
+  p.a = g;
+  p.b = w;
+  p.out = dx;
+  p.I = m;
+  p.J = p.ldb = k;
+  p.R = p.lda = n;
+  p.scale = scale;
+  p.scale_dt = scale_dt;
+  p.alpha = alpha;
+  p.x = x;
+  p.xs = xs;
+  p.dots = dots;
+  return m == 0 || k == 0 ? TT_OK : run_product(LAY_NN, LIN_DGRAD, dtype, p, ws, ws_bytes, s);
+}
+
+// dw [n, k] = alpha g^T x.
+int weight_gradient(const void* g, const void* x, int dtype, int64_t m, int64_t k, int64_t n,
+                    float alpha, void* dw, void* ws, size_t ws_bytes, hipStream_t s) {
+  LinArgs p{};
+  p.a = g;
+  p.b = x;
+  p.out = dw;
+  p.I = p.lda = n;
+  p.J = p.ldb = k;
+  p.R = m;
+  p.alpha = alpha;
+  return n == 0 || k == 0 ? TT_OK : run_product(LAY_TN, LIN_PLAIN, dtype, p, ws, ws_bytes, s);
+}
+
+// Passes over the rows of [m, n]: chunks of rows, tiles of columns.
+struct RowPass {
+  int64_t per, chunks, tiles;
+  RowPass(int64_t m, int64_t n)
+      : per(chunk_rows(m, n)), chunks((m + per - 1) / per), tiles((n + P_COLS - 1) / P_COLS) {}
+  dim3 grid() const { return dim3((unsigned)chunks, (unsigned)tiles); }
+};
+
+int column_sums(const float* part, const RowPass& rp, int64_t width, float alpha, void* out, int dt,
+                hipStream_t s) {
+  hipLaunchKernelGGL(linear_colsum_kernel, dim3((unsigned)((width + 31) / 32)), dim3(L_NT), 0, s,
+                     part, rp.chunks, width, alpha, out, dt);
+  return tt_check_launch("linear_colsum");
+}
+
+// A workspace handed out in 256-byte aligned pieces.
+struct Pieces {
+  char* at;
+  size_t left;
+  void* take(size_t bytes) {
+    const size_t n = round256(bytes);
+    if (n > left) return nullptr;
+    char* p = at;
+    at += n;
+    left -= n;
+    return p;
+  }
+};
+
+
 }  // namespace
 
 extern "C" size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t k, int64_t n) {
-  if (m <= 0 || k < 0 || n < 0) return 0;
-  // The larger of the two plans: which one runs also depends on the addresses.
-  auto parts = [&](int layout, int kind, int64_t I, int64_t J, int64_t R) {
-    const int64_t any = plan_of(layout, kind, I, J, R, false).split.splits;
-    const int64_t fast = fast_sizes(layout, kind, dtype, I, J, R)
-                             ? plan_of(layout, kind, I, J, R, true).split.splits : 1;
-    return part_bytes(kind, I, J, std::max(any, fast));
-  };
+  if (m <= 0 || k < 0 || n <= 0) return 0;
   switch (op) {
-    case TT_LINEAR_ACT: return parts(LAY_NT, LIN_ACT, m, n, k);
-    case TT_LINEAR_GATED: return parts(LAY_NT, LIN_GATED, m, n, k);
-    case TT_LINEAR_RESIDUAL: return parts(LAY_NT, LIN_RES, m, n, k);
-    case TT_LINEAR_DGRAD:  // dot products, then the split sums, later the bias's part
-      return dots_bytes(m, k) + std::max(parts(LAY_NN, LIN_DGRAD, m, k, n), (size_t)m * 4);
-    case TT_LINEAR_WGRAD: return parts(LAY_TN, LIN_PLAIN, n, k, m);
-    case TT_LINEAR_COLSUM: {
-      const int64_t per = chunk_rows(m, n);
-      return (size_t)((m + per - 1) / per) * 2 * n * 4;  // gated: both halves
-    }
+    case TT_LINEAR_ACT: return parts_of(LAY_NT, LIN_ACT, dtype, m, n, k);
+    case TT_LINEAR_GATED: return parts_of(LAY_NT, LIN_GATED, dtype, m, n, k);
+    case TT_LINEAR_RESIDUAL: return parts_of(LAY_NT, LIN_RES, dtype, m, n, k);
     default: return 0;
   }
 }
@@ -474,28 +537,52 @@ extern "C" int tt_linear_act_fwd(const void* x, const void* w, const void* bias,
                      S(stream));
 }
 
-extern "C" int tt_linear_act_bwd(const void* dy, const float* pre, int dtype, int64_t m, int64_t n,
-                                 int32_t act, int32_t gated, void* da, void* dbias, int bias_dtype,
+// Workspace: da where there is an activation, then the parts of one step at a time.
+extern "C" size_t tt_linear_act_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t n,
+                                              int32_t act, int32_t gated) {
+  if (m < 0 || k < 0 || n < 0) return 0;
+  const int64_t width = gated ? 2 * n : n;
+  const size_t sums = (size_t)RowPass(m, n).chunks * width * 4;
+  const size_t parts = std::max(parts_of(LAY_NN, LIN_DGRAD, dtype, m, k, width),
+                                parts_of(LAY_TN, LIN_PLAIN, dtype, width, k, m));
+  const bool own = act != ACT_NONE || gated;
+  return (own ? round256((size_t)m * width * tt_elem_size(dtype)) : 0) +
+         round256(std::max(sums, parts));
+}
+
+extern "C" int tt_linear_act_bwd(const void* dy, const void* x, const void* w, const float* pre,
+                                 int dtype, int64_t m, int64_t k, int64_t n, int32_t act,
+                                 int32_t gated, void* dx, void* dw, void* dbias, int bias_dtype,
                                  void* workspace, size_t workspace_bytes, void* stream) {
-  TT_TRY(sizes_ok(dtype, m, 0, n));
+  TT_TRY(sizes_ok(dtype, m, k, n));
   TT_TRY(vector_ok("the bias", dbias, bias_dtype));
   TT_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, "linear: unknown activation %d", act);
-  if (n == 0) return TT_OK;
-  const int64_t width = gated ? 2 * n : n, per = chunk_rows(m, n), chunks = (m + per - 1) / per;
-  const int64_t tiles = (n + P_COLS - 1) / P_COLS;
-  TT_REQUIRE(tiles <= 65535, "linear: too many columns");
-  TT_REQUIRE(dbias == nullptr || workspace_bytes >= (size_t)chunks * width * 4,
+  const bool own = act != ACT_NONE || gated;
+  TT_REQUIRE(workspace_bytes >= tt_linear_act_bwd_workspace(dtype, m, k, n, act, gated),
              "linear_act_bwd: the workspace is too small");
-  float* part = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
-  if (m > 0) {
-    const bool vec = n % 8 == 0 && all_aligned({dy, pre, da});
+  const int64_t width = gated ? 2 * n : n;
+  Pieces ws{static_cast<char*>(workspace), workspace_bytes};
+  void* const da = own ? ws.take((size_t)m * width * tt_elem_size(dtype)) : nullptr;
+  const RowPass rp(m, n);
+  TT_REQUIRE(rp.tiles <= 65535, "linear: too many columns");
+  float* const part = dbias != nullptr ? reinterpret_cast<float*>(ws.at) : nullptr;
+  if (m > 0 && n > 0 && (own || dbias != nullptr)) {
+    const bool vec = n % 8 == 0 && all_aligned({dy, pre});
     TT_TRY(typed(dtype, [&](auto tt) {
       typedef decltype(tt) TT;
       typedef typename TT::storage St;
-      const dim3 grid((unsigned)chunks, (unsigned)tiles), block(L_NT);
+      if (!own) {  // the bias's sums alone
+        auto go = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, rp.grid(), dim3(L_NT), 0, S(stream), static_cast<const St*>(dy),
+                             nullptr, 0, 0u, nullptr, nullptr, part, m, n, rp.per);
+          return tt_check_launch("linear_res_bwd");
+        };
+        return vec ? go(&linear_res_bwd_kernel<TT, false, true>)
+                   : go(&linear_res_bwd_kernel<TT, false, false>);
+      }
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, block, 0, S(stream), static_cast<const St*>(dy), pre,
-                           static_cast<St*>(da), part, m, n, per, (int)act);
+        hipLaunchKernelGGL(kernel, rp.grid(), dim3(L_NT), 0, S(stream), static_cast<const St*>(dy),
+                           pre, static_cast<St*>(da), part, m, n, rp.per, (int)act);
         return tt_check_launch("linear_act_bwd");
       };
       if (gated)
@@ -505,10 +592,15 @@ extern "C" int tt_linear_act_bwd(const void* dy, const float* pre, int dtype, in
                  : go(&linear_act_bwd_kernel<TT, false, false>);
     }));
   }
-  if (dbias == nullptr) return TT_OK;
-  hipLaunchKernelGGL(linear_colsum_kernel, dim3((unsigned)((width + 31) / 32)), dim3(L_NT), 0,
-                     S(stream), part, chunks, width, 1.0f, dbias, bias_dtype);
-  return tt_check_launch("linear_colsum");
+  if (dbias != nullptr && n > 0)
+    TT_TRY(column_sums(part, rp, width, 1.0f, dbias, bias_dtype, S(stream)));
+  const void* const g = own ? da : dy;
+  if (dx != nullptr)
+    TT_TRY(data_gradient(g, w, nullptr, nullptr, 0, dtype, m, k, width, 1.0f, dx, nullptr, nullptr,
+                         ws.at, ws.left, S(stream)));
+  if (dw != nullptr)
+    TT_TRY(weight_gradient(g, x, dtype, m, k, width, 1.0f, dw, ws.at, ws.left, S(stream)));
+  return TT_OK;
 }
 
 extern "C" int tt_linear_residual_fwd(const void* x, const void* w, const void* bias,
@@ -541,109 +633,90 @@ extern "C" int tt_linear_residual_fwd(const void* x, const void* w, const void* 
                      workspace_bytes, S(stream));
 }
 
-extern "C" int tt_linear_residual_bwd(const void* dy, const void* row_scale, int scale_dtype,
-                                      int dtype, int64_t m, int64_t n, int32_t threshold,
-                                      const int64_t* key, void* g, void* dbias, int bias_dtype,
-                                      void* workspace, size_t workspace_bytes, void* stream) {
-  TT_TRY(sizes_ok(dtype, m, 0, n));
-  TT_TRY(vector_ok("the bias", dbias, bias_dtype));
+// Workspace: dy without its dropped elements; with a row scale the scaled rows, the dot
+// products of its gradient and the bias's part of it; then the parts of one step at
+// a time.
+extern "C" size_t tt_linear_residual_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t n,
+                                                   int32_t scaled, int32_t dropped) {
+  if (m < 0 || k < 0 || n < 0) return 0;
+  const size_t es = tt_elem_size(dtype);
+  const size_t sums = (size_t)RowPass(m, n).chunks * n * 4;
+  const size_t parts = std::max(parts_of(LAY_NN, LIN_DGRAD, dtype, m, k, n),
+                                parts_of(LAY_TN, LIN_PLAIN, dtype, n, k, m));
+  return (dropped ? round256((size_t)m * n * es) : 0) +
+         (scaled ? round256((size_t)m * k * es) + dots_bytes(m, k) + round256((size_t)m * 4) : 0) +
+         round256(std::max(sums, parts));
+}
+
+extern "C" int tt_linear_residual_bwd(const void* dy, const void* x, const void* w,
+                                      const void* bias, int bias_dtype, const void* row_scale,
+                                      int scale_dtype, int dtype, int64_t m, int64_t k, int64_t n,
+                                      int32_t threshold, const int64_t* key, void* dx, void* dw,
+                                      void* dbias, void* dscale, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  TT_TRY(sizes_ok(dtype, m, k, n));
+  TT_TRY(vector_ok("the bias", bias != nullptr ? bias : dbias, bias_dtype));
   TT_TRY(vector_ok("the row scale", row_scale, scale_dtype));
   TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
-  TT_REQUIRE(threshold == 0 || (key != nullptr && g != nullptr),
-             "linear: dropout without a key or a place for its gradient");
-  if (n == 0) return TT_OK;
-  const int64_t per = chunk_rows(m, n), chunks = (m + per - 1) / per;
-  const int64_t tiles = (n + P_COLS - 1) / P_COLS;
-  TT_REQUIRE(tiles <= 65535, "linear: too many columns");
-  TT_REQUIRE(dbias == nullptr || workspace_bytes >= (size_t)chunks * n * 4,
+  TT_REQUIRE(threshold == 0 || key != nullptr, "linear: dropout without a key");
+  TT_REQUIRE(row_scale != nullptr || dscale == nullptr,
+             "linear_residual_bwd: the scale's gradient needs a row scale");
+  TT_REQUIRE(workspace_bytes >= tt_linear_residual_bwd_workspace(dtype, m, k, n,
+                                                                 row_scale != nullptr,
+                                                                 threshold != 0),
              "linear_residual_bwd: the workspace is too small");
-  float* part = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
-  if (m > 0 && (threshold != 0 || dbias != nullptr)) {
-    const bool vec = n % 8 == 0 && all_aligned({dy, threshold != 0 ? g : nullptr});
-    TT_TRY(typed(dtype, [&](auto tt) {
-      typedef decltype(tt) TT;
-      typedef typename TT::storage St;
-      const dim3 grid((unsigned)chunks, (unsigned)tiles), block(L_NT);
-      auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, block, 0, S(stream), static_cast<const St*>(dy), row_scale,
-                           scale_dtype, (uint32_t)threshold, key, static_cast<St*>(g), part, m, n,
-                           per);
-        return tt_check_launch("linear_res_bwd");
-      };
-      if (threshold != 0)
-        return vec ? go(&linear_res_bwd_kernel<TT, true, true>)
-                   : go(&linear_res_bwd_kernel<TT, true, false>);
-      return vec ? go(&linear_res_bwd_kernel<TT, false, true>)
-                 : go(&linear_res_bwd_kernel<TT, false, false>);
-    }));
-  }
-  if (dbias == nullptr) return TT_OK;
+  const size_t es = tt_elem_size(dtype);
   const float alpha = keep_inverse(threshold);
-  hipLaunchKernelGGL(linear_colsum_kernel, dim3((unsigned)((n + 31) / 32)), dim3(L_NT), 0,
-                     S(stream), part, chunks, n, alpha, dbias, bias_dtype);
-  return tt_check_launch("linear_colsum");
-}
-
-extern "C" int tt_linear_dgrad(const void* g, const void* w, const void* x, const void* row_scale,
-                               int scale_dtype, const void* bias, int bias_dtype, int dtype,
-                               int64_t m, int64_t k, int64_t n, int32_t threshold, void* dx,
-                               void* xs, void* dscale, void* workspace, size_t workspace_bytes,
-                               void* stream) {
-  TT_TRY(sizes_ok(dtype, m, k, n));
-  TT_TRY(vector_ok("the bias", bias, bias_dtype));
-  TT_TRY(vector_ok("the row scale", row_scale, scale_dtype));
-  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
-  TT_REQUIRE(row_scale != nullptr || (xs == nullptr && dscale == nullptr),
-             "linear_dgrad: scaled rows and the scale's gradient need a row scale");
-  TT_REQUIRE(row_scale == nullptr || x != nullptr || k == 0, "linear_dgrad: a row scale needs x");
-  if (m == 0) return TT_OK;
-  const size_t db = dscale != nullptr ? dots_bytes(m, k) : 0;
-  const int64_t nd = (k + LIN_DOT - 1) / LIN_DOT;
-  // The bias's part of the scale's gradient goes where the split sums were.
-  const size_t need = db + (dscale != nullptr && bias != nullptr ? (size_t)m * 4 : 0);
-  TT_REQUIRE(workspace_bytes >= need, "linear_dgrad: the workspace is too small");
-  char* const rest = static_cast<char*>(workspace) + db;
-  LinArgs p{};
-  p.a = g;
-  p.b = w;
-  p.out = dx;
-  p.I = m;
-  p.J = p.ldb = k;
-  p.R = p.lda = n;
-  p.scale = row_scale;
-  p.scale_dt = scale_dtype;
-  p.alpha = keep_inverse(threshold);
-  p.x = x;
-  p.xs = xs;
-  p.dots = dscale != nullptr ? static_cast<float*>(workspace) : nullptr;
-  if (k > 0)
-    TT_TRY(run_product(LAY_NN, LIN_DGRAD, dtype, p, rest, workspace_bytes - db, S(stream)));
-  if (dscale == nullptr) return TT_OK;
-  float* extra = nullptr;
-  if (bias != nullptr) {
-    extra = reinterpret_cast<float*>(rest);
-    hipLaunchKernelGGL(linear_rowdot_kernel, dim3((unsigned)((m + 3) / 4)), dim3(L_NT), 0,
-                       S(stream), g, dtype, bias, bias_dtype, m, n, extra);
-    TT_TRY(tt_check_launch("linear_rowdot"));
+  Pieces ws{static_cast<char*>(workspace), workspace_bytes};
+  void* const kept = threshold != 0 ? ws.take((size_t)m * n * es) : nullptr;
+  void* const rows = row_scale != nullptr ? ws.take((size_t)m * k * es) : nullptr;
+  float* const dots = row_scale != nullptr ? static_cast<float*>(ws.take(dots_bytes(m, k))) : nullptr;
+  float* const extra = row_scale != nullptr ? static_cast<float*>(ws.take((size_t)m * 4)) : nullptr;
+  if (n > 0) {
+    const RowPass rp(m, n);
+    TT_REQUIRE(rp.tiles <= 65535, "linear: too many columns");
+    float* const part = dbias != nullptr ? reinterpret_cast<float*>(ws.at) : nullptr;
+    if (m > 0 && (threshold != 0 || dbias != nullptr)) {
+      const bool vec = n % 8 == 0 && all_aligned({dy});
+      TT_TRY(typed(dtype, [&](auto tt) {
+        typedef decltype(tt) TT;
+        typedef typename TT::storage St;
+        auto go = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, rp.grid(), dim3(L_NT), 0, S(stream), static_cast<const St*>(dy),
+                             row_scale, scale_dtype, (uint32_t)threshold, key,
+                             static_cast<St*>(kept), part, m, n, rp.per);
+          return tt_check_launch("linear_res_bwd");
+        };
+        if (threshold != 0)
+          return vec ? go(&linear_res_bwd_kernel<TT, true, true>)
+                     : go(&linear_res_bwd_kernel<TT, true, false>);
+        return vec ? go(&linear_res_bwd_kernel<TT, false, true>)
+                   : go(&linear_res_bwd_kernel<TT, false, false>);
+      }));
+    }
+    if (dbias != nullptr) TT_TRY(column_sums(part, rp, n, alpha, dbias, bias_dtype, S(stream)));
   }
-  hipLaunchKernelGGL(linear_rowsum_kernel, dim3((unsigned)((m + L_NT - 1) / L_NT)), dim3(L_NT), 0,
-                     S(stream), p.dots, (int)nd, extra, p.alpha, m, dscale, scale_dtype);
-  return tt_check_launch("linear_rowsum");
-}
-
-extern "C" int tt_linear_wgrad(const void* g, const void* x, int dtype, int64_t m, int64_t k,
-                               int64_t n, int32_t threshold, void* dw, void* workspace,
-                               size_t workspace_bytes, void* stream) {
-  TT_TRY(sizes_ok(dtype, m, k, n));
-  TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
-  if (n == 0 || k == 0) return TT_OK;
-  LinArgs p{};
-  p.a = g;
-  p.b = x;
-  p.out = dw;
-  p.I = p.lda = n;
-  p.J = p.ldb = k;
-  p.R = m;
-  p.alpha = keep_inverse(threshold);
-  return run_product(LAY_TN, LIN_PLAIN, dtype, p, workspace, workspace_bytes, S(stream));
+  const void* const g = threshold != 0 ? kept : dy;
+  // The weight's gradient takes the rows times their scale, which the pass for dx writes;
+  // that pass runs for them, or for the scale's gradient, where dx is not wanted.
+  const bool scaled_rows = row_scale != nullptr && dw != nullptr;
+  if (dx != nullptr || dscale != nullptr || scaled_rows)
+    TT_TRY(data_gradient(g, w, x, row_scale, scale_dtype, dtype, m, k, n, alpha, dx,
+                         scaled_rows ? rows : nullptr, dscale != nullptr ? dots : nullptr, ws.at,
+                         ws.left, S(stream)));
+  if (dscale != nullptr && m > 0) {
+    if (bias != nullptr) {
+      hipLaunchKernelGGL(linear_rowdot_kernel, dim3((unsigned)((m + 3) / 4)), dim3(L_NT), 0,
+                         S(stream), g, dtype, bias, bias_dtype, m, n, extra);
+      TT_TRY(tt_check_launch("linear_rowdot"));
+    }
+    hipLaunchKernelGGL(linear_rowsum_kernel, dim3((unsigned)((m + L_NT - 1) / L_NT)), dim3(L_NT), 0,
+                       S(stream), dots, (int)((k + LIN_DOT - 1) / LIN_DOT),
+                       bias != nullptr ? extra : nullptr, alpha, m, dscale, scale_dtype);
+    TT_TRY(tt_check_launch("linear_rowsum"));
+  }
+  if (dw != nullptr)
+    TT_TRY(weight_gradient(g, scaled_rows ? rows : x, dtype, m, k, n, alpha, dw, ws.at, ws.left,
+                           S(stream)));
+  return TT_OK;
 }

@@ -64,8 +64,9 @@ class Dropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (key,) = ctx.saved_tensors
-        # The product with a fixed factor: differentiable again.
-        return Dropout.apply(dy, ctx.threshold, key), None, None
+        if torch.is_grad_enabled():  # a product with a fixed factor: differentiable again
+            return Dropout.apply(dy, ctx.threshold, key), None, None
+        return _drop(dy.contiguous(), ctx.threshold, key), None, None
 
 
 @register_op(op_name="dropout", impl_name="hip_dropout", kind=OpImplKind.CUSTOM,

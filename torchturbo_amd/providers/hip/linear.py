@@ -32,15 +32,11 @@ from .dropout import check_key, drop_threshold
 
 FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 ACTIVATIONS = {None: 0, F.silu: 1, F.gelu: 2}
-ACT, GATED, RESIDUAL, DGRAD, WGRAD, COLSUM = range(6)
+ACT, GATED, RESIDUAL = range(3)
 
 
-def _workspace(op, x, m, k, n):
-    """(tensor or None, bytes) of scratch for an op of these sizes."""
-    size = L.load().tt_linear_workspace(op, L.dtype_code(x.dtype), m, k, n)
-    if size == 0:
-        return None, 0
-    return torch.empty((size,), dtype=torch.uint8, device=x.device), size
+def _scratch(size, device):
+    return torch.empty((size,), dtype=torch.uint8, device=device) if size else None
 
 
 def _code(t):
@@ -51,62 +47,26 @@ def act_fwd(x, w, bias, act, gated, pre):
     """y [M, N] of x [M, K]; ``pre``: fp32 [M, N or 2 N] that takes the activation's input."""
     m, k = x.shape
     n = w.shape[0] // 2 if gated else w.shape[0]
-    y = x.new_empty((m, n))
-    ws, size = _workspace(GATED if gated else ACT, x, m, k, n)
-    L.call("tt_linear_act_fwd", L.ptr(x), L.ptr(w), L.ptr(bias), _code(bias),
-           L.dtype_code(x.dtype), m, k, n, act, int(gated), L.ptr(pre), L.ptr(y), L.ptr(ws), size,
-           L.stream(x.device))
+    dev, code = x.device, L.dtype_code(x.dtype)
+    y = torch.empty((m, n), dtype=x.dtype, device=dev)
+    size = L.load().tt_linear_workspace(GATED if gated else ACT, code, m, k, n)
+    ws = _scratch(size, dev)
+    L.call("tt_linear_act_fwd", L.ptr(x), L.ptr(w), L.ptr(bias), _code(bias), code, m, k, n, act,
+           gated, L.ptr(pre), L.ptr(y), L.ptr(ws), size, L.stream(dev))
     return y
 
 
 def residual_fwd(x, w, bias, residual, scale, threshold, key):
     m, k = x.shape
     n = w.shape[0]
-    y = x.new_empty((m, n))
-    ws, size = _workspace(RESIDUAL, x, m, k, n)
+    dev, code = x.device, L.dtype_code(x.dtype)
+    y = torch.empty((m, n), dtype=x.dtype, device=dev)
+    size = L.load().tt_linear_workspace(RESIDUAL, code, m, k, n)
+    ws = _scratch(size, dev)
     L.call("tt_linear_residual_fwd", L.ptr(x), L.ptr(w), L.ptr(bias), _code(bias), L.ptr(residual),
-           L.ptr(scale), _code(scale), L.dtype_code(x.dtype), m, k, n, threshold, L.ptr(key),
-           L.ptr(y), L.ptr(ws), size, L.stream(x.device))
+           L.ptr(scale), _code(scale), code, m, k, n, threshold, L.ptr(key), L.ptr(y), L.ptr(ws),
+           size, L.stream(dev))
     return y
-
-
-def residual_bwd(dy, scale, threshold, key, bias, want_bias):
-    """``(g, dbias)``: dy without its dropped elements, and the bias's gradient (or None)."""
-    m, n = dy.shape
-    if threshold == 0 and not want_bias:
-        return dy, None
-    g = torch.empty_like(dy) if threshold else dy
-    dbias = torch.empty_like(bias) if want_bias else None
-    ws, size = _workspace(COLSUM, dy, m, 0, n) if want_bias else (None, 0)
-    L.call("tt_linear_residual_bwd", L.ptr(dy), L.ptr(scale), _code(scale),
-           L.dtype_code(dy.dtype), m, n, threshold, L.ptr(key), L.ptr(g), L.ptr(dbias),
-           _code(dbias), L.ptr(ws), size, L.stream(dy.device))
-    return g, dbias
-
-
-def dgrad(g, w, x, scale, bias, threshold, want_x, want_rows, want_scale):
-    """``(dx, scaled rows, dscale)`` of the product's gradient g, each None unless wanted."""
-    m, n = g.shape
-    k = w.shape[1]
-    dx = g.new_empty((m, k)) if want_x else None
-    xs = torch.empty_like(x) if want_rows else None
-    ds = torch.empty_like(scale) if want_scale else None
-    ws, size = _workspace(DGRAD, g, m, k, n)
-    L.call("tt_linear_dgrad", L.ptr(g), L.ptr(w), L.ptr(x), L.ptr(scale), _code(scale),
-           L.ptr(bias) if want_scale else None, _code(bias), L.dtype_code(g.dtype), m, k, n,
-           threshold, L.ptr(dx), L.ptr(xs), L.ptr(ds), L.ptr(ws), size, L.stream(g.device))
-    return dx, xs, ds
-
-
-def wgrad(g, x, threshold):
-    """dw [N, K] = (inverse of the kept share) g^T x."""
-    m, n = g.shape
-    k = x.shape[1]
-    dw = g.new_empty((n, k))
-    ws, size = _workspace(WGRAD, g, m, k, n)
-    L.call("tt_linear_wgrad", L.ptr(g), L.ptr(x), L.dtype_code(g.dtype), m, k, n, threshold,
-           L.ptr(dw), L.ptr(ws), size, L.stream(g.device))
-    return dw
 
 
 class LinearAct(torch.autograd.Function):
@@ -129,18 +89,15 @@ class LinearAct(torch.autograd.Function):
         act, gated = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = dy.to(x.dtype).contiguous()
-        if pre is None:
-            da, dbias = residual_bwd(dy, None, 0, None, bias, need_b)
-        else:
-            m, n = dy.shape
-            da = dy.new_empty(pre.shape)
-            dbias = torch.empty_like(bias) if need_b else None
-            ws, size = _workspace(COLSUM, dy, m, 0, n) if need_b else (None, 0)
-            L.call("tt_linear_act_bwd", L.ptr(dy), L.ptr(pre), L.dtype_code(dy.dtype), m, n, act,
-                   int(gated), L.ptr(da), L.ptr(dbias), _code(dbias), L.ptr(ws), size,
-                   L.stream(dy.device))
-        dx = dgrad(da, w, None, None, None, 0, True, False, False)[0] if need_x else None
-        dw = wgrad(da, x, 0) if need_w else None
+        (m, n), k, dev, code = dy.shape, x.shape[1], x.device, L.dtype_code(x.dtype)
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty_like(w) if need_w else None
+        dbias = torch.empty_like(bias) if need_b else None
+        size = L.load().tt_linear_act_bwd_workspace(code, m, k, n, act, gated)
+        ws = _scratch(size, dev)
+        L.call("tt_linear_act_bwd", L.ptr(dy), L.ptr(x), L.ptr(w), L.ptr(pre), code, m, k, n, act,
+               gated, L.ptr(dx), L.ptr(dw), L.ptr(dbias), _code(dbias), L.ptr(ws), size,
+               L.stream(dev))
         return dx, dw, dbias, None, None
 
 
@@ -160,19 +117,20 @@ class LinearResidual(torch.autograd.Function):
         x, w, bias, scale, key = ctx.saved_tensors
         need_x, need_w, need_b, need_r, need_s = ctx.needs_input_grad[:5]
         d_residual = dy if need_r else None
+        if not (need_x or need_w or need_b or need_s):
+            return None, None, None, d_residual, None, None, None
         dy = dy.to(x.dtype).contiguous()
         t = ctx.threshold
-        g = dbias = dx = dw = ds = None
-        if need_x or need_w or need_b or need_s:
-            g, dbias = residual_bwd(dy, scale, t, key, bias, need_b)
-        # The weight's gradient needs the rows times their scale, which the pass for
-        # dx writes; that pass runs for them alone where dx is not wanted.
-        rows = need_w and scale is not None
-        if need_x or need_s or rows:
-            dx, xs, ds = dgrad(g, w, x if scale is not None else None, scale, bias, t, need_x,
-                               rows, need_s)
-        if need_w:
-            dw = wgrad(g, xs if rows else x, t)
+        (m, n), k, dev, code = dy.shape, x.shape[1], x.device, L.dtype_code(x.dtype)
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty_like(w) if need_w else None
+        dbias = torch.empty_like(bias) if need_b else None
+        ds = torch.empty_like(scale) if need_s else None
+        size = L.load().tt_linear_residual_bwd_workspace(code, m, k, n, scale is not None, t != 0)
+        ws = _scratch(size, dev)
+        L.call("tt_linear_residual_bwd", L.ptr(dy), L.ptr(x), L.ptr(w), L.ptr(bias), _code(bias),
+               L.ptr(scale), _code(scale), code, m, k, n, t, L.ptr(key), L.ptr(dx), L.ptr(dw),
+               L.ptr(dbias), L.ptr(ds), L.ptr(ws), size, L.stream(dev))
         return dx, dw, dbias, d_residual, ds, None, None
 
 
@@ -199,6 +157,8 @@ def _wants_grad(*tensors) -> bool:
 
 def _rows(t, width):
     """[..., width] as contiguous rows (their number from the other dimensions alone)."""
+    if t.dim() == 2:
+        return t.contiguous()
     count = 1
     for d in t.shape[:-1]:
         count *= d
@@ -226,7 +186,7 @@ class HipLinearAct(OpImpl):
             y = LinearAct.apply(x2, w, b, act, gated)
         else:
             y = act_fwd(x2, w, b, act, gated, None)
-        return y.view(*x.shape[:-1], n)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
 @register_op(op_name="linear_residual", impl_name="hip_linear_residual", kind=OpImplKind.CUSTOM,
@@ -260,4 +220,4 @@ class HipLinearResidual(OpImpl):
             y = LinearResidual.apply(x2, w, b, r, s, threshold, key)
         else:
             y = residual_fwd(x2, w, b, r, s, threshold, key)
-        return y.view(shape)
+        return y if x.dim() == 2 else y.view(shape)
