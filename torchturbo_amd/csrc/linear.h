@@ -234,10 +234,13 @@ __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t
 // TN: A [R, I], B [R, J].
 enum { LAY_NT = 0, LAY_NN = 1, LAY_TN = 2 };
 
+// The kernels: for any type, for few rows, and tiles of the 16-bit matrix instructions.
+enum { LIN_ANY = 0, LIN_ROWS = 1, LIN_T64 = 2, LIN_T128 = 3, LIN_T256x128 = 4, LIN_T256 = 5 };
+
 // fp32 matrix instructions on any type, size and alignment (linear_any.hip).
 int tt_linear_any(int kind, int dtype, const LinArgs& a, hipStream_t s);
-// 16-bit matrix instructions on tiles of `tile` (128 or 256) rows and columns, for
-// aligned rows of whole 16-byte vectors (linear_tile.hip).
+// 16-bit matrix instructions on tiles (LIN_T64 ...), for aligned rows of whole 16-byte
+// vectors (linear_tile.hip).
 int tt_linear_tile(int kind, int tile, int dtype, const LinArgs& a, hipStream_t s);
 // The same for at most 64 rows of x and NT operands under 2 GiB (linear_thin.hip).
 int tt_linear_thin(int kind, int dtype, const LinArgs& a, hipStream_t s);

@@ -105,10 +105,9 @@ Split split_of(int64_t R, int64_t wanted) {
   return Split{(int)((R + per - 1) / per), per};
 }
 
-// The kernel that runs a product (0: any type, 16: few rows, 64, 128 and 256: the tile
-// of linear_tile.hip) and how many parts its reduction is split into.
+// The kernel that runs a product and how many parts its reduction is split into.
 struct Plan {
-  int tile;
+  int kernel;
   Split split;
 };
 
@@ -131,12 +130,15 @@ int64_t least_splits(int layout, int64_t I, int64_t J, int64_t R) {
 double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sums, int64_t bytes) {
   const int64_t blocks = tiles * splits, full = blocks / 512, rest = blocks % 512;
   double us;
-  if (tile == 256) {
+  if (tile >= LIN_T256x128) {
+    const bool sq = tile == LIN_T256;
     const double fill = std::min(1.0, (double)blocks / 256);
-    us = 8 + (double)((blocks + 255) / 256) * (12 + (double)nkt * (0.85 + 0.35 * fill));
+    us = (sq ? 8 : 5) + (double)((blocks + 255) / 256) *
+                            ((sq ? 12 : 6) + (double)nkt * (sq ? 0.85 + 0.35 * fill : 0.5 + 0.2 * fill));
   } else {
-    const double one = tile == 64 ? 0.30 : 0.62, two = tile == 64 ? 0.5 : 1.0;
-    us = (tile == 64 ? 2.8 : 4.2) + (double)full * (tile == 64 ? 0.5 : 1.5) +
+    const bool small = tile == LIN_T64;
+    const double one = small ? 0.30 : 0.62, two = small ? 0.5 : 1.0;
+    us = (small ? 2.8 : 4.2) + (double)full * (small ? 0.5 : 1.5) +
          (double)nkt * ((double)full * two + (rest == 0 ? 0 : rest <= 256 ? one : two));
   }
   us = std::max(us, 2.8 + (double)bytes / 4.6e6);
@@ -155,30 +157,33 @@ double rows_us(int64_t blocks, int64_t I, int64_t J, int64_t R) {
 
 Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, bool fast) {
   const int64_t half = kind == LIN_GATED ? 2 : 1, width = half * J;
-  auto tiles = [&](int64_t t) { return ((I + t - 1) / t) * ((width + t - 1) / t); };
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((I + bm - 1) / bm) * ((width + bn - 1) / bn); };
   if (!fast) {
     // Enough blocks for the CUs, each reduction at least 256 long.
-    const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64), 1), R / 256);
-    return Plan{0, split_of(R, std::min<int64_t>(want, 32))};
+    const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64, 64), 1), R / 256);
+    return Plan{LIN_ANY, split_of(R, std::min<int64_t>(want, 32))};
   }
   const int64_t least = least_splits(layout, I, J, R);
-  Plan best{256, split_of(R, least)};
+  Plan best{LIN_T256, split_of(R, least)};
   double best_us = 1e30;
   if (layout == LAY_NT && I <= 64 && width * R * 2 < (1ll << 32)) {
-    best = Plan{16, split_of(R, 1)};
+    best = Plan{LIN_ROWS, split_of(R, 1)};
     best_us = rows_us((width + 15) / 16, I, width, R);
   }
-  for (int tile : {64, 128, 256})
+  for (int tile : {LIN_T64, LIN_T128, LIN_T256x128, LIN_T256}) {
+    const int64_t bm = tile == LIN_T64 ? 64 : tile == LIN_T128 ? 128 : 256;
+    const int64_t bn = tile == LIN_T64 ? 64 : tile == LIN_T256 ? 256 : 128;
     for (int64_t want = least; want <= std::max<int64_t>(least, 16); want *= 2) {
       const Split sp = split_of(R, want);
       if (sp.splits > least && sp.run < 256) break;
-      const double us = tile_us(tile, tiles(tile), sp.splits, sp.run / 64, I * width,
+      const double us = tile_us(tile, tiles(bm, bn), sp.splits, sp.run / 64, I * width,
                                 (I + width) * R * 2);
       if (us < best_us) {
         best_us = us;
         best = Plan{tile, sp};
       }
     }
+  }
   return best;
 }
 
@@ -208,15 +213,16 @@ int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_
   if (part_bytes(kind, p.I, p.J, pl.split.splits) > ws_bytes) {
     // Without room for the parts: a whole reduction, on the kernel for any size where
     // the tiles cannot walk it.
-    pl = Plan{fast && least_splits(layout, p.I, p.J, p.R) == 1 ? pl.tile : 0, split_of(p.R, 1)};
+    pl = Plan{fast && least_splits(layout, p.I, p.J, p.R) == 1 ? pl.kernel : LIN_ANY,
+              split_of(p.R, 1)};
   }
   const Split sp = pl.split;
   p.splits = sp.splits;
   p.rsplit = sp.run;
   p.part = sp.splits > 1 ? static_cast<float*>(ws) : nullptr;
-  const int rc = pl.tile == 0    ? tt_linear_any(kind, dtype, p, s)
-                 : pl.tile == 16 ? tt_linear_thin(kind, dtype, p, s)
-                                 : tt_linear_tile(kind, pl.tile, dtype, p, s);
+  const int rc = pl.kernel == LIN_ANY    ? tt_linear_any(kind, dtype, p, s)
+                 : pl.kernel == LIN_ROWS ? tt_linear_thin(kind, dtype, p, s)
+                                         : tt_linear_tile(kind, pl.kernel, dtype, p, s);
   if (rc != TT_OK || p.part == nullptr) return rc;
   switch (dtype) {
     case TT_BF16: return join_kind<BF16T>(kind, p, s);

@@ -439,27 +439,28 @@ __device__ __forceinline__ void mma16(f32x4_t& c, const uint4& a, const uint4& b
 // and the use of its result does not see assembly.
 __device__ __forceinline__ void mma_done() { asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory"); }
 
-// 256 x 256 tiles, 128 x 128 per wave (256 accumulators, one wave per SIMD), in
-// 16x16x32 products. Two k-tiles of A and three of B in LDS. k-step 0 multiplies,
-// reads the fragments of k-step 1 and loads B's k-tile kt + 2; then every wave has
-// read k-tile kt, and k-step 1 loads A's k-tile kt + 2 into its place, and after a
-// second barrier, which publishes k-tile kt + 1, reads that one's first fragments.
-template <int LAYOUT, int KIND, int ET, bool KMASK>
+// 256 x BN tiles, BN 256 or 128, 128 x BN / 2 per wave (one wave per SIMD), in
+// 16x16x32 products. LDS holds SA k-tiles of A and three of B; the k-tile after next is
+// loaded while one is multiplied. k-step 0 multiplies and reads the fragments of
+// k-step 1. With SA = 2 a barrier then frees A's stage for the loads of k-step 1 (with
+// three, the stage of the k-tile before is loaded). Half way through k-step 1 a
+// barrier publishes the next k-tile, whose first fragments the other half reads.
+template <int LAYOUT, int KIND, int ET, bool KMASK, int BN>
 __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int tj) {
-  typedef Tile<LAYOUT, KIND, 256, 256, 16> TL;
-  constexpr int FM = 8, FN = 8;
+  typedef Tile<LAYOUT, KIND, 256, BN, 16> TL;
+  constexpr int FM = 8, FN = BN / 32, SA = BN == 256 ? 2 : 3;
   constexpr int LA = TL::OpA::LOADS, LB = TL::OpB::LOADS;
-  static_assert(LA == 8 && LB == 8, "one load per eight or four products");
+  static_assert(LA == 8 && LB == FN, "loads per row of products");
   constexpr uint32_t BA = TL::OpA::BYTES, BB = TL::OpB::BYTES;
-  __shared__ __align__(16) char lds_raw[2 * BA + 3 * BB];  // two k-tiles of A, then three of B
+  __shared__ __align__(16) char lds_raw[SA * BA + 3 * BB];  // the k-tiles of A, then of B
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   TL t;
   t.setup(p, ti, tj, wave, lane);
   lds_char* const lds = (lds_char*)lds_raw;
   const uint32_t lds0 = lds_addr_of(lds);
-  const uint32_t wa0 = lds0 + (uint32_t)(LA * wave) * 1024u;           // the wave's part of A's stages
-  const uint32_t wb0 = lds0 + 2 * BA + (uint32_t)(LB * wave) * 1024u;  // and of B's
+  const uint32_t wa0 = lds0 + (uint32_t)(LA * wave) * 1024u;            // the wave's part of A's stages
+  const uint32_t wb0 = lds0 + SA * BA + (uint32_t)(LB * wave) * 1024u;  // and of B's
   uint4 fa[2][FM], fb[2][FN];
   f32x4_t acc[FM][FN] = {};
   t.a.template loads<KMASK, 0, LA>(t.wa.r, wa0, t.kn);
@@ -475,15 +476,17 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
 #pragma unroll
   for (int i = 0; i < FM; ++i) fa[0][i] = t.a.read(lds, i, 0);
 #pragma unroll
-  for (int i = 0; i < FN; ++i) fb[0][i] = t.b.read(lds + 2 * BA, i, 0);
-  int slot = 0;  // of B's k-tile kt
+  for (int i = 0; i < FN; ++i) fb[0][i] = t.b.read(lds + SA * BA, i, 0);
+  int slot = 0;  // of k-tile kt in a ring of three
   for (int kt = 0; kt < t.nkt; ++kt) {
     const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot == 0 ? 2 : slot - 1;
-    lds_char* const ca = lds + (uint32_t)(kt & 1) * BA;
-    lds_char* const na = lds + (uint32_t)((kt + 1) & 1) * BA;
-    lds_char* const cb = lds + 2 * BA + (uint32_t)slot * BB;
-    lds_char* const nb = lds + 2 * BA + (uint32_t)slot1 * BB;
-    const uint32_t to_a = wa0 + (uint32_t)(kt & 1) * BA, to_b = wb0 + (uint32_t)slot2 * BB;
+    const int a0 = SA == 3 ? slot : kt & 1, a1 = SA == 3 ? slot1 : (kt + 1) & 1;
+    lds_char* const ca = lds + (uint32_t)a0 * BA;
+    lds_char* const na = lds + (uint32_t)a1 * BA;
+    lds_char* const cb = lds + SA * BA + (uint32_t)slot * BB;
+    lds_char* const nb = lds + SA * BA + (uint32_t)slot1 * BB;
+    const uint32_t to_a = wa0 + (uint32_t)(SA == 3 ? slot2 : a0) * BA;
+    const uint32_t to_b = wb0 + (uint32_t)slot2 * BB;
     const int valid = t.kn - (kt + 2) * T_BK;
     // Products of row m and columns n, n + 1 of k-step s.
     auto mul = [&](int s, int m, int n) {
@@ -496,9 +499,27 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
 #pragma unroll
       for (int n = 0; n < FN; n += 2) {
         mul(0, m, n);
-        if (n == 0) fb[1][m] = t.b.read(cb, m, 1);
-        if (n == 4) fa[1][m] = t.a.read(ca, m, 1);
-        if (n == 6) t.b.template load<KMASK, m>(t.wb.r, to_b, valid);
+        if (n == 0 && m < FN) fb[1][m] = t.b.read(cb, m, 1);
+        if (n == (FN == 8 ? 4 : m < FN ? 2 : 0)) fa[1][m] = t.a.read(ca, m, 1);
+        if (n == FN - 2) {
+          if constexpr (m < LB) t.b.template load<KMASK, (m < LB ? m : 0)>(t.wb.r, to_b, valid);
+          else t.a.template load<KMASK, m - LB>(t.wa.r, to_a, valid);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // k-step 1, rows 0-3: with the rest of A's loads.
+    auto second = [&](auto m_c) {
+      constexpr int m = decltype(m_c)::value;
+#pragma unroll
+      for (int n = 0; n < FN; n += 2) {
+        mul(1, m, n);
+        if constexpr (FN == 8) {
+          if (n == 2) t.a.template load<KMASK, 2 * m>(t.wa.r, to_a, valid);
+          if (n == 6) t.a.template load<KMASK, 2 * m + 1>(t.wa.r, to_a, valid);
+        } else {
+          if (n == 0) t.a.template load<KMASK, 4 + m>(t.wa.r, to_a, valid);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -511,22 +532,11 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
     first(std::integral_constant<int, 6>{});
     first(std::integral_constant<int, 7>{});
     t.next_b(kt + 2);
-    TT_LDS_BARRIER();  // every wave has read k-tile kt
-    // Rows 0-2 of k-step 1, with A's loads.
-    auto load_a = [&](auto m_c) {
-      constexpr int m = decltype(m_c)::value;
-#pragma unroll
-      for (int n = 0; n < FN; n += 2) {
-        mul(1, m, n);
-        if (n == 2) t.a.template load<KMASK, 2 * m>(t.wa.r, to_a, valid);
-        if (n == 6) t.a.template load<KMASK, 2 * m + 1>(t.wa.r, to_a, valid);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    load_a(std::integral_constant<int, 0>{});
-    load_a(std::integral_constant<int, 1>{});
-    load_a(std::integral_constant<int, 2>{});
-    load_a(std::integral_constant<int, 3>{});
+    if constexpr (SA == 2) TT_LDS_BARRIER();  // every wave has read k-tile kt
+    second(std::integral_constant<int, 0>{});
+    second(std::integral_constant<int, 1>{});
+    second(std::integral_constant<int, 2>{});
+    second(std::integral_constant<int, 3>{});
     t.next_a(kt + 2);
     TT_WAIT_VMCNT(LA + LB);  // k-tile kt + 1 has landed
     TT_LDS_BARRIER();
@@ -535,9 +545,13 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
 #pragma unroll
       for (int n = 0; n < FN; n += 2) {
         mul(1, m, n);
-        const int i = 4 * (m - 4) + n / 2;
-        if (i < 8) fb[0][i] = t.b.read(nb, i, 0);
-        else fa[0][i - 8] = t.a.read(na, i - 8, 0);
+        constexpr int PS = FN == 8 ? 2 : 3;  // reads per two slots
+        const int at = (m - 4) * (FN / 2) + n / 2;
+#pragma unroll
+        for (int i = at * PS / 2; i < (at + 1) * PS / 2; ++i) {
+          if (i < FN) fb[0][i] = t.b.read(nb, i, 0);
+          else fa[0][i - FN] = t.a.read(na, i - FN, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     slot = slot1;
@@ -553,7 +567,7 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
       for (int n = 0; n < FN; ++n)
         put(16 * m + (lane & 15), 4 * n + (lane >> 4), acc[2 * mi + m][n]);
   };
-  tile_finish<KIND, ET, FM / 2, FN / 2>(p, stage, lds + wave * (32 * 128 * 4),
+  tile_finish<KIND, ET, FM / 2, FN / 2>(p, stage, lds + wave * (32 * (BN / 2) * 4),
                                         t.i0 + (wave >> 1) * 128,
                                         t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
@@ -631,23 +645,22 @@ __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int
 
 template <int LAYOUT, int KIND, int ET, bool KMASK>
 int launch(int tile, const LinArgs& p, hipStream_t s) {
-  const int bo = KIND == LIN_GATED ? tile / 2 : tile;
-  const int64_t ti = (p.I + tile - 1) / tile, tj = (p.J + bo - 1) / bo;
+  const int bm = tile == LIN_T64 ? 64 : tile == LIN_T128 ? 128 : 256;
+  const int bn = tile == LIN_T64 ? 64 : tile == LIN_T256 ? 256 : 128;
+  const int bo = KIND == LIN_GATED ? bn / 2 : bn;
+  const int64_t ti = (p.I + bm - 1) / bm, tj = (p.J + bo - 1) / bo;
   TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
-  const dim3 grid((unsigned)(ti * tj), (unsigned)p.splits), block(T_NT);
-  if (tile == 256)
-    hipLaunchKernelGGL((linear_big_kernel<LAYOUT, KIND, ET, KMASK>), grid, block, 0, s, p, (int)ti,
-                       (int)tj);
-  else if (tile == 64)
-    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 64, 4>), grid, block, 0, s, p,
-                       (int)ti, (int)tj);
-  else if (ti * tj * p.splits <= 256)
-    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 4>), grid, block, 0, s, p,
-                       (int)ti, (int)tj);
-  else
-    hipLaunchKernelGGL((linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 2>), grid, block, 0, s, p,
-                       (int)ti, (int)tj);
-  return tt_check_launch("linear");
+  const dim3 grid((unsigned)(ti * tj), (unsigned)p.splits);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(T_NT), 0, s, p, (int)ti, (int)tj);
+    return tt_check_launch("linear");
+  };
+  if (tile == LIN_T256) return go(&linear_big_kernel<LAYOUT, KIND, ET, KMASK, 256>);
+  if (tile == LIN_T256x128) return go(&linear_big_kernel<LAYOUT, KIND, ET, KMASK, 128>);
+  if (tile == LIN_T64) return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 64, 4>);
+  // A block has a CU to itself, and all of its memory, in a launch of at most one per CU.
+  if (ti * tj * p.splits <= 256) return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 4>);
+  return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 2>);
 }
 
 template <int LAYOUT, int KIND>
