@@ -2,7 +2,7 @@
 // mask of element (row, col) as in philox.h, so nothing but the key is stored
 // for the backward, which is the same call on the gradient. A dropped element is
 // 0 whatever it held (infinities and NaN included).
-#include "philox.h"
+#include "linear.h"
 
 namespace {
 
@@ -44,17 +44,11 @@ __global__ __launch_bounds__(DR_NT) void dropout_kernel(const typename TT::stora
       if (r >= rows) break;
       uint32_t w[4];
       philox(dk, (uint32_t)group, (uint32_t)r, w);
-      St o[8];
+      float o[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        o[j] = keeps(w, j, threshold) ? TT::from_f32(TT::to_f32(v[q][j]) * inv) : St(0);
-      if constexpr (VEC) {
-        __builtin_memcpy(y + r * cols + c0, o, sizeof(o));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c0 + j < cols) y[r * cols + c0 + j] = o[j];
-      }
+      for (int j = 0; j < 8; ++j) o[j] = keeps(w, j, threshold) ? TT::to_f32(v[q][j]) * inv : 0.f;
+      const int n = cols - c0 < 8 ? (int)(cols - c0) : 8;
+      lin_store<TT, 8, VEC>(y, r * cols + c0, n, o);
     }
   }
 }

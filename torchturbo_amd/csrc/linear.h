@@ -4,6 +4,7 @@
 
 #include <math.h>
 
+#include "gemm.h"
 #include "philox.h"
 
 // What becomes of the fp32 sums v = sum over r of A(i, r) B(r, j):
@@ -96,11 +97,18 @@ template <class TT, int W, bool VEC>
 __device__ __forceinline__ void lin_store(void* p, int64_t at, int n, const float (&v)[W]) {
   typedef typename TT::storage St;
   St* q = static_cast<St*>(p) + at;
-  if constexpr (VEC) {
+  if constexpr (VEC && sizeof(St) == 2) {
+    uint2 o[W / 4];
+#pragma unroll
+    for (int q = 0; q < W / 4; ++q)
+      o[q] = pack4<__is_same(TT, BF16T) ? TT_BF16 : TT_F16>(v[4 * q], v[4 * q + 1], v[4 * q + 2],
+                                                            v[4 * q + 3]);
+    __builtin_memcpy(__builtin_assume_aligned(q, W * 2), o, sizeof(o));
+  } else if constexpr (VEC) {
     St o[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) o[j] = TT::from_f32(v[j]);
-    __builtin_memcpy(__builtin_assume_aligned(q, sizeof(St) * W < 16 ? sizeof(St) * W : 16), o, sizeof(o));
+    __builtin_memcpy(__builtin_assume_aligned(q, 16), o, sizeof(o));
   } else {
 #pragma unroll
     for (int j = 0; j < W; ++j)

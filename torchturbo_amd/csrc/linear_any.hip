@@ -2,7 +2,6 @@
 // fp32 tensors, and 16-bit ones whose rows do not split into aligned 16-byte
 // vectors. Products and sums run in fp32 on v_mfma_f32_32x32x2_f32 (16-bit
 // operands widen exactly).
-#include "gemm.h"
 #include "linear.h"
 
 namespace {

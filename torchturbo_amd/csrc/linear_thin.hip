@@ -9,7 +9,6 @@
 // reduction elements of row l % 16), U steps at a time, the next ones in flight while
 // the ones before are multiplied. The waves' sums meet in LDS and are added in order.
 // GATED: a 16-row block of weights is eight gates and their eight ups.
-#include "gemm.h"
 #include "linear.h"
 
 namespace {

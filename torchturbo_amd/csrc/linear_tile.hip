@@ -11,7 +11,6 @@
 // ds_read_b64_tr_b16. Resources end with the operand, so rows past it read as
 // zeros; a K-major tail (R % 64) is masked per chunk; columns past J are read
 // from wherever they lead inside the resource and never stored.
-#include "gemm.h"
 #include "linear.h"
 
 #include <type_traits>

@@ -207,24 +207,25 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
         }
     };
     if (16 * wr < rows) {
-      // DROP: lanes l and l ^ 32 read the same eight elements of each 16 (and
-      // multiply four of them each); each makes two of the k-tile's four masks,
-      // one bit per element, and hands them to the other.
-      uint32_t kept = 0;
+      // DROP: lanes l and l ^ 32 read the same eight elements of each 16 (and multiply
+      // four of them each); each makes the masks of two of the k-tile's four, and the
+      // halves exchange them.
+      uint32_t kept[BK / 16][4];
       if constexpr (DROP) {
-        uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t w[4];
           philox(dk, (uint32_t)(kt * (BK / 8) + 2 * (2 * (g >> 1) + i) + (g & 1)),
                  (uint32_t)(row0 + row), w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            mine |= (keeps(w, e, drop.threshold) ? 1u : 0u) << (8 * i + e);
+          for (int q = 0; q < 4; ++q) {
+            // The lower lanes' mask is of 16 elements i, the upper ones' of 2 + i.
+            const uint32_t m = keep_mask(w[q], drop.threshold);
+            const auto v = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+            kept[i][q] = v[0];
+            kept[2 + i][q] = v[1];
+          }
         }
-        const uint32_t theirs = (uint32_t)__shfl_xor((int)mine, 32, 64);
-        kept = odd ? theirs | (mine << 16) : mine | (theirs << 16);
-        kept >>= odd ? 1 : 0;  // bit 8 b + 2 q: the element this lane multiplies
       }
       read(0);
 #pragma unroll
@@ -234,8 +235,7 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
         const uint32_t x[4] = {xv[b & 1].x, xv[b & 1].y, xv[b & 1].z, xv[b & 1].w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float a = widen1<TT, SCALE>(x[q], odd, s);
-          if constexpr (DROP) a = (kept >> (8 * b + 2 * q)) & 1u ? a : 0.f;
+          const float a = widen1<TT, SCALE>(DROP ? x[q] & kept[b][q] : x[q], odd, s);
 #pragma unroll
           for (int jt = 0; jt < CT; ++jt) acc[jt] = mfma16(a, wv[b & 1][q][jt], acc[jt]);
         }
@@ -381,8 +381,8 @@ __global__ __launch_bounds__(LR_NT, RT == 2 && WT ? 3 : 1) void lora_up_kernel(
     if constexpr (DROP) {
       uint32_t w[4];
       philox(dk, (uint32_t)(n >> 3), (uint32_t)(row0 + m), w);
-      v = uint4{keep_pair(v.x, w[0], drop.threshold), keep_pair(v.y, w[1], drop.threshold),
-                keep_pair(v.z, w[2], drop.threshold), keep_pair(v.w, w[3], drop.threshold)};
+      v = uint4{v.x & keep_mask(w[0], drop.threshold), v.y & keep_mask(w[1], drop.threshold),
+                v.z & keep_mask(w[2], drop.threshold), v.w & keep_mask(w[3], drop.threshold)};
     }
     if constexpr (BASE) {
       float d[8], b[8];
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(LR_NT) void lora_wgrad_kernel(const uint16_t* __res
     for (int q = 0; q < 4; ++q) {
       const bool ok = m0 + first + 2 * q < rows;
       uint32_t xq = ok && live ? x[buf][q] : 0;
-      if constexpr (DROP) xq = keep_pair(xq, w[q], drop.threshold);
+      if constexpr (DROP) xq &= keep_mask(w[q], drop.threshold);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float a = widen1<TT, SCALE>(xq, i == 1, s);

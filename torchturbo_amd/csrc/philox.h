@@ -46,11 +46,15 @@ __device__ __forceinline__ bool keeps(const uint32_t (&w)[4], int j, uint32_t th
   return ((w[j >> 1] >> (16 * (j & 1))) & 0xffffu) >= threshold;
 }
 
-// Packed 16-bit pair number i (elements 2 i, 2 i + 1) with its dropped halves cleared.
-__device__ __forceinline__ uint32_t keep_pair(uint32_t pair, uint32_t word, uint32_t threshold) {
-  const uint32_t lo = (word & 0xffffu) >= threshold ? 0x0000ffffu : 0u;
-  const uint32_t hi = (word >> 16) >= threshold ? 0xffff0000u : 0u;
-  return pair & (lo | hi);
+// Word i of a group as a mask of its two 16-bit elements 2 i and 2 i + 1: all ones
+// where kept. Thresholds 1 .. 65536.
+__device__ __forceinline__ uint32_t keep_mask(uint32_t word, uint32_t threshold) {
+  typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+  const unsigned short t = (unsigned short)(threshold - 1);
+  // w - (threshold - 1), not below 0, is at least 1 where w >= threshold.
+  const u16x2 over = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, word), u16x2{t, t});
+  const u16x2 one = __builtin_elementwise_min(over, u16x2{1, 1});
+  return __builtin_bit_cast(uint32_t, u16x2{0, 0} - one);
 }
 
 // 1 / (share that is kept): thresholds are in steps of 2^-16, 0 (nothing
