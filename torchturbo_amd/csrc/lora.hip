@@ -174,11 +174,32 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
   const int wr = wave / WC, wc = wave % WC;  // the wave's rows and columns
   const int row = 16 * wr + l16;
   f32x4 acc[CT] = {};
+  // DROP: lanes l and l ^ 32 read the same eight elements of each 16 (and multiply four
+  // of them each); each makes the masks of two of a k-tile's four 16s, and the halves
+  // exchange them. The masks of the next k-tile are made among the products of this one.
   DropKey dk{};
   if constexpr (DROP) dk = load_key(drop.key);
+  uint32_t kept[BK / 16][4], kept_next[BK / 16][4];
+  auto masks = [&](int kt, int i, uint32_t (&to)[BK / 16][4]) {
+    uint32_t w[4];
+    philox(dk, (uint32_t)(kt * (BK / 8) + 2 * (2 * (g >> 1) + i) + (g & 1)), (uint32_t)(row0 + row),
+           w);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // The lower lanes' mask is of the 16 elements i, the upper ones' of 2 + i.
+      const uint32_t m = keep_mask(w[q], drop.threshold);
+      const auto v = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+      to[i][q] = v[0];
+      to[2 + i][q] = v[1];
+    }
+  };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i)
     if (i < nkt) issue(i, i);
+  if constexpr (DROP) {
+    masks(0, 0, kept);
+    masks(0, 1, kept);
+  }
   int slot = 0;
   for (int kt = 0; kt < nkt; ++kt) {
     // k-tile kt has landed once at most the later ones are outstanding.
@@ -207,31 +228,13 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
         }
     };
     if (16 * wr < rows) {
-      // DROP: lanes l and l ^ 32 read the same eight elements of each 16 (and multiply
-      // four of them each); each makes the masks of two of the k-tile's four, and the
-      // halves exchange them.
-      uint32_t kept[BK / 16][4];
-      if constexpr (DROP) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t w[4];
-          philox(dk, (uint32_t)(kt * (BK / 8) + 2 * (2 * (g >> 1) + i) + (g & 1)),
-                 (uint32_t)(row0 + row), w);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            // The lower lanes' mask is of 16 elements i, the upper ones' of 2 + i.
-            const uint32_t m = keep_mask(w[q], drop.threshold);
-            const auto v = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-            kept[i][q] = v[0];
-            kept[2 + i][q] = v[1];
-          }
-        }
-      }
       read(0);
 #pragma unroll
       for (int b = 0; b < BK / 16; ++b) {
         if (b + 1 < BK / 16) read(b + 1);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (DROP)
+          if (b % 2 == 0) masks(kt + 1, b / 2, kept_next);
         const uint32_t x[4] = {xv[b & 1].x, xv[b & 1].y, xv[b & 1].z, xv[b & 1].w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -241,6 +244,12 @@ __global__ __launch_bounds__(LR_NT) void lora_down_kernel(const uint16_t* __rest
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    if constexpr (DROP) {
+#pragma unroll
+      for (int b = 0; b < BK / 16; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) kept[b][q] = kept_next[b][q];
     }
     slot = slot == S - 1 ? 0 : slot + 1;
   }
@@ -461,20 +470,25 @@ __global__ __launch_bounds__(LR_NT) void lora_wgrad_kernel(const uint16_t* __res
   };
   DropKey dk{};
   if constexpr (DROP) dk = load_key(drop.key);
-  auto multiply = [&](int64_t m0, int buf) {
+  // DROP: the four lanes of a group of eight columns make one row's words each, and a
+  // 4x4 transpose over them gives each lane its word of every row; those of the next
+  // 16 rows among the products of these.
+  uint32_t kept[2][4];
+  auto masks = [&](int64_t m0, int buf) {
+    const int i = lane & 3;
     uint32_t w[4];
-    if constexpr (DROP) {
-      // The four lanes of a group of eight columns make one row's words each,
-      // and a 4x4 transpose over them gives each lane its word of every row.
-      const int i = lane & 3;
-      philox(dk, (uint32_t)(c0 >> 3), (uint32_t)(row0 + m0 + first + 2 * i), w);
-      quad_transpose(w, i);
-    }
+    philox(dk, (uint32_t)(c0 >> 3), (uint32_t)(row0 + m0 + first + 2 * i), w);
+    quad_transpose(w, i);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) kept[buf][q] = keep_mask(w[q], drop.threshold);
+  };
+  auto multiply = [&](int64_t m0, int buf) {
+    if constexpr (DROP) masks(m0 + 16, buf ^ 1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const bool ok = m0 + first + 2 * q < rows;
       uint32_t xq = ok && live ? x[buf][q] : 0;
-      if constexpr (DROP) xq &= keep_mask(w[q], drop.threshold);
+      if constexpr (DROP) xq &= kept[buf][q];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float a = widen1<TT, SCALE>(xq, i == 1, s);
@@ -487,6 +501,7 @@ __global__ __launch_bounds__(LR_NT) void lora_wgrad_kernel(const uint16_t* __res
     }
   };
   if (rows > 0) load(0, 0);
+  if constexpr (DROP) masks(0, 0);
   for (int64_t m0 = 0; m0 < rows; m0 += 32) {
     if (m0 + 16 < rows) load(m0 + 16, 1);
     __builtin_amdgcn_sched_barrier(0);
