@@ -39,12 +39,13 @@ def threshold_of(p: float) -> int:
     return int(p) * 65536 if p in (0.0, 1.0) else min(max(round(p * 65536), 1), 65535)
 
 
-def factors(rows: int, cols: int, p: float, key) -> torch.Tensor:
-    """fp64 [rows, cols]: 0, or the inverse of the kept share."""
+def factors(rows: int, cols: int, p: float, key, first_row: int = 0) -> torch.Tensor:
+    """fp64 [rows, cols]: 0, or the inverse of the kept share (rows first_row ...)."""
     seed, offset = (int(v) % (1 << 64) for v in key.tolist())
     groups = (cols + 7) // 8
     c0 = np.broadcast_to(np.arange(groups, dtype=np.uint64), (rows, groups))
-    c1 = np.broadcast_to(np.arange(rows, dtype=np.uint64)[:, None], (rows, groups))
+    c1 = np.broadcast_to(np.arange(first_row, first_row + rows, dtype=np.uint64)[:, None],
+                         (rows, groups))
     words = philox4x32((c0, c1, np.full_like(c0, offset & 0xFFFFFFFF), np.full_like(c0, offset >> 32)),
                        (seed & 0xFFFFFFFF, seed >> 32))
     bits = np.empty((rows, groups, 8), dtype=np.int64)

@@ -336,9 +336,43 @@ def test_parts_of_the_gradient(hip_ops):
         torch.autograd.grad(g.sum(), full[0])
 
 
+def test_offsets_past_32_bits(hip_ops):
+    """Tensors of more than 2^31 elements and 4 GiB: the last rows of the output and of
+    the gradients are those of a call on these rows alone, and the weight's gradient, whose
+    operand no 32-bit offset spans, is the sum over slices of the rows."""
+    T, K, N, last = 72000, 64, 32768, 200
+    x, w = make((T, K), 1, BF), make((N, K), 2, BF, 0.1)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    dy = torch.empty((T, N), dtype=BF, device=DEV).normal_(generator=g)
+    s = torch.rand((T, 1), generator=g, device=DEV).to(BF)
+    leaves = [t.requires_grad_() for t in (x, w, s)]
+    y = hip_ops.linear_residual(x, w, None, dy, s)
+    dx, dw, ds = torch.autograd.grad(y, leaves, dy)
+    part = [x[-last:].detach().requires_grad_(), w, s[-last:].detach().requires_grad_()]
+    yp = hip_ops.linear_residual(part[0], w, None, dy[-last:], part[2])
+    dxp, dsp = torch.autograd.grad(yp, [part[0], part[2]], dy[-last:])
+    # The same roundings to 16 bits at the end of fp32 sums of at most N products.
+    for a, b in ((y[-last:], yp), (dx[-last:], dxp), (ds[-last:], dsp)):
+        assert (a.double() - b.double()).norm() <= 2 * unit(BF) * b.double().norm()
+    want = torch.zeros((N, K), dtype=torch.float64, device=DEV)
+    for at in range(0, T, 9000):
+        rows = (s[at:at + 9000].float() * x[at:at + 9000].float()).to(BF).detach()
+        want += (dy[at:at + 9000].float().t() @ rows.float()).double()
+    assert (dw.double() - want).norm() <= 2 * unit(BF) * want.norm()
+
+
 # ---------------------------------------------------------------------------
 # Dropout
 # ---------------------------------------------------------------------------
+def test_dropout_past_32_bits(hip_ops):
+    rows, cols = 1 << 20, 4104
+    x = torch.ones((rows, cols), dtype=BF, device=DEV)
+    key = torch.tensor([77, 78], device=DEV)
+    y = hip_ops.dropout(x, 0.5, key)
+    f = o_dropout.factors(3, cols, 0.5, key.cpu(), rows - 3)
+    assert torch.equal(y[-3:].double().cpu(), f)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
 @pytest.mark.parametrize("shape", [(1, 1), (3, 7), (5, 8), (9,), (130, 1024), (2, 4104), (3, 5, 13),
                                    (70000, 3), (2, 3, 4, 2056)])

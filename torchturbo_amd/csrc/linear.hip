@@ -202,7 +202,7 @@ bool fast_sizes(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R
   const bool a_ok = layout == LAY_TN ? I % 8 == 0 : R % 8 == 0;
   const bool b_ok = layout == LAY_NT ? R % 8 == 0 : J % 8 == 0;
   if (!a_ok || !b_ok || J % 8 != 0 || R == 0) return false;
-  const int64_t row = 2 * std::max(std::max(I, J), R);
+  const int64_t row = 2 * std::max(J, layout == LAY_TN ? I : R);  // of an operand or of C
   return row * 256 < (1ll << 31) && (kind != LIN_GATED || (J + 256) * R * 2 < (1ll << 31));
 }
 

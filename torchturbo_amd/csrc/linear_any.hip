@@ -6,7 +6,7 @@
 
 namespace {
 
-constexpr int A_NT = 256, A_BK = 16;
+constexpr int A_NT = 256, A_CHAIN = 512;
 
 // One block computes BT x BT of C (GATED: BT / 2 outputs, the tile's columns
 // being a gate's and its up's in runs of 32), each of the four waves a quarter.
@@ -16,6 +16,7 @@ template <int LAYOUT, int KIND, class TT, int BT>
 __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j, int vec) {
   typedef typename TT::storage St;
   constexpr bool A_K = LAYOUT != LAY_TN, B_K = LAYOUT == LAY_NT;
+  constexpr int A_BK = BT == 64 ? 32 : 16;   // small tiles wait for memory more than they multiply
   constexpr bool GATED = KIND == LIN_GATED;
   constexpr int F = BT / 64;                 // 32x32 blocks of a wave, each way
   constexpr int PER = BT * A_BK / A_NT;      // elements of an operand per thread and k-tile
@@ -111,7 +112,9 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
       else sb[buf][bk][br + e] = TT::to_f32(vb[e]);
     }
   };
-  f32x16 acc[F][F] = {};
+  // One chain of products is at most A_CHAIN long: a longer reduction adds chains, whose
+  // rounding grows with their number instead of its length.
+  f32x16 acc[F][F] = {}, total[F][F] = {};
   if (r0 < r1) {
     fetch(r0);
     put(0);
@@ -134,6 +137,15 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
             acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[n], fa[m], acc[m][n], 0, 0, 0);
       }
       if (more) put(buf ^ 1);
+      if (!more || (k0 - r0) % A_CHAIN == A_CHAIN - A_BK) {
+#pragma unroll
+        for (int m = 0; m < F; ++m)
+#pragma unroll
+          for (int n = 0; n < F; ++n) {
+            total[m][n] += acc[m][n];
+            acc[m][n] = f32x16{};
+          }
+      }
       __syncthreads();
       buf ^= 1;
     }
@@ -160,8 +172,8 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
         float v[4], u[4] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[e] = acc[m][n][4 * g + e];
-          if constexpr (GATED) u[e] = F == 1 ? acc[m][0][4 * ((g + 2) & 3) + e] : acc[m][(n + F / 2) % F][4 * g + e];
+          v[e] = total[m][n][4 * g + e];
+          if constexpr (GATED) u[e] = F == 1 ? total[m][0][4 * ((g + 2) & 3) + e] : total[m][(n + F / 2) % F][4 * g + e];
         }
         if (p.part != nullptr) {
           float* o = p.part + ((int64_t)blockIdx.y * p.I + i) * width + j;

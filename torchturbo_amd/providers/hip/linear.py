@@ -136,18 +136,18 @@ class LinearResidual(torch.autograd.Function):
 
 def _operands(op, x, weight, bias):
     """Checks shared by both products."""
-    if x.dim() < 1 or weight.dim() != 2:
+    dtype, w_shape, features = x.dtype, weight.shape, x.shape[-1] if x.dim() else -1
+    if features < 0 or len(w_shape) != 2:
         raise ValueError(f"{op} expects x [..., in] and weight [out, in]")
-    if x.dtype not in FLOATS or weight.dtype != x.dtype:
-        raise ValueError(f"{op}: x and weight must both be f32, bf16 or f16, got {x.dtype} and "
+    if dtype not in FLOATS or weight.dtype is not dtype:
+        raise ValueError(f"{op}: x and weight must both be f32, bf16 or f16, got {dtype} and "
                          f"{weight.dtype}")
-    if weight.shape[1] != x.shape[-1]:
-        raise ValueError(f"{op}: x has {x.shape[-1]} features, weight expects {weight.shape[1]}")
-    rows = weight.shape[0]
-    if bias is not None and (bias.dtype not in FLOATS or bias.shape != (rows,)):
-        raise ValueError(f"{op}: the bias must be a float tensor of shape [{rows}], got "
+    if w_shape[1] != features:
+        raise ValueError(f"{op}: x has {features} features, weight expects {w_shape[1]}")
+    if bias is not None and (bias.dtype not in FLOATS or bias.shape != w_shape[:1]):
+        raise ValueError(f"{op}: the bias must be a float tensor of shape [{w_shape[0]}], got "
                          f"{bias.dtype} {list(bias.shape)}")
-    if x.numel() // max(x.shape[-1], 1) >= 1 << 31:
+    if x.numel() >= (1 << 31) * max(features, 1):
         raise ValueError(f"{op} takes fewer than 2^31 rows")
 
 
