@@ -78,7 +78,8 @@ __device__ __forceinline__ void lin_act_grad(int act, float a, float& value, flo
   }
 }
 
-// W consecutive elements at p[at], widened; n of them exist (VEC: all, aligned).
+// W consecutive elements at p[at], widened; n of them exist (VEC: all, aligned; the
+// memory instructions take any address, and an aligned one is one line less).
 template <class TT, int W, bool VEC>
 __device__ __forceinline__ void lin_load(const void* p, int64_t at, int n, float (&o)[W]) {
   typedef typename TT::storage St;
@@ -86,6 +87,11 @@ __device__ __forceinline__ void lin_load(const void* p, int64_t at, int n, float
   if constexpr (VEC) {
     St v[W];
     __builtin_memcpy(v, __builtin_assume_aligned(q, sizeof(St) * W < 16 ? sizeof(St) * W : 16), sizeof(v));
+#pragma unroll
+    for (int j = 0; j < W; ++j) o[j] = TT::to_f32(v[j]);
+  } else if (n == W) {
+    St v[W];
+    __builtin_memcpy(v, q, sizeof(v));
 #pragma unroll
     for (int j = 0; j < W; ++j) o[j] = TT::to_f32(v[j]);
   } else {
@@ -97,18 +103,18 @@ template <class TT, int W, bool VEC>
 __device__ __forceinline__ void lin_store(void* p, int64_t at, int n, const float (&v)[W]) {
   typedef typename TT::storage St;
   St* q = static_cast<St*>(p) + at;
-  if constexpr (VEC && sizeof(St) == 2) {
-    uint2 o[W / 4];
+  if (VEC || n == W) {
+    constexpr int AT = VEC ? (sizeof(St) * W < 16 ? sizeof(St) * W : 16) : sizeof(St);
+    if constexpr (sizeof(St) == 2) {
+      uint2 o[W / 4];
 #pragma unroll
-    for (int q = 0; q < W / 4; ++q)
-      o[q] = pack4<__is_same(TT, BF16T) ? TT_BF16 : TT_F16>(v[4 * q], v[4 * q + 1], v[4 * q + 2],
-                                                            v[4 * q + 3]);
-    __builtin_memcpy(__builtin_assume_aligned(q, W * 2), o, sizeof(o));
-  } else if constexpr (VEC) {
-    St o[W];
-#pragma unroll
-    for (int j = 0; j < W; ++j) o[j] = TT::from_f32(v[j]);
-    __builtin_memcpy(__builtin_assume_aligned(q, 16), o, sizeof(o));
+      for (int e = 0; e < W / 4; ++e)
+        o[e] = pack4<__is_same(TT, BF16T) ? TT_BF16 : TT_F16>(v[4 * e], v[4 * e + 1], v[4 * e + 2],
+                                                              v[4 * e + 3]);
+      __builtin_memcpy(__builtin_assume_aligned(q, AT), o, sizeof(o));
+    } else {
+      __builtin_memcpy(__builtin_assume_aligned(q, AT), v, sizeof(v));
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < W; ++j)
@@ -166,6 +172,8 @@ __device__ __forceinline__ LinRow<TT, W> lin_row(const LinArgs& p, int64_t i, in
       if constexpr (VEC) {
         __builtin_memcpy(r.v, __builtin_assume_aligned(q, sizeof(St) * W < 16 ? sizeof(St) * W : 16),
                          sizeof(r.v));
+      } else if (n == W) {
+        __builtin_memcpy(r.v, q, sizeof(r.v));
       } else {
 #pragma unroll
         for (int e = 0; e < W; ++e)
@@ -242,13 +250,15 @@ __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t
 // TN: A [R, I], B [R, J].
 enum { LAY_NT = 0, LAY_NN = 1, LAY_TN = 2 };
 
-// The kernels: for any type, for few rows, and tiles of the 16-bit matrix instructions.
-enum { LIN_ANY = 0, LIN_ROWS = 1, LIN_T64 = 2, LIN_T128 = 3, LIN_T256x128 = 4, LIN_T256 = 5 };
+// The kernels: fp32, few rows, tiles of the 16-bit matrix instructions, and tiles for any
+// alignment.
+enum { LIN_F32 = 0, LIN_ROWS = 1, LIN_T64 = 2, LIN_T128 = 3, LIN_T256x128 = 4, LIN_T256 = 5,
+       LIN_ODD64 = 6, LIN_ODD128 = 7 };
 
-// fp32 matrix instructions on any type, size and alignment (linear_any.hip).
-int tt_linear_any(int kind, int dtype, const LinArgs& a, hipStream_t s);
+// fp32 tensors of any size and alignment (linear_f32.hip).
+int tt_linear_f32(int kind, const LinArgs& a, hipStream_t s);
 // 16-bit matrix instructions on tiles (LIN_T64 ...), for aligned rows of whole 16-byte
-// vectors (linear_tile.hip).
+// vectors, or (LIN_ODD64, LIN_ODD128) for any (linear_tile.hip).
 int tt_linear_tile(int kind, int tile, int dtype, const LinArgs& a, hipStream_t s);
-// The same for at most 64 rows of x and NT operands under 2 GiB (linear_thin.hip).
-int tt_linear_thin(int kind, int dtype, const LinArgs& a, hipStream_t s);
+// The same for at most 64 rows of x and NT operands under 2 GiB (linear_rows.hip).
+int tt_linear_rows(int kind, int dtype, const LinArgs& a, hipStream_t s);

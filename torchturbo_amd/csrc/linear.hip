@@ -155,13 +155,22 @@ double rows_us(int64_t blocks, int64_t I, int64_t J, int64_t R) {
   return 1.5 + work * std::max(1.0, 256.0 / (double)blocks);
 }
 
-Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, bool fast) {
+// `how` of a product: 16-bit on the tiles (FAST) or on those for any alignment (ODD), or fp32.
+enum { HOW_F32 = 0, HOW_ODD = 1, HOW_FAST = 2 };
+
+Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, int how) {
   const int64_t half = kind == LIN_GATED ? 2 : 1, width = half * J;
   auto tiles = [&](int64_t bm, int64_t bn) { return ((I + bm - 1) / bm) * ((width + bn - 1) / bn); };
-  if (!fast) {
+  if (how == HOW_ODD) {
+    // 128-wide tiles where they fill the CUs, else 64-wide ones, split as below.
+    const bool big = tiles(128, 128) >= 256;
+    const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64, 64), 1), R / 512);
+    return Plan{big ? LIN_ODD128 : LIN_ODD64, split_of(R, big ? 1 : std::min<int64_t>(want, 8))};
+  }
+  if (how == HOW_F32) {
     // Enough blocks for the CUs, each reduction at least 256 long.
     const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64, 64), 1), R / 256);
-    return Plan{LIN_ANY, split_of(R, std::min<int64_t>(want, 32))};
+    return Plan{LIN_F32, split_of(R, std::min<int64_t>(want, 32))};
   }
   const int64_t least = least_splits(layout, I, J, R);
   Plan best{LIN_T256, split_of(R, least)};
@@ -194,34 +203,39 @@ size_t dots_bytes(int64_t I, int64_t J) {
   return (((size_t)I * ((J + LIN_DOT - 1) / LIN_DOT) * 4) + 255) / 256 * 256;
 }
 
-// Whether the sizes of a product fit the 16-bit tiles: rows of whole 16-byte
-// vectors, and tiles within reach of a 32-bit offset (a gated tile's columns lie
-// half the weight apart).
-bool fast_sizes(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R) {
-  if (dtype != TT_BF16 && dtype != TT_F16) return false;
+// How the sizes of a product may run: the 16-bit tiles want rows of whole 16-byte
+// vectors and tiles within reach of a 32-bit offset (a gated tile's columns lie half
+// the weight apart); those for any alignment have 64-bit addresses.
+int how_sizes(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R) {
+  if (dtype == TT_F32) return HOW_F32;
+  if (R == 0) return HOW_ODD;
   const bool a_ok = layout == LAY_TN ? I % 8 == 0 : R % 8 == 0;
   const bool b_ok = layout == LAY_NT ? R % 8 == 0 : J % 8 == 0;
-  if (!a_ok || !b_ok || J % 8 != 0 || R == 0) return false;
+  if (!a_ok || !b_ok || J % 8 != 0) return HOW_ODD;
   const int64_t row = 2 * std::max(J, layout == LAY_TN ? I : R);  // of an operand or of C
-  return row * 256 < (1ll << 31) && (kind != LIN_GATED || (J + 256) * R * 2 < (1ll << 31));
+  const bool near = row * 256 < (1ll << 31) &&
+                    (kind != LIN_GATED || (J + 256) * R * 2 < (1ll << 31));
+  return near ? HOW_FAST : HOW_ODD;
 }
 
 int run_product(int layout, int kind, int dtype, LinArgs p, void* ws, size_t ws_bytes,
                 hipStream_t s) {
-  const bool fast = vectors(p) && fast_sizes(layout, kind, dtype, p.I, p.J, p.R);
-  Plan pl = plan_of(layout, kind, p.I, p.J, p.R, fast);
+  int how = how_sizes(layout, kind, dtype, p.I, p.J, p.R);
+  if (how == HOW_FAST && !vectors(p)) how = HOW_ODD;
+  Plan pl = plan_of(layout, kind, p.I, p.J, p.R, how);
   if (part_bytes(kind, p.I, p.J, pl.split.splits) > ws_bytes) {
-    // Without room for the parts: a whole reduction, on the kernel for any size where
-    // the tiles cannot walk it.
-    pl = Plan{fast && least_splits(layout, p.I, p.J, p.R) == 1 ? pl.kernel : LIN_ANY,
-              split_of(p.R, 1)};
+    // Without room for the parts: a whole reduction, on the kernel for any alignment
+    // where the tiles cannot walk it.
+    if (how == HOW_FAST && least_splits(layout, p.I, p.J, p.R) > 1)
+      pl = plan_of(layout, kind, p.I, p.J, p.R, HOW_ODD);
+    pl.split = split_of(p.R, 1);
   }
   const Split sp = pl.split;
   p.splits = sp.splits;
   p.rsplit = sp.run;
   p.part = sp.splits > 1 ? static_cast<float*>(ws) : nullptr;
-  const int rc = pl.kernel == LIN_ANY    ? tt_linear_any(kind, dtype, p, s)
-                 : pl.kernel == LIN_ROWS ? tt_linear_thin(kind, dtype, p, s)
+  const int rc = pl.kernel == LIN_F32    ? tt_linear_f32(kind, p, s)
+                 : pl.kernel == LIN_ROWS ? tt_linear_rows(kind, dtype, p, s)
                                          : tt_linear_tile(kind, pl.kernel, dtype, p, s);
   if (rc != TT_OK || p.part == nullptr) return rc;
   switch (dtype) {
@@ -437,10 +451,10 @@ bool all_aligned(std::initializer_list<const void*> ps) {
 // Bytes of the parts of a product, for the larger of its two plans: which one runs also
 // depends on the addresses.
 size_t parts_of(int layout, int kind, int dtype, int64_t I, int64_t J, int64_t R) {
-  const int64_t any = plan_of(layout, kind, I, J, R, false).split.splits;
-  const int64_t fast = fast_sizes(layout, kind, dtype, I, J, R)
-                           ? plan_of(layout, kind, I, J, R, true).split.splits : 1;
-  return part_bytes(kind, I, J, std::max(any, fast));
+  const int how = how_sizes(layout, kind, dtype, I, J, R);
+  int64_t splits = plan_of(layout, kind, I, J, R, how).split.splits;
+  if (how == HOW_FAST) splits = std::max<int64_t>(splits, plan_of(layout, kind, I, J, R, HOW_ODD).split.splits);
+  return part_bytes(kind, I, J, splits);
 }
 size_t round256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 

@@ -1,7 +1,5 @@
-// Dense product with an epilogue for every type, size and alignment (gfx950):
-// fp32 tensors, and 16-bit ones whose rows do not split into aligned 16-byte
-// vectors. Products and sums run in fp32 on v_mfma_f32_32x32x2_f32 (16-bit
-// operands widen exactly).
+// Dense product with an epilogue of fp32 tensors, any size and alignment (gfx950).
+// Products and sums run in fp32 on v_mfma_f32_32x32x2_f32.
 #include "linear.h"
 
 namespace {
@@ -12,9 +10,8 @@ constexpr int A_NT = 256, A_CHAIN = 512;
 // being a gate's and its up's in runs of 32), each of the four waves a quarter.
 // The next k-tile is loaded into registers while one is multiplied from LDS
 // (k-row-major, so that a fragment is 32 consecutive floats).
-template <int LAYOUT, int KIND, class TT, int BT>
-__global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j, int vec) {
-  typedef typename TT::storage St;
+template <int LAYOUT, int KIND, int BT>
+__global__ __launch_bounds__(A_NT) void linear_f32_kernel(LinArgs p, int tiles_j, int vec) {
   constexpr bool A_K = LAYOUT != LAY_TN, B_K = LAYOUT == LAY_NT;
   constexpr int A_BK = BT == 64 ? 32 : 16;   // small tiles wait for memory more than they multiply
   constexpr bool GATED = KIND == LIN_GATED;
@@ -29,8 +26,8 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
   const int64_t i0 = (int64_t)(blockIdx.x / tiles_j) * BT, j0 = (int64_t)(blockIdx.x % tiles_j) * BO;
   const int64_t r0 = (int64_t)blockIdx.y * p.rsplit;
   const int64_t r1 = r0 + p.rsplit < p.R ? r0 + p.rsplit : p.R;
-  const St* A = static_cast<const St*>(p.a);
-  const St* B = static_cast<const St*>(p.b);
+  const float* A = static_cast<const float*>(p.a);
+  const float* B = static_cast<const float*>(p.b);
   // Column of B that tile column c is, or -1. GATED (F of 32 columns per wave):
   // a wave's first half are gates, its second half their ups.
   auto bcol = [&](int c) -> int64_t {
@@ -50,66 +47,66 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
   const int br = B_K ? threadIdx.x / KT : (threadIdx.x % (BT / PER)) * PER;
   const int bk = B_K ? (threadIdx.x % KT) * PER : threadIdx.x / (BT / PER);
   const int64_t brow = bcol(br);
-  St va[PER], vb[PER];
+  float va[PER], vb[PER];
   auto fetch = [&](int64_t k0) {
     if constexpr (A_K) {
       const int64_t i = i0 + ar, k = k0 + ak;
-      const St* src = A + i * p.lda + k;
+      const float* src = A + i * p.lda + k;
       if (i >= p.I) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = St(0);
-      } else if (vec && k + PER <= r1) {
-        __builtin_memcpy(va, __builtin_assume_aligned(src, sizeof(St) * PER < 16 ? sizeof(St) * PER : 16), sizeof(va));
+        for (int e = 0; e < PER; ++e) va[e] = 0.f;
+      } else if (k + PER <= r1) {
+        __builtin_memcpy(va, src, sizeof(va));
       } else {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = k + e < r1 ? src[e] : St(0);
+        for (int e = 0; e < PER; ++e) va[e] = k + e < r1 ? src[e] : 0.f;
       }
     } else {
       const int64_t i = i0 + ar, k = k0 + ak;
-      const St* src = A + k * p.lda + i;
+      const float* src = A + k * p.lda + i;
       if (k >= r1) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = St(0);
-      } else if (vec && i + PER <= p.I) {
-        __builtin_memcpy(va, __builtin_assume_aligned(src, sizeof(St) * PER < 16 ? sizeof(St) * PER : 16), sizeof(va));
+        for (int e = 0; e < PER; ++e) va[e] = 0.f;
+      } else if (i + PER <= p.I) {
+        __builtin_memcpy(va, src, sizeof(va));
       } else {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = i + e < p.I ? src[e] : St(0);
+        for (int e = 0; e < PER; ++e) va[e] = i + e < p.I ? src[e] : 0.f;
       }
     }
     if constexpr (B_K) {
       const int64_t k = k0 + bk;
-      const St* src = B + brow * p.ldb + k;
+      const float* src = B + brow * p.ldb + k;
       if (brow < 0) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = St(0);
-      } else if (vec && k + PER <= r1) {
-        __builtin_memcpy(vb, __builtin_assume_aligned(src, sizeof(St) * PER < 16 ? sizeof(St) * PER : 16), sizeof(vb));
+        for (int e = 0; e < PER; ++e) vb[e] = 0.f;
+      } else if (k + PER <= r1) {
+        __builtin_memcpy(vb, src, sizeof(vb));
       } else {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = k + e < r1 ? src[e] : St(0);
+        for (int e = 0; e < PER; ++e) vb[e] = k + e < r1 ? src[e] : 0.f;
       }
     } else {
       const int64_t j = j0 + br, k = k0 + bk;
-      const St* src = B + k * p.ldb + j;
+      const float* src = B + k * p.ldb + j;
       if (k >= r1) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = St(0);
-      } else if (vec && j + PER <= p.J) {
-        __builtin_memcpy(vb, __builtin_assume_aligned(src, sizeof(St) * PER < 16 ? sizeof(St) * PER : 16), sizeof(vb));
+        for (int e = 0; e < PER; ++e) vb[e] = 0.f;
+      } else if (j + PER <= p.J) {
+        __builtin_memcpy(vb, src, sizeof(vb));
       } else {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = j + e < p.J ? src[e] : St(0);
+        for (int e = 0; e < PER; ++e) vb[e] = j + e < p.J ? src[e] : 0.f;
       }
     }
   };
   auto put = [&](int buf) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      if constexpr (A_K) sa[buf][ak + e][ar] = TT::to_f32(va[e]);
-      else sa[buf][ak][ar + e] = TT::to_f32(va[e]);
-      if constexpr (B_K) sb[buf][bk + e][br] = TT::to_f32(vb[e]);
-      else sb[buf][bk][br + e] = TT::to_f32(vb[e]);
+      if constexpr (A_K) sa[buf][ak + e][ar] = va[e];
+      else sa[buf][ak][ar + e] = va[e];
+      if constexpr (B_K) sb[buf][bk + e][br] = vb[e];
+      else sb[buf][bk][br + e] = vb[e];
     }
   };
   // One chain of products is at most A_CHAIN long: a longer reduction adds chains, whose
@@ -181,12 +178,12 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
             o[e] = v[e];
             if (GATED) o[p.J + e] = u[e];
           }
-        } else if (vec && p.J % 4 == 0) {
-          dots[n] += lin_finish<KIND, TT, 4, true>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
-                                             lin_row<KIND, TT, 4, true>(p, i, j, left));
+        } else if (p.J % 4 == 0) {
+          dots[n] += lin_finish<KIND, F32T, 4, true>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
+                                             lin_row<KIND, F32T, 4, true>(p, i, j, left));
         } else {
-          dots[n] += lin_finish<KIND, TT, 4, false>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
-                                             lin_row<KIND, TT, 4, false>(p, i, j, left));
+          dots[n] += lin_finish<KIND, F32T, 4, false>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
+                                             lin_row<KIND, F32T, 4, false>(p, i, j, left));
         }
       }
     if constexpr (KIND == LIN_DGRAD) {
@@ -204,49 +201,37 @@ __global__ __launch_bounds__(A_NT) void linear_any_kernel(LinArgs p, int tiles_j
   }
 }
 
-template <int LAYOUT, int KIND, class TT, int BT>
+template <int LAYOUT, int KIND, int BT>
 int launch(const LinArgs& p, hipStream_t s) {
   const int bo = KIND == LIN_GATED ? BT / 2 : BT;
   const int64_t ti = (p.I + BT - 1) / BT, tj = (p.J + bo - 1) / bo;
   TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
-  // Whole vectors of four (or eight 16-bit) elements, aligned.
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) |
-                       reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.res) |
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.res) |
                        reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.xs) |
                        reinterpret_cast<uintptr_t>(p.pre);
-  const int vec = at % 16 == 0 && p.lda % 8 == 0 && p.ldb % 8 == 0 && p.J % 8 == 0;
-  hipLaunchKernelGGL((linear_any_kernel<LAYOUT, KIND, TT, BT>),
+  hipLaunchKernelGGL((linear_f32_kernel<LAYOUT, KIND, BT>),
                      dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(A_NT), 0, s, p, (int)tj,
-                     vec);
-  return tt_check_launch("linear");
-}
-
-template <int LAYOUT, int KIND, class TT>
-int sized(const LinArgs& p, hipStream_t s) {
-  // 64-wide tiles while 128-wide ones leave CUs without a block.
-  const int64_t tiles = ((p.I + 127) / 128) * ((p.J + 127) / 128) * p.splits;
-  if (tiles >= 256) return launch<LAYOUT, KIND, TT, 128>(p, s);
-  return launch<LAYOUT, KIND, TT, 64>(p, s);
+                     (int)(at % 16 == 0 && p.J % 4 == 0));
+  return tt_check_launch("linear_f32");
 }
 
 template <int LAYOUT, int KIND>
-int typed(int dtype, const LinArgs& p, hipStream_t s) {
-  switch (dtype) {
-    case TT_BF16: return sized<LAYOUT, KIND, BF16T>(p, s);
-    case TT_F16: return sized<LAYOUT, KIND, F16T>(p, s);
-    default: return sized<LAYOUT, KIND, F32T>(p, s);
-  }
+int sized(const LinArgs& p, hipStream_t s) {
+  // 64-wide tiles while 128-wide ones leave CUs without a block.
+  const int64_t width = KIND == LIN_GATED ? 2 * p.J : p.J;
+  const int64_t tiles = ((p.I + 127) / 128) * ((width + 127) / 128) * p.splits;
+  return tiles >= 256 ? launch<LAYOUT, KIND, 128>(p, s) : launch<LAYOUT, KIND, 64>(p, s);
 }
 
 }  // namespace
 
-int tt_linear_any(int kind, int dtype, const LinArgs& p, hipStream_t s) {
+int tt_linear_f32(int kind, const LinArgs& p, hipStream_t s) {
   switch (kind) {
-    case LIN_ACT: return typed<LAY_NT, LIN_ACT>(dtype, p, s);
-    case LIN_GATED: return typed<LAY_NT, LIN_GATED>(dtype, p, s);
-    case LIN_RES: return typed<LAY_NT, LIN_RES>(dtype, p, s);
-    case LIN_DROP: return typed<LAY_NT, LIN_DROP>(dtype, p, s);
-    case LIN_DGRAD: return typed<LAY_NN, LIN_DGRAD>(dtype, p, s);
-    default: return typed<LAY_TN, LIN_PLAIN>(dtype, p, s);
+    case LIN_ACT: return sized<LAY_NT, LIN_ACT>(p, s);
+    case LIN_GATED: return sized<LAY_NT, LIN_GATED>(p, s);
+    case LIN_RES: return sized<LAY_NT, LIN_RES>(p, s);
+    case LIN_DROP: return sized<LAY_NT, LIN_DROP>(p, s);
+    case LIN_DGRAD: return sized<LAY_NN, LIN_DGRAD>(p, s);
+    default: return sized<LAY_TN, LIN_PLAIN>(p, s);
   }
 }

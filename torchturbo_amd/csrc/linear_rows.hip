@@ -27,7 +27,7 @@ __device__ __forceinline__ f32x4_t mma16(const u32x4& a, const u32x4& b, const f
 }
 
 template <int KIND, class TT, int MB, int NB, int U>
-__global__ __launch_bounds__(N_NT) void linear_thin_kernel(LinArgs p) {
+__global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
   constexpr bool GATED = KIND == LIN_GATED;
   constexpr int ET = sizeof(typename TT::storage) == 2 && __is_same(TT, BF16T) ? TT_BF16 : TT_F16;
   constexpr int CB = GATED ? 8 * NB : 16 * NB;  // output columns of a block
@@ -127,9 +127,9 @@ int launch(const LinArgs& p, hipStream_t s) {
   constexpr int CB = KIND == LIN_GATED ? 8 * NB : 16 * NB;
   const int64_t blocks = (p.J + CB - 1) / CB;
   TT_REQUIRE(blocks < 0x7fffffff, "linear: grid too large");
-  hipLaunchKernelGGL((linear_thin_kernel<KIND, TT, MB, NB, U>), dim3((unsigned)blocks), dim3(N_NT),
+  hipLaunchKernelGGL((linear_rows_kernel<KIND, TT, MB, NB, U>), dim3((unsigned)blocks), dim3(N_NT),
                      0, s, p);
-  return tt_check_launch("linear_thin");
+  return tt_check_launch("linear_rows");
 }
 
 template <int KIND, class TT>
@@ -146,7 +146,7 @@ int typed(int dtype, const LinArgs& p, hipStream_t s) {
 
 }  // namespace
 
-int tt_linear_thin(int kind, int dtype, const LinArgs& p, hipStream_t s) {
+int tt_linear_rows(int kind, int dtype, const LinArgs& p, hipStream_t s) {
   switch (kind) {
     case LIN_ACT: return typed<LIN_ACT>(dtype, p, s);
     case LIN_GATED: return typed<LIN_GATED>(dtype, p, s);

@@ -642,6 +642,155 @@ __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int
                                 t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
 
+// Tiles of operands whose rows do not start at multiples of 16 bytes, or end inside a
+// vector: BT x BT as in linear_mid_kernel, but a k-tile goes through registers (loads
+// of 16 bytes at any address, single elements at a row's end, zeros past it) into
+// the same LDS layouts, two stages; and results are stored the same way. 777 x 515 ->
+// 1001, with dropout, forward and backward XX us; on the fp32 instructions YY.
+template <int LAYOUT, int KIND, int ET, int BT>
+__global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int tj) {
+  typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;
+  typedef typename TypeOf<ET>::type TT;
+  constexpr bool GATED = KIND == LIN_GATED;
+  constexpr int FM = BT / 64, FN = BT / 64;
+  constexpr int LA = TL::OpA::LOADS, LB = TL::OpB::LOADS;
+  __shared__ __align__(16) char lds_raw[2 * TL::STAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  TL t;
+  t.setup(p, ti, tj, wave, lane);
+  lds_char* const lds = (lds_char*)lds_raw;
+  const int64_t r0 = (int64_t)blockIdx.y * p.rsplit;
+  // Chunk q of an operand: `rows` of it exist from the tile's first on (K-major rows, or
+  // MN-major columns), of which this lane takes row / chunk as Operand::setup lays out.
+  auto chunk = [&](const char* base, int64_t ld, int64_t rows, bool kmaj, bool gate, int br, int q,
+                   int kt) -> uint4 {
+    const int valid = t.kn - kt * T_BK;
+    int64_t at;
+    int n;
+    if (kmaj) {
+      const int r = (br / 4) * wave + 8 * q + (lane >> 3);
+      const int c = (lane & 7) ^ ((r >> 1) & 7);
+      int64_t row = r, in = r;
+      if (gate) {
+        const int w = r / (br / 2), i = r % (br / 2);
+        in = w * (br / 4) + i % (br / 4);
+        row = (i / (br / 4)) * p.J + in;
+      }
+      at = row * ld + (int64_t)kt * T_BK + 8 * c;
+      n = in < rows ? valid - 8 * c : 0;
+    } else {
+      const int lpr = br / 8, kr = 16 * wave + (64 / lpr) * q + lane / lpr;
+      const int c = (lane % lpr) ^ (4 * (kr & 3) & (lpr - 1));
+      at = ((int64_t)kt * T_BK + kr) * ld + 8 * c;
+      n = kr < valid ? (int)(rows - 8 * c < 8 ? rows - 8 * c : 8) : 0;
+    }
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(base) + at;
+    uint4 v = {0, 0, 0, 0};
+    if (n >= 8) {
+      __builtin_memcpy(&v, src, 16);
+    } else if (n > 0) {
+      uint32_t w[4] = {};
+#pragma unroll
+      for (int e = 0; e < 7; ++e)
+        if (e < n) w[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
+      v = uint4{w[0], w[1], w[2], w[3]};
+    }
+    return v;
+  };
+  const char* const pa = static_cast<const char*>(p.a) +
+                         (TL::A_K ? t.i0 * p.lda + r0 : r0 * p.lda + t.i0) * 2;
+  const char* const pb = static_cast<const char*>(p.b) +
+                         (TL::B_K ? t.j0 * p.ldb + r0 : r0 * p.ldb + t.j0) * 2;
+  const int64_t ra = p.I - t.i0, rb = p.J - t.j0;
+  uint4 va[LA], vb[LB];
+  auto fetch = [&](int kt) {
+#pragma unroll
+    for (int q = 0; q < LA; ++q) va[q] = chunk(pa, p.lda, ra, TL::A_K, false, BT, q, kt);
+#pragma unroll
+    for (int q = 0; q < LB; ++q) vb[q] = chunk(pb, p.ldb, rb, TL::B_K, GATED, BT, q, kt);
+  };
+  auto put = [&](int slot) {
+    lds_char* const at = lds + slot * TL::STAGE + lane * 16;
+#pragma unroll
+    for (int q = 0; q < LA; ++q)
+      *reinterpret_cast<lds_u32x4*>(at + (LA * wave + q) * 1024) = __builtin_bit_cast(u32x4, va[q]);
+#pragma unroll
+    for (int q = 0; q < LB; ++q)
+      *reinterpret_cast<lds_u32x4*>(at + TL::OpA::BYTES + (LB * wave + q) * 1024) =
+          __builtin_bit_cast(u32x4, vb[q]);
+  };
+  f32x16 acc[FM][FN] = {};
+  if (t.nkt > 0) fetch(0);
+  for (int kt = 0; kt < t.nkt; ++kt) {
+    // The other stage is free: every wave passed the barrier of k-tile kt - 1 after it.
+    put(kt & 1);
+    TT_LDS_BARRIER();
+    if (kt + 1 < t.nkt) fetch(kt + 1);
+    lds_char* const stg = lds + (kt & 1) * TL::STAGE;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      uint4 fa[FM], fb[FN];
+#pragma unroll
+      for (int m = 0; m < FM; ++m) fa[m] = t.a.read(stg, m, s);
+#pragma unroll
+      for (int n = 0; n < FN; ++n) fb[n] = t.b.read(stg + TL::OpA::BYTES, n, s);
+#pragma unroll
+      for (int m = 0; m < FM; ++m)
+#pragma unroll
+        for (int n = 0; n < FN; ++n) acc[m][n] = Mma<ET>::run(fb[n], fa[m], acc[m][n]);
+    }
+  }
+  __syncthreads();
+  // 32 rows at a time through the wave's LDS, rows of W floats and four more.
+  constexpr int W = 32 * FN, LD = W + 4, OUT = GATED ? W / 2 : W, NG = OUT / 8;
+  static_assert(4 * 32 * LD * 4 <= 2 * TL::STAGE, "the waves' rows");
+  float* const region = reinterpret_cast<float*>(lds_raw) + wave * (32 * LD);
+  const int64_t iw = t.i0 + (wave >> 1) * (BT / 2), jw = t.j0 + (wave & 1) * OUT;
+  const int64_t width = GATED ? 2 * p.J : p.J;
+  DropKey dk{};
+  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
+#pragma unroll
+  for (int mi = 0; mi < FM; ++mi) {
+#pragma unroll
+    for (int ni = 0; ni < FN; ++ni)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          region[(lane & 31) * LD + 32 * ni + 8 * g + 4 * (lane >> 5) + e] = acc[mi][ni][4 * g + e];
+#pragma unroll 1
+    for (int it = lane; it < 32 * NG; it += 64) {
+      const int r = it / NG, gi = it % NG;
+      const int64_t i = iw + 32 * mi + r, j = jw + 8 * gi;
+      const bool live = i < p.I && j < p.J;
+      const int n = !live ? 0 : p.J - j < 8 ? (int)(p.J - j) : 8;
+      float v[8], u[8] = {}, dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = region[r * LD + 8 * gi + e];
+        if constexpr (GATED) u[e] = region[r * LD + OUT + 8 * gi + e];
+      }
+      if (live && p.part != nullptr) {
+        const int64_t at = ((int64_t)blockIdx.y * p.I + i) * width + j;
+        lin_store<F32T, 8, false>(p.part, at, n, v);
+        if constexpr (GATED) lin_store<F32T, 8, false>(p.part, at + p.J, n, u);
+      } else if (live) {
+        dot = lin_finish<KIND, TT, 8, false>(p, i, j, n, v, u, dk, lin_cols<KIND, 8>(p, j, n),
+                                             lin_row<KIND, TT, 8, false>(p, i, j, n));
+      }
+      if constexpr (KIND == LIN_DGRAD) {
+        if (p.dots != nullptr && p.part == nullptr) {
+          static_assert(NG % 4 == 0, "four lanes of a run in one row");
+          dot = sum4(dot);
+          if (live && (lane & 3) == 0)
+            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
+        }
+      }
+    }
+  }
+}
+
 template <int LAYOUT, int KIND, int ET, bool KMASK>
 int launch(int tile, const LinArgs& p, hipStream_t s) {
   const int bm = tile == LIN_T64 ? 64 : tile == LIN_T128 ? 128 : 256;
@@ -662,8 +811,25 @@ int launch(int tile, const LinArgs& p, hipStream_t s) {
   return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 2>);
 }
 
+template <int LAYOUT, int KIND, int ET, int BT>
+int launch_odd(const LinArgs& p, hipStream_t s) {
+  constexpr int BO = KIND == LIN_GATED ? BT / 2 : BT;
+  const int64_t ti = (p.I + BT - 1) / BT, tj = (p.J + BO - 1) / BO;
+  TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
+  hipLaunchKernelGGL((linear_odd_kernel<LAYOUT, KIND, ET, BT>),
+                     dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(T_NT), 0, s, p, (int)ti,
+                     (int)tj);
+  return tt_check_launch("linear_odd");
+}
+
 template <int LAYOUT, int KIND>
 int typed(int tile, int dtype, const LinArgs& p, hipStream_t s) {
+  if (tile == LIN_ODD64)
+    return dtype == TT_BF16 ? launch_odd<LAYOUT, KIND, TT_BF16, 64>(p, s)
+                            : launch_odd<LAYOUT, KIND, TT_F16, 64>(p, s);
+  if (tile == LIN_ODD128)
+    return dtype == TT_BF16 ? launch_odd<LAYOUT, KIND, TT_BF16, 128>(p, s)
+                            : launch_odd<LAYOUT, KIND, TT_F16, 128>(p, s);
   const bool mask = LAYOUT != LAY_TN && p.R % T_BK != 0;
   if (dtype == TT_BF16)
     return mask ? launch<LAYOUT, KIND, TT_BF16, LAYOUT != LAY_TN>(tile, p, s)
