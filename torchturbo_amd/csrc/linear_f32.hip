@@ -4,7 +4,7 @@
 
 namespace {
 
-constexpr int A_NT = 256, A_CHAIN = 512;
+constexpr int A_NT = 256, A_BK = 32, A_CHAIN = 512;
 
 // One block computes BT x BT of C (GATED: BT / 2 outputs, the tile's columns
 // being a gate's and its up's in runs of 32), each of the four waves a quarter.
@@ -13,7 +13,6 @@ constexpr int A_NT = 256, A_CHAIN = 512;
 template <int LAYOUT, int KIND, int BT>
 __global__ __launch_bounds__(A_NT) void linear_f32_kernel(LinArgs p, int tiles_j, int vec) {
   constexpr bool A_K = LAYOUT != LAY_TN, B_K = LAYOUT == LAY_NT;
-  constexpr int A_BK = BT == 64 ? 32 : 16;   // small tiles wait for memory more than they multiply
   constexpr bool GATED = KIND == LIN_GATED;
   constexpr int F = BT / 64;                 // 32x32 blocks of a wave, each way
   constexpr int PER = BT * A_BK / A_NT;      // elements of an operand per thread and k-tile

@@ -207,8 +207,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* m, int64
 // columns of 32 rows) nor the reads (a row's chunks) of eight lanes meet in a bank.
 // One wave per SIMD has nothing to hide instructions behind, so memory is reached
 // through resources with 32-bit offsets, conversions are the hardware's, and what a
-// row needs is fetched 32 rows ahead: 4096 x 4096 x 512 with a residual 48 -> XX us,
-// the gradient's form 73 -> XX.
+// row needs is fetched 32 rows ahead: 4096 x 4096 x 512 with a residual 48 -> 31 us,
+// the gradient with a row scale 73 -> 41.
 // stage(mi, put): calls put(row, chunk, four sums) for the lane's part of the 32 rows mi.
 template <int KIND, int ET, int FM, int FN, typename F>
 __device__ __forceinline__ void tile_finish(const LinArgs& p, F stage, lds_char* region, int64_t i0,
@@ -642,12 +642,94 @@ __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int
                                 t.j0 + (wave & 1) * (TL::BO / 2), lane);
 }
 
+// An operand of linear_odd_kernel, chunks laid out as Operand::setup does. A load is
+// always of 16 bytes, at an address moved back where they would pass the operand's
+// end, so that it never waits for another; the elements are put in place, and those past
+// a row's end cleared, when it has arrived.
+// TINY: an operand may have fewer than eight elements in all.
+template <bool KM, int BR, bool GATE, bool TINY>
+struct OddOperand {
+  static constexpr int LOADS = BR / 32;
+  const uint16_t* base;
+  int64_t last;        // the last element that 16 bytes can start at
+  int64_t off[LOADS];  // of the chunk in k-tile 0
+  int64_t step;        // elements of a k-tile
+  int at[LOADS];       // the chunk's place in the reduction
+  int most[LOADS];     // its elements that exist, by the other dimension
+  bool inside;         // every row of the tile exists
+
+  // rows x R elements (GATE: 2 x rows), from row `first` and reduction element r0 on.
+  __device__ __forceinline__ void setup(const uint16_t* p, int64_t ld, int64_t rows, int64_t R,
+                                        int64_t first, int64_t r0, int64_t half, int wave, int lane) {
+    base = p;
+    last = rows * R * (GATE ? 2 : 1) - 8;
+    step = KM ? T_BK : T_BK * ld;
+    inside = first + (GATE ? BR / 2 : BR) <= rows;
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) {
+      if constexpr (KM) {
+        const int r = (BR / 4) * wave + 8 * q + (lane >> 3), c = (lane & 7) ^ ((r >> 1) & 7);
+        int64_t row = r, in = r;
+        if constexpr (GATE) {
+          in = r / (BR / 2) * (BR / 4) + r % (BR / 2) % (BR / 4);
+          row = (r % (BR / 2) / (BR / 4)) * half + in;
+        }
+        off[q] = (first + row) * ld + r0 + 8 * c;
+        at[q] = 8 * c;
+        most[q] = first + in < rows ? 8 : 0;
+      } else {
+        constexpr int LPR = BR / 8;
+        const int kr = 16 * wave + (64 / LPR) * q + lane / LPR;
+        const int c = (lane % LPR) ^ (4 * (kr & 3) & (LPR - 1));
+        const int64_t left = rows - first - 8 * c;
+        off[q] = (r0 + kr) * ld + first + 8 * c;
+        at[q] = kr;
+        most[q] = left <= 0 ? 0 : left < 8 ? (int)left : 8;
+      }
+    }
+  }
+  __device__ __forceinline__ int64_t start(int q, int kt) const { return off[q] + kt * step; }
+  // Whether all of k-tile kt of kn elements exists.
+  __device__ __forceinline__ bool whole(int kt, int kn) const {
+    return inside && (kt + 1) * T_BK <= kn;
+  }
+  __device__ __forceinline__ uint4 load(int q, int kt) const {
+    const int64_t o = start(q, kt);
+    uint4 v;
+    if constexpr (!TINY) {
+      __builtin_memcpy(&v, base + (o < last ? o : last), 16);
+    } else {
+      uint32_t w[4] = {};
+      for (int e = 0; e < 8; ++e)
+        if (o + e < last + 8) w[e >> 1] |= (uint32_t)base[o + e] << (16 * (e & 1));
+      v = uint4{w[0], w[1], w[2], w[3]};
+    }
+    return v;
+  }
+  // What `load` brought for k-tile kt, of which kn reduction elements exist from k-tile 0 on.
+  __device__ __forceinline__ u32x4 trim(const uint4& v, int q, int kt, int kn) const {
+    const int left = kn - kt * T_BK - at[q];
+    int n = KM ? (left < most[q] ? left : most[q]) : (left > 0 ? most[q] : 0);
+    n = n > 0 ? n : 0;
+    const int64_t o = start(q, kt);
+    const int moved = !TINY && o > last ? (int)(o - last < 8 ? o - last : 8) : 0;
+    uint64_t lo = ((uint64_t)v.y << 32) | v.x, hi = ((uint64_t)v.w << 32) | v.z;
+    if (moved != 0) {  // down by `moved` elements
+      const int s = 16 * moved;
+      lo = s >= 64 ? (s >= 128 ? 0 : hi >> (s - 64)) : (lo >> s) | (hi << (64 - s));
+      hi = s >= 64 ? 0 : hi >> s;
+    }
+    lo = n >= 4 ? lo : lo & ((1ull << (16 * n)) - 1);
+    hi = n >= 8 ? hi : n <= 4 ? 0 : hi & ((1ull << (16 * (n - 4))) - 1);
+    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
+};
+
 // Tiles of operands whose rows do not start at multiples of 16 bytes, or end inside a
-// vector: BT x BT as in linear_mid_kernel, but a k-tile goes through registers (loads
-// of 16 bytes at any address, single elements at a row's end, zeros past it) into
-// the same LDS layouts, two stages; and results are stored the same way. 777 x 515 ->
-// 1001, with dropout, forward and backward XX us; on the fp32 instructions YY.
-template <int LAYOUT, int KIND, int ET, int BT>
+// vector: BT x BT as in linear_mid_kernel, but a k-tile goes through registers
+// (OddOperand) into the same LDS layouts, two stages; and results are stored at any
+// address, single elements at a row's end.
+template <int LAYOUT, int KIND, int ET, int BT, bool TINY>
 __global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;
   typedef typename TypeOf<ET>::type TT;
@@ -661,73 +743,38 @@ __global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int
   t.setup(p, ti, tj, wave, lane);
   lds_char* const lds = (lds_char*)lds_raw;
   const int64_t r0 = (int64_t)blockIdx.y * p.rsplit;
-  // Chunk q of an operand: `rows` of it exist from the tile's first on (K-major rows, or
-  // MN-major columns), of which this lane takes row / chunk as Operand::setup lays out.
-  auto chunk = [&](const char* base, int64_t ld, int64_t rows, bool kmaj, bool gate, int br, int q,
-                   int kt) -> uint4 {
-    const int valid = t.kn - kt * T_BK;
-    int64_t at;
-    int n;
-    if (kmaj) {
-      const int r = (br / 4) * wave + 8 * q + (lane >> 3);
-      const int c = (lane & 7) ^ ((r >> 1) & 7);
-      int64_t row = r, in = r;
-      if (gate) {
-        const int w = r / (br / 2), i = r % (br / 2);
-        in = w * (br / 4) + i % (br / 4);
-        row = (i / (br / 4)) * p.J + in;
-      }
-      at = row * ld + (int64_t)kt * T_BK + 8 * c;
-      n = in < rows ? valid - 8 * c : 0;
-    } else {
-      const int lpr = br / 8, kr = 16 * wave + (64 / lpr) * q + lane / lpr;
-      const int c = (lane % lpr) ^ (4 * (kr & 3) & (lpr - 1));
-      at = ((int64_t)kt * T_BK + kr) * ld + 8 * c;
-      n = kr < valid ? (int)(rows - 8 * c < 8 ? rows - 8 * c : 8) : 0;
-    }
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(base) + at;
-    uint4 v = {0, 0, 0, 0};
-    if (n >= 8) {
-      __builtin_memcpy(&v, src, 16);
-    } else if (n > 0) {
-      uint32_t w[4] = {};
+  OddOperand<TL::A_K, BT, false, TINY> oa;
+  OddOperand<TL::B_K, BT, GATED, TINY> ob;
+  oa.setup(static_cast<const uint16_t*>(p.a), p.lda, p.I, p.R, t.i0, r0, 0, wave, lane);
+  ob.setup(static_cast<const uint16_t*>(p.b), p.ldb, p.J, p.R, t.j0, r0, p.J, wave, lane);
+  // k-tiles kt + 1 and kt + 2 are on their way while kt is multiplied. Loads past the last
+  // one are made all the same (and trimmed to nothing), in whole pairs of k-tiles: where
+  // some are skipped, the compiler waits for all of them.
+  uint4 va[2][LA], vb[2][LB];
+  auto fetch = [&](int kt, int buf) {
 #pragma unroll
-      for (int e = 0; e < 7; ++e)
-        if (e < n) w[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
-      v = uint4{w[0], w[1], w[2], w[3]};
-    }
-    return v;
-  };
-  const char* const pa = static_cast<const char*>(p.a) +
-                         (TL::A_K ? t.i0 * p.lda + r0 : r0 * p.lda + t.i0) * 2;
-  const char* const pb = static_cast<const char*>(p.b) +
-                         (TL::B_K ? t.j0 * p.ldb + r0 : r0 * p.ldb + t.j0) * 2;
-  const int64_t ra = p.I - t.i0, rb = p.J - t.j0;
-  uint4 va[LA], vb[LB];
-  auto fetch = [&](int kt) {
+    for (int q = 0; q < LA; ++q) va[buf][q] = oa.load(q, kt);
 #pragma unroll
-    for (int q = 0; q < LA; ++q) va[q] = chunk(pa, p.lda, ra, TL::A_K, false, BT, q, kt);
-#pragma unroll
-    for (int q = 0; q < LB; ++q) vb[q] = chunk(pb, p.ldb, rb, TL::B_K, GATED, BT, q, kt);
-  };
-  auto put = [&](int slot) {
-    lds_char* const at = lds + slot * TL::STAGE + lane * 16;
-#pragma unroll
-    for (int q = 0; q < LA; ++q)
-      *reinterpret_cast<lds_u32x4*>(at + (LA * wave + q) * 1024) = __builtin_bit_cast(u32x4, va[q]);
-#pragma unroll
-    for (int q = 0; q < LB; ++q)
-      *reinterpret_cast<lds_u32x4*>(at + TL::OpA::BYTES + (LB * wave + q) * 1024) =
-          __builtin_bit_cast(u32x4, vb[q]);
+    for (int q = 0; q < LB; ++q) vb[buf][q] = ob.load(q, kt);
   };
   f32x16 acc[FM][FN] = {};
-  if (t.nkt > 0) fetch(0);
-  for (int kt = 0; kt < t.nkt; ++kt) {
-    // The other stage is free: every wave passed the barrier of k-tile kt - 1 after it.
-    put(kt & 1);
+  auto step = [&](int kt, int buf) {
+    // This stage is free: every wave passed the barrier of k-tile kt - 1 after kt - 2.
+    lds_char* const stg = lds + buf * TL::STAGE;
+    lds_char* const at = stg + lane * 16;
+    auto put = [&](auto& op, uint4* v, int first, int loads) {
+      const bool all = op.whole(kt, t.kn);
+#pragma unroll
+      for (int q = 0; q < loads; ++q) {
+        u32x4 w = __builtin_bit_cast(u32x4, v[q]);
+        if (!all) w = op.trim(v[q], q, kt, t.kn);
+        *reinterpret_cast<lds_u32x4*>(at + first + (loads * wave + q) * 1024) = w;
+      }
+    };
+    put(oa, va[buf], 0, LA);
+    put(ob, vb[buf], TL::OpA::BYTES, LB);
+    fetch(kt + 2, buf);
     TT_LDS_BARRIER();
-    if (kt + 1 < t.nkt) fetch(kt + 1);
-    lds_char* const stg = lds + (kt & 1) * TL::STAGE;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       uint4 fa[FM], fb[FN];
@@ -740,6 +787,12 @@ __global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int
 #pragma unroll
         for (int n = 0; n < FN; ++n) acc[m][n] = Mma<ET>::run(fb[n], fa[m], acc[m][n]);
     }
+  };
+  fetch(0, 0);
+  fetch(1, 1);
+  for (int kt = 0; kt < t.nkt; kt += 2) {
+    step(kt, 0);
+    step(kt + 1, 1);
   }
   __syncthreads();
   // 32 rows at a time through the wave's LDS, rows of W floats and four more.
@@ -816,10 +869,14 @@ int launch_odd(const LinArgs& p, hipStream_t s) {
   constexpr int BO = KIND == LIN_GATED ? BT / 2 : BT;
   const int64_t ti = (p.I + BT - 1) / BT, tj = (p.J + BO - 1) / BO;
   TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
-  hipLaunchKernelGGL((linear_odd_kernel<LAYOUT, KIND, ET, BT>),
-                     dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(T_NT), 0, s, p, (int)ti,
-                     (int)tj);
-  return tt_check_launch("linear_odd");
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(T_NT), 0, s, p,
+                       (int)ti, (int)tj);
+    return tt_check_launch("linear_odd");
+  };
+  if constexpr (BT == 64)
+    if (p.I * p.R < 8 || p.J * p.R < 8) return go(&linear_odd_kernel<LAYOUT, KIND, ET, BT, true>);
+  return go(&linear_odd_kernel<LAYOUT, KIND, ET, BT, false>);
 }
 
 template <int LAYOUT, int KIND>
