@@ -223,6 +223,25 @@ def test_empty_sizes(hip_ops, dtype):
             assert g.shape == t.shape
 
 
+@pytest.mark.parametrize("T, K, N", [(0, 2048, 2048), (0, 2049, 2051), (2048, 0, 2056), (5, 2049, 2051)])
+def test_reductions_of_nearly_nothing_over_many_tiles(hip_ops, T, K, N):
+    # 256 and more tiles of 128 x 128, each with at most five products to an element.
+    x, w = make((T, K), 1, BF), make((2 * N, K), 2, BF)
+    if T and K:
+        check_act(hip_ops, x, w, None, F.silu, True)
+        return
+    x.requires_grad_()
+    w.requires_grad_()
+    y = hip_ops.linear_act(x, w, activation_func=F.silu, gated=True)
+    assert y.shape == (T, N) and not y.any()
+    for t, g in zip((x, w), torch.autograd.grad(y, (x, w), torch.ones_like(y))):
+        assert g.shape == t.shape and not g.any()
+    y = hip_ops.linear_residual(x, w)
+    assert y.shape == (T, 2 * N) and not y.any()
+    for t, g in zip((x, w), torch.autograd.grad(y, (x, w), torch.ones_like(y))):
+        assert g.shape == t.shape and not g.any()
+
+
 def test_strides_alignment_and_dimensions(hip_ops):
     """Transposed, sliced, expanded and unaligned operands and leading dimensions give the
     contiguous, aligned call's values."""

@@ -162,8 +162,9 @@ Plan plan_of(int layout, int kind, int64_t I, int64_t J, int64_t R, int how) {
   const int64_t half = kind == LIN_GATED ? 2 : 1, width = half * J;
   auto tiles = [&](int64_t bm, int64_t bn) { return ((I + bm - 1) / bm) * ((width + bn - 1) / bn); };
   if (how == HOW_ODD) {
-    // 128-wide tiles where they fill the CUs, else 64-wide ones, split as below.
-    const bool big = tiles(128, 128) >= 256;
+    // 128-wide tiles where they fill the CUs, else 64-wide ones, split as below. Those
+    // take operands of fewer than eight elements, too.
+    const bool big = R >= 8 && tiles(128, 128) >= 256;
     const int64_t want = std::min<int64_t>(256 / std::max<int64_t>(tiles(64, 64), 1), R / 512);
     return Plan{big ? LIN_ODD128 : LIN_ODD64, split_of(R, big ? 1 : std::min<int64_t>(want, 8))};
   }
