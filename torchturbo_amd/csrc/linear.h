@@ -185,7 +185,7 @@ __device__ __forceinline__ LinRow<TT, W> lin_row(const LinArgs& p, int64_t i, in
 }
 
 // The sums v (GATED: gate v and up u) of row i, columns j .. j + W - 1 (n of
-// them exist) to what KIND makes of them. j is a multiple of W; W is 4 or 8.
+// them exist) to what KIND makes of them. j is a multiple of W, which is 8.
 // Returns DGRAD's share of the row's dot product.
 template <int KIND, class TT, int W, bool VEC>
 __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t j, int n,
@@ -211,13 +211,11 @@ __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t
   } else if constexpr (KIND == LIN_RES || KIND == LIN_DROP) {
     uint32_t w[4] = {};
     if constexpr (KIND == LIN_DROP) philox(dk, (uint32_t)(j >> 3), (uint32_t)i, w);
-    const bool upper = W == 4 && (j & 4) != 0;  // the upper four of the group
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       float t = v[e] + col.b[e];
       if constexpr (KIND == LIN_DROP) {
-        const bool keep = upper ? keeps(w, 4 + (e & 3), p.threshold) : keeps(w, e, p.threshold);
-        t = keep ? t * p.alpha : 0.f;
+        t = keeps(w, e, p.threshold) ? t * p.alpha : 0.f;
       }
       if (p.scale != nullptr) t *= row.s;
       v[e] = p.res != nullptr ? t + TT::to_f32(row.v[e]) : t;
@@ -244,6 +242,67 @@ __device__ __forceinline__ float lin_finish(const LinArgs& p, int64_t i, int64_t
   return dot;
 }
 
+// Sum over the four lanes of a quad.
+__device__ __forceinline__ float sum4(float v) {
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true));  // ^ 1
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true));  // ^ 2
+  return v;
+}
+
+// The sums of a wave's (32 FM) x (32 FN) part of a tile to what KIND makes of them, from
+// row iw and output column jw on, at any alignment: 32 rows at a time through the wave's LDS,
+// so that a lane gets eight consecutive columns (GATED: the first half of the wave's columns
+// are gates, the second half their ups). stage(mi, put): calls put(row, column, four sums)
+// for the lane's part of the 32 rows mi.
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+template <int FN>
+constexpr int LIN_WAVE_FLOATS = 32 * (32 * FN + 4);  // rows of the wave's sums and four more
+
+template <int KIND, class TT, int FM, int FN, typename F>
+__device__ __forceinline__ void lin_finish_wave(const LinArgs& p, const F& stage, float* region,
+                                                int64_t iw, int64_t jw, int lane) {
+  constexpr bool GATED = KIND == LIN_GATED;
+  constexpr int W = 32 * FN, LD = W + 4, OUT = GATED ? W / 2 : W, NG = OUT / 8;
+  const int64_t width = GATED ? 2 * p.J : p.J;
+  DropKey dk{};
+  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
+#pragma unroll
+  for (int mi = 0; mi < FM; ++mi) {
+    stage(mi, [&](int row, int column, const f32x4_t& v) {
+      *reinterpret_cast<f32x4_t*>(region + row * LD + column) = v;
+    });
+#pragma unroll 1
+    for (int it = lane; it < 32 * NG; it += 64) {
+      const int r = it / NG, gi = it % NG;
+      const int64_t i = iw + 32 * mi + r, j = jw + 8 * gi;
+      const bool live = i < p.I && j < p.J;
+      const int n = !live ? 0 : p.J - j < 8 ? (int)(p.J - j) : 8;
+      float v[8], u[8] = {}, dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = region[r * LD + 8 * gi + e];
+        if constexpr (GATED) u[e] = region[r * LD + OUT + 8 * gi + e];
+      }
+      if (live && p.part != nullptr) {
+        const int64_t at = ((int64_t)blockIdx.y * p.I + i) * width + j;
+        lin_store<F32T, 8, false>(p.part, at, n, v);
+        if constexpr (GATED) lin_store<F32T, 8, false>(p.part, at + p.J, n, u);
+      } else if (live) {
+        dot = lin_finish<KIND, TT, 8, false>(p, i, j, n, v, u, dk, lin_cols<KIND, 8>(p, j, n),
+                                             lin_row<KIND, TT, 8, false>(p, i, j, n));
+      }
+      if constexpr (KIND == LIN_DGRAD) {
+        if (p.dots != nullptr && p.part == nullptr) {
+          static_assert(NG % 4 == 0, "four lanes of a run in one row");
+          dot = sum4(dot);
+          if (live && (lane & 3) == 0)
+            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
+        }
+      }
+    }
+  }
+}
+
 }  // namespace
 
 // Operand layouts of a product: NT: A [I, R], B [J, R]. NN: A [I, R], B [R, J].
@@ -260,5 +319,5 @@ int tt_linear_f32(int kind, const LinArgs& a, hipStream_t s);
 // 16-bit matrix instructions on tiles (LIN_T64 ...), for aligned rows of whole 16-byte
 // vectors, or (LIN_ODD64, LIN_ODD128) for any (linear_tile.hip).
 int tt_linear_tile(int kind, int tile, int dtype, const LinArgs& a, hipStream_t s);
-// The same for at most 64 rows of x and NT operands under 2 GiB (linear_rows.hip).
+// The same for at most 64 rows of x, NT, aligned (linear_rows.hip).
 int tt_linear_rows(int kind, int dtype, const LinArgs& a, hipStream_t s);

@@ -1,225 +1,259 @@
 // Dense product with an epilogue of fp32 tensors, any size and alignment (gfx950).
-// Products and sums run in fp32 on v_mfma_f32_32x32x2_f32.
+// Products and sums run in fp32 on v_mfma_f32_32x32x2_f32. 2048 x 8192 -> 2048 613 us (112
+// TFLOP/s; a plain product of torch 454), 4096 x 1024 -> 3000 298 us, 512 x 256 -> 512 11 us;
+// with 4001 x 1201 -> 1703, whose rows start at no multiple of 16 bytes, 192 us NT, 205 NN
+// and 311 TN. Tiles of 128 x 128 are 2 to 7 % faster where they fill the CUs in whole rounds
+// (2048 cubed 177 in place of 189) and up to half slower where not (4001 x 1703 -> 1201 313
+// us); v_mfma_f32_16x16x4_f32 is 2 to 5 % slower.
 #include "linear.h"
 
 namespace {
 
-constexpr int A_NT = 256, A_BK = 32, A_CHAIN = 512;
+constexpr int A_NT = 256, A_BT = 64, A_BK = 32, A_CHAIN = 512;
 
-// One block computes BT x BT of C (GATED: BT / 2 outputs, the tile's columns
-// being a gate's and its up's in runs of 32), each of the four waves a quarter.
-// The next k-tile is loaded into registers while one is multiplied from LDS
-// (k-row-major, so that a fragment is 32 consecutive floats).
-template <int LAYOUT, int KIND, int BT>
-__global__ __launch_bounds__(A_NT) void linear_f32_kernel(LinArgs p, int tiles_j, int vec) {
-  constexpr bool A_K = LAYOUT != LAY_TN, B_K = LAYOUT == LAY_NT;
+// An operand of a tile of A_BT rows (columns): 32-deep k-tiles in chunks of four elements,
+// LOADS of them per thread. A load is always of 16 bytes, at an address moved back where
+// they would pass the operand's end, so that it never waits for another; the
+// elements are put in place, and those past a row's end cleared, when it has arrived.
+// In LDS a K-major operand lies row by row, the other one k-row by k-row, each with a
+// stride that spreads a fragment's lanes over all banks.
+// GATE: per half of the tile, A_BT / 4 rows of the operand's first half, then their ups.
+// FAR: rows too far apart for 32-bit offsets, or an operand of fewer than four elements:
+// every element by itself.
+template <bool KM, bool GATE, bool FAR>
+struct Operand32 {
+  static constexpr int LOADS = A_BT / 32;
+  static constexpr int LD = KM ? A_BK + 4 : A_BT + 8;
+  static constexpr int FLOATS = LD * (KM ? A_BT : A_BK);
+  const float* base;
+  int64_t last;        // the last element that 16 bytes can start at
+  int64_t first_at;    // the tile's first element in k-tile 0
+  uint64_t off[LOADS]; // bytes from there to the chunk
+  int64_t step;        // elements of a k-tile
+  int at[LOADS];       // the chunk's place in the reduction
+  int most[LOADS];     // its elements that exist, by the other dimension
+  int slot[LOADS];     // its place in LDS
+  bool inside;         // every row of the tile exists
+
+  // rows x R elements (GATE: 2 x rows), from row `first` and reduction element r0 on.
+  __device__ __forceinline__ void setup(const void* p, int64_t ld, int64_t rows, int64_t R,
+                                        int64_t first, int64_t r0) {
+    base = static_cast<const float*>(p);
+    last = rows * R * (GATE ? 2 : 1) - 4;
+    first_at = KM ? first * ld + r0 : r0 * ld + first;
+    step = KM ? A_BK : A_BK * ld;
+    inside = first + (GATE ? A_BT / 2 : A_BT) <= rows;
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) {
+      const int id = threadIdx.x + A_NT * q;
+      if constexpr (KM) {
+        const int r = id / (A_BK / 4), c = id % (A_BK / 4);
+        int64_t row = r, in = r;
+        if constexpr (GATE) {
+          in = r / (A_BT / 2) * (A_BT / 4) + r % (A_BT / 2) % (A_BT / 4);
+          row = (r % (A_BT / 2) / (A_BT / 4)) * rows + in;
+        }
+        off[q] = (uint64_t)(row * ld + 4 * c) * 4;
+        at[q] = 4 * c;
+        most[q] = first + in < rows ? 4 : 0;
+        slot[q] = r * LD + 4 * c;
+      } else {
+        const int kr = id / (A_BT / 4), c = id % (A_BT / 4);
+        const int64_t left = rows - first - 4 * c;
+        off[q] = (uint64_t)(kr * ld + 4 * c) * 4;
+        at[q] = kr;
+        most[q] = left <= 0 ? 0 : left < 4 ? (int)left : 4;
+        slot[q] = kr * LD + 4 * c;
+      }
+    }
+  }
+  // Whether 32-bit offsets reach a tile's elements.
+  static bool near(int64_t ld, int64_t rows) {
+    return (KM ? (A_BT + (GATE ? rows : 0)) * ld : (int64_t)A_BK * ld + A_BT) * 4 < (1ll << 32) - 1024;
+  }
+  __device__ __forceinline__ void load(f32x4_t (&v)[LOADS], int kt) const {
+    const int64_t at_kt = first_at + kt * step;
+    if constexpr (!FAR) {
+      const int64_t from = at_kt < last ? at_kt : last, left = (last - from) * 4;
+      const char* const p = reinterpret_cast<const char*>(base + from);
+      const uint32_t reach = left < 0xfffffff0ll ? (uint32_t)left : 0xfffffff0u;
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q) {
+        const uint32_t o = (uint32_t)off[q];
+        __builtin_memcpy(&v[q], p + (o < reach ? o : reach), 16);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q) {
+        const int64_t o = at_kt + (int64_t)(off[q] / 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[q][e] = o + e < last + 4 ? base[o + e] : 0.f;
+      }
+    }
+  }
+  // What `load` brought for k-tile kt, of which kn reduction elements exist from k-tile 0 on.
+  __device__ __forceinline__ f32x4_t trim(const f32x4_t& v, int q, int kt, int kn) const {
+    const int left = kn - kt * A_BK - at[q];
+    const int n = KM ? (left < most[q] ? left : most[q]) : (left > 0 ? most[q] : 0);
+    const int64_t o = first_at + kt * step + (int64_t)(off[q] / 4);
+    const int moved = !FAR && o > last ? (int)(o - last < 4 ? o - last : 4) : 0;
+    f32x4_t r{};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int f = e; f < 4; ++f) r[e] = e < n && e + moved == f ? v[f] : r[e];
+    return r;
+  }
+  // Into LDS.
+  __device__ __forceinline__ void put(float* lds, const f32x4_t (&v)[LOADS], int kt, int kn) const {
+    if (inside && (kt + 1) * A_BK <= kn) {
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q) *reinterpret_cast<f32x4_t*>(lds + slot[q]) = v[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q)
+        *reinterpret_cast<f32x4_t*>(lds + slot[q]) = trim(v[q], q, kt, kn);
+    }
+  }
+  // Reduction elements 8 s + 4 h + 0..3 of row r.
+  static __device__ __forceinline__ f32x4_t fragment(const float* lds, int r, int s, int h) {
+    if constexpr (KM) {
+      return *reinterpret_cast<const f32x4_t*>(lds + r * LD + 8 * s + 4 * h);
+    } else {
+      const float* p = lds + (8 * s + 4 * h) * LD + r;
+      return f32x4_t{p[0], p[LD], p[2 * LD], p[3 * LD]};
+    }
+  }
+};
+
+// One block computes A_BT x A_BT of C (GATED: A_BT / 2 outputs, each half of the tile's columns
+// being gates and their ups), each of the four waves a quarter. While a k-tile is
+// multiplied from LDS the next one goes there and the two after it are on their way. Product j of four takes
+// reduction elements j and 4 + j of eight, so that a fragment is 16 consecutive bytes of a
+// K-major operand.
+template <int LAYOUT, int KIND, bool FAR>
+__global__ __launch_bounds__(A_NT) void linear_f32_kernel(LinArgs p, int tiles_j) {
   constexpr bool GATED = KIND == LIN_GATED;
-  constexpr int F = BT / 64;                 // 32x32 blocks of a wave, each way
-  constexpr int PER = BT * A_BK / A_NT;      // elements of an operand per thread and k-tile
-  constexpr int LD = BT + 4;
-  constexpr int BO = GATED ? BT / 2 : BT;    // output columns of a tile
-  __shared__ float sa[2][A_BK][LD], sb[2][A_BK][LD];
+  constexpr int F = A_BT / 64;             // 32x32 blocks of a wave, each way
+  constexpr int BO = GATED ? A_BT / 2 : A_BT;  // output columns of a tile
+  typedef Operand32<LAYOUT != LAY_TN, false, FAR> OpA;
+  typedef Operand32<LAYOUT == LAY_NT, GATED, FAR> OpB;
+  constexpr int FLOATS = 2 * (OpA::FLOATS + OpB::FLOATS);
+  __shared__ __align__(16) float lds[FLOATS];
+  float* const sa[2] = {lds, lds + OpA::FLOATS};
+  float* const sb[2] = {lds + 2 * OpA::FLOATS, lds + 2 * OpA::FLOATS + OpB::FLOATS};
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wr = (wave >> 1) * (BT / 2), wc = (wave & 1) * (BT / 2);
+  const int wr = (wave >> 1) * (A_BT / 2), wc = (wave & 1) * (A_BT / 2);
   const int l32 = lane & 31, h = lane >> 5;
-  const int64_t i0 = (int64_t)(blockIdx.x / tiles_j) * BT, j0 = (int64_t)(blockIdx.x % tiles_j) * BO;
+  const int64_t i0 = (int64_t)(blockIdx.x / tiles_j) * A_BT, j0 = (int64_t)(blockIdx.x % tiles_j) * BO;
   const int64_t r0 = (int64_t)blockIdx.y * p.rsplit;
-  const int64_t r1 = r0 + p.rsplit < p.R ? r0 + p.rsplit : p.R;
-  const float* A = static_cast<const float*>(p.a);
-  const float* B = static_cast<const float*>(p.b);
-  // Column of B that tile column c is, or -1. GATED (F of 32 columns per wave):
-  // a wave's first half are gates, its second half their ups.
-  auto bcol = [&](int c) -> int64_t {
-    if constexpr (GATED) {
-      const int w = c / (BT / 2), in = c % (BT / 2), up = in / (BT / 4);
-      const int64_t o = j0 + w * (BT / 4) + in % (BT / 4);
-      return o < p.J ? o + (up ? p.J : 0) : -1;
-    }
-    return j0 + c < p.J ? j0 + c : -1;
-  };
-  // Operand elements of a thread: K-major: PER consecutive k of one row, else
-  // PER consecutive rows (columns) of one k.
-  constexpr int KT = A_BK / PER > 0 ? A_BK / PER : 1;
-  static_assert(PER <= A_BK, "a thread's elements lie in one row");
-  const int ar = A_K ? threadIdx.x / KT : (threadIdx.x % (BT / PER)) * PER;
-  const int ak = A_K ? (threadIdx.x % KT) * PER : threadIdx.x / (BT / PER);
-  const int br = B_K ? threadIdx.x / KT : (threadIdx.x % (BT / PER)) * PER;
-  const int bk = B_K ? (threadIdx.x % KT) * PER : threadIdx.x / (BT / PER);
-  const int64_t brow = bcol(br);
-  float va[PER], vb[PER];
-  auto fetch = [&](int64_t k0) {
-    if constexpr (A_K) {
-      const int64_t i = i0 + ar, k = k0 + ak;
-      const float* src = A + i * p.lda + k;
-      if (i >= p.I) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = 0.f;
-      } else if (k + PER <= r1) {
-        __builtin_memcpy(va, src, sizeof(va));
-      } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = k + e < r1 ? src[e] : 0.f;
-      }
-    } else {
-      const int64_t i = i0 + ar, k = k0 + ak;
-      const float* src = A + k * p.lda + i;
-      if (k >= r1) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = 0.f;
-      } else if (i + PER <= p.I) {
-        __builtin_memcpy(va, src, sizeof(va));
-      } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) va[e] = i + e < p.I ? src[e] : 0.f;
-      }
-    }
-    if constexpr (B_K) {
-      const int64_t k = k0 + bk;
-      const float* src = B + brow * p.ldb + k;
-      if (brow < 0) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = 0.f;
-      } else if (k + PER <= r1) {
-        __builtin_memcpy(vb, src, sizeof(vb));
-      } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = k + e < r1 ? src[e] : 0.f;
-      }
-    } else {
-      const int64_t j = j0 + br, k = k0 + bk;
-      const float* src = B + k * p.ldb + j;
-      if (k >= r1) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = 0.f;
-      } else if (j + PER <= p.J) {
-        __builtin_memcpy(vb, src, sizeof(vb));
-      } else {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) vb[e] = j + e < p.J ? src[e] : 0.f;
-      }
-    }
-  };
-  auto put = [&](int buf) {
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if constexpr (A_K) sa[buf][ak + e][ar] = va[e];
-      else sa[buf][ak][ar + e] = va[e];
-      if constexpr (B_K) sb[buf][bk + e][br] = vb[e];
-      else sb[buf][bk][br + e] = vb[e];
-    }
+  const int kn = (int)(r0 + p.rsplit < p.R ? p.rsplit : p.R - r0), nkt = (kn + A_BK - 1) / A_BK;
+  OpA oa;
+  OpB ob;
+  oa.setup(p.a, p.lda, p.I, p.R, i0, r0);
+  ob.setup(p.b, p.ldb, p.J, p.R, j0, r0);
+  // Loads past the last k-tile are made all the same (and trimmed to nothing), in whole
+  // pairs of k-tiles: where some are skipped, the compiler waits for all of them.
+  f32x4_t va[2][OpA::LOADS], vb[2][OpB::LOADS];
+  auto fetch = [&](int kt, int buf) {
+    oa.load(va[buf], kt);
+    ob.load(vb[buf], kt);
   };
   // One chain of products is at most A_CHAIN long: a longer reduction adds chains, whose
   // rounding grows with their number instead of its length.
   f32x16 acc[F][F] = {}, total[F][F] = {};
-  if (r0 < r1) {
-    fetch(r0);
-    put(0);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k0 = r0; k0 < r1; k0 += A_BK) {
-      const bool more = k0 + A_BK < r1;
-      if (more) fetch(k0 + A_BK);
+  f32x4_t fa[2][F], fb[2][F];
+  auto read = [&](int buf, int s) {
 #pragma unroll
-      for (int s = 0; s < A_BK / 2; ++s) {
-        float fa[F], fb[F];
+    for (int m = 0; m < F; ++m) fa[s & 1][m] = OpA::fragment(sa[buf], wr + 32 * m + l32, s, h);
 #pragma unroll
-        for (int m = 0; m < F; ++m) fa[m] = sa[buf][2 * s + h][wr + 32 * m + l32];
+    for (int n = 0; n < F; ++n) fb[s & 1][n] = OpB::fragment(sb[buf], wc + 32 * n + l32, s, h);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](int s) {
 #pragma unroll
-        for (int m = 0; m < F; ++m) fb[m] = sb[buf][2 * s + h][wc + 32 * m + l32];
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int m = 0; m < F; ++m)
+      for (int m = 0; m < F; ++m)
 #pragma unroll
-          for (int n = 0; n < F; ++n)
-            acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[n], fa[m], acc[m][n], 0, 0, 0);
-      }
-      if (more) put(buf ^ 1);
-      if (!more || (k0 - r0) % A_CHAIN == A_CHAIN - A_BK) {
-#pragma unroll
-        for (int m = 0; m < F; ++m)
-#pragma unroll
-          for (int n = 0; n < F; ++n) {
-            total[m][n] += acc[m][n];
-            acc[m][n] = f32x16{};
-          }
-      }
-      __syncthreads();
-      buf ^= 1;
+        for (int n = 0; n < F; ++n)
+          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[s & 1][n][j], fa[s & 1][m][j],
+                                                           acc[m][n], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Multiplies k-tile kt, a fragment's eight deep at a time while the next ones are read.
+  // After the first, kt + 1 goes to LDS and kt + 3 is asked for; before the last, a barrier
+  // publishes kt + 1, and frees kt's stage.
+  auto step = [&](int kt, int buf) {
+    read(buf, 1);
+    multiply(0);
+    oa.put(sa[buf ^ 1], va[buf ^ 1], kt + 1, kn);
+    ob.put(sb[buf ^ 1], vb[buf ^ 1], kt + 1, kn);
+    fetch(kt + 3, buf ^ 1);
+    read(buf, 2);
+    multiply(1);
+    read(buf, 3);
+    multiply(2);
+    TT_LDS_BARRIER();
+    read(buf ^ 1, 0);
+    multiply(3);
+  };
+  fetch(0, 0);
+  fetch(1, 1);
+  oa.put(sa[0], va[0], 0, kn);
+  ob.put(sb[0], vb[0], 0, kn);
+  fetch(2, 0);
+  TT_LDS_BARRIER();
+  read(0, 0);
+  for (int first = 0; first < nkt; first += A_CHAIN / A_BK) {
+    const int end = first + A_CHAIN / A_BK < nkt ? first + A_CHAIN / A_BK : nkt;
+    for (int kt = first; kt < end; kt += 2) {
+      step(kt, 0);
+      step(kt + 1, 1);
     }
-  }
-  // Lane l holds row 32 m + l % 32, columns 32 n + 8 g + 4 (l / 32) + 0..3 of the wave's.
-  DropKey dk{};
-  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
-  const int64_t width = GATED ? 2 * p.J : p.J;
 #pragma unroll
-  for (int m = 0; m < F; ++m) {
-    const int64_t i = i0 + wr + 32 * m + l32;
-    const bool live = i < p.I;
-    float dots[F] = {};  // of each 32 columns
+    for (int m = 0; m < F; ++m)
 #pragma unroll
-    for (int n = 0; n < (GATED ? (F + 1) / 2 : F); ++n)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        // GATED with one block per wave: columns 0-15 of it are gates, 16-31 their ups.
-        if (GATED && F == 1 && g >= 2) continue;
-        const int64_t j = GATED ? j0 + (wave & 1) * (BT / 4) + 32 * n + 8 * g + 4 * h
-                                : j0 + wc + 32 * n + 8 * g + 4 * h;
-        if (!live || j >= p.J) continue;
-        const int left = p.J - j < 4 ? (int)(p.J - j) : 4;
-        float v[4], u[4] = {};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = total[m][n][4 * g + e];
-          if constexpr (GATED) u[e] = F == 1 ? total[m][0][4 * ((g + 2) & 3) + e] : total[m][(n + F / 2) % F][4 * g + e];
-        }
-        if (p.part != nullptr) {
-          float* o = p.part + ((int64_t)blockIdx.y * p.I + i) * width + j;
-          for (int e = 0; e < left; ++e) {
-            o[e] = v[e];
-            if (GATED) o[p.J + e] = u[e];
-          }
-        } else if (p.J % 4 == 0) {
-          dots[n] += lin_finish<KIND, F32T, 4, true>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
-                                             lin_row<KIND, F32T, 4, true>(p, i, j, left));
-        } else {
-          dots[n] += lin_finish<KIND, F32T, 4, false>(p, i, j, left, v, u, dk, lin_cols<KIND, 4>(p, j, left),
-                                             lin_row<KIND, F32T, 4, false>(p, i, j, left));
-        }
+      for (int n = 0; n < F; ++n) {
+        total[m][n] += acc[m][n];
+        acc[m][n] = f32x16{};
       }
-    if constexpr (KIND == LIN_DGRAD) {
-      static_assert(LIN_DOT == 32, "a block's columns");
-      if (p.dots != nullptr && p.part == nullptr) {
-#pragma unroll
-        for (int n = 0; n < F; ++n) {
-          const float dot = dots[n] + __shfl_xor(dots[n], 32, 64);
-          const int64_t j = j0 + wc + 32 * n;
-          if (live && h == 0 && j < p.J)
-            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
-        }
-      }
-    }
   }
+  __syncthreads();
+  static_assert(LIN_WAVE_FLOATS<F> * 4 <= FLOATS, "the waves' rows");
+  // Lane l holds row 32 m + l % 32, columns 32 n + 8 g + 4 (l / 32) + 0..3.
+  auto stage = [&](int m, auto put) {
+#pragma unroll
+    for (int n = 0; n < F; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        put(l32, 32 * n + 8 * g + 4 * h,
+            f32x4_t{total[m][n][4 * g], total[m][n][4 * g + 1], total[m][n][4 * g + 2],
+                    total[m][n][4 * g + 3]});
+  };
+  lin_finish_wave<KIND, F32T, F, F>(p, stage, lds + wave * LIN_WAVE_FLOATS<F>, i0 + wr,
+                                    j0 + (GATED ? wc / 2 : wc), lane);
 }
 
-template <int LAYOUT, int KIND, int BT>
+template <int LAYOUT, int KIND, bool FAR>
 int launch(const LinArgs& p, hipStream_t s) {
-  const int bo = KIND == LIN_GATED ? BT / 2 : BT;
-  const int64_t ti = (p.I + BT - 1) / BT, tj = (p.J + bo - 1) / bo;
+  const int bo = KIND == LIN_GATED ? A_BT / 2 : A_BT;
+  const int64_t ti = (p.I + A_BT - 1) / A_BT, tj = (p.J + bo - 1) / bo;
   TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.res) |
-                       reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.xs) |
-                       reinterpret_cast<uintptr_t>(p.pre);
-  hipLaunchKernelGGL((linear_f32_kernel<LAYOUT, KIND, BT>),
-                     dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(A_NT), 0, s, p, (int)tj,
-                     (int)(at % 16 == 0 && p.J % 4 == 0));
+  hipLaunchKernelGGL((linear_f32_kernel<LAYOUT, KIND, FAR>),
+                     dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(A_NT), 0, s, p,
+                     (int)tj);
   return tt_check_launch("linear_f32");
 }
 
 template <int LAYOUT, int KIND>
 int sized(const LinArgs& p, hipStream_t s) {
-  // 64-wide tiles while 128-wide ones leave CUs without a block.
-  const int64_t width = KIND == LIN_GATED ? 2 * p.J : p.J;
-  const int64_t tiles = ((p.I + 127) / 128) * ((width + 127) / 128) * p.splits;
-  return tiles >= 256 ? launch<LAYOUT, KIND, 128>(p, s) : launch<LAYOUT, KIND, 64>(p, s);
+  constexpr bool GATED = KIND == LIN_GATED;
+  typedef Operand32<LAYOUT != LAY_TN, false, false> OpA;
+  typedef Operand32<LAYOUT == LAY_NT, GATED, false> OpB;
+  if (p.I * p.R < 4 || p.J * p.R < 4 || !OpA::near(p.lda, p.I) || !OpB::near(p.ldb, p.J))
+    return launch<LAYOUT, KIND, true>(p, s);
+  return launch<LAYOUT, KIND, false>(p, s);
 }
 
 }  // namespace

@@ -1,9 +1,10 @@
 // Dense product with an epilogue on the 16-bit matrix instructions (gfx950):
-// C [I, J] = sum over r of A(i, r) B(r, j), rows of whole aligned 16-byte
-// vectors, then what linear.h makes of the fp32 sums.
+// C [I, J] = sum over r of A(i, r) B(r, j), then what linear.h makes of the fp32 sums.
+// Rows of whole aligned 16-byte vectors take linear_big_kernel or linear_mid_kernel,
+// all others linear_odd_kernel.
 //
-// Both kernels compute a tile with four waves, two by two, in 32x32 blocks of
-// v_mfma_f32_32x32x16 whose operands are swapped, so that a lane holds four
+// A tile is computed by four waves, two by two, in blocks of v_mfma_f32_16x16x32 (256-row
+// tiles) or v_mfma_f32_32x32x16 whose operands are swapped, so that a lane holds four
 // consecutive columns of one row. 64-deep k-tiles go from memory straight into LDS.
 // LDS layouts: K-major operands: 128 bytes per row, chunk c in slot
 // c ^ ((row >> 1) & 7), read with ds_read_b128; the others: k-row by k-row as in
@@ -160,7 +161,6 @@ struct TypeOf<TT_BF16> { typedef BF16T type; };
 template <>
 struct TypeOf<TT_F16> { typedef F16T type; };
 
-typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((address_space(3))) f32x4_t lds_f32x4;
 
 // Eight 16-bit values of four dwords, and back (hardware round to nearest even).
@@ -181,13 +181,6 @@ template <int ET>
 __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
   const uint2 lo = pack4<ET>(v[0], v[1], v[2], v[3]), hi = pack4<ET>(v[4], v[5], v[6], v[7]);
   return u32x4{lo.x, lo.y, hi.x, hi.y};
-}
-
-// Sum over the four lanes of a quad.
-__device__ __forceinline__ float sum4(float v) {
-  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true));  // ^ 1
-  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true));  // ^ 2
-  return v;
 }
 
 // The wave's rows [i0, I) of a matrix of `ld` elements of `size` bytes per row, from column
@@ -444,6 +437,10 @@ __device__ __forceinline__ void mma_done() { asm volatile("s_nop 7\n\ts_nop 7\n\
 // k-step 1. With SA = 2 a barrier then frees A's stage for the loads of k-step 1 (with
 // three, the stage of the k-tile before is loaded). Half way through k-step 1 a
 // barrier publishes the next k-tile, whose first fragments the other half reads.
+// Large products run at the part's power limit, where the 16x16x32 instructions draw less
+// than the 32x32x16 ones (2.0 GHz in place of 1.78), and the sums stay in the accumulation
+// registers. 4096 x 7168 -> 4096 in bf16, tiles of 256 x 256: NT 159 us (1.51 PFLOP/s),
+// NN 163, TN 161; a plain product of torch 151, 177 and 211.
 template <int LAYOUT, int KIND, int ET, bool KMASK, int BN>
 __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, 256, BN, 16> TL;
@@ -572,7 +569,9 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
 }
 
 // BT x BT tiles (64 or 128), a quarter per wave, a ring of S stages (16 or 32 KiB) with
-// one barrier per k-tile, which publishes k-tile kt and frees the stage of kt - 1.
+// one barrier per k-tile, which publishes k-tile kt and frees the stage of kt - 1. Several
+// blocks share a CU and hide one another's waits and epilogues: 512 x 2048 -> 7168 24.7 us
+// (0.61 PFLOP/s), 1000 x 704 -> 1024 6.5 us.
 template <int LAYOUT, int KIND, int ET, bool KMASK, int BT, int S>
 __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;
@@ -728,7 +727,9 @@ struct OddOperand {
 // Tiles of operands whose rows do not start at multiples of 16 bytes, or end inside a
 // vector: BT x BT as in linear_mid_kernel, but a k-tile goes through registers
 // (OddOperand) into the same LDS layouts, two stages; and results are stored at any
-// address, single elements at a row's end.
+// address, single elements at a row's end. It is bound by the instructions that move
+// k-tiles, not by products: 4001 x 1201 -> 1703 in bf16 62 us NT, 71 NN, 71 TN (0.26
+// PFLOP/s; 228, 316 and 366 us on the fp32 matrix instructions).
 template <int LAYOUT, int KIND, int ET, int BT, bool TINY>
 __global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;
@@ -795,53 +796,20 @@ __global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int
     step(kt + 1, 1);
   }
   __syncthreads();
-  // 32 rows at a time through the wave's LDS, rows of W floats and four more.
-  constexpr int W = 32 * FN, LD = W + 4, OUT = GATED ? W / 2 : W, NG = OUT / 8;
-  static_assert(4 * 32 * LD * 4 <= 2 * TL::STAGE, "the waves' rows");
-  float* const region = reinterpret_cast<float*>(lds_raw) + wave * (32 * LD);
-  const int64_t iw = t.i0 + (wave >> 1) * (BT / 2), jw = t.j0 + (wave & 1) * OUT;
-  const int64_t width = GATED ? 2 * p.J : p.J;
-  DropKey dk{};
-  if constexpr (KIND == LIN_DROP) dk = load_key(p.key);
-#pragma unroll
-  for (int mi = 0; mi < FM; ++mi) {
+  static_assert(LIN_WAVE_FLOATS<FN> * 4 * 4 <= 2 * TL::STAGE, "the waves' rows");
+  // Lane l holds row 32 mi + l % 32, columns 32 ni + 8 g + 4 (l / 32) + 0..3.
+  auto stage = [&](int mi, auto put) {
 #pragma unroll
     for (int ni = 0; ni < FN; ++ni)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          region[(lane & 31) * LD + 32 * ni + 8 * g + 4 * (lane >> 5) + e] = acc[mi][ni][4 * g + e];
-#pragma unroll 1
-    for (int it = lane; it < 32 * NG; it += 64) {
-      const int r = it / NG, gi = it % NG;
-      const int64_t i = iw + 32 * mi + r, j = jw + 8 * gi;
-      const bool live = i < p.I && j < p.J;
-      const int n = !live ? 0 : p.J - j < 8 ? (int)(p.J - j) : 8;
-      float v[8], u[8] = {}, dot = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = region[r * LD + 8 * gi + e];
-        if constexpr (GATED) u[e] = region[r * LD + OUT + 8 * gi + e];
-      }
-      if (live && p.part != nullptr) {
-        const int64_t at = ((int64_t)blockIdx.y * p.I + i) * width + j;
-        lin_store<F32T, 8, false>(p.part, at, n, v);
-        if constexpr (GATED) lin_store<F32T, 8, false>(p.part, at + p.J, n, u);
-      } else if (live) {
-        dot = lin_finish<KIND, TT, 8, false>(p, i, j, n, v, u, dk, lin_cols<KIND, 8>(p, j, n),
-                                             lin_row<KIND, TT, 8, false>(p, i, j, n));
-      }
-      if constexpr (KIND == LIN_DGRAD) {
-        if (p.dots != nullptr && p.part == nullptr) {
-          static_assert(NG % 4 == 0, "four lanes of a run in one row");
-          dot = sum4(dot);
-          if (live && (lane & 3) == 0)
-            p.dots[i * ((p.J + LIN_DOT - 1) / LIN_DOT) + j / LIN_DOT] = dot;
-        }
-      }
-    }
-  }
+        put(lane & 31, 32 * ni + 8 * g + 4 * (lane >> 5),
+            f32x4_t{acc[mi][ni][4 * g], acc[mi][ni][4 * g + 1], acc[mi][ni][4 * g + 2],
+                    acc[mi][ni][4 * g + 3]});
+  };
+  lin_finish_wave<KIND, TT, FM, FN>(p, stage, reinterpret_cast<float*>(lds_raw) + wave * LIN_WAVE_FLOATS<FN>,
+                                    t.i0 + (wave >> 1) * (BT / 2),
+                                    t.j0 + (wave & 1) * (GATED ? BT / 4 : BT / 2), lane);
 }
 
 template <int LAYOUT, int KIND, int ET, bool KMASK>

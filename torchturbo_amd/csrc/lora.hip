@@ -19,6 +19,12 @@
 // scalings and sums; forward and backward 2821 -> 1211 us, at 4096 tokens r 8
 // 4098 -> 1843 us, r 64 5017 -> 2980. (Sums split over the waves of a block
 // took 354 us, but in an order of their own: other last bits.)
+//
+// With dropout the rows' masks are made in the kernels that read or write them, among the
+// products: K 2048, r 16, 16384 rows, down 36 -> 57 us, dx 42 -> 48, dA 33 -> 68, for
+// Philox's 40 32-bit multiplies to eight elements (a quarter of the rate of adds). Passes of
+// their own over x and dx would take about as long together (134 MB each, 26 us at a
+// copy's rate), and keep the 67 MB of dropped rows for the backward.
 #include "gemm.h"
 #include "philox.h"
 
