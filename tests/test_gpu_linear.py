@@ -383,6 +383,41 @@ def test_offsets_past_32_bits(hip_ops):
 # ---------------------------------------------------------------------------
 # Dropout
 # ---------------------------------------------------------------------------
+def test_few_rows_with_a_weight_past_32_bits(hip_ops):
+    """Columns of a weight of more than 4 GiB against a call on their rows of it alone."""
+    T, K, N = 3, 32768, 69640
+    x = make((T, K), 1, BF)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    w = torch.empty((N, K), dtype=BF, device=DEV).normal_(0.0, 0.01, generator=g)
+    assert w.numel() * 2 > 1 << 32
+    y = hip_ops.linear_residual(x, w)
+    for at in (0, 65528, N - 200):
+        part = hip_ops.linear_residual(x, w[at:at + 200])
+        want = part.double()
+        # Roundings to 16 bits at the end of fp32 sums of K products.
+        assert (y[:, at:at + 200].double() - want).norm() <= 2 * unit(BF) * want.norm()
+    exact = x.double() @ w[-200:].double().t()
+    assert (y[:, -200:].double() - exact).norm() <= 2 * unit(BF) * exact.norm()
+
+
+def test_fp32_rows_further_apart_than_32_bits(hip_ops):
+    # 64 rows of a tile span more than 4 GiB; whole numbers, so that every sum is exact.
+    K = (1 << 24) + 1001
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randint(-1, 2, (2, K), generator=g, device=DEV).float().requires_grad_()
+    w = torch.randint(-1, 2, (3, K), generator=g, device=DEV).float().requires_grad_()
+    dy = torch.tensor([[1.0, -2.0, 3.0], [0.0, 4.0, -5.0]], device=DEV)
+    y = hip_ops.linear_residual(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with torch.no_grad():
+        for i in range(2):
+            for j in range(3):
+                assert y[i, j].item() == (x[i].double() * w[j].double()).sum().item()
+            assert torch.equal(dx[i], sum(dy[i, j] * w[j] for j in range(3)))
+        for j in range(3):
+            assert torch.equal(dw[j], sum(dy[i, j] * x[i] for i in range(2)))
+
+
 def test_dropout_past_32_bits(hip_ops):
     rows, cols = 1 << 20, 4104
     x = torch.ones((rows, cols), dtype=BF, device=DEV)
