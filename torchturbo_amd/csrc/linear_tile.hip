@@ -827,7 +827,8 @@ int launch(int tile, const LinArgs& p, hipStream_t s) {
   if (tile == LIN_T256) return go(&linear_big_kernel<LAYOUT, KIND, ET, KMASK, 256>);
   if (tile == LIN_T256x128) return go(&linear_big_kernel<LAYOUT, KIND, ET, KMASK, 128>);
   if (tile == LIN_T64) return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 64, 4>);
-  // A block has a CU to itself, and all of its memory, in a launch of at most one per CU.
+  // A block has a CU to itself, and all of its memory, in a launch of at most one per CU
+  // (four stages / two: 512 x 2048 -> 7168 24.0 / 25.0 us, 2048 cubed 24.8 / 25.6).
   if (ti * tj * p.splits <= 256) return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 4>);
   return go(&linear_mid_kernel<LAYOUT, KIND, ET, KMASK, 128, 2>);
 }
