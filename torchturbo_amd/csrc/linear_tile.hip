@@ -729,7 +729,7 @@ struct OddOperand {
 // (OddOperand) into the same LDS layouts, two stages; and results are stored at any
 // address, single elements at a row's end. It is bound by the instructions that move
 // k-tiles, not by products: 4001 x 1201 -> 1703 in bf16 62 us NT, 71 NN, 71 TN (0.26
-// PFLOP/s; 228, 316 and 366 us on the fp32 matrix instructions).
+// PFLOP/s; 228, 340 and 366 us on the fp32 matrix instructions).
 template <int LAYOUT, int KIND, int ET, int BT, bool TINY>
 __global__ __launch_bounds__(T_NT) void linear_odd_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;
