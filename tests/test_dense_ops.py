@@ -341,3 +341,37 @@ def test_lora_counter_dropout_is_opt_in(process_ops):
     torch.testing.assert_close(got, want)
     lora.eval()
     assert torch.equal(lora(x, counts, probs)[0], lora(x, counts, probs)[0])
+
+
+# ---------------------------------------------------------------------------
+# What autograd has to see
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", range(5))
+def test_tangents_and_transforms_are_refused(monkeypatch, which, grad):
+    """A dual tensor does not require gradients: a native call on its address would lose
+    the tangent without a word, so the operators raise, as all others of the package do."""
+    from torchturbo_amd.providers.hip import linear as hip_linear
+
+    # The native calls stubbed, everything before them as it is.
+    monkeypatch.setattr(hip_linear, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(hip_linear, "act_fwd", lambda x, w, *a: torch.zeros(x.shape[0], w.shape[0]))
+    monkeypatch.setattr(hip_linear, "residual_fwd",
+                        lambda x, w, *a: torch.zeros(x.shape[0], w.shape[0]))
+    leaves = [torch.ones(s) for s in ((4, 8), (6, 8), (6,), (4, 6), (4, 1))]
+    calls = [lambda v: HipLinearResidual()(*v)]
+    if which < 3:
+        calls.append(lambda v: HipLinearAct()(*v[:3]))
+    fwd = torch.autograd.forward_ad
+    for call in calls:
+        def of(t):
+            return call([t if i == which else v for i, v in enumerate(leaves)])
+
+        with torch.set_grad_enabled(grad):
+            assert of(leaves[which]).shape == (4, 6)
+            with fwd.dual_level():
+                assert of(leaves[which]).shape == (4, 6)  # no tangent: nothing to lose
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    of(fwd.make_dual(leaves[which], torch.ones_like(leaves[which])))
+            with pytest.raises(RuntimeError, match="autograd.Function"):
+                torch.func.jvp(of, (leaves[which],), (torch.ones_like(leaves[which]),))

@@ -151,8 +151,14 @@ def _operands(op, x, weight, bias):
         raise ValueError(f"{op} takes fewer than 2^31 rows")
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _autograd_sees(*tensors) -> bool:
+    """Whether the call has to go through its autograd function: for gradients, and for the
+    tangents and function transforms that the function refuses and a native call on addresses
+    would lose (a dual tensor does not require gradients)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return (torch.autograd.forward_ad._current_level >= 0
+            or torch._C._are_functorch_transforms_active())
 
 
 def _rows(t, width):
@@ -182,7 +188,7 @@ class HipLinearAct(OpImpl):
         n = weight.shape[0] // 2 if gated else weight.shape[0]
         x2, w = _rows(x, x.shape[-1]), weight.contiguous()
         b = None if bias is None else bias.contiguous()
-        if _wants_grad(x2, w, b):
+        if _autograd_sees(x2, w, b):
             y = LinearAct.apply(x2, w, b, act, gated)
         else:
             y = act_fwd(x2, w, b, act, gated, None)
@@ -216,7 +222,7 @@ class HipLinearResidual(OpImpl):
         b = None if bias is None else bias.contiguous()
         r = None if residual is None else _rows(residual, n)
         s = None if row_scale is None else row_scale.reshape(-1).contiguous()
-        if _wants_grad(x2, w, b, r, s):
+        if _autograd_sees(x2, w, b, r, s):
             y = LinearResidual.apply(x2, w, b, r, s, threshold, key)
         else:
             y = residual_fwd(x2, w, b, r, s, threshold, key)
