@@ -375,3 +375,39 @@ def test_tangents_and_transforms_are_refused(monkeypatch, which, grad):
                     of(fwd.make_dual(leaves[which], torch.ones_like(leaves[which])))
             with pytest.raises(RuntimeError, match="autograd.Function"):
                 torch.func.jvp(of, (leaves[which],), (torch.ones_like(leaves[which]),))
+
+
+# ---------------------------------------------------------------------------
+# What a caller attaches to the modules
+# ---------------------------------------------------------------------------
+def shared_layer(expert):
+    torch.manual_seed(6)
+    cfg = shared_config()
+    layer = MoELayer(cfg, None, MoESubmodules(experts=ModuleSpec(module=GroupedMLP)))
+    layer.shared_expert = expert(cfg)
+    layer.shared_expert_gate = torch.nn.Linear(16, 1, bias=False)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.normal_(std=0.2)
+    return layer
+
+
+def test_another_shared_expert_runs_before_its_gate(process_ops):
+    """The order of the reference: that of hooks, and of random draws in either of the two."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    layer = shared_layer(lambda cfg: torch.nn.Sequential(torch.nn.Linear(16, 16),
+                                                         torch.nn.Dropout(0.5)))
+    layer.shared_expert_gate = torch.nn.Sequential(torch.nn.Dropout(0.5), torch.nn.Linear(16, 1))
+    seen = []
+    layer.shared_expert.register_forward_hook(lambda *a: seen.append("expert"))
+    layer.shared_expert_gate.register_forward_hook(lambda *a: seen.append("gate"))
+    x = torch.randn(3, 5, 16)
+    torch.manual_seed(1)
+    got, _ = layer(x)
+    assert seen == ["expert", "gate"]
+    expert, gate = layer.shared_expert, layer.shared_expert_gate
+    layer.shared_expert = None
+    routed, _ = layer(x)
+    torch.manual_seed(1)
+    shared = expert(x)
+    assert torch.equal(got, routed + F.sigmoid(gate(x)) * shared)

@@ -168,13 +168,18 @@ class MoELayer(BaseMoELayer):
                 output = self._dispatched_experts(hidden_states, probs, routing_map,
                                                   expert_indices)
         if self.shared_expert is not None:
-            gate = F.sigmoid(self.shared_expert_gate(hidden_states))
-            if (type(self.shared_expert) is SharedExpertMLP
-                    and gate.shape == (*hidden_states.shape[:-1], 1)):
-                # The token's gate and the sum in the expert's last product.
-                output = self.shared_expert(hidden_states, output, gate)
+            if type(self.shared_expert) is SharedExpertMLP:
+                gate = F.sigmoid(self.shared_expert_gate(hidden_states))
+                if gate.shape == (*hidden_states.shape[:-1], 1):
+                    # The token's gate and the sum in the expert's last product.
+                    output = self.shared_expert(hidden_states, output, gate)
+                else:
+                    output = output + gate * self.shared_expert(hidden_states)
             else:
-                output = output + gate * self.shared_expert(hidden_states)
+                # Any other module runs before its gate (moe_layer.py:175-182): hooks and random
+                # draws keep their order.
+                shared = self.shared_expert(hidden_states)
+                output = output + F.sigmoid(self.shared_expert_gate(hidden_states)) * shared
         if self.shared_experts is not None:
             if type(self.shared_experts) is SharedExpertMLP:
                 output = self.shared_experts(hidden_states, output)
