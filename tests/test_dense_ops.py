@@ -411,3 +411,74 @@ def test_another_shared_expert_runs_before_its_gate(process_ops):
     torch.manual_seed(1)
     shared = expert(x)
     assert torch.equal(got, routed + F.sigmoid(gate(x)) * shared)
+
+
+class _FusedOps:
+    """Stands in for the process dispatcher where the HIP operators are chosen."""
+
+    def __init__(self, **chosen):
+        self.chosen = {"lora_residual": "hip_lora_residual", "dropout": "hip_dropout",
+                       "grouped_matmul": "hip_grouped_matmul",
+                       "linear_residual": "hip_linear_residual", **chosen}
+        self.calls = []
+
+    def selected_impl_name(self, op):
+        return self.chosen[op]
+
+    def lora_residual(self, base, x, a, b, counts, scale, **dropout):
+        self.calls.append(("lora_residual", sorted(dropout)))
+        return base
+
+    def dropout(self, x, p, key):
+        self.calls.append(("dropout", p))
+        return x
+
+
+def _hook(drop):
+    drop.register_forward_hook(lambda *a: None)
+
+
+def _pre_hook(drop):
+    drop.register_forward_pre_hook(lambda *a: None)
+
+
+def _backward_hook(drop):
+    drop.register_full_backward_hook(lambda *a: None)
+
+
+def _replaced(drop):
+    drop.forward = type(drop).forward.__get__(drop)
+
+
+class _OnGpu:
+    is_cuda, device = True, torch.device("cpu")
+
+
+@pytest.mark.filterwarnings("ignore:For backward hooks to be called")
+@pytest.mark.parametrize("attach, chosen, fused", [
+    (None, {}, True), (_hook, {}, False), (_pre_hook, {}, False), (_backward_hook, {}, False),
+    (_replaced, {}, False), (None, {"dropout": "other"}, False),
+    (None, {"lora_residual": "other"}, False)])
+def test_lora_calls_a_dropout_that_something_is_attached_to(monkeypatch, attach, chosen, fused):
+    """The fused operator makes the mask itself only where calling the module would do
+    nothing else: hooks run, and another implementation that was chosen is called."""
+    from torchturbo_amd.moe import dropout as m_dropout
+    from torchturbo_amd.moe import lora as m_lora
+
+    fake = _FusedOps(**chosen)
+    monkeypatch.setattr(m_lora, "ops", fake)
+    monkeypatch.setattr(m_dropout, "ops", fake)
+    monkeypatch.setattr(m_lora, "op_resolves", lambda name: True)
+    cfg = MoEConfig(hidden_size=8, moe_ffn_hidden_size=6, gated_linear_unit=True,
+                    activation_func=F.silu)
+    lora = GroupedMLPLoRA(GroupedMLP(2, False, cfg), "default", r=2, lora_dropout=0.3,
+                          counter_dropout=True)
+    drop = lora.lora_dropout["default"]
+    x, counts = _OnGpu(), torch.tensor([4, 5])
+    if attach is not None:
+        attach(drop)
+    lora._add_residual(torch.zeros(1), x, counts, "default", lora.lora_A, lora.lora_B)
+    if fused:
+        assert fake.calls == [("lora_residual", ["dropout_key", "dropout_p"])]
+    else:
+        assert fake.calls == [("dropout", 0.3), ("lora_residual", [])]

@@ -32,6 +32,7 @@ import torch.nn as nn
 from ..dispatch import op_resolves, ops
 from .dropout import CounterDropout
 from .experts import GroupedMLP
+from .module import attached
 
 try:  # PEFT integration is optional (the reference requires it)
     from peft.tuners.tuners_utils import BaseTunerLayer as _TunerBase
@@ -276,7 +277,11 @@ class GroupedMLPLoRA(nn.Module, _TunerBase):
         # In place of the HIP grouped product only: another one chosen for it is called.
         fused = (x.is_cuda and op_resolves("lora_residual")
                  and ops.selected_impl_name("grouped_matmul") == "hip_grouped_matmul")
+        # The op makes the mask in place of a CounterDropout that nothing is attached to, where
+        # neither of the two ops has been replaced.
         if (fused and type(drop) is CounterDropout and drop.active
+                and not attached(drop, "draw_key")
+                and ops.selected_impl_name("lora_residual") == "hip_lora_residual"
                 and ops.selected_impl_name("dropout") == "hip_dropout"):
             key = drop.draw_key(x.device)
             y = ops.lora_residual(base, x, a.weight, b.weight, counts, scale, dropout_p=drop.p,
