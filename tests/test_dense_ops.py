@@ -482,3 +482,57 @@ def test_lora_calls_a_dropout_that_something_is_attached_to(monkeypatch, attach,
         assert fake.calls == [("lora_residual", ["dropout_key", "dropout_p"])]
     else:
         assert fake.calls == [("dropout", 0.3), ("lora_residual", [])]
+
+
+@pytest.mark.parametrize("attach", [_hook, _pre_hook, _backward_hook, _replaced, "module"])
+@pytest.mark.parametrize("scaled", [True, False])
+def test_shared_expert_calls_a_dropout_that_something_is_attached_to(process_ops, monkeypatch,
+                                                                     attach, scaled):
+    """The same values as with the mask made in the product's epilogue."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    torch.manual_seed(4)
+    mlp = SharedExpertMLP(shared_config(), dropout=0.4)
+    x, r, s = torch.randn(7, 16), torch.randn(7, 16), torch.rand(7) if scaled else None
+    torch.manual_seed(5)
+    want = mlp(x, r, s)
+    calls, forward = [], CounterDropout.forward
+    monkeypatch.setattr(CounterDropout, "forward",
+                        lambda self, v: calls.append(v.shape) or forward(self, v))
+    if attach == "module":
+        mlp.dropout = torch.nn.Sequential(mlp.dropout)
+    else:
+        attach(mlp.dropout)
+    torch.manual_seed(5)
+    torch.testing.assert_close(mlp(x, r, s), want)
+    assert calls == [(7, 16)]
+    torch.manual_seed(5)
+    torch.testing.assert_close(mlp(x), want - r if s is None else (want - r) / s[:, None],
+                               rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("chosen, calls", [
+    ({}, [("linear_residual", True)]),
+    ({"dropout": "other"}, [("linear_residual", False), ("dropout", 0.4)]),
+    # Another product brings a dropout of its own.
+    ({"dropout": "other", "linear_residual": "other"}, [("linear_residual", True)])])
+def test_shared_expert_uses_the_dropout_that_was_chosen(monkeypatch, chosen, calls):
+    from torchturbo_amd.moe import dropout as m_dropout
+    from torchturbo_amd.moe import shared_experts as m_shared
+
+    fake = _FusedOps(**chosen)
+    fake.linear_act = lambda x, w, b, **how: x @ w[:12].t()
+
+    def linear_residual(x, w, b, residual=None, row_scale=None, *, dropout_p=0.0, dropout_key=None):
+        fake.calls.append(("linear_residual", dropout_p > 0))
+        return x @ w.t()
+
+    fake.linear_residual = linear_residual
+    for module in (m_dropout, m_shared):
+        monkeypatch.setattr(module, "ops", fake)
+    mlp = SharedExpertMLP(shared_config(), dropout=0.4)
+    mlp(torch.randn(7, 16), torch.randn(7, 16))
+    assert fake.calls == calls
+    fake.calls.clear()
+    mlp.eval()  # nothing to drop: one product, whatever is chosen
+    mlp(torch.randn(7, 16), torch.randn(7, 16))
+    assert fake.calls == [("linear_residual", False)]

@@ -16,6 +16,7 @@ from torch.nn.parameter import Parameter
 
 from ..dispatch import ops
 from .dropout import CounterDropout
+from .module import attached
 from .moe_config import MoEConfig
 
 
@@ -64,11 +65,26 @@ class SharedExpertMLP(torch.nn.Module):
         h = ops.linear_act(hidden_states, self.weight1, self.bias1,
                            activation_func=self.config.activation_func,
                            gated=self.config.gated_linear_unit)
+        drop = self.dropout
+        if not self._dropout_in_epilogue(drop):
+            y = drop(ops.linear_residual(h, self.weight2, self.bias2))
+            if row_scale is not None:
+                y = y * row_scale.reshape(*y.shape[:-1], 1)
+            return (y if residual is None else residual + y).to(hidden_states.dtype)
         p, key = 0.0, None
-        if self.dropout.active:
-            p, key = self.dropout.p, self.dropout.draw_key(hidden_states.device)
+        if drop.active:
+            p, key = drop.p, drop.draw_key(hidden_states.device)
         return ops.linear_residual(h, self.weight2, self.bias2, residual, row_scale, dropout_p=p,
                                    dropout_key=key)
+
+    @staticmethod
+    def _dropout_in_epilogue(drop) -> bool:
+        """Whether ``linear_residual`` may make the mask in place of a call of ``drop``: nothing
+        is attached to it, and the HIP product's mask is that of the ``dropout`` op chosen."""
+        if type(drop) is not CounterDropout or attached(drop, "draw_key"):
+            return False
+        return (not drop.active or ops.selected_impl_name("dropout") == "hip_dropout"
+                or ops.selected_impl_name("linear_residual") != "hip_linear_residual")
 
 
 __all__ = ["SharedExpertMLP"]
