@@ -536,3 +536,28 @@ def test_shared_expert_uses_the_dropout_that_was_chosen(monkeypatch, chosen, cal
     mlp.eval()  # nothing to drop: one product, whatever is chosen
     mlp(torch.randn(7, 16), torch.randn(7, 16))
     assert fake.calls == [("linear_residual", False)]
+
+
+@pytest.mark.parametrize("name", ["shared_expert", "shared_experts"])
+@pytest.mark.parametrize("attach", ["hook", "pre_hook", "replaced"])
+def test_what_is_attached_to_a_shared_expert_sees_the_expert_alone(process_ops, name, attach):
+    """Its input, and its output without the gate and the routed experts, as with any module."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    layer = shared_layer(SharedExpertMLP)
+    expert = layer.shared_expert
+    if name == "shared_experts":
+        layer.shared_expert, layer.shared_experts = None, expert
+    x = torch.randn(3, 5, 16)
+    want, own = layer(x)[0], expert(x)
+    seen = []
+    if attach == "hook":
+        expert.register_forward_hook(lambda m, args, out: seen.append((args, out)))
+    elif attach == "pre_hook":
+        expert.register_forward_pre_hook(lambda m, args: seen.append((args, own)))
+    else:
+        forward = expert.forward
+        expert.forward = lambda v: seen.append(((v,), forward(v))) or seen[-1][1]
+    torch.testing.assert_close(layer(x)[0], want)
+    (args, out), = seen
+    assert len(args) == 1 and torch.equal(args[0], x)
+    torch.testing.assert_close(out, own)

@@ -18,7 +18,7 @@ import torch.nn.functional as F
 
 from ..dispatch import ops
 from .experts import Fp8GroupedMLP, GroupedMLP
-from .module import ModuleSpec, build_module
+from .module import ModuleSpec, attached, build_module
 from .moe_config import MoEConfig
 from .router import TopKRouter
 from .shared_experts import SharedExpertMLP
@@ -168,7 +168,7 @@ class MoELayer(BaseMoELayer):
                 output = self._dispatched_experts(hidden_states, probs, routing_map,
                                                   expert_indices)
         if self.shared_expert is not None:
-            if type(self.shared_expert) is SharedExpertMLP:
+            if self._adds_itself(self.shared_expert):
                 gate = F.sigmoid(self.shared_expert_gate(hidden_states))
                 if gate.shape == (*hidden_states.shape[:-1], 1):
                     # The token's gate and the sum in the expert's last product.
@@ -181,11 +181,17 @@ class MoELayer(BaseMoELayer):
                 shared = self.shared_expert(hidden_states)
                 output = output + F.sigmoid(self.shared_expert_gate(hidden_states)) * shared
         if self.shared_experts is not None:
-            if type(self.shared_experts) is SharedExpertMLP:
+            if self._adds_itself(self.shared_experts):
                 output = self.shared_experts(hidden_states, output)
             else:
                 output = output + self.shared_experts(hidden_states)
         return output
+
+    @staticmethod
+    def _adds_itself(expert) -> bool:
+        """Whether ``expert`` takes the sum (and a token's gate) into its last product. With
+        something attached it is called as any module is: hooks see its own output."""
+        return type(expert) is SharedExpertMLP and not attached(expert)
 
     def _dispatched_experts(self, hidden_states, probs, routing_map, expert_indices):
         d = self.token_dispatcher
