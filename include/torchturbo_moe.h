@@ -417,6 +417,7 @@ int tt_moe_experts_fwd(const void* x, int dtype, int64_t num_tokens, int64_t hid
  * fp32 and are rounded once, where they are stored. Any size, 0 included, any
  * alignment of the elements; 16-bit operands whose k and n are multiples of 8 and whose
  * addresses are multiples of 16 run fastest. A workspace is aligned to 256 bytes.
+ * Tensors that a call reads or writes are not NULL, unless they have no elements.
  * activation: 0 none, 1 SiLU, 2 GELU (erf form).
  *
  * tt_linear_workspace: bytes of scratch of a forward of these sizes (0: none). With

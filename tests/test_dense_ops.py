@@ -561,3 +561,70 @@ def test_what_is_attached_to_a_shared_expert_sees_the_expert_alone(process_ops, 
     (args, out), = seen
     assert len(args) == 1 and torch.equal(args[0], x)
     torch.testing.assert_close(out, own)
+
+
+# ---------------------------------------------------------------------------
+# Pointers of the entry points
+# ---------------------------------------------------------------------------
+def pointers(name, given, **sizes):
+    """A call of a C entry point whose pointers are NULL but for those ``given`` (an address
+    that no kernel ever gets: every such call is refused)."""
+    s = {"m": 4, "k": 8, "n": 8, "t": 0, "act": 1, "gated": 1, "bytes": 1 << 40, **sizes}
+    size = (L.TT_BF16, s["m"], s["k"], s["n"])
+    given = given if isinstance(given, dict) else dict.fromkeys(given, 4096)
+    g = {n: ctypes.c_void_p(v) for n, v in given.items()}.get
+    L.call(name, *{
+        "tt_linear_act_fwd": lambda: (g("x"), g("w"), g("bias"), 0, *size, s["act"], s["gated"],
+                                      g("pre"), g("y"), g("ws"), s["bytes"], None),
+        "tt_linear_act_bwd": lambda: (g("dy"), g("x"), g("w"), g("pre"), *size, s["act"],
+                                      s["gated"], g("dx"), g("dw"), g("db"), 0, g("ws"),
+                                      s["bytes"], None),
+        "tt_linear_residual_fwd": lambda: (g("x"), g("w"), g("bias"), 0, g("res"), g("scale"), 0,
+                                           *size, s["t"], g("key"), g("y"), g("ws"), s["bytes"],
+                                           None),
+        "tt_linear_residual_bwd": lambda: (g("dy"), g("x"), g("w"), g("bias"), 0, g("scale"), 0,
+                                           *size, s["t"], g("key"), g("dx"), g("dw"), g("db"),
+                                           g("ds"), g("ws"), s["bytes"], None),
+    }[name]())
+
+
+@pytest.mark.parametrize("name, given, missing", [
+    ("tt_linear_act_fwd", "w y ws", "x"),
+    ("tt_linear_act_fwd", "x y ws", "w"),
+    ("tt_linear_act_fwd", "x w ws", "y"),
+    ("tt_linear_act_fwd", "x w y", "the workspace"),
+    ("tt_linear_act_bwd", "x w pre dx dw ws", "dy"),
+    ("tt_linear_act_bwd", "dy x w dx ws", "pre"),
+    ("tt_linear_act_bwd", "dy db ws", "pre"),
+    ("tt_linear_act_bwd", "dy x pre dx ws", "w"),
+    ("tt_linear_act_bwd", "dy w pre dw ws", "x"),
+    ("tt_linear_act_bwd", "dy x w pre dx dw", "the workspace"),
+    ("tt_linear_residual_fwd", "w y ws", "x"),
+    ("tt_linear_residual_fwd", "x y ws res scale bias", "w"),
+    ("tt_linear_residual_fwd", "x w ws", "y"),
+    ("tt_linear_residual_fwd", "x w y", "the workspace"),
+    ("tt_linear_residual_bwd", "x w dx dw ws", "dy"),
+    ("tt_linear_residual_bwd", "db ws", "dy"),
+    ("tt_linear_residual_bwd", "dy x dx ws", "w"),
+    ("tt_linear_residual_bwd", "dy x scale dw ws", "w"),
+    ("tt_linear_residual_bwd", "dy x scale ds ws", "w"),
+    ("tt_linear_residual_bwd", "dy w dw ws", "x"),
+    ("tt_linear_residual_bwd", "dy w scale ds ws", "x"),
+    ("tt_linear_residual_bwd", "dy x w dx db", "the workspace"),
+])
+def test_null_pointers_are_refused(name, given, missing):
+    with pytest.raises(ValueError, match=rf"null pointer \({missing}\)"):
+        pointers(name, given.split())
+
+
+@pytest.mark.parametrize("name, given", [
+    ("tt_linear_act_fwd", "x w y"), ("tt_linear_residual_fwd", "x w y"),
+    ("tt_linear_act_bwd", "dy x w pre dx"), ("tt_linear_residual_bwd", "dy x w dx")])
+def test_a_workspace_off_its_alignment_is_refused(name, given):
+    with pytest.raises(ValueError, match="aligned to 256 bytes"):
+        pointers(name, {**{n: 4096 for n in given.split()}, "ws": 4096 + 16})
+
+
+def test_calls_that_ask_for_no_gradient_launch_nothing():
+    pointers("tt_linear_act_bwd", [])
+    pointers("tt_linear_residual_bwd", ["scale", "key"], t=7)

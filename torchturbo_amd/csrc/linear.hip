@@ -438,6 +438,19 @@ int vector_ok(const char* what, const void* p, int dtype) {
     if (rc_ != TT_OK) return rc_; \
   } while (0)
 
+// A pointer that the call reads or writes (`used`) has to be there, a workspace that it
+// takes anything of has to be there and aligned: the kernels get addresses and cannot tell.
+int pointer_ok(const char* what, const void* p, bool used) {
+  TT_REQUIRE(p != nullptr || !used, "linear: null pointer (%s)", what);
+  return TT_OK;
+}
+int workspace_ok(const void* ws, size_t bytes) {
+  TT_TRY(pointer_ok("the workspace", ws, bytes != 0));
+  TT_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 256 == 0,
+             "linear: the workspace must be aligned to 256 bytes");
+  return TT_OK;
+}
+
 template <typename F>
 int typed(int dtype, F f) {
   switch (dtype) {
@@ -547,6 +560,10 @@ extern "C" int tt_linear_act_fwd(const void* x, const void* w, const void* bias,
   TT_TRY(vector_ok("the bias", bias, bias_dtype));
   TT_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, "linear: unknown activation %d", act);
   if (m == 0 || n == 0) return TT_OK;
+  TT_TRY(pointer_ok("x", x, k > 0));
+  TT_TRY(pointer_ok("w", w, k > 0));
+  TT_TRY(pointer_ok("y", y, true));
+  TT_TRY(workspace_ok(workspace, workspace_bytes));
   LinArgs p{};
   p.a = x;
   p.b = w;
@@ -583,8 +600,15 @@ extern "C" int tt_linear_act_bwd(const void* dy, const void* x, const void* w, c
   TT_TRY(vector_ok("the bias", dbias, bias_dtype));
   TT_REQUIRE(act >= ACT_NONE && act <= ACT_GELU, "linear: unknown activation %d", act);
   const bool own = act != ACT_NONE || gated;
-  TT_REQUIRE(workspace_bytes >= tt_linear_act_bwd_workspace(dtype, m, k, n, act, gated),
-             "linear_act_bwd: the workspace is too small");
+  const size_t needed = tt_linear_act_bwd_workspace(dtype, m, k, n, act, gated);
+  TT_REQUIRE(workspace_bytes >= needed, "linear_act_bwd: the workspace is too small");
+  if (dx == nullptr && dw == nullptr && dbias == nullptr) return TT_OK;
+  const bool products = m > 0 && k > 0 && n > 0;
+  TT_TRY(pointer_ok("dy", dy, m > 0 && n > 0));
+  TT_TRY(pointer_ok("pre", pre, own && m > 0 && n > 0));
+  TT_TRY(pointer_ok("w", w, dx != nullptr && products));
+  TT_TRY(pointer_ok("x", x, dw != nullptr && products));
+  TT_TRY(workspace_ok(workspace, needed));
   const int64_t width = gated ? 2 * n : n;
   Pieces ws{static_cast<char*>(workspace), workspace_bytes};
   void* const da = own ? ws.take((size_t)m * width * tt_elem_size(dtype)) : nullptr;
@@ -639,6 +663,10 @@ extern "C" int tt_linear_residual_fwd(const void* x, const void* w, const void* 
   TT_REQUIRE(threshold >= 0 && threshold <= 65536, "linear: the threshold must be in [0, 65536]");
   TT_REQUIRE(threshold == 0 || key != nullptr, "linear: dropout without a key");
   if (m == 0 || n == 0) return TT_OK;
+  TT_TRY(pointer_ok("x", x, k > 0));
+  TT_TRY(pointer_ok("w", w, k > 0));
+  TT_TRY(pointer_ok("y", y, true));
+  TT_TRY(workspace_ok(workspace, workspace_bytes));
   LinArgs p{};
   p.a = x;
   p.b = w;
@@ -686,10 +714,16 @@ extern "C" int tt_linear_residual_bwd(const void* dy, const void* x, const void*
   TT_REQUIRE(threshold == 0 || key != nullptr, "linear: dropout without a key");
   TT_REQUIRE(row_scale != nullptr || dscale == nullptr,
              "linear_residual_bwd: the scale's gradient needs a row scale");
-  TT_REQUIRE(workspace_bytes >= tt_linear_residual_bwd_workspace(dtype, m, k, n,
-                                                                 row_scale != nullptr,
-                                                                 threshold != 0),
-             "linear_residual_bwd: the workspace is too small");
+  const size_t needed =
+      tt_linear_residual_bwd_workspace(dtype, m, k, n, row_scale != nullptr, threshold != 0);
+  TT_REQUIRE(workspace_bytes >= needed, "linear_residual_bwd: the workspace is too small");
+  if (dx == nullptr && dw == nullptr && dbias == nullptr && dscale == nullptr) return TT_OK;
+  // With a row scale the weight's gradient takes the rows that the product for dx scales.
+  const bool back = dx != nullptr || dscale != nullptr || (row_scale != nullptr && dw != nullptr);
+  TT_TRY(pointer_ok("dy", dy, m > 0 && n > 0));
+  TT_TRY(pointer_ok("w", w, back && m > 0 && k > 0 && n > 0));
+  TT_TRY(pointer_ok("x", x, (dw != nullptr || dscale != nullptr) && m > 0 && k > 0));
+  TT_TRY(workspace_ok(workspace, needed));
   const size_t es = tt_elem_size(dtype);
   const float alpha = keep_inverse(threshold);
   Pieces ws{static_cast<char*>(workspace), workspace_bytes};
@@ -725,7 +759,7 @@ extern "C" int tt_linear_residual_bwd(const void* dy, const void* x, const void*
   // The weight's gradient takes the rows times their scale, which the pass for dx writes;
   // that pass runs for them, or for the scale's gradient, where dx is not wanted.
   const bool scaled_rows = row_scale != nullptr && dw != nullptr;
-  if (dx != nullptr || dscale != nullptr || scaled_rows)
+  if (back)
     TT_TRY(data_gradient(g, w, x, row_scale, scale_dtype, dtype, m, k, n, alpha, dx,
                          scaled_rows ? rows : nullptr, dscale != nullptr ? dots : nullptr, ws.at,
                          ws.left, S(stream)));
