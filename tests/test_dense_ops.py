@@ -628,3 +628,12 @@ def test_a_workspace_off_its_alignment_is_refused(name, given):
 def test_calls_that_ask_for_no_gradient_launch_nothing():
     pointers("tt_linear_act_bwd", [])
     pointers("tt_linear_residual_bwd", ["scale", "key"], t=7)
+
+
+@pytest.mark.parametrize("name", ["tt_lora_down_dropout", "tt_lora_up_dropout",
+                                  "tt_lora_wgrad_dropout"])
+@pytest.mark.parametrize("missing", range(4))
+def test_null_pointers_of_the_adapters_are_refused(name, missing):
+    at = [None if i == missing else ctypes.c_void_p(4096) for i in range(4)]
+    with pytest.raises(ValueError, match="null pointer"):
+        L.call(name, at[0], at[1], L.TT_BF16, 4, 8, 4, 2, at[2], 5, P, at[3], None)

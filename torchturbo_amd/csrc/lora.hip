@@ -624,9 +624,11 @@ int lora_checks(int dtype, int64_t m, int64_t c, int r, int E, const void* p0, c
   TT_REQUIRE(row_blocks(m, E) * ((c + 255) / 256) < 0x7fffffff, "lora: grid too large");
   return TT_OK;
 }
-int drop_checks(int32_t threshold, const int64_t* key) {
+// `there`: whether every tensor that the call reads or writes is (an empty one may be NULL).
+int drop_checks(int32_t threshold, const int64_t* key, bool there) {
   TT_REQUIRE(threshold >= 1 && threshold <= 65536, "lora: the threshold must be in [1, 65536]");
   TT_REQUIRE(key != nullptr, "lora: dropout without a key");
+  TT_REQUIRE(there, "lora: null pointer");
   return TT_OK;
 }
 Drop drop_of(int32_t threshold, const int64_t* key) {
@@ -656,7 +658,8 @@ extern "C" int tt_lora_down_dropout(const void* in, const float* w, int dtype, i
                                     int32_t threshold, const int64_t* key, float* out,
                                     void* stream) {
   int rc = lora_checks(dtype, m, c, r, num_experts, in, w, nullptr);
-  if (rc == TT_OK) rc = drop_checks(threshold, key);
+  const bool there = m == 0 || (out && counts && (c == 0 || (in && w)));
+  if (rc == TT_OK) rc = drop_checks(threshold, key, there);
   if (rc != TT_OK) return rc;
   if (m == 0) return TT_OK;
   const LoraArgs a{static_cast<const uint16_t*>(in), w, nullptr, out, m, (int)c, r, 1.0f,
@@ -688,7 +691,8 @@ extern "C" int tt_lora_up_dropout(const float* h, const float* w, int dtype, int
                                   int32_t r, int32_t num_experts, const int64_t* counts,
                                   int32_t threshold, const int64_t* key, void* out, void* stream) {
   int rc = lora_checks(dtype, m, c, r, num_experts, w, out, nullptr);
-  if (rc == TT_OK) rc = drop_checks(threshold, key);
+  const bool there = m == 0 || c == 0 || (h && w && counts && out);
+  if (rc == TT_OK) rc = drop_checks(threshold, key, there);
   if (rc != TT_OK) return rc;
   if (m == 0 || c == 0) return TT_OK;
   const LoraArgs a{nullptr, w, nullptr, out, m, (int)c, r, 1.0f, num_experts, counts,
@@ -719,7 +723,8 @@ extern "C" int tt_lora_wgrad_dropout(const void* in, const float* v, int dtype, 
                                      const int64_t* counts, int32_t threshold, const int64_t* key,
                                      float* out, void* stream) {
   int rc = lora_checks(dtype, m, c, r, num_experts, in, out, nullptr);
-  if (rc == TT_OK) rc = drop_checks(threshold, key);
+  const bool there = c == 0 || (counts && out && (m == 0 || (in && v)));
+  if (rc == TT_OK) rc = drop_checks(threshold, key, there);
   if (rc != TT_OK) return rc;
   if (c == 0) return TT_OK;
   const LoraArgs a{static_cast<const uint16_t*>(in), nullptr, nullptr, out, m, (int)c, r, 1.0f,
