@@ -637,3 +637,17 @@ def test_null_pointers_of_the_adapters_are_refused(name, missing):
     at = [None if i == missing else ctypes.c_void_p(4096) for i in range(4)]
     with pytest.raises(ValueError, match="null pointer"):
         L.call(name, at[0], at[1], L.TT_BF16, 4, 8, 4, 2, at[2], 5, P, at[3], None)
+
+
+@pytest.mark.parametrize("m, base, transposed, taken", [
+    (0, None, 0, True), (0, P, 0, True), (0, None, 1, True), (0, P, 1, False),
+    (4, None, 0, False), (4, P, 1, False)])
+def test_base_of_the_up_projection(m, base, transposed, taken):
+    """A base in the gradient's form is refused, of an empty call too, whose base may
+    be NULL in the forward's."""
+    args = ("tt_lora_up", P, P, base, L.TT_BF16, m, 8, 4, transposed, 1.0, 2, P, P, None)
+    if taken:
+        L.call(*args)
+    else:
+        with pytest.raises(ValueError, match="forward form only"):
+            L.call(*args)

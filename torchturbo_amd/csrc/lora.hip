@@ -674,9 +674,11 @@ extern "C" int tt_lora_up(const float* h, const float* w, const void* base, int 
                           int32_t num_experts, const int64_t* counts, void* out, void* stream) {
   const int rc = lora_checks(dtype, m, c, r, num_experts, base, w, out);
   if (rc != TT_OK) return rc;
-  if (m == 0 || c == 0) return TT_OK;
-  TT_REQUIRE((base == nullptr) == (transposed != 0),
+  // The base of an empty call may be NULL.
+  const bool empty = m == 0 || c == 0;
+  TT_REQUIRE(transposed ? base == nullptr : empty || base != nullptr,
              "lora: the base is added in the forward form only");
+  if (empty) return TT_OK;
   const LoraArgs a{nullptr, w, static_cast<const uint16_t*>(base), out, m, (int)c, r, scale,
                    num_experts, counts, Drop{}};
   return typed(dtype, r, [&](auto tt, auto rt) {
