@@ -658,3 +658,23 @@ def test_shared_expert_and_adapters_in_the_layer(process_ops):
     near(out, want.detach(), "out")
     for n in wg:
         near(grads[n], wg[n], n)
+
+
+# ---------------------------------------------------------------------------
+# Ends of tiles
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("K", [40, 72, 200, 1032])
+def test_scale_gradient_counts_its_columns_alone(hip_ops, K):
+    """Finite operands with a finite gradient: a tile's columns past K hold sums of one row of
+    dy with the weight's next row, here past the largest fp32 number, and count for nothing."""
+    T, N = 70, 48
+    x, w = make((T, K), 1, BF), make((N, K), 2, BF)
+    s, dy = make((T, 1), 3, BF), make((T, N), 4, BF)
+    w[0], w[1, :32], dy[5, 0], dy[5, 1] = 0.0, 4.0, 3e38, 0.0
+    leaf = s.clone().requires_grad_()
+    ds, = torch.autograd.grad(hip_ops.linear_residual(x, w, None, None, leaf), leaf, dy)
+    X, W, G = wide(x, w, dy)
+    want, mag = (X * (G @ W)).sum(1), (X.abs() * (G.abs() @ W.abs())).sum(1)
+    assert want.abs().max() < 1e6
+    within(ds.reshape(-1), want, unit(BF) * want.abs() +
+           1.01 * (gamma(N) + gamma(K) + 2.0 ** -22) * mag, "ds")

@@ -336,7 +336,8 @@ __device__ __forceinline__ void tile_finish(const LinArgs& p, F stage, lds_char*
         __builtin_amdgcn_raw_buffer_store_b128(pack8<ET>(x), xs, (int)(col_ok ? at16 : DM_OOB), 0, 0);
         if (p.dots != nullptr) {
           static_assert(LIN_DOT == 32, "four lanes of eight columns");
-          dot = sum4(dot);
+          // Sums past column J are of other rows of B: 0 times an infinite one is no number.
+          dot = sum4(col_ok ? dot : 0.f);
           const int64_t i = i0 + q + rr;
           if ((lane & 3) == 0 && i < p.I && col_ok) p.dots[i * nd + j / LIN_DOT] = dot;
         }
