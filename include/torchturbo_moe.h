@@ -424,6 +424,11 @@ int tt_moe_experts_fwd(const void* x, int dtype, int64_t num_tokens, int64_t hid
  * less, it does not split its reduction. The backward's scratch has a query of its own
  * and is needed in full.
  *
+ * tt_linear_plan: which kernel runs a product of operation `op` (TT_LINEAR_...) of these
+ * sizes, one of TT_LINEAR_KERNEL_..., plus 256 times the parts its reduction is split into.
+ * pass: 0 the forward, 1 the gradient of x, 2 that of w; aligned: whether the operands'
+ * addresses are multiples of 16. Host arithmetic; -1 for sizes that no call takes, or empty
+ * results.
  * tt_linear_act_fwd: a = x w^T + bias; y [m, n] = act(a), w [n, k]; gated: y =
  *   act(a[:, :n]) * a[:, n:], w [2n, k], the gate's rows first. pre (or NULL): a in
  *   fp32, [m, n] or [m, 2n], for the backward (not needed for activation 0 without gate).
@@ -437,6 +442,11 @@ int tt_moe_experts_fwd(const void* x, int dtype, int64_t num_tokens, int64_t hid
  *   row_scale g, dscale [m] = <x_i, (g w)_i> + <g_i, bias>; each skipped when NULL.
  *   bias is read for dscale only; bias_dtype is dbias's as well. */
 enum { TT_LINEAR_ACT = 0, TT_LINEAR_GATED = 1, TT_LINEAR_RESIDUAL = 2 };
+enum { TT_LINEAR_KERNEL_F32 = 0, TT_LINEAR_KERNEL_ROWS = 1, TT_LINEAR_KERNEL_T64 = 2,
+       TT_LINEAR_KERNEL_T128 = 3, TT_LINEAR_KERNEL_T256X128 = 4, TT_LINEAR_KERNEL_T256 = 5,
+       TT_LINEAR_KERNEL_ODD64 = 6, TT_LINEAR_KERNEL_ODD128 = 7 };
+int tt_linear_plan(int32_t op, int32_t pass, int dtype, int64_t m, int64_t k, int64_t n,
+                   int32_t aligned);
 size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t k, int64_t n);
 int tt_linear_act_fwd(const void* x, const void* w, const void* bias, int bias_dtype, int dtype,
                       int64_t m, int64_t k, int64_t n, int32_t activation, int32_t gated,

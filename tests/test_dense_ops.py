@@ -651,3 +651,30 @@ def test_base_of_the_up_projection(m, base, transposed, taken):
     else:
         with pytest.raises(ValueError, match="forward form only"):
             L.call(*args)
+
+
+# ---------------------------------------------------------------------------
+# Which kernel runs a product
+# ---------------------------------------------------------------------------
+def test_sizes_of_the_gpu_tests_take_the_kernels_they_name():
+    from test_gpu_linear import BF, HF, WIDE, plan
+
+    for op, T, K, N, plans in WIDE:
+        for dtype in (BF, HF):
+            assert " ".join(plan(op, i, T, K, N, dtype) for i in range(3)) == plans, (op, T, K, N)
+    # A weight of more than 4 GiB goes to the tiles however few the rows are.
+    assert plan("residual", 0, 3, 32768, 69640) == "T64/1"
+    assert plan("residual", 0, 3, 8192, 8192) == plan("gated", 0, 1, 7168, 2048) == "ROWS/1"
+
+
+def test_plan_query():
+    query = L.load().tt_linear_plan
+    f32, bf = L.TT_F32, L.TT_BF16
+    assert query(2, 0, f32, 512, 256, 512, 1) % 256 == 0
+    # An address off 16 bytes, or a size off eight elements: the kernels of any alignment.
+    assert query(0, 0, bf, 200, 128, 128, 1) % 256 == 2 and query(0, 0, bf, 200, 128, 128, 0) % 256 == 6
+    assert query(0, 0, bf, 200, 127, 128, 1) % 256 == 6
+    for bad in ((3, 0, bf, 4, 8, 8), (-1, 0, bf, 4, 8, 8), (0, 3, bf, 4, 8, 8), (0, -1, bf, 4, 8, 8),
+                (0, 0, L.TT_F64, 4, 8, 8), (0, 0, bf, -1, 8, 8), (0, 0, bf, 0, 8, 8),
+                (0, 1, bf, 4, 0, 8), (0, 2, bf, 4, 8, 0)):
+        assert query(*bad, 1) == -1

@@ -678,3 +678,90 @@ def test_scale_gradient_counts_its_columns_alone(hip_ops, K):
     assert want.abs().max() < 1e6
     within(ds.reshape(-1), want, unit(BF) * want.abs() +
            1.01 * (gamma(N) + gamma(K) + 2.0 ** -22) * mag, "ds")
+
+
+# ---------------------------------------------------------------------------
+# Sizes that take the wide tiles
+# ---------------------------------------------------------------------------
+KERNELS = "F32 ROWS T64 T128 T256x128 T256 ODD64 ODD128".split()  # TT_LINEAR_KERNEL_...
+OPS = {"act": 0, "gated": 1, "residual": 2}
+
+
+def plan(op, which, T, K, N, dtype=BF, aligned=True):
+    """Kernel / parts of a product: which 0 the forward, 1 the gradient of x, 2 of w."""
+    from torchturbo_amd import _lib as L
+
+    v = L.load().tt_linear_plan(OPS[op], which, L.dtype_code(dtype), T, K, N, int(aligned))
+    return f"{KERNELS[v % 256]}/{v // 256}"
+
+
+# Operation, sizes and the plans of its three products: every wide kernel in every layout, whole
+# and split, with rows, columns and reductions that end inside a tile.
+WIDE = [
+    ("gated", 3850, 2056, 3400, "T256/1 T256/1 T256/1"),
+    ("residual", 3850, 2056, 3400, "T256/1 T256/1 T256x128/1"),
+    ("act", 3850, 2056, 3400, "T256/1 T256/1 T256x128/1"),
+    ("residual", 1542, 5016, 1552, "T256x128/2 T256/1 T256/1"),
+    ("gated", 257, 1440, 5472, "T256x128/1 T64/4 T128/1"),
+    ("gated", 202, 4592, 2080, "T256x128/4 T128/4 T128/1"),
+    ("gated", 4411, 72, 4424, "T128/1 T256x128/8 T256x128/4"),
+    ("gated", 1869, 2184, 552, "T128/1 T256x128/1 T128/1"),
+    ("residual", 5484, 1096, 712, "T256x128/1 T128/1 T128/4"),
+    ("residual", 135, 4616, 5488, "T256x128/4 T64/1 T128/1"),
+    ("residual", 131, 5448, 4984, "T64/1 T256x128/4 T128/1"),
+    ("residual", 838, 4680, 1120, "T128/4 T256x128/1 T128/1"),
+    ("residual", 4743, 136, 5528, "T128/1 T64/1 T256x128/4"),
+    ("act", 1000, 5632, 2048, "T256x128/4 T256x128/1 T128/1"),
+    ("gated", 2051, 2051, 2051, "ODD128/1 ODD128/1 ODD128/1"),
+    ("residual", 2051, 2051, 2051, "ODD128/1 ODD128/1 ODD128/1"),
+    ("act", 4001, 1201, 1703, "ODD128/1 ODD128/1 ODD64/1"),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("op, T, K, N, plans", WIDE)
+def test_wide_tiles(hip_ops, op, T, K, N, plans, dtype):
+    assert " ".join(plan(op, i, T, K, N, dtype) for i in range(3)) == plans
+    x = make((T, K), 1, dtype)
+    if op == "residual":
+        w, b = make((N, K), 2, dtype, K ** -0.5), make((N,), 3, dtype, 0.3)
+        r, s = make((T, N), 4, dtype), make((T, 1), 5, dtype)
+        key = torch.tensor([T * 123456789, -K], device=DEV)
+        check_residual(hip_ops, x, w, b, r, s, 0.2, key)
+        check_residual(hip_ops, x, w, None, r, None)
+        check_residual(hip_ops, x, w, None, None, s.float())
+    else:
+        rows = 2 * N if op == "gated" else N
+        w, b = make((rows, K), 2, dtype, K ** -0.5), make((rows,), 3, dtype, 0.3)
+        check_act(hip_ops, x, w, None, F.silu, op == "gated")
+        check_act(hip_ops, x, w, b, F.gelu if op == "gated" else None, op == "gated")
+
+
+@pytest.mark.parametrize("T, K, N, gated, residual", [
+    (2048, 2048, 2048, "ODD128/1 ODD128/1 ODD128/1", "ODD128/1 ODD128/1 ODD128/1"),
+    (1030, 2056, 2104, "ODD128/1 ODD64/1 ODD128/1", "ODD64/1 ODD64/1 ODD128/1")])
+def test_wide_tiles_of_unaligned_operands(hip_ops, T, K, N, gated, residual):
+    for op, plans in (("gated", gated), ("residual", residual)):
+        assert " ".join(plan(op, i, T, K, N, aligned=False) for i in range(3)) == plans
+
+    def off(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].copy_(t.reshape(-1)).view(t.shape)
+
+    x, w = off(make((T, K), 1, BF)), off(make((2 * N, K), 2, BF, K ** -0.5))
+    assert x.data_ptr() % 16 and w.data_ptr() % 16
+    check_act(hip_ops, x, w, None, F.silu, True)
+    r, s = off(make((T, N), 4, BF)), make((T, 1), 5, BF)
+    check_residual(hip_ops, x, off(w[:N]), None, r, s, 0.2, torch.tensor([1, 2], device=DEV))
+
+
+def test_few_rows_of_the_largest_weights(hip_ops):
+    """The most that the kernel of few rows streams: above about 620 MB the tiles are taken."""
+    for T, K, N, gated in ((1, 41168, 7560, False), (1, 55680, 2784, True)):
+        assert plan("gated" if gated else "residual", 0, T, K, N) == "ROWS/1"
+        x = make((T, K), 1, BF)
+        g = torch.Generator(device=DEV).manual_seed(4)
+        w = torch.empty((N * (1 + gated), K), dtype=BF, device=DEV).normal_(0.0, K ** -0.5, generator=g)
+        if gated:
+            check_act(hip_ops, x, w, None, F.silu, True, backward=False)
+        else:
+            check_residual(hip_ops, x, w, None, make((T, N), 5, BF), None, backward=False)

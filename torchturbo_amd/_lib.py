@@ -76,6 +76,7 @@ _PROTOS: dict[str, list] = {
     "tt_lora_down_dropout": [P, P, c_int, I64, I64, I32, I32, P, I32, P, P, P],
     "tt_lora_up_dropout": [P, P, c_int, I64, I64, I32, I32, P, I32, P, P, P],
     "tt_lora_wgrad_dropout": [P, P, c_int, I64, I64, I32, I32, P, I32, P, P, P],
+    "tt_linear_plan": [I32, I32, c_int, I64, I64, I64, I32],
     "tt_linear_workspace": [I32, c_int, I64, I64, I64],
     "tt_linear_act_fwd": [P, P, P, c_int, c_int, I64, I64, I64, I32, I32, P, P, P, c_size_t, P],
     "tt_linear_act_bwd_workspace": [c_int, I64, I64, I64, I32, I32],

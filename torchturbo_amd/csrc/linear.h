@@ -311,8 +311,10 @@ enum { LAY_NT = 0, LAY_NN = 1, LAY_TN = 2 };
 
 // The kernels: fp32, few rows, tiles of the 16-bit matrix instructions, and tiles for any
 // alignment.
-enum { LIN_F32 = 0, LIN_ROWS = 1, LIN_T64 = 2, LIN_T128 = 3, LIN_T256x128 = 4, LIN_T256 = 5,
-       LIN_ODD64 = 6, LIN_ODD128 = 7 };
+enum { LIN_F32 = TT_LINEAR_KERNEL_F32, LIN_ROWS = TT_LINEAR_KERNEL_ROWS,
+       LIN_T64 = TT_LINEAR_KERNEL_T64, LIN_T128 = TT_LINEAR_KERNEL_T128,
+       LIN_T256x128 = TT_LINEAR_KERNEL_T256X128, LIN_T256 = TT_LINEAR_KERNEL_T256,
+       LIN_ODD64 = TT_LINEAR_KERNEL_ODD64, LIN_ODD128 = TT_LINEAR_KERNEL_ODD128 };
 
 // fp32 tensors of any size and alignment (linear_f32.hip).
 int tt_linear_f32(int kind, const LinArgs& a, hipStream_t s);

@@ -552,6 +552,27 @@ extern "C" size_t tt_linear_workspace(int32_t op, int dtype, int64_t m, int64_t 
   }
 }
 
+extern "C" int tt_linear_plan(int32_t op, int32_t pass, int dtype, int64_t m, int64_t k, int64_t n,
+                              int32_t aligned) {
+  if (op < TT_LINEAR_ACT || op > TT_LINEAR_RESIDUAL || pass < 0 || pass > 2 || m < 0 || k < 0 ||
+      n < 0 || (dtype != TT_F32 && dtype != TT_BF16 && dtype != TT_F16))
+    return -1;
+  const bool gated = op == TT_LINEAR_GATED;
+  const int64_t width = gated ? 2 * n : n;
+  const int layout = pass == 0 ? LAY_NT : pass == 1 ? LAY_NN : LAY_TN;
+  const int kind = pass == 1   ? LIN_DGRAD
+                   : pass == 2 ? LIN_PLAIN
+                   : gated     ? LIN_GATED
+                               : LIN_ACT;  // RES's and DROP's plan as well
+  const int64_t I = pass == 2 ? width : m, J = pass == 0 ? n : k;
+  const int64_t R = pass == 0 ? k : pass == 1 ? width : m;
+  if (I == 0 || J == 0) return -1;
+  int how = how_sizes(layout, kind, dtype, I, J, R);
+  if (how == HOW_FAST && !aligned) how = HOW_ODD;
+  const Plan pl = plan_of(layout, kind, I, J, R, how);
+  return pl.kernel + 256 * pl.split.splits;
+}
+
 extern "C" int tt_linear_act_fwd(const void* x, const void* w, const void* bias, int bias_dtype,
                                  int dtype, int64_t m, int64_t k, int64_t n, int32_t act,
                                  int32_t gated, float* pre, void* y, void* workspace,
