@@ -678,3 +678,19 @@ def test_plan_query():
                 (0, 0, L.TT_F64, 4, 8, 8), (0, 0, bf, -1, 8, 8), (0, 0, bf, 0, 8, 8),
                 (0, 1, bf, 4, 0, 8), (0, 2, bf, 4, 8, 0)):
         assert query(*bad, 1) == -1
+
+
+@pytest.mark.parametrize("name, given", [("tt_linear_act_fwd", "x w y"),
+                                         ("tt_linear_residual_fwd", "x w y")])
+def test_more_tiles_than_a_launch_has_are_refused(name, given):
+    """A launch ends below 2^32 threads, 2^24 blocks of 256."""
+    with pytest.raises(ValueError, match="grid too large"):
+        pointers(name, given.split(), m=(1 << 30) + 1, k=4, bytes=0)
+
+
+@pytest.mark.parametrize("name, rows, rank", [("tt_lora_down_dropout", 1 << 29, 64),
+                                              ("tt_lora_up_dropout", 1 << 30, 4)])
+def test_more_blocks_of_the_adapters_than_a_launch_has_are_refused(name, rows, rank):
+    at = ctypes.c_void_p(4096)
+    with pytest.raises(ValueError, match="grid too large"):
+        L.call(name, at, at, L.TT_BF16, rows, 8, rank, 2, at, 5, P, at, None)

@@ -765,3 +765,36 @@ def test_few_rows_of_the_largest_weights(hip_ops):
             check_act(hip_ops, x, w, None, F.silu, True, backward=False)
         else:
             check_residual(hip_ops, x, w, None, make((T, N), 5, BF), None, backward=False)
+
+
+def test_more_rows_than_one_launch_of_a_wave_each(hip_ops):
+    """2^26 rows and some more: the scale's gradient takes a wave per row, and a launch ends
+    below 2^32 threads. The last rows against a call on them alone."""
+    T, K, N, last = (1 << 26) + 5, 8, 8, 300
+    g = torch.Generator(device=DEV).manual_seed(6)
+
+    def normal(*shape):
+        return torch.empty(shape, dtype=BF, device=DEV).normal_(generator=g)
+
+    x, w, b, s, dy = normal(T, K), normal(N, K), normal(N), normal(T, 1), normal(T, N)
+    s.requires_grad_()
+    ds, = torch.autograd.grad(hip_ops.linear_residual(x, w, b, None, s), s, dy)
+    part = s[-last:].detach().requires_grad_()
+    want, = torch.autograd.grad(hip_ops.linear_residual(x[-last:], w, b, None, part), part, dy[-last:])
+    # fp32 sums of 8 + 8 products, rounded once: at most the order of the sums differs.
+    X, W, B, G = wide(x[-last:], w, b, dy[-last:])
+    mag = (X.abs() * (G.abs() @ W.abs())).sum(1) + G.abs() @ B.abs()
+    exact = (X * (G @ W)).sum(1) + G @ B
+    tol = unit(BF) * exact.abs() + 1.01 * (gamma(N) + gamma(K)) * mag
+    within(ds[-last:].reshape(-1), exact, tol, "ds")
+    within(want.reshape(-1), exact, tol, "ds of the last rows")
+
+
+def test_dropout_of_more_rows_than_its_launch_has(hip_ops):
+    rows, cols = (1 << 22) + 3, 1032  # four rows to a block of threads at a time
+    x = torch.ones((rows, cols), dtype=BF, device=DEV)
+    key = torch.tensor([79, 80], device=DEV)
+    y = hip_ops.dropout(x, 0.5, key)
+    for at in (0, (1 << 22) - 2, rows - 3):
+        f = o_dropout.factors(3, cols, 0.5, key.cpu(), at)
+        assert torch.equal(y[at:at + 3].double().cpu(), f), at

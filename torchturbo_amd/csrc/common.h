@@ -146,6 +146,12 @@ __device__ __forceinline__ int lane_id() { return threadIdx.x & (TT_WAVE - 1); }
 void tt_set_error(const char* fmt, ...);
 int tt_check_launch(const char* what);
 
+// Whether a launch of these blocks runs whole: one of 2^32 threads or more runs a part of
+// its blocks, and reports no error.
+static inline bool tt_grid_ok(int64_t blocks, int threads) {
+  return blocks * threads < (1ll << 32);
+}
+
 #define TT_REQUIRE(cond, ...)               \
   do {                                      \
     if (!(cond)) {                          \

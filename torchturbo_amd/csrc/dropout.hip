@@ -12,6 +12,7 @@ namespace {
 
 constexpr int DR_NT = 256;
 constexpr int DR_ROWS = 4;  // rows in flight per thread
+constexpr int64_t DR_BLOCKS = 1 << 20;  // along rows; with more rows they take them in turn
 
 // Lanes along the groups of eight columns (L of a block's 256 threads, a power
 // of two), the others along rows; a thread keeps its group and walks rows.
@@ -67,7 +68,7 @@ int launch(const void* x, void* y, int64_t rows, int64_t cols, int32_t threshold
   const int64_t gy = (groups + L - 1) / L;
   int64_t gx = (rows + (DR_NT / L) * DR_ROWS - 1) / ((DR_NT / L) * DR_ROWS);
   TT_REQUIRE(gy <= 65535, "dropout: too many columns (%lld)", (long long)cols);
-  if (gx > 0x7fffffff) gx = 0x7fffffff;
+  if (gx > DR_BLOCKS) gx = DR_BLOCKS;
   const bool vec = cols % 8 == 0 && ((reinterpret_cast<uintptr_t>(x) |
                                       reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   const dim3 grid((unsigned)gx, (unsigned)gy), block(DR_NT);

@@ -11,6 +11,7 @@ namespace {
 inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 constexpr int L_NT = 256;
+constexpr int64_t MAX_BLOCKS = 1 << 20;  // of a pass whose blocks take rows in turn
 
 // ---------------------------------------------------------------------------
 // Joins the sums of a split reduction, in the order of the splits. A thread
@@ -69,7 +70,7 @@ template <int KIND, class TT>
 int join(const LinArgs& p, hipStream_t s) {
   const int64_t run = LIN_DOT / 8, groups = ((p.J + 7) / 8 + run - 1) / run * run;
   const int64_t blocks = (p.I * groups + L_NT - 1) / L_NT;
-  TT_REQUIRE(blocks < 0x7fffffff, "linear: grid too large");
+  TT_REQUIRE(tt_grid_ok(blocks, L_NT), "linear: grid too large");
   if (vectors(p))
     hipLaunchKernelGGL((linear_join_kernel<KIND, TT, true>), dim3((unsigned)blocks), dim3(L_NT), 0,
                        s, p, groups);
@@ -380,18 +381,18 @@ __global__ __launch_bounds__(L_NT) void linear_colsum_kernel(const float* __rest
   store_from_f32(out, dt, j, alpha * t);
 }
 
-// out[i] = sum over j of g[i, j] * bias[j], one wave per row.
+// out[i] = sum over j of g[i, j] * bias[j], one wave per row at a time.
 __global__ __launch_bounds__(L_NT) void linear_rowdot_kernel(const void* __restrict__ g, int dtype,
                                                              const void* __restrict__ bias,
                                                              int bias_dt, int64_t rows, int64_t J,
                                                              float* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= rows) return;
-  float t = 0.f;
-  for (int64_t j = threadIdx.x & 63; j < J; j += 64)
-    t += load_as_f32(g, dtype, i * J + j) * load_as_f32(bias, bias_dt, j);
-  t = wave_sum(t);
-  if ((threadIdx.x & 63) == 0) out[i] = t;
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += 4ll * gridDim.x) {
+    float t = 0.f;
+    for (int64_t j = threadIdx.x & 63; j < J; j += 64)
+      t += load_as_f32(g, dtype, i * J + j) * load_as_f32(bias, bias_dt, j);
+    t = wave_sum(t);
+    if ((threadIdx.x & 63) == 0) out[i] = t;
+  }
 }
 
 // out[i] = the dots of row i, in order, + alpha * extra[i].
@@ -786,8 +787,9 @@ extern "C" int tt_linear_residual_bwd(const void* dy, const void* x, const void*
                          ws.left, S(stream)));
   if (dscale != nullptr && m > 0) {
     if (bias != nullptr) {
-      hipLaunchKernelGGL(linear_rowdot_kernel, dim3((unsigned)((m + 3) / 4)), dim3(L_NT), 0,
-                         S(stream), g, dtype, bias, bias_dtype, m, n, extra);
+      const int64_t blocks = std::min<int64_t>((m + 3) / 4, MAX_BLOCKS);
+      hipLaunchKernelGGL(linear_rowdot_kernel, dim3((unsigned)blocks), dim3(L_NT), 0, S(stream), g,
+                         dtype, bias, bias_dtype, m, n, extra);
       TT_TRY(tt_check_launch("linear_rowdot"));
     }
     hipLaunchKernelGGL(linear_rowsum_kernel, dim3((unsigned)((m + L_NT - 1) / L_NT)), dim3(L_NT), 0,

@@ -239,7 +239,7 @@ template <int LAYOUT, int KIND, bool FAR>
 int launch(const LinArgs& p, hipStream_t s) {
   const int bo = KIND == LIN_GATED ? A_BT / 2 : A_BT;
   const int64_t ti = (p.I + A_BT - 1) / A_BT, tj = (p.J + bo - 1) / bo;
-  TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
+  TT_REQUIRE(tt_grid_ok(ti * tj, A_NT), "linear: grid too large");
   hipLaunchKernelGGL((linear_f32_kernel<LAYOUT, KIND, FAR>),
                      dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(A_NT), 0, s, p,
                      (int)tj);

@@ -127,7 +127,7 @@ template <int KIND, class TT, int MB, int NB, int U>
 int launch(const LinArgs& p, hipStream_t s) {
   constexpr int CB = KIND == LIN_GATED ? 8 * NB : 16 * NB;
   const int64_t blocks = (p.J + CB - 1) / CB;
-  TT_REQUIRE(blocks < 0x7fffffff, "linear: grid too large");
+  TT_REQUIRE(tt_grid_ok(blocks, N_NT), "linear: grid too large");
   hipLaunchKernelGGL((linear_rows_kernel<KIND, TT, MB, NB, U>), dim3((unsigned)blocks), dim3(N_NT),
                      0, s, p);
   return tt_check_launch("linear_rows");

@@ -819,7 +819,7 @@ int launch(int tile, const LinArgs& p, hipStream_t s) {
   const int bn = tile == LIN_T64 ? 64 : tile == LIN_T256 ? 256 : 128;
   const int bo = KIND == LIN_GATED ? bn / 2 : bn;
   const int64_t ti = (p.I + bm - 1) / bm, tj = (p.J + bo - 1) / bo;
-  TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
+  TT_REQUIRE(tt_grid_ok(ti * tj, T_NT), "linear: grid too large");
   const dim3 grid((unsigned)(ti * tj), (unsigned)p.splits);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(T_NT), 0, s, p, (int)ti, (int)tj);
@@ -838,7 +838,7 @@ template <int LAYOUT, int KIND, int ET, int BT>
 int launch_odd(const LinArgs& p, hipStream_t s) {
   constexpr int BO = KIND == LIN_GATED ? BT / 2 : BT;
   const int64_t ti = (p.I + BT - 1) / BT, tj = (p.J + BO - 1) / BO;
-  TT_REQUIRE(ti * tj < 0x7fffffff, "linear: grid too large");
+  TT_REQUIRE(tt_grid_ok(ti * tj, T_NT), "linear: grid too large");
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(ti * tj), (unsigned)p.splits), dim3(T_NT), 0, s, p,
                        (int)ti, (int)tj);

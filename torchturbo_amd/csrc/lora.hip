@@ -562,8 +562,10 @@ int64_t row_blocks(int64_t M, int E, int bm = 64) { return M / bm + (M < E ? M :
 
 template <class TT, int RT, bool WT, bool SCALE, int WC, bool DROP>
 int launch_down_wc(const LoraArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((lora_down_kernel<TT, RT, WT, SCALE, WC, DROP>),
-                     dim3((unsigned)row_blocks(a.M, a.E, 64 / WC)), dim3(LR_NT), 0, s, a.in, a.w,
+  const int64_t blocks = row_blocks(a.M, a.E, 64 / WC);
+  TT_REQUIRE(tt_grid_ok(blocks, LR_NT), "lora: grid too large");
+  hipLaunchKernelGGL((lora_down_kernel<TT, RT, WT, SCALE, WC, DROP>), dim3((unsigned)blocks),
+                     dim3(LR_NT), 0, s, a.in, a.w,
                      static_cast<float*>(a.out), a.C, a.r, a.s, a.E, a.counts, a.drop);
   return tt_check_launch("lora_down");
 }
@@ -587,9 +589,11 @@ int launch_down(const LoraArgs& a, hipStream_t s) {
 template <class TT, int RT, bool WT, bool BASE, bool DROP>
 int launch_up(const LoraArgs& a, const float* h, hipStream_t s) {
   const int tn = (a.C + 255) / 256;
-  hipLaunchKernelGGL((lora_up_kernel<TT, RT, WT, BASE, DROP>),
-                     dim3((unsigned)(row_blocks(a.M, a.E) * tn)), dim3(LR_NT), 0, s, h, a.w, a.base,
-                     static_cast<uint16_t*>(a.out), a.C, a.r, a.s, a.E, a.counts, tn, a.drop);
+  const int64_t blocks = row_blocks(a.M, a.E) * tn;
+  TT_REQUIRE(tt_grid_ok(blocks, LR_NT), "lora: grid too large");
+  hipLaunchKernelGGL((lora_up_kernel<TT, RT, WT, BASE, DROP>), dim3((unsigned)blocks),
+                     dim3(LR_NT), 0, s, h, a.w, a.base, static_cast<uint16_t*>(a.out), a.C, a.r,
+                     a.s, a.E, a.counts, tn, a.drop);
   return tt_check_launch("lora_up");
 }
 template <class TT, int RT, bool GT, bool SCALE, bool DROP>
@@ -621,7 +625,6 @@ int lora_checks(int dtype, int64_t m, int64_t c, int r, int E, const void* p0, c
   TT_REQUIRE(((reinterpret_cast<uintptr_t>(p0) | reinterpret_cast<uintptr_t>(p1) |
                reinterpret_cast<uintptr_t>(p2)) & 15) == 0,
              "lora: operands must be 16-byte aligned");
-  TT_REQUIRE(row_blocks(m, E) * ((c + 255) / 256) < 0x7fffffff, "lora: grid too large");
   return TT_OK;
 }
 // `there`: whether every tensor that the call reads or writes is (an empty one may be NULL).
