@@ -2,7 +2,7 @@
 // most 64, 16-bit x [I, R] and w [rows, R]: the decode of one or some sequences.
 //
 // Such a call reads the weight once and is bound by that stream. A block takes 16
-// NB rows of the weight and all of x, and its eight waves split the reduction
+// rows of the weight and all of x, and its eight waves split the reduction
 // among them, so that every CU streams with a few blocks however few columns there
 // are, with no second launch to join parts. Operands go from memory to registers
 // in the layout of the 16x16x32 products (a lane's 16 bytes are eight consecutive
@@ -16,6 +16,7 @@
 namespace {
 
 constexpr int N_NT = 512, N_W = N_NT / 64;
+constexpr int U = 4;  // 32-deep steps fetched together
 
 template <int ET>
 __device__ __forceinline__ f32x4_t mma16(const u32x4& a, const u32x4& b, const f32x4_t& c) {
@@ -27,12 +28,12 @@ __device__ __forceinline__ f32x4_t mma16(const u32x4& a, const u32x4& b, const f
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <int KIND, class TT, int MB, int NB, int U>
+template <int KIND, class TT, int MB>
 __global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
   constexpr bool GATED = KIND == LIN_GATED;
   constexpr int ET = sizeof(typename TT::storage) == 2 && __is_same(TT, BF16T) ? TT_BF16 : TT_F16;
-  constexpr int CB = GATED ? 8 * NB : 16 * NB;  // output columns of a block
-  constexpr int LD = 16 * NB + 4;               // row stride of the sums: 16-byte chunks, spread
+  constexpr int CB = GATED ? 8 : 16;  // output columns of a block
+  constexpr int LD = 16 + 4;          // row stride of the sums: 16-byte chunks, spread
   __shared__ __align__(16) float sums[N_W][16 * MB][LD];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
   const int s0 = steps * wave / N_W, s1 = steps * (wave + 1) / N_W;
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<void*>(p.a), (short)0, (int)(uint32_t)(p.I * p.lda * 2), 0x00020000);
-  uint32_t xo[MB], wo[NB];
+  uint32_t xo[MB];
   const char* const w0 = static_cast<const char*>(p.b) + j0 * p.ldb * 2;
   const int64_t wleft = ((GATED ? 2 : 1) * p.J - j0) * p.ldb * 2;
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
@@ -53,24 +54,19 @@ __global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
 #pragma unroll
   for (int m = 0; m < MB; ++m)
     xo[m] = 16 * m + r < p.I ? (uint32_t)(((16 * m + r) * p.lda + 8 * g) * 2) : DM_OOB;
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int64_t c = GATED ? 8 * n + (r & 7) : 16 * n + r;  // column of the block
-    const int64_t row = GATED && r >= 8 ? p.J + c : c;
-    wo[n] = j0 + c < p.J ? (uint32_t)((row * p.ldb + 8 * g) * 2) : DM_OOB;
-  }
-  f32x4_t acc[MB][NB] = {};
-  u32x4 xv[2][U][MB], wv[2][U][NB];
+  const int64_t c = GATED ? r & 7 : r;  // column of the block
+  const int64_t row = GATED && r >= 8 ? p.J + c : c;
+  const uint32_t wo = j0 + c < p.J ? (uint32_t)((row * p.ldb + 8 * g) * 2) : DM_OOB;
+  f32x4_t acc[MB] = {};
+  u32x4 xv[2][U][MB], wv[2][U];
   auto fetch = [&](int s, int buf) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       // Steps past the wave's last and elements past the row's end read as zeros.
       const bool ok = s + q < s1 && 32 * (s + q) + 8 * g < R;
       const uint32_t at = (uint32_t)(s + q) * 64u;
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-        wv[buf][q][n] = __builtin_amdgcn_raw_buffer_load_b128(
-            rw, (int)(ok && wo[n] != DM_OOB ? wo[n] + at : DM_OOB), 0, 0);
+      wv[buf][q] = __builtin_amdgcn_raw_buffer_load_b128(
+          rw, (int)(ok && wo != DM_OOB ? wo + at : DM_OOB), 0, 0);
 #pragma unroll
       for (int m = 0; m < MB; ++m)
         xv[buf][q][m] = __builtin_amdgcn_raw_buffer_load_b128(
@@ -81,9 +77,7 @@ __global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
 #pragma unroll
     for (int q = 0; q < U; ++q)
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) acc[m][n] = mma16<ET>(wv[buf][q][n], xv[buf][q][m], acc[m][n]);
+      for (int m = 0; m < MB; ++m) acc[m] = mma16<ET>(wv[buf][q], xv[buf][q][m], acc[m]);
   };
   if (s0 < s1) fetch(s0, 0);
   for (int s = s0; s < s1; s += 2 * U) {
@@ -95,12 +89,10 @@ __global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
     __builtin_amdgcn_sched_barrier(0);
     multiply(1);
   }
-  // Lane l holds row 16 m + l % 16 of x, rows 16 n + 4 (l / 16) + 0..3 of the weights.
+  // Lane l holds row 16 m + l % 16 of x, rows 4 (l / 16) + 0..3 of the weights.
 #pragma unroll
   for (int m = 0; m < MB; ++m)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-      *reinterpret_cast<f32x4_t*>(&sums[wave][16 * m + r][16 * n + 4 * g]) = acc[m][n];
+    *reinterpret_cast<f32x4_t*>(&sums[wave][16 * m + r][4 * g]) = acc[m];
   __syncthreads();
   constexpr int NG = CB / 8;  // groups of eight outputs
   DropKey dk{};
@@ -123,21 +115,21 @@ __global__ __launch_bounds__(N_NT) void linear_rows_kernel(LinArgs p) {
   }
 }
 
-template <int KIND, class TT, int MB, int NB, int U>
+template <int KIND, class TT, int MB>
 int launch(const LinArgs& p, hipStream_t s) {
-  constexpr int CB = KIND == LIN_GATED ? 8 * NB : 16 * NB;
+  constexpr int CB = KIND == LIN_GATED ? 8 : 16;
   const int64_t blocks = (p.J + CB - 1) / CB;
   TT_REQUIRE(tt_grid_ok(blocks, N_NT), "linear: grid too large");
-  hipLaunchKernelGGL((linear_rows_kernel<KIND, TT, MB, NB, U>), dim3((unsigned)blocks), dim3(N_NT),
+  hipLaunchKernelGGL((linear_rows_kernel<KIND, TT, MB>), dim3((unsigned)blocks), dim3(N_NT),
                      0, s, p);
   return tt_check_launch("linear_rows");
 }
 
 template <int KIND, class TT>
 int rows(const LinArgs& p, hipStream_t s) {
-  if (p.I <= 16) return launch<KIND, TT, 1, 1, 4>(p, s);
-  if (p.I <= 32) return launch<KIND, TT, 2, 1, 4>(p, s);
-  return launch<KIND, TT, 4, 1, 4>(p, s);
+  if (p.I <= 16) return launch<KIND, TT, 1>(p, s);
+  if (p.I <= 32) return launch<KIND, TT, 2>(p, s);
+  return launch<KIND, TT, 4>(p, s);
 }
 
 template <int KIND>
