@@ -3,9 +3,10 @@
 // for the backward, which is the same call on the gradient. A dropped element is
 // 0 whatever it held (infinities and NaN included).
 //
-// One read and one write, 131072 x 2048 bf16 in 206 us: 5.2 TB/s, the rate of a copy. The
+// One read and one write, 131072 x 2048 bf16 in 207 us: 5.2 TB/s, the rate of a copy. The
 // ten rounds of a group of eight are about 80 instructions, four rows of them in flight
-// per thread: under the time of their memory accesses.
+// per thread: under the time of their memory accesses. Widths off eight elements and
+// unaligned rows are loaded one element at a time: 131072 x 2047 in 291 us.
 #include "linear.h"
 
 namespace {

@@ -123,10 +123,14 @@ int64_t least_splits(int layout, int64_t I, int64_t J, int64_t R) {
 // k-tile of a 64-wide tile takes 0.30 us where a CU has one block and 0.5 with two,
 // of a 128-wide one 0.62 and 1.0, of a 256-wide one (one block per CU) 0.85 on a few
 // CUs and 1.2 on all (the part is then at its power limit); the rest are starts and
-// epilogues. Measured / this estimate: 1000 x 704 -> 1024 (352 tiles of 64) 6.5 / 7.2,
-// 2048 x 768 -> 2048 (1024 of 64) 15.8 / 15.8, in 256 tiles of 128 13.0 / 11.6, 512 x
-// 2048 -> 7168 (224 of 128) 24.7 / 24.0, 1000 rows (448 of 128) 34.2 / 34.6, 2048 rows
-// (224 of 256) 54 / 57; 24 x 7168 -> 4096 in four parts (256 blocks of 64) 15.6 / 15.0.
+// epilogues. Measured (back to back in a graph) / this estimate: 1000 x 704 -> 1024 (256
+// tiles of 64) 7.4 / 6.1, 1000 x 1024 -> 1408 (352) 10.5 / 10.8, 2048 x 768 -> 2048 (1024 of
+// 64) 16.4 / 15.8, in 256 tiles of 128 13.8 / 11.6, 512 x 2048 -> 7168 (224 of 128) 26.1 /
+// 24.0, 1000 rows (448 of 128) 35.0 / 36.2, 2048 rows (224 of 256) 52.2 / 57.0; 24 x 7168 ->
+// 4096 in four parts (256 blocks of 64) 16.3 / 19.1, 24 x 2048 -> 7168 (112 of 64) 12.7 / 12.4
+// and in four parts 10.6 / 13.1. Over 170 random sizes the choice took 1.03 (forward), 1.01
+// (gradient of x) and 1.02 (of the weight) times the best kernel's time in the mean, at
+// most 1.2, 1.3 and 1.3 times among the tiles.
 // No plan is faster than its operands' bytes at 4.6 TB/s.
 double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sums, int64_t bytes) {
   const int64_t blocks = tiles * splits, full = blocks / 512, rest = blocks % 512;
@@ -149,8 +153,10 @@ double tile_us(int tile, int64_t tiles, int64_t splits, int64_t nkt, int64_t sum
 
 // The same of the kernel of few rows: the weight at 4.6 TB/s and, for each block of its
 // columns, all of x at 9 TB/s, with fewer than 256 blocks accordingly slower. Measured /
-// this estimate: 1 x 7168 -> 2 x 2048 13.8 / 14.7, 24 x 2048 -> 7168 12.8 / 12.8, 24 x
-// 2048 -> 2 x 768 8.1 / 8.0, 64 x 7168 -> 2 x 2048 40.9 / 40.3.
+// this estimate: 1 x 7168 -> 2 x 2048 12.5 / 14.7, 16 x 2048 -> 7168 10.5 / 11.1, 24 rows
+// 12.8 / 12.8 (the 64-wide tiles, chosen there, 12.7), 24 x 2048 -> 2 x 768 8.5 / 7.9, 64 x
+// 7168 -> 2 x 2048 35.5 / 40.4. Bytes alone are too little for a short reduction: 52 x 152 ->
+// 2 x 4304 10.6 / 3.0, where the tiles take 4.7.
 double rows_us(int64_t blocks, int64_t I, int64_t J, int64_t R) {
   const double work = (double)(J * R) * 2 / 4.6e6 + (double)(blocks * I * R) * 2 / 9e6;
   return 1.5 + work * std::max(1.0, 256.0 / (double)blocks);

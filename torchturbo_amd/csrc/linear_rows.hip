@@ -8,8 +8,8 @@
 // in the layout of the 16x16x32 products (a lane's 16 bytes are eight consecutive
 // reduction elements of row l % 16), U steps at a time, the next ones in flight while
 // the ones before are multiplied. The waves' sums meet in LDS and are added in order.
-// 1 x 7168 -> 2 x 2048 12.6 us (the 59 MB of weights at 4.7 TB/s); with more rows the
-// blocks' reading of x is the bound, 24 x 2048 -> 7168 12.8 us (2.3 TB/s).
+// 1 x 7168 -> 2 x 2048 12.5 us (the 59 MB of weights at 4.7 TB/s); with more rows the
+// blocks' reading of x is the bound, 16 x 2048 -> 7168 10.5 us (2.8 TB/s).
 // GATED: a 16-row block of weights is eight gates and their eight ups.
 #include "linear.h"
 

@@ -571,8 +571,8 @@ __global__ __launch_bounds__(T_NT) void linear_big_kernel(LinArgs p, int ti, int
 
 // BT x BT tiles (64 or 128), a quarter per wave, a ring of S stages (16 or 32 KiB) with
 // one barrier per k-tile, which publishes k-tile kt and frees the stage of kt - 1. Several
-// blocks share a CU and hide one another's waits and epilogues: 512 x 2048 -> 7168 24.7 us
-// (0.61 PFLOP/s), 1000 x 704 -> 1024 6.5 us.
+// blocks share a CU and hide one another's waits and epilogues: 512 x 2048 -> 7168 26.1 us
+// (0.58 PFLOP/s), 1000 x 704 -> 1024 7.4 us.
 template <int LAYOUT, int KIND, int ET, bool KMASK, int BT, int S>
 __global__ __launch_bounds__(T_NT) void linear_mid_kernel(LinArgs p, int ti, int tj) {
   typedef Tile<LAYOUT, KIND, BT, BT, 32> TL;

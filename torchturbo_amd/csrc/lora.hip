@@ -21,8 +21,10 @@
 // took 354 us, but in an order of their own: other last bits.)
 //
 // With dropout the rows' masks are made in the kernels that read or write them, among the
-// products: K 2048, r 16, 16384 rows, down 36 -> 57 us, dx 42 -> 48, dA 33 -> 68, for
-// Philox's 40 32-bit multiplies to eight elements (a quarter of the rate of adds). Passes of
+// products: K 2048, r 16, 16384 rows, down 36 -> 58 us, dx 42 -> 49, dA 33 -> 67, for
+// Philox's twenty 32 x 32 bit multiplies with 64-bit results to eight elements, each at a
+// quarter of the rate of adds; in dA also for the masks' passage through LDS, where the
+// compiler puts the words that quad_transpose selects among (12 KB). Passes of
 // their own over x and dx would take about as long together (134 MB each, 26 us at a
 // copy's rate), and keep the 67 MB of dropped rows for the backward.
 #include "gemm.h"
