@@ -112,3 +112,35 @@ def test_shape_queries_answer_without_a_gpu(lib):
     # gathering weight gradients take sources of fewer than 2^24 rows (24-bit offsets)
     assert gs(2, bf, (1 << 24) - 1, 1 << 24, 64, 64, 8) == 1
     assert gs(2, bf, 1 << 24, 1 << 24, 64, 64, 8) == 0
+
+
+AT = ctypes.c_void_p(4096)  # an address that no kernel ever gets: every such call is refused
+BIG = 1 << 24  # blocks of 256 threads that make 2^32
+
+
+@pytest.mark.parametrize("name,args", [
+    ("tt_permute_scatter", (AT, 1, BIG, 2048, 1, AT, AT)),
+    ("tt_unpermute_gather", (AT, 1, BIG, 4096, 1, AT, None, None, 0, 1, AT)),
+    ("tt_unpermute_gather", (AT, 1, 2 * BIG, 2048, 1, AT, AT, AT, 0, 4, AT)),  # 128 threads
+    ("tt_unpermute_gather", (AT, 1, BIG, 2048, 9, AT, None, None, 0, 1, AT)),
+    ("tt_unpermute_gather", (AT, 1, BIG, 257, 1, AT, None, None, 0, 1, AT)),
+    ("tt_unpermute_gather_bwd", (AT, AT, 1, BIG, 64, 1, AT, AT, AT, 0, 4, AT, AT)),
+    ("tt_packed_probs_bwd", (AT, 0, 4 * BIG, 2, 8, AT, AT, AT)),
+    ("tt_swiglu_fwd", (AT, 1, 4 * BIG, 512, None, 0, AT)),
+    ("tt_swiglu_fwd", (AT, 1, 4 * BIG, 65, None, 0, AT)),
+    ("tt_swiglu_bwd", (AT, 1, BIG, 4096, None, 0, AT, AT, None)),
+    ("tt_swiglu_bwd", (AT, 1, 4 * BIG, 512, None, 0, AT, AT, None)),
+    ("tt_swiglu_bwd", (AT, 1, 4 * BIG, 65, None, 0, AT, AT, None)),
+    ("tt_gated_act_fwd", (AT, 1, 4 * BIG, 512, 1, 0.0, 0, None, 0, AT)),
+    ("tt_gated_act_fwd", (AT, 1, 4 * BIG, 65, 1, 0.0, 0, None, 0, AT)),
+    ("tt_gated_act_bwd", (AT, 1, 4 * BIG, 512, 1, 0.0, 0, None, 0, AT, AT, None)),
+    ("tt_gated_act_bwd", (AT, 1, 4 * BIG, 65, 1, 0.0, 0, None, 0, AT, AT, None)),
+    ("tt_router_topk_fwd", (AT, 0, 4 * BIG, 8, 2, 0, 0, None, 0, 0, 1.0, None, AT, AT, AT)),
+    ("tt_router_topk_bwd", (AT, 0, 4 * BIG, 8, 2, 0, 0, 1.0, AT, AT, AT)),
+    ("tt_router_loss_bwd", (AT, 0, 4 * BIG, 8, 0, None, AT, AT, AT, AT, AT)),
+])
+def test_launches_of_2_to_the_32_threads_are_refused(lib, name, args):
+    """Such a launch runs a part of its blocks and reports no error."""
+    args = list(args) + [None] * (len(L._PROTOS[name]) - len(args))
+    with pytest.raises(ValueError, match="grid too large"):
+        L.call(name, *args)

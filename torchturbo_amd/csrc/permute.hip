@@ -421,6 +421,7 @@ int launch_unpermute(const void* packed, int64_t T, int64_t H, int K, const int3
     // loads at once.
     if (nvb % 128 == 0 && nvb / 2 <= 1024) {
       const dim3 blk((unsigned)(nvb / 2));
+      TT_REQUIRE(tt_grid_ok(T, (int)blk.x), "unpermute: grid too large");
       if (probs == nullptr) {
         if (K <= 2)
           hipLaunchKernelGGL((unpermute_small_kernel<TT, XD, kNoProbs, V, 2, 2>), grid, blk, 0, s, p, H, K, rows, experts, probs, E, o, M);
@@ -441,6 +442,7 @@ int launch_unpermute(const void* packed, int64_t T, int64_t H, int K, const int3
     const unsigned nthr =
         nvb <= 256 ? block_for(nvb) : (unsigned)(nvb <= 1024 ? ((nvb + 63) / 64) * 64 : 1024);
     const dim3 blk(nthr);
+    TT_REQUIRE(tt_grid_ok(T, (int)nthr), "unpermute: grid too large");
     if (probs == nullptr) {
       if (K <= 2)
         hipLaunchKernelGGL((unpermute_small_kernel<TT, XD, kNoProbs, V, 2, 1>), grid, blk, 0, s, p, H, K, rows, experts, probs, E, o, M);
@@ -458,9 +460,11 @@ int launch_unpermute(const void* packed, int64_t T, int64_t H, int K, const int3
     }
   } else if (al % 16 == 0) {
     constexpr int V = 16 / sizeof(St);
+    TT_REQUIRE(tt_grid_ok(T, (int)block_for(H / V)), "unpermute: grid too large");
     hipLaunchKernelGGL((unpermute_gather_kernel<TT, V>), dim3(T), dim3(block_for(H / V)), 0, s, p,
                        H, K, rows, experts, probs, pdt, E, prod_dt, o, M);
   } else {
+    TT_REQUIRE(tt_grid_ok(T, (int)block_for(H)), "unpermute: grid too large");
     hipLaunchKernelGGL((unpermute_gather_kernel<TT, 1>), dim3(T), dim3(block_for(H)), 0, s, p, H,
                        K, rows, experts, probs, pdt, E, prod_dt, o, M);
   }
@@ -476,6 +480,7 @@ int launch_unpermute_bwd_k(const void* gout, const void* packed, int64_t T, int6
   const uintptr_t al = reinterpret_cast<uintptr_t>(gout) | reinterpret_cast<uintptr_t>(packed) |
                        reinterpret_cast<uintptr_t>(gpacked) |
                        static_cast<uintptr_t>(H * sizeof(St));
+  TT_REQUIRE(tt_grid_ok(T, 256), "unpermute_bwd: grid too large");
   if (al % 16 == 0) {
     constexpr int V = 16 / sizeof(St);
     hipLaunchKernelGGL((unpermute_bwd_kernel<TT, V, KMAX>), dim3(T), dim3(256), 0, s,
@@ -523,6 +528,7 @@ extern "C" int tt_permute_scatter(const void* tokens, int dtype, int64_t num_tok
   const int64_t nvb = row_bytes / vb;
   const unsigned blk =
       nvb <= 256 ? block_for(nvb) : (unsigned)(nvb <= 1024 ? ((nvb + 63) / 64) * 64 : 1024);
+  TT_REQUIRE(tt_grid_ok(num_tokens, (int)blk), "permute: grid too large");
   const char* a = static_cast<const char*>(tokens);
   char* b = static_cast<char*>(packed);
   switch (vb) {
@@ -588,6 +594,7 @@ extern "C" int tt_packed_probs_bwd(const void* grad_packed_probs, int dtype, int
   if (n == 0) return TT_OK;
   const size_t lds = (size_t)4 * num_experts * sizeof(float);
   TT_REQUIRE(lds <= 64 * 1024, "packed_probs_bwd: too many experts (%d)", num_experts);
+  TT_REQUIRE(tt_grid_ok((num_tokens + 3) / 4, 256), "packed_probs_bwd: grid too large");
   hipLaunchKernelGGL(packed_probs_bwd_kernel, dim3((unsigned)((num_tokens + 3) / 4)), dim3(256),
                      lds, S(stream), grad_packed_probs, dtype, num_tokens, topk, num_experts,
                      row_indices, expert_indices, grad_probs_dense, num_tokens * topk);

@@ -1447,6 +1447,8 @@ extern "C" int tt_router_topk_fwd(const void* logits, int logits_dtype, int64_t 
     TT_REQUIRE(topk <= group_topk * gs, "router: topk exceeds the experts of the kept groups");
   }
   if (num_tokens == 0) return TT_OK;
+  TT_REQUIRE(tt_grid_ok((num_tokens + kRouterWaves - 1) / kRouterWaves, 256),
+             "router: grid too large");
   const dim3 grid((unsigned)((num_tokens + kRouterWaves - 1) / kRouterWaves));
   const int gk = fixed_indices ? 0 : group_topk;
   switch (epl) {
@@ -1475,6 +1477,8 @@ extern "C" int tt_router_topk_bwd(const void* logits, int logits_dtype, int64_t 
   TT_REQUIRE(topk >= 1 && topk <= 64 && topk <= num_experts, "router_bwd: bad topk");
   TT_REQUIRE(score_function >= 0 && score_function <= 2, "router_bwd: bad score function");
   if (num_tokens == 0) return TT_OK;
+  TT_REQUIRE(tt_grid_ok((num_tokens + kRouterWaves - 1) / kRouterWaves, 256),
+             "router: grid too large");
   const dim3 grid((unsigned)((num_tokens + kRouterWaves - 1) / kRouterWaves));
   switch (epl_for(num_experts)) {
 #define TT_CASE(N)                                                                            \
@@ -1662,6 +1666,8 @@ static int loss_bwd_run(const void* logits, int logits_dtype, int64_t num_tokens
              "router_loss_bwd: num_experts must be in [1, 1024]");
   TT_REQUIRE(score_function >= 0 && score_function <= 2, "router_loss_bwd: bad score function");
   if (num_tokens == 0) return TT_OK;
+  TT_REQUIRE(tt_grid_ok((num_tokens + kRouterWaves - 1) / kRouterWaves, 256),
+             "router: grid too large");
   const dim3 grid((unsigned)((num_tokens + kRouterWaves - 1) / kRouterWaves));
   switch (epl_for(num_experts)) {
 #define TT_CASE(N)                                                                               \

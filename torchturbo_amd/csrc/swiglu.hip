@@ -360,7 +360,9 @@ int launch_fwd_p(const void* x, int64_t rows, int64_t F, const void* probs, void
     constexpr int V = 16 / sizeof(St);
     split(F / V, nseg, seg);
     const int L = lanes_per_row(seg);
-    const dim3 grid((unsigned)((rows * nseg + 4 * (64 / L) - 1) / (4 * (64 / L))));
+    const int64_t blocks = (rows * nseg + 4 * (64 / L) - 1) / (4 * (64 / L));
+    TT_REQUIRE(tt_grid_ok(blocks, 256), "swiglu: grid too large");
+    const dim3 grid((unsigned)blocks);
     if (nseg > 1)
       hipLaunchKernelGGL((swiglu_fwd_kernel<TT, PD, V, true>), grid, dim3(256), 0, s, xp, rows,
                          F, probs, L, nseg, seg, op);
@@ -370,7 +372,9 @@ int launch_fwd_p(const void* x, int64_t rows, int64_t F, const void* probs, void
   } else {
     split(F, nseg, seg);
     const int L = lanes_per_row(seg);
-    const dim3 grid((unsigned)((rows * nseg + 4 * (64 / L) - 1) / (4 * (64 / L))));
+    const int64_t blocks = (rows * nseg + 4 * (64 / L) - 1) / (4 * (64 / L));
+    TT_REQUIRE(tt_grid_ok(blocks, 256), "swiglu: grid too large");
+    const dim3 grid((unsigned)blocks);
     if (nseg > 1)
       hipLaunchKernelGGL((swiglu_fwd_kernel<TT, PD, 1, true>), grid, dim3(256), 0, s, xp, rows,
                          F, probs, L, nseg, seg, op);
@@ -397,11 +401,13 @@ int launch_bwd_p(const void* x, int64_t rows, int64_t F, const void* probs, cons
     const int64_t nv = F / V;
     if (nv > 256) {
       const int64_t seg = (((nv + 3) / 4 + 63) / 64) * 64;
+      TT_REQUIRE(tt_grid_ok(rows, 256), "swiglu_bwd: grid too large");
       hipLaunchKernelGGL((swiglu_bwd_kernel<TT, PD, V, GP, true>), dim3((unsigned)rows),
                          dim3(256), 0, s, xp, rows, F, probs, 64, seg, gp, dxp, gprobs);
     } else {
       const int L = lanes_per_row(nv);
       const int64_t rpb = 4 * (64 / L);
+      TT_REQUIRE(tt_grid_ok((rows + rpb - 1) / rpb, 256), "swiglu: grid too large");
       hipLaunchKernelGGL((swiglu_bwd_kernel<TT, PD, V, GP, false>),
                          dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, s, xp, rows, F,
                          probs, L, nv, gp, dxp, gprobs);
@@ -409,6 +415,7 @@ int launch_bwd_p(const void* x, int64_t rows, int64_t F, const void* probs, cons
   } else {
     const int L = lanes_per_row(F);
     const int64_t rpb = 4 * (64 / L);
+    TT_REQUIRE(tt_grid_ok((rows + rpb - 1) / rpb, 256), "swiglu: grid too large");
     hipLaunchKernelGGL((swiglu_bwd_kernel<TT, PD, 1, GP, false>),
                        dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, s, xp, rows, F,
                        probs, L, F, gp, dxp, gprobs);
@@ -463,11 +470,13 @@ int launch_gated_fwd_p(const void* x, int64_t rows, int64_t F, const void* probs
     constexpr int V = 16 / sizeof(St);
     const int L = lanes_per_row(F / V);
     const int64_t rpb = 4 * (64 / L);
+    TT_REQUIRE(tt_grid_ok((rows + rpb - 1) / rpb, 256), "swiglu: grid too large");
     hipLaunchKernelGGL((gated_fwd_kernel<TT, PD, V>), dim3((unsigned)((rows + rpb - 1) / rpb)),
                        dim3(256), 0, s, xp, rows, F, probs, L, ga.act, ga.mode, ga.lim, op);
   } else {
     const int L = lanes_per_row(F);
     const int64_t rpb = 4 * (64 / L);
+    TT_REQUIRE(tt_grid_ok((rows + rpb - 1) / rpb, 256), "swiglu: grid too large");
     hipLaunchKernelGGL((gated_fwd_kernel<TT, PD, 1>), dim3((unsigned)((rows + rpb - 1) / rpb)),
                        dim3(256), 0, s, xp, rows, F, probs, L, ga.act, ga.mode, ga.lim, op);
   }
@@ -487,12 +496,14 @@ int launch_gated_bwd_p(const void* x, int64_t rows, int64_t F, const void* probs
     constexpr int V = 16 / sizeof(St);
     const int L = lanes_per_row(F / V);
     const int64_t rpb = 4 * (64 / L);
+    TT_REQUIRE(tt_grid_ok((rows + rpb - 1) / rpb, 256), "swiglu: grid too large");
     hipLaunchKernelGGL((gated_bwd_kernel<TT, PD, V, GP>),
                        dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, s, xp, rows, F,
                        probs, L, ga.act, ga.mode, ga.lim, gp, dxp, gprobs);
   } else {
     const int L = lanes_per_row(F);
     const int64_t rpb = 4 * (64 / L);
+    TT_REQUIRE(tt_grid_ok((rows + rpb - 1) / rpb, 256), "swiglu: grid too large");
     hipLaunchKernelGGL((gated_bwd_kernel<TT, PD, 1, GP>),
                        dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, s, xp, rows, F,
                        probs, L, ga.act, ga.mode, ga.lim, gp, dxp, gprobs);
