@@ -127,14 +127,14 @@ BIG = 1 << 24  # blocks of 256 threads that make 2^32
     ("tt_unpermute_gather_bwd", (AT, AT, 1, BIG, 64, 1, AT, AT, AT, 0, 4, AT, AT)),
     ("tt_packed_probs_bwd", (AT, 0, 4 * BIG, 2, 8, AT, AT, AT)),
     ("tt_swiglu_fwd", (AT, 1, 4 * BIG, 512, None, 0, AT)),
-    ("tt_swiglu_fwd", (AT, 1, 4 * BIG, 65, None, 0, AT)),
+    ("tt_swiglu_fwd", (AT, 1, 4 * BIG, 63, None, 0, AT)),
     ("tt_swiglu_bwd", (AT, 1, BIG, 4096, None, 0, AT, AT, None)),
     ("tt_swiglu_bwd", (AT, 1, 4 * BIG, 512, None, 0, AT, AT, None)),
-    ("tt_swiglu_bwd", (AT, 1, 4 * BIG, 65, None, 0, AT, AT, None)),
+    ("tt_swiglu_bwd", (AT, 1, 4 * BIG, 63, None, 0, AT, AT, None)),
     ("tt_gated_act_fwd", (AT, 1, 4 * BIG, 512, 1, 0.0, 0, None, 0, AT)),
-    ("tt_gated_act_fwd", (AT, 1, 4 * BIG, 65, 1, 0.0, 0, None, 0, AT)),
+    ("tt_gated_act_fwd", (AT, 1, 4 * BIG, 63, 1, 0.0, 0, None, 0, AT)),
     ("tt_gated_act_bwd", (AT, 1, 4 * BIG, 512, 1, 0.0, 0, None, 0, AT, AT, None)),
-    ("tt_gated_act_bwd", (AT, 1, 4 * BIG, 65, 1, 0.0, 0, None, 0, AT, AT, None)),
+    ("tt_gated_act_bwd", (AT, 1, 4 * BIG, 63, 1, 0.0, 0, None, 0, AT, AT, None)),
     ("tt_router_topk_fwd", (AT, 0, 4 * BIG, 8, 2, 0, 0, None, 0, 0, 1.0, None, AT, AT, AT)),
     ("tt_router_topk_bwd", (AT, 0, 4 * BIG, 8, 2, 0, 0, 1.0, AT, AT, AT)),
     ("tt_router_loss_bwd", (AT, 0, 4 * BIG, 8, 0, None, AT, AT, AT, AT, AT)),
