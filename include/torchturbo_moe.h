@@ -493,6 +493,62 @@ int tt_lora_wgrad_dropout(const void* x, const float* dh, int dtype, int64_t m, 
                           int32_t r, int32_t num_experts, const int64_t* counts, int32_t threshold,
                           const int64_t* key, float* da, void* stream);
 
+/* ---- Microscaling formats, products with 4-bit weights, the norm ----------
+ * Groups of 32 consecutive elements of a row share a power of two, kept as a byte c of
+ * value 2^(c - 127), 255 for NaN (E8M0). Elements are E2M1 (weights, two to a byte, the
+ * lower index in the low four bits) or E4M3 (rows). Rows are whole groups; tensors are
+ * row-major and contiguous. The reference has no counterpart as one op (it dequantises
+ * such checkpoints offline, scripts/dequant/).
+ *
+ * tt_mxfp4_quantize / tt_mxfp8_quantize: x [rows, cols] (f32 / bf16 / f16) to codes [rows,
+ *   cols / 2] or [rows, cols] and scales [rows, cols / 32], as the formats' specification
+ *   converts: c = floor(log2 amax) - 2 (8) + 127, elements rounded to nearest even and kept
+ *   within +-6 (448); a group of zeros has c = 0, NaN or infinity in a group makes it NaN.
+ * tt_mxfp4_dequantize / tt_mxfp8_dequantize: the values they stand for, rounded to dtype.
+ *
+ * tt_mx_product: y [M, N] = epilogue(x W[e]^T), rows grouped by expert as in tt_gmm_fwd
+ *   (tokens_per_expert NULL: one expert takes all M rows). x: bf16 [M, K], or with x_scales
+ *   E4M3 codes [M, K] and E8M0 [M, K / 32]; row_map (or NULL): row r of the product is row
+ *   row_map[r] of x, which has src_rows rows. codes [E, W, K / 2], scales [E, W, K / 32],
+ *   W = N, or gated 2 N with the gates' rows first. epilogue: act (0 none, 1 SiLU, 2 GELU) of
+ *   the product, gated: act of the first half times the second half; times probs[r] (f32 /
+ *   bf16 / f16, or NULL). y: bf16, or with y_scales E4M3 codes and their E8M0 bytes (N a
+ *   multiple of 32). Products are exact, sums run in fp32 and are rounded once.
+ * tt_mx_dgrad: dx [M, K] = dy [M, N] W[e], bf16, of weights that stay as they are.
+ * x, codes and dx are 16-byte aligned; K is a multiple of 32; any M, N.
+ *
+ * tt_rms_norm_fwd: h = x + residual (or x), y = h (mean(h^2) + eps)^(-1/2) weight over the
+ *   last of [rows, cols], each of y, sum (h, rounded), rstd [rows] and codes / scales (y in
+ *   E4M3, cols a multiple of 32) skipped when NULL. weight [cols] may have another dtype.
+ * tt_rms_norm_bwd: with h as rounded, a = gy weight, xh = h rstd: dx = rstd (a - xh
+ *   mean(a xh)) + gsum (or without, NULL), dweight = the sum over rows of gy xh, joined in a
+ *   fixed order; either skipped when NULL. workspace (dweight): tt_rms_norm_bwd_workspace
+ *   bytes, 4-byte aligned. */
+int tt_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, uint8_t* codes,
+                      uint8_t* scales, void* stream);
+int tt_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols,
+                        void* out, int dtype, void* stream);
+int tt_mxfp8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, uint8_t* codes,
+                      uint8_t* scales, void* stream);
+int tt_mxfp8_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols,
+                        void* out, int dtype, void* stream);
+int tt_mx_product(const void* x, const uint8_t* x_scales, const int32_t* row_map, int64_t src_rows,
+                  const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int64_t N,
+                  int32_t num_experts, const int64_t* tokens_per_expert, int32_t gated,
+                  int32_t act, const void* probs, int probs_dtype, void* y, uint8_t* y_scales,
+                  void* stream);
+int tt_mx_dgrad(const void* dy, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K,
+                int64_t N, int32_t num_experts, const int64_t* tokens_per_expert, void* dx,
+                void* stream);
+int tt_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
+                    int dtype, int64_t rows, int64_t cols, float eps, void* y, void* sum,
+                    float* rstd, uint8_t* codes, uint8_t* scales, void* stream);
+size_t tt_rms_norm_bwd_workspace(int64_t rows, int64_t cols);
+int tt_rms_norm_bwd(const void* h, const void* weight, int weight_dtype, const float* rstd,
+                    const void* gy, const void* gsum, int dtype, int64_t rows, int64_t cols,
+                    void* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,442 @@
+"""HIP quantisers of the microscaling formats and products with 4-bit weights against the oracle
+in 64 bits.
+
+Quantisation is exact arithmetic on its inputs: codes and bytes are equal. Products, with A the
+sum of the magnitudes of a result's K terms: a bf16 output is off by 2^-8 of itself; bf16 rows add
+K 2^-24 A (fp32 sums of exact products). The scaled matrix instruction adds products in sets of
+eight and keeps, of a set, what is at least 2^-13 of its largest: at most seven times that is lost,
+2^-10 of the set's magnitudes, so rows in 8 bits add 2^-10 A. On integers of a narrow range nothing
+is lost and every sum below 2^24 is exact: the output is the exact sum rounded once, to the bit.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle.native_providers import mx as o_mx
+from torchturbo_amd.dispatch import MxRows
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+def _weights(shape, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return o_mx.quantize_mxfp4(torch.randn(shape, generator=g) * 0.05)
+
+
+def _rows(m, k, mx, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g)
+    return o_mx.quantize_mxfp8(x) if mx else x.to(BF16)
+
+
+def _dev(x):
+    if isinstance(x, MxRows):
+        return MxRows(x.codes.to(DEV), x.scales.to(DEV))
+    return x.to(DEV)
+
+
+def _integers(m, k, n, mx, seed=0):
+    """Rows of whole numbers up to 4 and weights of 1, 2, 4 and 6 (E2M1 groups of byte 127) or 0."""
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.tensor([0, 2, 4, 6, 10, 12, 14, 15])[torch.randint(0, 8, (n, k), generator=g)]
+    codes = (codes[:, 0::2] + 16 * codes[:, 1::2]).to(torch.uint8)
+    x = torch.randint(-4, 5, (m, k), generator=g).float()
+    ones = lambda r: torch.full((r, k // 32), 127, dtype=torch.uint8)  # noqa: E731
+    rows = MxRows(x.to(torch.float8_e4m3fn), ones(m)) if mx else x.to(BF16)
+    return rows, codes, ones(n)
+
+
+def _bound(x, codes, scales, y):
+    """Of the plain product."""
+    v = o_mx.values_of(x)
+    w = o_mx.dequantize_mxfp4(codes, scales, torch.float64)
+    share = 2.0 ** -10 if isinstance(x, MxRows) else 0.0
+    return 2.0 ** -8 * y.abs() + (share + v.shape[1] * 2.0 ** -24) * (v.abs() @ w.abs().t()) + 1e-30
+
+
+def _within(got, want, bound, what=""):
+    got = got.double().cpu()
+    assert got.shape == want.shape, (got.shape, want.shape)
+    bad = ~((got - want).abs() <= bound)
+    assert not bad.any(), (what, int(bad.sum()), bad.nonzero()[:4].tolist(), got[bad][:4],
+                           want[bad][:4])
+
+
+# ---------------------------------------------------------------------------
+# Quantisers
+# ---------------------------------------------------------------------------
+def _spread(shape, dtype, seed=0):
+    """Groups from 2^-140 to 2^120 with ties, zeros, infinities and NaN among them."""
+    g = torch.Generator().manual_seed(seed)
+    v = torch.randn(shape, generator=g, dtype=torch.float64).unflatten(-1, (-1, 32))
+    low, high = (-24, 14) if dtype is torch.float16 else (-130, 118)
+    e = torch.randint(low, high, v.shape[:-1] + (1,), generator=g)
+    v = v * o_mx.power(e)
+    flat = v.view(-1, 32)
+    n = flat.shape[0]
+    flat[0] = 0
+    if n > 8:
+        flat[1] = torch.arange(32) * 0.25 - 4  # ties of both formats
+        flat[2] = torch.arange(32) * 32.0 - 500
+        flat[3, 5], flat[4, 31], flat[5, 0] = float("nan"), float("inf"), -float("inf")
+        flat[6] = torch.tensor([448.0, 464.0, 480.0, 511.0] * 8) * 2.0 ** -9
+        flat[7] = -0.0
+    return v.flatten(-2).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 32), (40, 96), (3, 5, 256), (0, 64), (7, 0)])
+def test_quantise_bits(hip_ops, dtype, shape):
+    x = _spread(shape, dtype) if all(shape) else torch.zeros(shape, dtype=dtype)
+    codes, scales = hip_ops.quantize_mxfp4(x.to(DEV))
+    want_c, want_s = o_mx.quantize_mxfp4(x)
+    assert torch.equal(scales.cpu(), want_s)
+    assert codes.shape == want_c.shape
+    # Equal values: a negative element that rounds to zero keeps its sign or not.
+    assert torch.equal(o_mx.e2m1_values(codes.cpu()), o_mx.e2m1_values(want_c))
+    rows, want = hip_ops.quantize_mxfp8(x.to(DEV)), o_mx.quantize_mxfp8(x)
+    assert torch.equal(rows.scales.cpu(), want.scales)
+    assert torch.equal(rows.codes.float().cpu().nan_to_num(nan=777.0),
+                       want.codes.float().nan_to_num(nan=777.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, torch.float16])
+def test_dequantise_every_code_and_byte(hip_ops, dtype):
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
+    scales = torch.arange(256, dtype=torch.uint8).unsqueeze(1).repeat(1, 16)
+    got = hip_ops.dequantize_mxfp4(codes.to(DEV), scales.to(DEV), dtype).cpu()
+    want = o_mx.dequantize_mxfp4(codes, scales, torch.float64)
+    if dtype is torch.float16:  # through fp32, whose subnormals f16 rounds to zero like the rest
+        want = want.float()
+    assert torch.equal(got.nan_to_num(nan=777.0), want.to(dtype).nan_to_num(nan=777.0))
+    eight = MxRows(torch.arange(256, dtype=torch.uint8).repeat(256, 1).view(torch.float8_e4m3fn),
+                   torch.arange(256, dtype=torch.uint8).unsqueeze(1).repeat(1, 8))
+    got = hip_ops.dequantize_mxfp8(_dev(eight), dtype).cpu()
+    want = o_mx.dequantize_mxfp8(eight, torch.float64).float().to(dtype)
+    assert torch.equal(got.nan_to_num(nan=777.0), want.nan_to_num(nan=777.0))
+
+
+def test_quantise_views_and_torch_types(hip_ops):
+    x = _spread((24, 128), BF16, seed=3).nan_to_num(nan=1.0, posinf=2.0, neginf=-2.0)
+    want = hip_ops.quantize_mxfp4(x.to(DEV))
+    store = torch.empty(24 * 128 + 1, dtype=BF16, device=DEV)
+    for view in (store[1:].view(24, 128).copy_(x),
+                 torch.empty(128, 24, dtype=BF16, device=DEV).t().copy_(x)):
+        assert all(torch.equal(a, b) for a, b in zip(hip_ops.quantize_mxfp4(view), want))
+    typed = (want[0].view(torch.float4_e2m1fn_x2), want[1].view(torch.float8_e8m0fnu))
+    assert torch.equal(hip_ops.dequantize_mxfp4(*typed), hip_ops.dequantize_mxfp4(*want))
+    rows = _dev(_rows(3, 128, False))
+    assert torch.equal(hip_ops.linear_mxfp4(rows, *typed), hip_ops.linear_mxfp4(rows, *want))
+
+
+# ---------------------------------------------------------------------------
+# Dense products
+# ---------------------------------------------------------------------------
+SIZES = [(1, 32, 1), (1, 7168, 96), (2, 64, 17), (3, 96, 40), (16, 160, 130), (17, 128, 48), (31, 512, 33),
+         (48, 256, 272), (65, 192, 100), (127, 1024, 64), (130, 288, 300), (300, 128, 520),
+         (257, 640, 257)]
+
+
+@pytest.mark.parametrize("m, k, n", SIZES)
+@pytest.mark.parametrize("mx", [False, True])
+def test_linear_integers_to_the_bit(hip_ops, m, k, n, mx):
+    x, codes, scales = _integers(m, k, n, mx, seed=m + n)
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV))
+    want = o_mx.linear(x, codes, scales).to(BF16)
+    assert torch.equal(got.cpu(), want), (got.cpu() != want).nonzero()[:8]
+
+
+@pytest.mark.parametrize("m, k, n", SIZES)
+@pytest.mark.parametrize("mx", [False, True])
+def test_linear(hip_ops, m, k, n, mx):
+    x, (codes, scales) = _rows(m, k, mx), _weights((n, k))
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV))
+    want = o_mx.linear(x, codes, scales)
+    _within(got, want, _bound(x, codes, scales, want))
+
+
+def _epilogue_bound(a, bound, act, gated, y):
+    """What an error ``bound`` of the product ``a`` makes of the epilogue's result, |act'| <= 1.13,
+    |act(v)| <= |v|, the exponential's 2^-20, and the output's rounding."""
+    n = a.shape[1] // 2
+    if gated:
+        gate, up, bg, bu = a[:, :n], a[:, n:], bound[:, :n], bound[:, n:]
+        value = act(gate)
+        e = 1.13 * bg * (up.abs() + bu) + value.abs() * bu + 2.0 ** -20 * (gate * up).abs()
+    else:
+        e = 1.13 * bound + 2.0 ** -20 * a.abs()
+    return e + 2.0 ** -8 * y.abs() + 1e-30
+
+
+ACTS = [(F.silu, True), (F.gelu, True), (F.silu, False), (F.gelu, False), (None, True)]
+
+
+@pytest.mark.parametrize("m, k, n", [(1, 128, 8), (3, 96, 13), (20, 256, 40), (70, 160, 136),
+                                     (200, 512, 160)])
+@pytest.mark.parametrize("act, gated", ACTS)
+@pytest.mark.parametrize("mx", [False, True])
+def test_linear_epilogues(hip_ops, m, k, n, act, gated, mx):
+    x, (codes, scales) = _rows(m, k, mx), _weights((2 * n if gated else n, k), seed=5)
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), activation_func=act,
+                               gated=gated)
+    a = o_mx.linear(x, codes, scales)
+    y = o_mx.epilogue(a, act, gated)
+    plain = _bound(x, codes, scales, torch.zeros_like(a))
+    _within(got, y, _epilogue_bound(a, plain, act or (lambda v: v), gated, y))
+
+
+def _within_8_bits(rows, y, bound):
+    """Each value within half a step of its group (or its group's top) and ``bound`` of y."""
+    got = o_mx.dequantize_mxfp8(MxRows(rows.codes.cpu(), rows.scales.cpu()), torch.float64)
+    step = o_mx.power(rows.scales.cpu().int() - 127).unsqueeze(-1)
+    v, b = y.unflatten(-1, (-1, 32)), bound.unflatten(-1, (-1, 32))
+    # The byte fits the group: 2^8 steps reach its largest magnitude, 2^9 exceed it.
+    amax, ab = v.abs().amax(-1, keepdim=True), b.amax(-1, keepdim=True)
+    assert ((256 * step <= amax + ab) & (512 * step > amax - ab)).all()
+    exponent = torch.log2(((v.abs() + b) / step).clamp(min=2.0 ** -6)).floor()
+    half = torch.maximum(2.0 ** (exponent - 4) * step, v.abs() - 448 * step)
+    _within(got, y, (half + 2 * b).flatten(-2), "8 bits")
+
+
+@pytest.mark.parametrize("m, k, n", [(1, 128, 32), (5, 96, 96), (40, 256, 160), (150, 128, 288),
+                                     (260, 512, 128)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("mx", [False, True])
+def test_linear_output_in_8_bits(hip_ops, m, k, n, gated, mx):
+    act = F.silu if gated else None
+    x, (codes, scales) = _rows(m, k, mx), _weights((2 * n if gated else n, k), seed=6)
+    rows = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), activation_func=act,
+                                gated=gated, mx_out=True)
+    a = o_mx.linear(x, codes, scales)
+    y = o_mx.epilogue(a, act, gated)
+    plain = _bound(x, codes, scales, torch.zeros_like(a))
+    _within_8_bits(rows, y, _epilogue_bound(a, plain, act or (lambda v: v), gated, 0 * y))
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_nan_and_infinity_stay_where_they_belong(hip_ops, mx):
+    m, k, n = 70, 256, 96
+    x, (codes, scales) = _rows(m, k, mx), _weights((n, k))
+    clean = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV)).cpu()
+    scales = scales.clone()
+    scales[11, 3] = 255  # a NaN group of the weights: column 11 of every row
+    if mx:
+        x.scales[20, 7] = 255
+    else:
+        x[20, 255] = float("nan")
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV)).cpu()
+    nan = torch.zeros(m, n, dtype=torch.bool)
+    nan[:, 11] = nan[20] = True
+    assert got[nan].isnan().all() and torch.equal(got[~nan], clean[~nan])
+
+
+def test_leading_dimensions_empty_and_views(hip_ops):
+    codes, scales = (t.to(DEV) for t in _weights((40, 64)))
+    x = _rows(12, 64, False).to(DEV)
+    y = hip_ops.linear_mxfp4(x, codes, scales)
+    assert torch.equal(hip_ops.linear_mxfp4(x.view(3, 4, 64), codes, scales), y.view(3, 4, 40))
+    assert torch.equal(hip_ops.linear_mxfp4(x[0], codes, scales), y[0])
+    assert hip_ops.linear_mxfp4(x[:0], codes, scales).shape == (0, 40)
+    assert torch.equal(hip_ops.linear_mxfp4(x[:, :0], codes[:, :0], scales[:, :0]),
+                       torch.zeros_like(y))
+    store = torch.empty(12 * 64 + 1, dtype=BF16, device=DEV)
+    assert torch.equal(hip_ops.linear_mxfp4(store[1:].view(12, 64).copy_(x), codes, scales), y)
+    odd = torch.empty(40 * 32 + 5, dtype=torch.uint8, device=DEV)[5:].view(40, 32).copy_(codes)
+    assert torch.equal(hip_ops.linear_mxfp4(x, odd, scales), y)
+    wide = torch.empty(12, 128, dtype=BF16, device=DEV)[:, ::2].copy_(x)
+    assert torch.equal(hip_ops.linear_mxfp4(wide, codes, scales), y)
+
+
+@pytest.mark.parametrize("m, k, n", [(1, 32, 1), (3, 96, 40), (17, 128, 33), (64, 512, 64), (130, 160, 72),
+                                     (129, 256, 520), (300, 288, 65)])
+def test_linear_gradient(hip_ops, m, k, n):
+    x, (codes, scales) = _rows(m, k, False), _weights((n, k), seed=2)
+    dy = torch.randn(m, n, generator=torch.Generator().manual_seed(9)).to(BF16)
+    xd = x.to(DEV).requires_grad_()
+    y = hip_ops.linear_mxfp4(xd, codes.to(DEV), scales.to(DEV))
+    want = o_mx.linear(x, codes, scales)
+    _within(y.detach(), want, _bound(x, codes, scales, want))
+    dx, = torch.autograd.grad(y, xd, dy.to(DEV))
+    w = o_mx.dequantize_mxfp4(codes, scales, torch.float64)
+    dwant = dy.double() @ w
+    _within(dx, dwant, 2.0 ** -8 * dwant.abs() + n * 2.0 ** -24 * (dy.double().abs() @ w.abs()) + 1e-30)
+    ints, icodes, iscales = _integers(m, k, n, False, seed=4)
+    idy = torch.randint(-4, 5, (m, n), generator=torch.Generator().manual_seed(3)).to(BF16)
+    xd = ints.to(DEV).requires_grad_()
+    dx, = torch.autograd.grad(hip_ops.linear_mxfp4(xd, icodes.to(DEV), iscales.to(DEV)), xd,
+                              idy.to(DEV))
+    assert torch.equal(dx.cpu(), (idy.double() @ o_mx.dequantize_mxfp4(icodes, iscales, torch.float64)).to(BF16))
+
+
+def test_linear_gradient_through_the_activation(hip_ops):
+    """The bf16 product between the two passes is off by 2^-8 of itself."""
+    m, k, n = 33, 128, 48
+    x, (codes, scales) = _rows(m, k, False), _weights((2 * n, k), seed=2)
+    dy = torch.randn(m, n, generator=torch.Generator().manual_seed(9)).to(BF16)
+    for act, gated in ACTS:
+        w = (codes, scales) if gated else (codes[:n], scales[:n])
+        xd = x.to(DEV).requires_grad_()
+        y = hip_ops.linear_mxfp4(xd, *(t.to(DEV) for t in w), activation_func=act, gated=gated)
+        dx, = torch.autograd.grad(y, xd, dy.to(DEV))
+        xw = x.double().requires_grad_()
+        want, = torch.autograd.grad(o_mx.linear(xw, *w, activation_func=act, gated=gated), xw,
+                                    dy.double())
+        # Roundings of the product, of its gradient and of dx: some 2^-8 each of terms that the
+        # sum over the features averages; the norm is off by three such steps at most.
+        assert (dx.double().cpu() - want).norm() <= 3 * 2.0 ** -8 * want.norm(), (act, gated)
+
+
+# ---------------------------------------------------------------------------
+# Experts
+# ---------------------------------------------------------------------------
+COUNTS = [[5], [0, 0, 3], [1, 0, 17, 2], [40, 0, 0, 33, 64, 1], [130, 5, 0, 300], [0, 0], [16] * 9,
+          [0] * 60 + [1, 0, 0, 2]]
+
+
+@pytest.mark.parametrize("counts", COUNTS)
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("k, n", [(96, 40), (256, 136)])
+def test_grouped_integers_to_the_bit(hip_ops, counts, mx, k, n):
+    m, e = sum(counts), len(counts)
+    x, codes, scales = _integers(m, k, n * e, mx, seed=len(counts))
+    codes, scales = codes.view(e, n, -1), scales.view(e, n, -1)
+    want = o_mx.grouped(x, codes, scales, counts).to(BF16)
+    args = _dev(x), codes.to(DEV), scales.to(DEV)
+    for given in (counts, torch.tensor(counts), torch.tensor(counts, device=DEV)):
+        assert torch.equal(hip_ops.grouped_matmul_mxfp4(*args, given).cpu(), want)
+    perm = torch.randperm(m, generator=torch.Generator().manual_seed(1))
+    inverse = torch.argsort(perm).int().to(DEV)
+    shuffled = MxRows(x.codes.view(torch.uint8)[perm].view(torch.float8_e4m3fn), x.scales[perm]) \
+        if mx else x[perm]
+    got = hip_ops.grouped_matmul_mxfp4(_dev(shuffled), *args[1:], counts, row_map=inverse)
+    assert torch.equal(got.cpu(), want)
+    if not mx and m:
+        idy = torch.randint(-4, 5, (m, n), generator=torch.Generator().manual_seed(3)).to(BF16)
+        xd = _dev(x).requires_grad_()
+        dx, = torch.autograd.grad(hip_ops.grouped_matmul_mxfp4(xd, *args[1:], counts), xd, idy.to(DEV))
+        w = o_mx.dequantize_mxfp4(codes, scales, torch.float64)
+        parts = [p @ w[i] for i, p in enumerate(idy.double().split(counts))]
+        assert torch.equal(dx.cpu(), torch.cat(parts).to(BF16))
+
+
+@pytest.mark.parametrize("counts", [[1, 0, 17, 2], [40, 0, 90, 33], [3] * 12])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("pdt", [None, torch.float32, BF16])
+def test_grouped_gated(hip_ops, counts, mx, pdt):
+    m, e, k, n = sum(counts), len(counts), 160, 64
+    x, (codes, scales) = _rows(m, k, mx), _weights((e, 2 * n, k), seed=7)
+    g = torch.Generator().manual_seed(8)
+    probs = None if pdt is None else torch.rand(m, generator=g).to(pdt)
+    dprobs = None if pdt is None else probs.to(DEV)
+    a = o_mx.grouped(x, codes, scales, counts)
+    y = o_mx.epilogue(a, F.silu, True, probs)
+    v, at, bounds = o_mx.values_of(x), 0, []
+    for i, c in enumerate(counts):
+        part = MxRows(x.codes[at:at + c], x.scales[at:at + c]) if mx else x[at:at + c]
+        bounds.append(_bound(part, codes[i], scales[i], torch.zeros(c, 2 * n, dtype=torch.float64)))
+        at += c
+    factor = 1.0 if probs is None else probs.double().unsqueeze(1)
+    bound = _epilogue_bound(a, torch.cat(bounds), F.silu, True, 0 * y) * factor
+    args = _dev(x), codes.to(DEV), scales.to(DEV), counts
+    got = hip_ops.grouped_matmul_mxfp4(*args, gated=True, probs=dprobs)
+    _within(got, y, bound + 2.0 ** -8 * y.abs())
+    rows = hip_ops.grouped_matmul_mxfp4(*args, gated=True, probs=dprobs, mx_out=True)
+    _within_8_bits(rows, y, bound + 1e-30)
+    assert v.shape == (m, k)
+
+
+def test_grouped_gradients_of_rows_and_probabilities(hip_ops):
+    counts, k, n = [20, 0, 7, 50], 128, 64
+    m, e = sum(counts), len(counts)
+    x, (codes, scales) = _rows(m, k, False), _weights((e, 2 * n, k), seed=7)
+    g = torch.Generator().manual_seed(8)
+    probs, dy = torch.rand(m, generator=g), torch.randn(m, n, generator=g).to(BF16)
+    for gated in (True, False):
+        w = (codes, scales) if gated else (codes[:, :n].contiguous(), scales[:, :n].contiguous())
+        leaves = [x.to(DEV).requires_grad_(), probs.to(DEV).requires_grad_()]
+        y = hip_ops.grouped_matmul_mxfp4(leaves[0], *(t.to(DEV) for t in w), counts, probs=leaves[1],
+                                         gated=gated)
+        got = torch.autograd.grad(y, leaves, dy.to(DEV))
+        wide = [x.double().requires_grad_(), probs.double().requires_grad_()]
+        yw = o_mx.grouped(wide[0], *w, counts, probs=wide[1], gated=gated)
+        want = torch.autograd.grad(yw, wide, dy.double())
+        for a, b in zip(got, want):  # three roundings of 2^-8, averaged by the sums
+            assert (a.double().cpu() - b).norm() <= 3 * 2.0 ** -8 * b.norm()
+
+
+def test_experts_of_many_rows_and_offsets_past_32_bits(hip_ops):
+    """Weights past 4 GiB: the last expert's product is its own."""
+    e, n, k = 34, 16384, 16384
+    codes = torch.empty((e, n, k // 2), dtype=torch.uint8, device=DEV)
+    scales = torch.full((e, n, k // 32), 127, dtype=torch.uint8, device=DEV)
+    codes[:-1].fill_(0x77)
+    x, small, _ = _integers(3, k, 64, False, seed=5)
+    codes[-1].zero_()
+    codes[-1, -64:] = small.to(DEV)
+    for m, mx in ((3, False), (3, True)):
+        rows = MxRows(x.float().to(torch.float8_e4m3fn).to(DEV),
+                      torch.full((3, k // 32), 127, dtype=torch.uint8, device=DEV)) if mx else x.to(DEV)
+        y = hip_ops.grouped_matmul_mxfp4(rows, codes, scales, [0] * (e - 1) + [m])
+        want = o_mx.linear(x, small, torch.full((64, k // 32), 127, dtype=torch.uint8)).to(BF16)
+        assert torch.equal(y[:, -64:].cpu(), want) and not y[:, :-64].any()
+    xd = x.to(DEV).requires_grad_()
+    dy = torch.zeros(3, n, dtype=BF16, device=DEV)
+    dy[:, -64:] = torch.randint(-4, 5, (3, 64)).to(BF16).to(DEV)
+    dx, = torch.autograd.grad(hip_ops.grouped_matmul_mxfp4(xd, codes, scales, [0] * (e - 1) + [3]), xd, dy)
+    w = o_mx.dequantize_mxfp4(small, torch.full((64, k // 32), 127, dtype=torch.uint8), torch.float64)
+    assert torch.equal(dx.cpu(), (dy[:, -64:].double().cpu() @ w).to(BF16))
+
+
+def test_more_experts_than_rows_and_repeats(hip_ops):
+    e, k, n = 1000, 64, 32
+    x, codes, scales = _integers(10, k, n * e, False)
+    codes, scales = codes.view(e, n, -1), scales.view(e, n, -1)
+    counts = torch.zeros(e, dtype=torch.int64)
+    counts[torch.tensor([0, 3, 63, 64, 255, 256, 511, 700, 998, 999])] = 1
+    want = o_mx.grouped(x, codes, scales, counts).to(BF16)
+    args = x.to(DEV), codes.to(DEV), scales.to(DEV), counts.to(DEV)
+    first = hip_ops.grouped_matmul_mxfp4(*args)
+    assert torch.equal(first.cpu(), want)
+    assert all(torch.equal(hip_ops.grouped_matmul_mxfp4(*args), first) for _ in range(3))
+
+
+def test_graph_replay_and_another_stream(hip_ops):
+    counts = torch.tensor([20, 0, 7, 50], device=DEV)
+    k, n = 128, 64
+    m = 77
+    x = _rows(m, k, False).to(DEV)
+    codes, scales = (t.to(DEV) for t in _weights((4, 2 * n, k), seed=7))
+    dy = torch.randn(m, 2 * n, device=DEV).to(BF16)
+
+    def step():
+        with torch.no_grad():
+            rows = hip_ops.quantize_mxfp8(x)
+            h = hip_ops.grouped_matmul_mxfp4(rows, codes, scales, counts, gated=True, mx_out=True)
+            d = hip_ops.linear_mxfp4(rows, codes[0], scales[0])
+        xd = x.detach().requires_grad_()
+        y = hip_ops.grouped_matmul_mxfp4(xd, codes, scales, counts)
+        dx, = torch.autograd.grad(y, xd, dy)
+        return [rows.scales, h.codes.view(torch.uint8), h.scales, d, y.detach(), dx]
+
+    eager = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(eager, other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(3):
+        x.copy_(_rows(m, k, False, seed=20 + seed))
+        counts.copy_(torch.tensor([[1, 70, 6, 0], [0, 0, 77, 0], [19, 19, 19, 20]][seed]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, step()))

@@ -89,12 +89,22 @@ _PROTOS: dict[str, list] = {
                                P, P, c_size_t, P],
     "tt_dropout": [P, c_int, I64, I64, I32, P, P, P],
     "tt_fp8_quantize_blocks": [P, c_int, I64, I64, I64, P, P, c_int, P],
+    "tt_mxfp4_quantize": [P, c_int, I64, I64, P, P, P],
+    "tt_mxfp4_dequantize": [P, P, I64, I64, P, c_int, P],
+    "tt_mxfp8_quantize": [P, c_int, I64, I64, P, P, P],
+    "tt_mxfp8_dequantize": [P, P, I64, I64, P, c_int, P],
+    "tt_mx_product": [P, P, P, I64, P, P, I64, I64, I64, I32, P, I32, I32, P, c_int, P, P, P],
+    "tt_mx_dgrad": [P, P, P, I64, I64, I64, I32, P, P, P],
+    "tt_rms_norm_fwd": [P, P, P, c_int, c_int, I64, I64, c_float, P, P, P, P, P, P],
+    "tt_rms_norm_bwd_workspace": [I64, I64],
+    "tt_rms_norm_bwd": [P, P, c_int, P, P, P, c_int, I64, I64, P, P, P, c_size_t, P],
 }
 _RESTYPES = {"tt_last_error": ctypes.c_char_p, "tt_route_index_workspace": c_size_t,
              "tt_route_index_rejected_offset": c_size_t, "tt_router_loss_workspace": c_size_t,
              "tt_moe_experts_workspace": c_size_t, "tt_router_gate_bwd_workspace": c_size_t,
              "tt_linear_workspace": c_size_t, "tt_linear_act_bwd_workspace": c_size_t,
-             "tt_linear_residual_bwd_workspace": c_size_t}
+             "tt_linear_residual_bwd_workspace": c_size_t,
+             "tt_rms_norm_bwd_workspace": c_size_t}
 ABI_VERSION = 1
 
 _LIB: ctypes.CDLL | None = None

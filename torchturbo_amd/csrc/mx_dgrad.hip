@@ -1,0 +1,219 @@
+// Gradient of bf16 rows through frozen 4-bit weights (gfx950): dx [M, K] = dy [M, N] W[e], with
+// W [N, K] in groups of 32 along K.
+//
+// The reduction runs across the rows of W, whose elements lie along K, so the matrix instructions
+// need W transposed: a block turns a 64 x 128 piece of codes into bf16 (exact, two codes an
+// instruction, each thread one group with its scale) and writes it to LDS as it lies; the transposing
+// LDS reads then give each lane eight reduction elements of a column. dy goes straight from memory
+// to LDS. Both are double-buffered: the next k-tile's loads are in flight while a tile is
+// multiplied. Every product is exact in fp32; sums run in fp32 and dx is rounded once.
+#include "mx_gemm.h"
+
+namespace {
+
+constexpr int D_NT = 256, D_BM = 128, D_BN = 128, D_BK = 64;
+constexpr int D_A = D_BM * D_BK * 2, D_B = D_BN * D_BK * 2, D_STAGE = D_A + D_B;
+
+// ALIGNED: rows of dy are multiples of 16 bytes at 16-byte addresses.
+template <bool ALIGNED>
+__global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
+    const char* __restrict__ dy, const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
+    char* __restrict__ dx, int64_t M, int64_t K, int64_t N, int E,
+    const int64_t* __restrict__ counts, int tiles_j) {
+  __shared__ __align__(16) char lds_raw[2 * D_STAGE];
+  RowTile t;
+  if (counts != nullptr) {
+    if (!row_tile<D_BM, D_NT>(counts, E, tiles_j, lds_raw, t)) return;
+    // Counts that sum to more than M end at its last row.
+    if (t.seg0 + t.nrows > M) t.nrows = M - t.seg0;
+    if ((int64_t)t.mt * D_BM >= t.nrows) return;
+  } else {
+    t.e = 0;
+    const int tiles_i = (int)((M + D_BM - 1) / D_BM);
+    const int slot = xcd_remap(blockIdx.x, tiles_i * tiles_j);
+    t.mt = slot % tiles_i;
+    t.nt = slot / tiles_i;
+    t.seg0 = 0;
+    t.nrows = M;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t i0 = (int64_t)t.mt * D_BM, j0 = (int64_t)t.nt * D_BN;
+  const int64_t rows = t.nrows - i0;
+  const int nkt = (int)((N + D_BK - 1) / D_BK);
+  lds_char* const lds = (lds_char*)lds_raw;
+
+  // dy: wave w loads rows 32 w + 8 q + lane / 8, chunk slot lane % 8 holding chunk
+  // slot ^ ((row >> 1) & 7); rows past the expert's and elements past a row's end read as zeros.
+  const char* const a0 = dy + (t.seg0 + i0) * N * 2;
+  const i32x4 ra = make_rsrc(a0, (rows < D_BM ? rows : D_BM) * N * 2);
+  uint32_t aoff[4];
+  int akof[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = 32 * wave + 8 * q + (lane >> 3);
+    const int c = (lane & 7) ^ ((r >> 1) & 7);
+    akof[q] = 8 * c;
+    aoff[q] = (uint32_t)(r * N + 8 * c) * 2u;
+  }
+  // W: thread t takes row t / 4 of a k-tile, group t % 4 of the tile's columns. Groups past a row's
+  // end read the last one again: their columns are not stored.
+  const int wr = tid >> 2;
+  const int64_t groups = K / MX_GROUP;
+  int64_t wg = j0 / MX_GROUP + (tid & 3);
+  wg = wg < groups ? wg : groups - 1;
+  const uint8_t* const wp = w + (int64_t)t.e * N * (K / 2) + wg * 16;
+  const uint8_t* const wsp = ws + (int64_t)t.e * N * groups + wg;
+
+  uint4 wv;
+  uint32_t wsv;
+  auto load = [&](int kt, int buf) {
+    const int64_t n = (int64_t)kt * D_BK + wr;
+    wv = uint4{0, 0, 0, 0};
+    wsv = 127u;
+    if (n < N) {
+      wv = *reinterpret_cast<const uint4*>(wp + n * (K / 2));
+      wsv = wsp[n * groups];
+    }
+    lds_char* const a = lds + buf * D_STAGE;
+    if constexpr (ALIGNED) {
+      const uint32_t base = lds_addr_of(a) + (uint32_t)(4 * wave) * 1024u;
+      const i32x4 rk = advance_rsrc(ra, (uint32_t)kt * (D_BK * 2));
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        dma16((int64_t)kt * D_BK + akof[q] < N ? aoff[q] : DM_OOB, rk, base + q * 1024u);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = 32 * wave + 8 * q + (lane >> 3);
+        const int64_t n0 = (int64_t)kt * D_BK + akof[q];
+        const uint16_t* const p = reinterpret_cast<const uint16_t*>(a0) + r * N + n0;
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = r < rows && n0 + 2 * e < N ? p[2 * e] : 0u;
+          const uint32_t hi = r < rows && n0 + 2 * e + 1 < N ? p[2 * e + 1] : 0u;
+          v[e] = lo | hi << 16;
+        }
+        *reinterpret_cast<lds_u32x4*>(a + (4 * wave + q) * 1024 + 16 * lane) =
+            u32x4{v[0], v[1], v[2], v[3]};
+      }
+    }
+  };
+  // The k-row's chunk c (eight columns) lies in slot c ^ (4 (row % 4)).
+  auto put = [&](int buf) {
+    lds_char* const b = lds + buf * D_STAGE + D_A + wr * 256;
+    const uint32_t q[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = mx_bf16x8(q[i], wsv);
+      const int c = 4 * (tid & 3) + i;
+      *reinterpret_cast<lds_u32x4*>(b + ((c ^ (4 * (wr & 3))) << 4)) = u32x4{v.x, v.y, v.z, v.w};
+    }
+  };
+  // Wave w multiplies rows 64 (w / 2) .. + 63 and columns 64 (w % 2) .. + 63.
+  const int m0 = 64 * (wave >> 1), n0 = 64 * (wave & 1);
+  uint32_t fa[4], fb[4][2];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    fa[s] = fragk64(m0, s, lane);
+    const int g = lane >> 4, i = lane & 15;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int col = n0 + 32 * b + 16 * (g & 1) + 4 * (i & 3);
+      const int kr = 16 * s + 8 * (g >> 1) + (i >> 2);
+      fb[s][b] = D_A + (uint32_t)(kr * 256 + (((col >> 3) ^ (4 * (kr & 3))) << 4) + (col & 7) * 2);
+    }
+  }
+  f32x16 acc[2][2] = {};
+  if (nkt > 0) {
+    load(0, 0);
+    put(0);
+  }
+  TT_WAIT_VMCNT(0);
+  TT_LDS_BARRIER();
+  for (int kt = 0; kt < nkt; ++kt) {
+    const int buf = kt & 1;
+    if (kt + 1 < nkt) load(kt + 1, buf ^ 1);
+    lds_char* const st = lds + buf * D_STAGE;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      uint4 b[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(st + fb[s][j]));
+        const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(st + fb[s][j] + 1024));
+        const uint2 p0 = __builtin_bit_cast(uint2, v0), p1 = __builtin_bit_cast(uint2, v1);
+        b[j] = uint4{p0.x, p0.y, p1.x, p1.y};
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 a = read_k(st, fa[s] + i * 4096);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = Mma<TT_BF16>::run(b[j], a, acc[i][j]);
+      }
+    }
+    if (kt + 1 < nkt) put(buf ^ 1);
+    TT_WAIT_VMCNT(0);
+    TT_LDS_BARRIER();
+  }
+  // The tile through LDS, rows of 256 bytes, chunk c of row r in slot c ^ (r % 16). Register 4 q + e
+  // of lane l: row l % 32, column 8 q + 4 (l / 32) + e.
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = m0 + 32 * i + (lane & 31), c = (n0 + 32 * j) / 8 + q;
+        const uint2 v = pack4<TT_BF16>(acc[i][j][4 * q], acc[i][j][4 * q + 1],
+                                       acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        *reinterpret_cast<lds_u32x2*>(lds + r * 256 + ((c ^ (r & 15)) << 4) + 8 * (lane >> 5)) =
+            u32x2{v.x, v.y};
+      }
+  TT_LDS_BARRIER();
+  const int c = tid & 15;
+  if (j0 + 8 * c >= K) return;
+#pragma unroll
+  for (int p = 0; p < D_BM / 16; ++p) {
+    const int r = 16 * p + (tid >> 4);
+    if (r < rows)
+      *reinterpret_cast<uint4*>(dx + ((t.seg0 + i0 + r) * K + j0 + 8 * c) * 2) =
+          read_k(lds, (uint32_t)(r * 256 + ((c ^ (r & 15)) << 4)));
+  }
+}
+
+}  // namespace
+
+extern "C" int tt_mx_dgrad(const void* dy, const uint8_t* codes, const uint8_t* scales, int64_t M,
+                           int64_t K, int64_t N, int32_t num_experts,
+                           const int64_t* tokens_per_expert, void* dx, void* stream) {
+  TT_REQUIRE(M >= 0 && K >= 0 && N >= 0 && num_experts > 0, "mx dgrad: bad sizes");
+  TT_REQUIRE(K % MX_GROUP == 0, "mx dgrad: the weights' rows are whole groups of 32 elements");
+  TT_REQUIRE(K < (1ll << 31) && N < (1ll << 24) && M < (1ll << 31) && num_experts <= 65536,
+             "mx dgrad: sizes past 2^31 (2^24 columns)");
+  TT_REQUIRE(tokens_per_expert != nullptr || num_experts == 1,
+             "mx dgrad: several experts need their counts");
+  if (M == 0 || K == 0) return TT_OK;
+  TT_REQUIRE(dx != nullptr && (N == 0 || (dy != nullptr && codes != nullptr && scales != nullptr)),
+             "mx dgrad: NULL tensor");
+  TT_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(dx)) & 15) == 0,
+             "mx dgrad: codes and dx must be 16-byte aligned");
+  const int64_t tiles_j = (K + D_BN - 1) / D_BN;
+  int64_t tiles_i = (M + D_BM - 1) / D_BM;
+  if (tokens_per_expert != nullptr) tiles_i = M / D_BM + (num_experts < M ? num_experts : M);
+  TT_REQUIRE(tiles_i * tiles_j < (1ll << 31) && tt_grid_ok(tiles_i * tiles_j, D_NT),
+             "mx dgrad: grid too large");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(tiles_i * tiles_j));
+  const bool aligned = N % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
+  if (aligned)
+    hipLaunchKernelGGL((mx_dgrad_kernel<true>), grid, dim3(D_NT), 0, s, static_cast<const char*>(dy),
+                       codes, scales, static_cast<char*>(dx), M, K, N, num_experts,
+                       tokens_per_expert, (int)tiles_j);
+  else
+    hipLaunchKernelGGL((mx_dgrad_kernel<false>), grid, dim3(D_NT), 0, s,
+                       static_cast<const char*>(dy), codes, scales, static_cast<char*>(dx), M, K, N,
+                       num_experts, tokens_per_expert, (int)tiles_j);
+  return tt_check_launch("mx_dgrad");
+}

@@ -3,12 +3,15 @@
 from .base import OpImpl, OpImplKind, OpPolicy, OpSpec
 from .dispatcher import OpDispatcher
 from .moe import MoEPermutation, get_expert_indices
+from .mx import MxRows, NormRows
 from .ops import get_ops, get_or_create_ops, op_resolves, ops, reset_ops
 from .providers import add_provider_package, iter_provider_modules, remove_provider_package
 from .registry import OpRegistry, register_op, registry
 
 __all__ = [
     "MoEPermutation",
+    "MxRows",
+    "NormRows",
     "OpDispatcher",
     "OpImpl",
     "OpImplKind",

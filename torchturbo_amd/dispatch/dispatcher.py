@@ -258,6 +258,32 @@ class OpDispatcher:
         position of an element. No reference counterpart."""
         return self._dispatch("dropout", x, p, key, impl=impl)
 
+    def rms_norm(self, x, weight, eps: float = 1e-6, *, residual=None, impl: str | None = None):
+        """``y = h / sqrt(mean(h^2) + eps) * weight`` of ``h = x + residual``; ``(y, h)`` with a
+        residual."""
+        return self._dispatch("rms_norm", x, weight, eps, residual=residual, impl=impl)
+
+    def rms_norm_mx(self, x, weight, eps: float = 1e-6, *, residual=None, with_y: bool = False,
+                    impl: str | None = None):
+        """``rms_norm`` with its output in 8 bits (``NormRows``). No reference counterpart."""
+        return self._dispatch("rms_norm_mx", x, weight, eps, residual=residual, with_y=with_y,
+                              impl=impl)
+
+    def linear_mxfp4(self, x, codes, scales, *, activation_func=None, gated: bool = False,
+                     mx_out: bool = False, impl: str | None = None):
+        """``act(x @ W.T)`` with 4-bit ``W``, rows in bf16 or 8 bits (``MxRows``). No reference
+        counterpart."""
+        return self._dispatch("linear_mxfp4", x, codes, scales, activation_func=activation_func,
+                              gated=gated, mx_out=mx_out, impl=impl)
+
+    def grouped_matmul_mxfp4(self, x, codes, scales, tokens_per_expert, *, probs=None,
+                             gated: bool = False, row_map=None, mx_out: bool = False,
+                             impl: str | None = None):
+        """``grouped_matmul`` with 4-bit weights; gated: SwiGLU; times ``probs``. No reference
+        counterpart."""
+        return self._dispatch("grouped_matmul_mxfp4", x, codes, scales, tokens_per_expert,
+                              probs=probs, gated=gated, row_map=row_map, mx_out=mx_out, impl=impl)
+
     def moe_permutation(
         self,
         tokens: torch.Tensor,

@@ -1,0 +1,283 @@
+"""HIP products with 4-bit weights, and the quantisers of the microscaling formats.
+
+Weights ``[..., N, K]`` are kept as E2M1 codes (uint8 ``[..., N, K / 2]``, the lower index in
+the low four bits) with one power of two per 32 elements of a row (uint8 ``[..., N,
+K / 32]``, ``2^(byte - 127)``, 255 for NaN); rows in 8 bits are ``MxRows``. torch's own
+``float4_e2m1fn_x2`` and ``float8_e8m0fnu`` tensors are taken as well.
+
+* ``quantize_mxfp4(weight)`` -> ``(codes, scales)``, ``dequantize_mxfp4(codes, scales, dtype)``;
+  ``quantize_mxfp8(x)`` -> ``MxRows``, ``dequantize_mxfp8(rows, dtype)``. The conversion of the
+  formats' specification (OCP MX 1.0).
+* ``linear_mxfp4(x, codes, scales, activation_func, gated, mx_out)``: ``act(x W^T)``, gated with
+  the gate's rows first in ``W [2 N, K]``: ``act(a[..., :N]) * a[..., N:]``.
+* ``grouped_matmul_mxfp4(x, codes, scales, tokens_per_expert, probs, gated, row_map, mx_out)``:
+  the same for every expert's rows, SwiGLU where gated, each row times its probability.
+  ``row_map`` (int32 ``[M]``): row r is row ``row_map[r]`` of x.
+
+``x`` is bf16 or ``MxRows``; the output bf16, or with ``mx_out`` ``MxRows``. Every product of two
+elements is exact, sums run in fp32 and are rounded once. The weights are frozen: gradients flow
+to a bf16 ``x`` (and to ``probs``). With gradients the activation is a pass of its own over the
+product, rounded to bf16, as in ``GroupedMLP``; rows in 8 bits, in or out, have none.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ... import _lib as L
+from ...dispatch import MxRows, OpImpl, OpImplKind, register_op
+from ...dispatch.mx import GROUP
+from ...runtime import TurboDevice
+from . import PRIORITY
+from ._functions import GatedActivation, SwiGLU, device_counts, require_cuda
+from .available import hip_available
+from .linear import ACTIVATIONS, FLOATS, _autograd_sees, _rows
+
+
+
+def _aligned(t, size):
+    """``t``, contiguous at a multiple of ``size`` bytes (copied where a view is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % size == 0 else t.clone()
+
+
+def _bytes(op, name, t, kind):
+    if t.dtype not in (torch.uint8, kind):
+        raise ValueError(f"{op}: {name} must be uint8 or {kind}, got {t.dtype}")
+    return t if t.dtype is torch.uint8 else t.view(torch.uint8)
+
+
+def check_weights(op, codes, scales, dims):
+    """Codes ``[..., N, K / 2]`` and scales as uint8, contiguous; ``ValueError`` otherwise."""
+    codes = _bytes(op, "codes", codes, torch.float4_e2m1fn_x2)
+    scales = _bytes(op, "scales", scales, torch.float8_e8m0fnu)
+    if codes.dim() != dims:
+        raise ValueError(f"{op} expects codes of {dims} dimensions ([..., out, in / 2]), got "
+                         f"{list(codes.shape)}")
+    k = 2 * codes.shape[-1]
+    want = (*codes.shape[:-1], k // GROUP)
+    if k % GROUP or tuple(scales.shape) != want:
+        raise ValueError(f"{op}: codes {list(codes.shape)} need scales {list(want)} and whole groups "
+                         f"of {GROUP} elements, got {list(scales.shape)}")
+    return _aligned(codes, 16), scales.contiguous()
+
+
+def check_rows(op, x, k):
+    """``(values [T, K], scales or None, leading shape)`` of bf16 rows or ``MxRows``."""
+    if isinstance(x, MxRows):
+        codes, scales = x.codes, _bytes(op, "the rows' scales", x.scales, torch.float8_e8m0fnu)
+        if codes.dtype is not torch.float8_e4m3fn or codes.dim() == 0 or codes.shape[-1] % GROUP \
+                or tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] // GROUP):
+            raise ValueError(f"{op}: rows in 8 bits are float8_e4m3fn [..., K] with uint8 scales "
+                             f"[..., K / {GROUP}], got {codes.dtype} {list(codes.shape)} and "
+                             f"{list(scales.shape)}")
+        values = _rows(codes, codes.shape[-1])
+        scales = _rows(scales, scales.shape[-1])
+    else:
+        if x.dtype is not torch.bfloat16 or x.dim() == 0:
+            raise ValueError(f"{op} takes bf16 rows [..., in] or MxRows, got {x.dtype}")
+        codes, values, scales = x, _rows(x, x.shape[-1]), None
+    if k is not None and values.shape[1] != k:
+        raise ValueError(f"{op}: x has {values.shape[1]} features, weight expects {k}")
+    return _aligned(values, 16), scales, codes.shape[:-1]
+
+
+def product(values, xs, codes, scales, counts, *, gated=False, act=0, probs=None, row_map=None,
+            mx_out=False):
+    """``tt_mx_product`` of checked operands: bf16 [M, N], or its codes and scales."""
+    m = values.shape[0] if row_map is None else row_map.shape[0]
+    k, dev = values.shape[1], values.device
+    experts = 1 if counts is None else codes.shape[0]
+    n = codes.shape[-2] // (2 if gated else 1)
+    y = torch.empty((m, n), dtype=torch.float8_e4m3fn if mx_out else torch.bfloat16, device=dev)
+    ys = torch.empty((m, n // GROUP), dtype=torch.uint8, device=dev) if mx_out else None
+    L.call("tt_mx_product", L.ptr(values), L.ptr(xs), L.ptr(row_map), values.shape[0],
+           L.ptr(codes), L.ptr(scales), m, k, n, experts, L.ptr(counts), int(gated), act,
+           L.ptr(probs), 0 if probs is None else L.dtype_code(probs.dtype), L.ptr(y), L.ptr(ys),
+           L.stream(dev))
+    return (y, ys) if mx_out else y
+
+
+class MxProduct(torch.autograd.Function):
+    """``(x bf16 [M, K], codes, scales, counts or None) -> x W^T``; gradient to x."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, counts):
+        ctx.save_for_backward(codes, scales, counts)
+        ctx.x_shape = x.shape
+        return product(x, None, codes, scales, counts)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, scales, counts = ctx.saved_tensors
+        dy = dy.to(torch.bfloat16).contiguous()
+        dx = torch.empty(ctx.x_shape, dtype=torch.bfloat16, device=dy.device)
+        L.call("tt_mx_dgrad", L.ptr(dy), L.ptr(codes), L.ptr(scales), *dx.shape, dy.shape[1],
+               1 if counts is None else codes.shape[0], L.ptr(counts), L.ptr(dx),
+               L.stream(dy.device))
+        return dx, None, None, None
+
+
+def _no_gradient(op, what):
+    return RuntimeError(f"{op}: {what} have no gradient: call it under torch.no_grad()")
+
+
+@register_op(op_name="linear_mxfp4", impl_name="hip_linear_mxfp4", kind=OpImplKind.CUSTOM,
+             priority=PRIORITY, devices=(TurboDevice.CUDA,))
+class HipLinearMxfp4(OpImpl):
+    def available(self) -> bool:
+        return hip_available()
+
+    def __call__(self, x, codes, scales, *, activation_func=None, gated=False, mx_out=False):
+        op = "linear_mxfp4"
+        if activation_func not in ACTIVATIONS:
+            raise ValueError(f"{op} only supports no activation, F.silu and F.gelu")
+        codes, scales = check_weights(op, codes, scales, 2)
+        if gated and codes.shape[0] % 2:
+            raise ValueError(f"{op}: a gated weight needs an even number of rows")
+        n = codes.shape[0] // 2 if gated else codes.shape[0]
+        if mx_out and n % GROUP:
+            raise ValueError(f"{op}: outputs in 8 bits are whole groups of {GROUP}, got {n}")
+        values, xs, lead = check_rows(op, x, 2 * codes.shape[1])
+        require_cuda(values, xs, codes, scales)
+        if _autograd_sees(values):
+            if mx_out:
+                raise _no_gradient(op, "outputs in 8 bits")
+            y = MxProduct.apply(values, codes, scales, None)
+            if gated:
+                y = (GatedActivation.apply(y, None, ACTIVATIONS[activation_func] - 1, 0.0, False)
+                     if activation_func is not None else y[:, :n] * y[:, n:])
+            elif activation_func is not None:
+                y = activation_func(y)
+            return y.view(*lead, n)
+        y = product(values, xs, codes, scales, None, gated=bool(gated),
+                    act=ACTIVATIONS[activation_func], mx_out=mx_out)
+        if mx_out:
+            return MxRows(y[0].view(*lead, n), y[1].view(*lead, n // GROUP))
+        return y.view(*lead, n)
+
+
+@register_op(op_name="grouped_matmul_mxfp4", impl_name="hip_grouped_matmul_mxfp4",
+             kind=OpImplKind.CUSTOM, priority=PRIORITY, devices=(TurboDevice.CUDA,))
+class HipGroupedMatmulMxfp4(OpImpl):
+    def available(self) -> bool:
+        return hip_available()
+
+    def __call__(self, x, codes, scales, tokens_per_expert, *, probs=None, gated=False,
+                 row_map=None, mx_out=False):
+        op = "grouped_matmul_mxfp4"
+        codes, scales = check_weights(op, codes, scales, 3)
+        experts, width = codes.shape[:2]
+        if experts == 0:
+            raise ValueError(f"{op} needs at least one expert")
+        if gated and width % 2:
+            raise ValueError(f"{op}: a gated weight needs an even number of rows")
+        n = width // 2 if gated else width
+        if mx_out and n % GROUP:
+            raise ValueError(f"{op}: outputs in 8 bits are whole groups of {GROUP}, got {n}")
+        values, xs, lead = check_rows(op, x, 2 * codes.shape[2])
+        if len(lead) != 1:
+            raise ValueError(f"{op} expects packed rows [M, in], got {[*lead, values.shape[1]]}")
+        m = values.shape[0]
+        if row_map is not None:
+            if row_map.dtype is not torch.int32 or row_map.dim() != 1:
+                raise ValueError(f"{op}: row_map must be int32 [M], got {row_map.dtype} "
+                                 f"{list(row_map.shape)}")
+            m = row_map.shape[0]
+            row_map = row_map.contiguous()
+        if probs is not None:
+            if probs.dtype not in FLOATS or tuple(probs.shape) not in ((m,), (m, 1)):
+                raise ValueError(f"{op}: probs must be a float tensor of shape [{m}], got "
+                                 f"{probs.dtype} {list(probs.shape)}")
+            probs = probs.reshape(-1).contiguous()
+        dev = require_cuda(values, xs, codes, scales, row_map, probs)
+        counts = device_counts(tokens_per_expert, experts, dev, m=m)
+        if _autograd_sees(values, probs):
+            if mx_out:
+                raise _no_gradient(op, "outputs in 8 bits")
+            if xs is not None:
+                raise _no_gradient(op, "rows in 8 bits")
+            if row_map is not None:
+                raise _no_gradient(op, "rows taken through row_map")
+            y = MxProduct.apply(values, codes, scales, counts)
+            if gated:
+                return SwiGLU.apply(y, probs)
+            return y if probs is None else (y * probs.unsqueeze(-1)).to(y.dtype)
+        y = product(values, xs, codes, scales, counts, gated=bool(gated), act=int(bool(gated)),
+                    probs=probs, row_map=row_map, mx_out=mx_out)
+        return MxRows(*y) if mx_out else y
+
+
+def _quantized(op, x, bits):
+    if x.dtype not in FLOATS or x.dim() == 0 or x.shape[-1] % GROUP:
+        raise ValueError(f"{op} takes f32, bf16 or f16 rows of whole groups of {GROUP} elements, got "
+                         f"{x.dtype} {list(x.shape)}")
+    require_cuda(x)
+    x2 = _rows(x.detach(), x.shape[-1])
+    t, k = x2.shape
+    lead = x.shape[:-1]
+    codes = torch.empty((*lead, k * bits // 8), device=x.device,
+                        dtype=torch.uint8 if bits == 4 else torch.float8_e4m3fn)
+    scales = torch.empty((*lead, k // GROUP), dtype=torch.uint8, device=x.device)
+    L.call(f"tt_mxfp{bits}_quantize", L.ptr(x2), L.dtype_code(x.dtype), t, k, L.ptr(codes),
+           L.ptr(scales), L.stream(x.device))
+    return codes, scales
+
+
+def _dequantized(op, codes, scales, k, dtype, bits):
+    if dtype not in FLOATS:
+        raise ValueError(f"{op} gives f32, bf16 or f16, not {dtype}")
+    require_cuda(codes, scales)
+    codes, scales = _aligned(codes, 8), scales.contiguous()
+    out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=codes.device)
+    rows = out.numel() // k if k else 0
+    L.call(f"tt_mxfp{bits}_dequantize", L.ptr(codes), L.ptr(scales), rows, k, L.ptr(out),
+           L.dtype_code(dtype), L.stream(codes.device))
+    return out
+
+
+@register_op(op_name="quantize_mxfp4", impl_name="hip_quantize_mxfp4", kind=OpImplKind.CUSTOM,
+             priority=PRIORITY, devices=(TurboDevice.CUDA,))
+class HipQuantizeMxfp4(OpImpl):
+    def available(self) -> bool:
+        return hip_available()
+
+    def __call__(self, weight):
+        return _quantized("quantize_mxfp4", weight, 4)
+
+
+@register_op(op_name="dequantize_mxfp4", impl_name="hip_dequantize_mxfp4", kind=OpImplKind.CUSTOM,
+             priority=PRIORITY, devices=(TurboDevice.CUDA,))
+class HipDequantizeMxfp4(OpImpl):
+    def available(self) -> bool:
+        return hip_available()
+
+    def __call__(self, codes, scales, dtype=torch.bfloat16):
+        codes, scales = check_weights("dequantize_mxfp4", codes, scales, codes.dim() or 1)
+        return _dequantized("dequantize_mxfp4", codes, scales, 2 * codes.shape[-1], dtype, 4)
+
+
+@register_op(op_name="quantize_mxfp8", impl_name="hip_quantize_mxfp8", kind=OpImplKind.CUSTOM,
+             priority=PRIORITY, devices=(TurboDevice.CUDA,))
+class HipQuantizeMxfp8(OpImpl):
+    def available(self) -> bool:
+        return hip_available()
+
+    def __call__(self, x):
+        return MxRows(*_quantized("quantize_mxfp8", x, 8))
+
+
+@register_op(op_name="dequantize_mxfp8", impl_name="hip_dequantize_mxfp8", kind=OpImplKind.CUSTOM,
+             priority=PRIORITY, devices=(TurboDevice.CUDA,))
+class HipDequantizeMxfp8(OpImpl):
+    def available(self) -> bool:
+        return hip_available()
+
+    def __call__(self, rows, dtype=torch.bfloat16):
+        if not isinstance(rows, MxRows):
+            raise ValueError(f"dequantize_mxfp8 takes MxRows, got {type(rows).__name__}")
+        values, scales, lead = check_rows("dequantize_mxfp8", rows, None)
+        out = _dequantized("dequantize_mxfp8", values, scales, values.shape[1], dtype, 8)
+        return out.view(*lead, values.shape[1])
