@@ -97,3 +97,6 @@ __device__ __forceinline__ void mx_store_rows(const MxArgs& p, int64_t r, int64_
 
 // Few rows per expert (mx_rows.hip); operands already checked.
 int tt_mx_rows(const MxArgs& p, bool gated, hipStream_t s);
+// Many rows per expert (mx_tile.hip), and whether the sizes and addresses fit its offsets.
+int tt_mx_tile(const MxArgs& p, bool gated, hipStream_t s);
+bool tt_mx_tile_takes(const MxArgs& p, bool gated);

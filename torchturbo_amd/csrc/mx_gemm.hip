@@ -3,6 +3,9 @@
 
 namespace {
 
+// Rows per expert on average up to which the weights' stream bounds a product.
+constexpr int64_t ROWS_LIMIT = 64;
+
 int check(const MxArgs& p) {
   TT_REQUIRE(p.M >= 0 && p.K >= 0 && p.N >= 0 && p.E > 0, "mx product: bad sizes");
   TT_REQUIRE(p.K % MX_GROUP == 0, "mx product: the reduction is whole groups of 32 elements");
@@ -38,5 +41,8 @@ extern "C" int tt_mx_product(const void* x, const uint8_t* x_scales, const int32
                     tokens_per_expert, act, probs, probs_dtype, y, y_scales};
   const int rc = check(p);
   if (rc != TT_OK || M == 0 || N == 0) return rc;
-  return tt_mx_rows(p, gated != 0, reinterpret_cast<hipStream_t>(stream));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int64_t per = M / num_experts;  // rows per expert on average
+  if (per > ROWS_LIMIT && tt_mx_tile_takes(p, gated != 0)) return tt_mx_tile(p, gated != 0, s);
+  return tt_mx_rows(p, gated != 0, s);
 }
