@@ -514,6 +514,8 @@ int tt_lora_wgrad_dropout(const void* x, const float* dh, int dtype, int64_t m, 
  *   the product, gated: act of the first half times the second half; times probs[r] (f32 /
  *   bf16 / f16, or NULL). y: bf16, or with y_scales E4M3 codes and their E8M0 bytes (N a
  *   multiple of 32). Products are exact, sums run in fp32 and are rounded once.
+ *   tt_mx_product_workspace: bytes of scratch of a call of these sizes (0: none), 16-byte
+ *   aligned; with less it does not split its reduction.
  * tt_mx_dgrad: dx [M, K] = dy [M, N] W[e], bf16, of weights that stay as they are.
  * x, codes and dx are 16-byte aligned; K is a multiple of 32; any M, N.
  *
@@ -536,7 +538,8 @@ int tt_mx_product(const void* x, const uint8_t* x_scales, const int32_t* row_map
                   const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K, int64_t N,
                   int32_t num_experts, const int64_t* tokens_per_expert, int32_t gated,
                   int32_t act, const void* probs, int probs_dtype, void* y, uint8_t* y_scales,
-                  void* stream);
+                  void* workspace, size_t workspace_bytes, void* stream);
+size_t tt_mx_product_workspace(int64_t M, int64_t K, int64_t N, int32_t grouped, int32_t gated);
 int tt_mx_dgrad(const void* dy, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t K,
                 int64_t N, int32_t num_experts, const int64_t* tokens_per_expert, void* dx,
                 void* stream);

@@ -160,6 +160,61 @@ def test_linear(hip_ops, m, k, n, mx):
     _within(got, want, _bound(x, codes, scales, want))
 
 
+# The tiles of 64 x 128 with a split reduction, of 128 x 128 and of 128 x 256, the reduction a multiple
+# of 128 or not.
+TILES = [(40, 6400, 200), (200, 4096, 64), (65, 6272, 30), (600, 256, 4500), (600, 160, 4500),
+         (1700, 128, 4200), (1700, 224, 4200)]
+
+
+@pytest.mark.parametrize("m, k, n", TILES)
+@pytest.mark.parametrize("mx", [False, True])
+def test_every_tile_on_integers(hip_ops, m, k, n, mx):
+    x, codes, scales = _integers(m, k, n, mx, seed=m + n)
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV))
+    want = o_mx.linear(x, codes, scales).to(BF16)
+    assert torch.equal(got.cpu(), want), (got.cpu() != want).nonzero()[:8]
+
+
+@pytest.mark.parametrize("m, k, n, gated", [(40, 6400, 64, True), (300, 128, 2400, True),
+                                            (1700, 128, 2112, True), (40, 6400, 160, False),
+                                            (1700, 224, 4224, False)])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("mx_out", [False, True])
+def test_every_tile_with_its_epilogue(hip_ops, m, k, n, gated, mx, mx_out):
+    x, (codes, scales) = _rows(m, k, mx), _weights((2 * n if gated else n, k), seed=5)
+    act = F.silu if gated else None
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), activation_func=act,
+                               gated=gated, mx_out=mx_out)
+    a = o_mx.linear(x, codes, scales)
+    y = o_mx.epilogue(a, act, gated)
+    plain = _bound(x, codes, scales, torch.zeros_like(a))
+    if mx_out:
+        _within_8_bits(got, y, _epilogue_bound(a, plain, act or (lambda v: v), gated, 0 * y))
+    else:
+        _within(got, y, _epilogue_bound(a, plain, act or (lambda v: v), gated, y))
+
+
+@pytest.mark.parametrize("counts", [[700, 0, 900, 100, 1400], [60] * 20, [40, 300, 0, 20]])
+@pytest.mark.parametrize("mx", [False, True])
+def test_every_tile_of_experts(hip_ops, counts, mx):
+    m, e, k, n = sum(counts), len(counts), 128, 2600
+    x, codes, scales = _integers(m, k, n * e, mx)
+    codes, scales = codes.view(e, n, -1), scales.view(e, n, -1)
+    got = hip_ops.grouped_matmul_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), counts)
+    assert torch.equal(got.cpu(), o_mx.grouped(x, codes, scales, counts).to(BF16))
+    if not mx:
+        dy = torch.randint(-4, 5, (m, n), generator=torch.Generator().manual_seed(3)).to(BF16)
+        for dk in (128, 8192):  # tiles of 128 x 128, and of 256 x 256 for experts of many rows
+            xi, ci, si = _integers(m, dk, n * e, False, seed=2)
+            ci, si = ci.view(e, n, -1).to(DEV), si.view(e, n, -1).to(DEV)
+            xd = xi.to(DEV).requires_grad_()
+            dx, = torch.autograd.grad(hip_ops.grouped_matmul_mxfp4(xd, ci, si, counts), xd, dy.to(DEV))
+            w = hip_ops.dequantize_mxfp4(ci, si, torch.float32)
+            parts = [p.float().to(DEV) @ w[i] for i, p in enumerate(dy.split(counts))]
+            # Whole numbers below 2^24: exact in fp32 in any order.
+            assert torch.equal(dx, torch.cat(parts).to(BF16))
+
+
 def _epilogue_bound(a, bound, act, gated, y):
     """What an error ``bound`` of the product ``a`` makes of the epilogue's result, |act'| <= 1.13,
     |act(v)| <= |v|, the exponential's 2^-20, and the output's rounding."""

@@ -93,7 +93,9 @@ _PROTOS: dict[str, list] = {
     "tt_mxfp4_dequantize": [P, P, I64, I64, P, c_int, P],
     "tt_mxfp8_quantize": [P, c_int, I64, I64, P, P, P],
     "tt_mxfp8_dequantize": [P, P, I64, I64, P, c_int, P],
-    "tt_mx_product": [P, P, P, I64, P, P, I64, I64, I64, I32, P, I32, I32, P, c_int, P, P, P],
+    "tt_mx_product": [P, P, P, I64, P, P, I64, I64, I64, I32, P, I32, I32, P, c_int, P, P, P,
+                      c_size_t, P],
+    "tt_mx_product_workspace": [I64, I64, I64, I32, I32],
     "tt_mx_dgrad": [P, P, P, I64, I64, I64, I32, P, P, P],
     "tt_rms_norm_fwd": [P, P, P, c_int, c_int, I64, I64, c_float, P, P, P, P, P, P],
     "tt_rms_norm_bwd_workspace": [I64, I64],
@@ -104,7 +106,7 @@ _RESTYPES = {"tt_last_error": ctypes.c_char_p, "tt_route_index_workspace": c_siz
              "tt_moe_experts_workspace": c_size_t, "tt_router_gate_bwd_workspace": c_size_t,
              "tt_linear_workspace": c_size_t, "tt_linear_act_bwd_workspace": c_size_t,
              "tt_linear_residual_bwd_workspace": c_size_t,
-             "tt_rms_norm_bwd_workspace": c_size_t}
+             "tt_rms_norm_bwd_workspace": c_size_t, "tt_mx_product_workspace": c_size_t}
 ABI_VERSION = 1
 
 _LIB: ctypes.CDLL | None = None

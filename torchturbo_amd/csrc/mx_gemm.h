@@ -20,6 +20,12 @@ struct MxArgs {
   int pdt;
   void* y;                // bf16 [M, N], or E4M3 codes
   uint8_t* ys;            // E8M0 [M, N / 32], NULL: bf16
+  float* part;            // sums of the parts of a split reduction
+};
+
+// Tile of a product of many rows, and the parts that its reduction is split into (1: none).
+struct MxPlan {
+  int bm, bn, parts;
 };
 
 namespace {
@@ -98,5 +104,5 @@ __device__ __forceinline__ void mx_store_rows(const MxArgs& p, int64_t r, int64_
 // Few rows per expert (mx_rows.hip); operands already checked.
 int tt_mx_rows(const MxArgs& p, bool gated, hipStream_t s);
 // Many rows per expert (mx_tile.hip), and whether the sizes and addresses fit its offsets.
-int tt_mx_tile(const MxArgs& p, bool gated, hipStream_t s);
+int tt_mx_tile(const MxArgs& p, bool gated, MxPlan plan, hipStream_t s);
 bool tt_mx_tile_takes(const MxArgs& p, bool gated);

@@ -3,8 +3,43 @@
 
 namespace {
 
-// Rows per expert on average up to which the weights' stream bounds a product.
-constexpr int64_t ROWS_LIMIT = 64;
+int64_t tiles(int64_t rows, int64_t cols, int bm, int bn) {
+  return (rows + bm - 1) / bm * ((cols + bn - 1) / bn);
+}
+
+// Whether a product takes the kernel of few rows, which reads x once per weight tile from memory.
+// us, rows / tiles (the plan's), bf16 rows: dense 17 x 7168 -> 2 x 2048 17.6 / 21.1, 24 x 2048 ->
+// 7168 8.6 / 15.0, 64 x 7168 -> 2 x 2048 21.9 / 21.3, 64 x 4096 -> 2 x 14336 79 / 31; 128 experts
+// of 2048 -> 2 x 768 with 512 rows 59 / 57, with 1024 74 / 64, of 768 -> 2048 with 512 28 / 40; 64 of
+// 7168 -> 2 x 2048 with 256 rows 279 / 263. E4M3 rows: 15.2 / 15.4, 7.4 / 9.9, 18.7 / 15.7, 66 / 24;
+// 54 / 46, 68 / 53, 26 / 32; 269 / 201.
+bool few_rows(int64_t M, int64_t K, int64_t W, int E, bool grouped) {
+  if (grouped) return M <= (int64_t)E * (K <= 1024 ? 8 : 3);
+  return M <= 16 || (M <= 32 && W < 512 * 16);
+}
+
+// Tile and parts. The largest tile reads least, but wants a block for nearly each of the 256 CUs (and
+// experts that fill it); then 128 x 128; the smallest, for dense products split until the blocks fill
+// the CUs, while a part keeps 1536 elements (the second kernel and its reads cost some 5 us). us, bf16
+// rows, 128 x 256 / 128 x 128 / 64 x 128 / 64 x 128 in 2 / in 4 parts: 128 x 7168 -> 2 x 2048 98 / 67 /
+// 46 / 30 / 22, 256 rows 99 / 68 / 46 / 31 / 30, 1531 x 5632 -> 2048 92 / 57 / 59 / 61 / 67, 1024 x
+// 7168 -> 2 x 2048 100 / 70 / 78 / 93, 2048 rows 112 / 119 / 163, 4096 204 / 264 / 325. 128 experts of
+// 2048 -> 2 x 768 with 32 rows each 95 / 96 / 77, with 64 115 / 117 / 104, with 128 148 / 164 / 161; 64
+// of 7168 -> 2 x 2048 with 64 479 / 494 / 528, E4M3 rows 375 / 339 / 363, with 256 625 / 714 / 873.
+MxPlan plan(int64_t M, int64_t K, int64_t W, int E, bool grouped) {
+  const int64_t per = grouped ? M / E : M;
+  if (per > 96 && tiles(M, W, 128, 256) >= 224) return MxPlan{128, 256, 1};
+  if (per > 48 && tiles(M, W, 128, 128) >= 160) return MxPlan{128, 128, 1};
+  int parts = 1;
+  if (!grouped)
+    while (parts < 4 && tiles(M, W, 64, 128) * parts * 2 <= 256 && K / (parts * 2) >= 1536) parts *= 2;
+  return MxPlan{64, 128, parts};
+}
+
+size_t part_bytes(const MxPlan& pl, int64_t M, int64_t W) {
+  if (pl.parts == 1) return 0;
+  return (size_t)(tiles(M, W, pl.bm, pl.bn) * pl.parts) * pl.bm * pl.bn * sizeof(float);
+}
 
 int check(const MxArgs& p) {
   TT_REQUIRE(p.M >= 0 && p.K >= 0 && p.N >= 0 && p.E > 0, "mx product: bad sizes");
@@ -36,13 +71,31 @@ extern "C" int tt_mx_product(const void* x, const uint8_t* x_scales, const int32
                              int64_t M, int64_t K, int64_t N, int32_t num_experts,
                              const int64_t* tokens_per_expert, int32_t gated, int32_t act,
                              const void* probs, int probs_dtype, void* y, uint8_t* y_scales,
-                             void* stream) {
-  const MxArgs p = {x, x_scales, row_map, src_rows, codes, scales, M, K, N, num_experts,
-                    tokens_per_expert, act, probs, probs_dtype, y, y_scales};
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  MxArgs p = {x, x_scales, row_map, src_rows, codes, scales, M, K, N, num_experts,
+                    tokens_per_expert, act, probs, probs_dtype, y, y_scales, nullptr};
   const int rc = check(p);
   if (rc != TT_OK || M == 0 || N == 0) return rc;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t per = M / num_experts;  // rows per expert on average
-  if (per > ROWS_LIMIT && tt_mx_tile_takes(p, gated != 0)) return tt_mx_tile(p, gated != 0, s);
-  return tt_mx_rows(p, gated != 0, s);
+  const int64_t W = gated ? 2 * N : N;
+  const bool grouped = tokens_per_expert != nullptr;
+  if (few_rows(M, K, W, num_experts, grouped) || !tt_mx_tile_takes(p, gated != 0))
+    return tt_mx_rows(p, gated != 0, s);
+  MxPlan pl = plan(M, K, W, num_experts, grouped);
+  if (pl.parts > 1) {
+    if (workspace != nullptr && workspace_bytes >= part_bytes(pl, M, W) &&
+        (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)
+      p.part = static_cast<float*>(workspace);
+    else
+      pl.parts = 1;
+  }
+  return tt_mx_tile(p, gated != 0, pl, s);
+}
+
+extern "C" size_t tt_mx_product_workspace(int64_t M, int64_t K, int64_t N,
+                                          int32_t grouped, int32_t gated) {
+  if (M <= 0 || K <= 0 || N <= 0 || grouped) return 0;
+  const int64_t W = gated ? 2 * N : N;
+  if (few_rows(M, K, W, 1, false)) return 0;
+  return part_bytes(plan(M, K, W, 1, false), M, W);
 }

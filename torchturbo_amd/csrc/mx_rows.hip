@@ -11,9 +11,7 @@
 
 namespace {
 
-constexpr int U = 2;
-
-template <bool MX, bool GATED, bool OUT8, int MB, int NB, int W>
+template <bool MX, bool GATED, bool OUT8, int MB, int NB, int W, int U>
 __global__ __launch_bounds__(64 * W) void mx_rows_kernel(MxArgs p, int tiles_j) {
   constexpr int NT = 64 * W;
   constexpr int CB = (GATED ? 8 : 16) * NB;  // output columns of a block
@@ -181,7 +179,7 @@ __global__ __launch_bounds__(64 * W) void mx_rows_kernel(MxArgs p, int tiles_j) 
   }
 }
 
-template <bool MX, bool GATED, bool OUT8, int MB, int NB, int W>
+template <bool MX, bool GATED, bool OUT8, int MB, int NB, int W, int U>
 int launch(const MxArgs& p, hipStream_t s) {
   constexpr int CB = (GATED ? 8 : 16) * NB;
   const int64_t tiles_j = (p.N + CB - 1) / CB;
@@ -191,18 +189,25 @@ int launch(const MxArgs& p, hipStream_t s) {
   TT_REQUIRE(tiles_i < (1ll << 31) && tiles_j < (1ll << 31) && tiles_i * tiles_j < (1ll << 31) &&
                  tt_grid_ok(tiles_i * tiles_j, 64 * W),
              "mx product: grid too large");
-  hipLaunchKernelGGL((mx_rows_kernel<MX, GATED, OUT8, MB, NB, W>), dim3((unsigned)(tiles_i * tiles_j)),
+  hipLaunchKernelGGL((mx_rows_kernel<MX, GATED, OUT8, MB, NB, W, U>), dim3((unsigned)(tiles_i * tiles_j)),
                      dim3(64 * W), 0, s, p, (int)tiles_j);
   return tt_check_launch("mx_rows");
 }
 
+// Weight tiles and waves of a block by how many 16-row tiles the launch has (those of the experts
+// that can have rows): few tiles are spread over all CUs with the reduction split eight ways, many
+// share their reads of x and their block's start. us, bf16 rows, <1, 8> / <4, 4> / <4, 2>:
+// 1 x 7168 -> 2 x 2048 (256 tiles) 8.4 / 18.0 / 20.9, 4 x 4096 -> 2 x 14336 (1792) 34.6 / 24.5 /
+// 25.7, 128 rows of 128 experts 2048 -> 2 x 768 (12288) 129 / 34.7 / 33.0, 768 -> 2048 91 / 22.8 / 18.5.
 template <bool MX, bool GATED, bool OUT8>
 int rows(const MxArgs& p, hipStream_t s) {
-  const int64_t per = p.counts != nullptr ? (p.M + p.E - 1) / p.E : p.M;
   constexpr int N8 = GATED ? 4 : 2;  // weight tiles of 32 outputs, a group's
-  if (per <= 16) return launch<MX, GATED, OUT8, 1, OUT8 ? N8 : 1, 8>(p, s);
-  if (per <= 32) return launch<MX, GATED, OUT8, 2, OUT8 ? N8 : 2, 4>(p, s);
-  return launch<MX, GATED, OUT8, 4, OUT8 ? N8 : 2, 4>(p, s);
+  const int64_t per = p.counts != nullptr ? (p.M + p.E - 1) / p.E : p.M;
+  const int64_t tiles = ((GATED ? 2 : 1) * p.N + 15) / 16 * (p.counts == nullptr || p.E < p.M ? p.E : p.M);
+  if (per > 16) return launch<MX, GATED, OUT8, 2, OUT8 ? N8 : 2, 4, 2>(p, s);
+  if (tiles < 1024) return launch<MX, GATED, OUT8, 1, OUT8 ? N8 : 1, 8, 1>(p, s);
+  if (tiles < 4096) return launch<MX, GATED, OUT8, 1, OUT8 ? N8 : 4, 4, 1>(p, s);
+  return launch<MX, GATED, OUT8, 1, OUT8 ? N8 : 4, 2, 1>(p, s);
 }
 
 template <bool MX, bool GATED>

@@ -2,12 +2,13 @@
 //
 // A block computes 128 rows by 256 weight rows (gated: 128 columns, a wave's blocks of 32 weight
 // rows alternating between gates and their ups), four waves of 64 x 128 each on 32-wide matrix
-// instructions. k-tiles go from memory straight to LDS, swizzled so that fragment reads are
+// instructions; 128 x 128 or 64 x 128 where the launch would have too few blocks, and dense products
+// of fewer still split their reduction, the parts' sums joined in order by a second kernel. k-tiles go from memory straight to LDS, swizzled so that fragment reads are
 // free of bank conflicts; two blocks share a CU, so that one's matrix instructions cover the
 // other's waits, prologue and epilogue. Rows of 4-bit weights are a quarter of bf16 rows' bytes
 // (half of E4M3 rows'), which is why the tile is twice as wide in them.
 //
-// E4M3 rows: k-tiles of 128, two stages; codes are multiplied as they are, with the groups' bytes as
+// E4M3 rows: k-tiles of 128, two stages (four of the smallest tile); codes are multiplied as they are, with the groups' bytes as
 // the instruction's scales (a row's four bytes of a k-tile are one word in LDS).
 // bf16 rows: k-tiles of 64, three stages; a lane's 16 bytes of codes are one group of a weight row,
 // which it turns into four bf16 fragments with the group's scale. The order of the reduction
@@ -19,19 +20,23 @@
 
 namespace {
 
-constexpr int T_NT = 256, T_BM = 128, T_BN = 256;
+constexpr int T_NT = 256;
 
-template <bool MX>
+template <bool MX, int BM_, int BN_>
 struct Tile {
+  static constexpr int BM = BM_, BN = BN_;           // rows of x and of W
   static constexpr int BK = MX ? 128 : 64;
-  static constexpr int STAGES = MX ? 2 : 3;
-  static constexpr int XB = T_BM * 128;              // rows of x: 128 bytes per k-tile
+  static constexpr int STAGES = MX ? (BM == 64 ? 4 : 2) : 3;
+  static constexpr int XB = BM * 128;                // rows of x: 128 bytes per k-tile
   static constexpr int WR = MX ? 64 : 32;            // bytes of a weight row per k-tile
-  static constexpr int WB = T_BN * WR;
+  static constexpr int WB = BN * WR;
   static constexpr int STAGE = XB + WB;
-  // Scales of 128 elements, one word per row: weight rows, then x's; two buffers.
-  static constexpr int SB = (T_BN + (MX ? T_BM : 0)) * 4;
-  static constexpr int LDS = STAGES * STAGE + 2 * SB;
+  // Scales of 128 elements, one word per row: weight rows, then x's. A buffer per stage, or two where
+  // a word lasts two k-tiles.
+  static constexpr int SB = (BN + (MX ? BM : 0)) * 4;
+  static constexpr int SBS = MX ? STAGES : 2;
+  static constexpr int LDS = STAGES * STAGE + SBS * SB;
+  static constexpr int MI = BM / 64, NJ = BN / 64;   // 32-wide blocks of a wave
 };
 
 // Bytes 0..3 of a scale word: groups past the reduction's end are 127 (their codes are zeros).
@@ -42,206 +47,20 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* p, int left) {
   return v;
 }
 
-// KA: K is a multiple of 128 and scales are 4-byte aligned.
-template <bool MX, bool GATED, bool OUT8, bool KA>
-__global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j) {
-  typedef Tile<MX> L;
-  constexpr int CB = GATED ? T_BN / 2 : T_BN;  // output columns
-  constexpr int ES = MX ? 1 : 2;               // bytes of an element of x
-  __shared__ __align__(16) char lds_raw[L::LDS];
-  RowTile t;
-  if (p.counts != nullptr) {
-    if (!row_tile<T_BM, T_NT>(p.counts, p.E, tiles_j, lds_raw, t)) return;
-    // Counts that sum to more than M end at its last row.
-    if (t.seg0 + t.nrows > p.M) t.nrows = p.M - t.seg0;
-    if ((int64_t)t.mt * T_BM >= t.nrows) return;
-  } else {
-    t.e = 0;
-    const int tiles_i = (int)((p.M + T_BM - 1) / T_BM);
-    const int slot = xcd_remap(blockIdx.x, tiles_i * tiles_j);
-    t.mt = slot % tiles_i;
-    t.nt = slot / tiles_i;
-    t.seg0 = 0;
-    t.nrows = p.M;
-  }
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t K = p.K, i0 = (int64_t)t.mt * T_BM, j0 = (int64_t)t.nt * CB;
-  const int64_t rows = t.nrows - i0;  // valid rows of the tile, at least one
-  const int groups = (int)(K / MX_GROUP);
-  const int nkt = (int)((K + L::BK - 1) / L::BK);
-  lds_char* const lds = (lds_char*)lds_raw;
-  lds_char* const lds_s = lds + L::STAGES * L::STAGE;
-
-  // x: wave w loads rows 32 w + 8 q + lane / 8, chunk slot lane % 8 holding chunk
-  // slot ^ ((row >> 1) & 7). Rows past the expert's read as zeros.
-  const bool gather = p.arow != nullptr;
-  const int64_t first = t.seg0 + i0;
-  const char* const xbase = static_cast<const char*>(p.x) + (gather ? 0 : first * K * ES);
-  const i32x4 rx = make_rsrc(xbase, (gather ? p.src_rows : (rows < T_BM ? rows : T_BM)) * K * ES);
-  uint32_t xoff[4];
-  int xk[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int r = 32 * wave + 8 * q + (lane >> 3);
-    const int c = (lane & 7) ^ ((r >> 1) & 7);
-    xk[q] = c * (16 / ES);
-    xoff[q] = DM_OOB;
-    if (r < rows) xoff[q] = (uint32_t)((gather ? mx_source_row(p, first + r) : r) * K * ES + 16 * c);
-  }
-  // W: rows of WR bytes. Tile row r is weight row `weight_row(r)`; those past the last read it again
-  // (their columns are not stored). A wave's instruction covers 1 KiB.
-  const int64_t width = GATED ? 2 * p.N : p.N;
-  const uint8_t* const wbase = p.w + (int64_t)t.e * width * (K / 2);
-  const uint8_t* const sbase = p.ws + (int64_t)t.e * width * groups;
-  const i32x4 rw = make_rsrc(wbase, width * (K / 2));
-  const i32x4 rs = make_rsrc(sbase, width * groups);
-  auto weight_row = [&](int r) -> int64_t {
-    int64_t n = GATED ? j0 + 32 * (r >> 6) + (r & 31) : j0 + r;
-    n = n < p.N ? n : p.N - 1;
-    return GATED && (r & 32) ? n + p.N : n;
-  };
-  constexpr int WQ = L::WB / 4096;  // instructions per wave
-  constexpr int CW = L::WR / 16;    // chunks of a row
-  uint32_t woff[WQ];
-  int wk[WQ];
-#pragma unroll
-  for (int q = 0; q < WQ; ++q) {
-    const int r = (64 * wave) + (64 / CW) * q + lane / CW;
-    const int c = (lane % CW) ^ (MX ? (r >> 2) & 3 : (r >> 3) & 1);
-    wk[q] = 32 * c;
-    woff[q] = (uint32_t)(weight_row(r) * (K / 2) + 16 * c);
-  }
-  // Scales: thread t takes weight row t, and of x row t % 128 (the first 128 threads).
-  const int64_t srow = weight_row(tid);
-  const uint32_t soff = (uint32_t)(srow * groups);
-  const uint8_t* const xsbase = MX ? p.xs + (gather ? 0 : first * groups) : nullptr;
-  const i32x4 rxs = make_rsrc(xsbase, MX ? (gather ? p.src_rows : (rows < T_BM ? rows : T_BM)) * groups : 0);
-  uint32_t xsoff = DM_OOB;
-  if (MX && tid < T_BM && tid < rows)
-    xsoff = (uint32_t)((gather ? mx_source_row(p, first + tid) : tid) * groups);
-
-  // The words of 128 elements from group g0 on into scale buffer b.
-  auto load_scales = [&](int g0, int b) {
-    const uint32_t at = lds_addr_of(lds_s) + (uint32_t)(b * L::SB);
-    if constexpr (KA) {
-      dma4(soff, advance_rsrc(rs, (uint32_t)g0), at + 256u * wave);
-      if (MX && wave < 2)
-        dma4(xsoff, advance_rsrc(rxs, (uint32_t)g0), at + T_BN * 4 + 256u * wave);
-    } else {
-      uint32_t* const to = reinterpret_cast<uint32_t*>(lds_raw + L::STAGES * L::STAGE + b * L::SB);
-      to[tid] = scale_word(sbase + soff + g0, groups - g0);
-      if constexpr (MX)
-        if (tid < T_BM) to[T_BN + tid] = xsoff == DM_OOB ? 0x7f7f7f7fu : scale_word(xsbase + xsoff + g0, groups - g0);
-    }
-  };
-  auto issue = [&](int kt, int stage) {
-    const uint32_t base = lds_addr_of(lds) + (uint32_t)(stage * L::STAGE);
-    const i32x4 rxk = advance_rsrc(rx, (uint32_t)(kt * L::BK * ES));
-    const i32x4 rwk = advance_rsrc(rw, (uint32_t)(kt * (L::BK / 2)));
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      dma16(KA || kt * L::BK + xk[q] < (int)K ? xoff[q] : DM_OOB, rxk,
-            base + (uint32_t)(4 * wave + q) * 1024u);
-#pragma unroll
-    for (int q = 0; q < WQ; ++q)
-      dma16(KA || kt * L::BK + wk[q] < (int)K ? woff[q] : DM_OOB, rwk,
-            base + L::XB + (uint32_t)(WQ * wave + q) * 1024u);
-    if (MX || (kt & 1) == 0) load_scales(kt * (L::BK / MX_GROUP), MX ? kt & 1 : (kt >> 1) & 1);
-  };
-
-  // Wave w multiplies rows 64 (w / 2) .. + 63 by weight rows 128 (w % 2) .. + 127.
-  const int m0 = 64 * (wave >> 1), n0 = 128 * (wave & 1);
-  const int r32 = lane & 31, g = lane >> 5;
-  f32x16 acc[2][4] = {};
-  auto multiply = [&](int kt, int stage) {
-    lds_char* const st = lds + stage * L::STAGE;
-    const char* const sw = lds_raw + L::STAGES * L::STAGE + (MX ? kt & 1 : (kt >> 1) & 1) * L::SB;
-    const int shift = MX ? 8 * g : 8 * (2 * (kt & 1) + g);
-    uint32_t ws[4], xs[2];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      ws[j] = *reinterpret_cast<const uint32_t*>(sw + 4 * (n0 + 32 * j + r32)) >> shift;
-    if constexpr (MX) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        xs[i] = *reinterpret_cast<const uint32_t*>(sw + 4 * (T_BN + m0 + 32 * i + r32)) >> shift;
-      auto step = [&](auto sc) {
-        constexpr int s = decltype(sc)::value;
-        uint4 w[4], x[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = m0 + 32 * i + r32;
-          const uint32_t at = (uint32_t)(r * 128), sz = (uint32_t)((r >> 1) & 7);
-          x[i][0] = read_k(st, at + (((4 * s + g) ^ sz) << 4));
-          x[i][1] = read_k(st, at + (((4 * s + 2 + g) ^ sz) << 4));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = n0 + 32 * j + r32;
-          w[j] = read_k(st, L::XB + (uint32_t)(r * 64 + (((2 * s + g) ^ ((r >> 2) & 3)) << 4)));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            acc[i][j] = mx_mma32<2 * s, 2 * s>(w[j], x[i][0], x[i][1], ws[j], xs[i], acc[i][j]);
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-    } else {
-      uint4 w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = n0 + 32 * j + r32;
-        w[j] = read_k(st, L::XB + (uint32_t)(r * 32 + ((g ^ ((r >> 3) & 1)) << 4)));
-        ws[j] &= 255u;
-      }
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        uint4 x[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = m0 + 32 * i + r32;
-          x[i] = read_k(st, (uint32_t)(r * 128 + (((4 * g + s) ^ ((r >> 1) & 7)) << 4)));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t q = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w;
-          const uint4 a = mx_bf16x8(q, ws[j]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) acc[i][j] = Mma<TT_BF16>::run(a, x[i], acc[i][j]);
-        }
-      }
-    }
-  };
-
-#pragma unroll
-  for (int s = 0; s < L::STAGES - 1; ++s)
-    if (s < nkt) issue(s, s);
-  int stage = 0;
-  for (int kt = 0; kt < nkt; ++kt) {
-    // k-tile kt has landed once at most the loads of later ones are outstanding: at least the x and
-    // W pieces of kt + 1 where three stages are used.
-    if (L::STAGES == 3 && KA && kt + 1 < nkt) TT_WAIT_VMCNT(4 + WQ);
-    else TT_WAIT_VMCNT(0);
-    TT_LDS_BARRIER();
-    const int next = stage == 0 ? L::STAGES - 1 : stage - 1;  // the stage of kt - 1
-    if (kt + L::STAGES - 1 < nkt) issue(kt + L::STAGES - 1, next);
-    multiply(kt, stage);
-    stage = stage == L::STAGES - 1 ? 0 : stage + 1;
-  }
-
-  // Epilogue. Register 4 q + e of lane l in block (i, j): row m0 + 32 i + l % 32, weight row
-  // n0 + 32 j + 8 q + 4 g + e. A wave's rows go through its own 16 KiB of LDS, in rows of RB bytes,
-  // chunk c of row r in slot c ^ (r % (RB / 16)).
-  TT_LDS_BARRIER();  // every wave is past its fragment reads
-  constexpr int JN = GATED ? 2 : 4;              // 32-column blocks of a wave
+// Epilogue of a wave's MI x NJ blocks: register 4 q + e of lane l in block (i, j) is row
+// m0 + 32 i + l % 32 of the tile's (`rows` valid, the first is output row `first`), weight row
+// 32 j + 8 q + 4 (l / 32) + e of the wave's; gated: odd blocks are the ups of the even ones. Output
+// columns from c0. Rows go through the wave's own LDS at `out`, RB bytes each, chunk c of row r in
+// slot c ^ (r % (RB / 16)).
+template <bool GATED, bool OUT8, int MI, int NJ>
+__device__ __forceinline__ void mx_tile_store(const MxArgs& p, const f32x16 (&acc)[MI][NJ],
+                                              lds_char* out, int64_t first, int64_t rows, int m0,
+                                              int64_t c0) {
+  constexpr int JN = GATED ? NJ / 2 : NJ;        // 32-column blocks of a wave
   constexpr int RB = 32 * JN * (OUT8 ? 1 : 2);   // bytes of a row
-  lds_char* const out = lds + wave * 16384;
-  const int64_t c0 = j0 + (GATED ? n0 / 2 : n0);  // the wave's first column
+  const int lane = lane_id(), r32 = lane & 31, g = lane >> 5;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < MI; ++i) {
     const int r = 32 * i + r32;
     const int64_t row = first + m0 + r;
     const bool valid = m0 + r < rows;
@@ -291,7 +110,7 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j)
   const int64_t col = c0 + PER * (lane % LR);
   const bool whole = OUT8 || (p.N & 7) == 0;
 #pragma unroll
-  for (int q = 0; q < LR; ++q) {
+  for (int q = 0; q < MI * LR / 2; ++q) {
     const int r = q * (64 / LR) + lane / LR;
     if (m0 + r >= rows || col >= p.N) continue;
     const uint4 v = read_k(out, (uint32_t)(r * RB + (((lane % LR) ^ (r & (LR - 1))) << 4)));
@@ -307,29 +126,285 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j)
   }
 }
 
-template <bool MX, bool GATED, bool OUT8, bool KA>
-int launch(const MxArgs& p, hipStream_t s) {
-  constexpr int CB = GATED ? T_BN / 2 : T_BN;
+// KA: K is a multiple of 128 and scales are 4-byte aligned.
+template <bool MX, bool GATED, bool OUT8, bool KA, int T_BM, int T_BN>
+__global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j, int parts) {
+  typedef Tile<MX, T_BM, T_BN> L;
+  constexpr int CB = GATED ? T_BN / 2 : T_BN;  // output columns
+  constexpr int ES = MX ? 1 : 2;               // bytes of an element of x
+  constexpr int MI = L::MI, NJ = L::NJ;
+  __shared__ __align__(16) char lds_raw[L::LDS];
+  RowTile t;
+  int slot = 0, part = 0;  // of a dense product
+  if (p.counts != nullptr) {
+    if (!row_tile<T_BM, T_NT>(p.counts, p.E, tiles_j, lds_raw, t)) return;
+    // Counts that sum to more than M end at its last row.
+    if (t.seg0 + t.nrows > p.M) t.nrows = p.M - t.seg0;
+    if ((int64_t)t.mt * T_BM >= t.nrows) return;
+  } else {
+    t.e = 0;
+    const int tiles_i = (int)((p.M + T_BM - 1) / T_BM);
+    slot = xcd_remap(blockIdx.x, tiles_i * tiles_j * parts);
+    part = slot % parts;
+    t.mt = slot / parts % tiles_i;
+    t.nt = slot / parts / tiles_i;
+    t.seg0 = 0;
+    t.nrows = p.M;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t K = p.K, i0 = (int64_t)t.mt * T_BM, j0 = (int64_t)t.nt * CB;
+  const int64_t rows = t.nrows - i0;  // valid rows of the tile, at least one
+  const int groups = (int)(K / MX_GROUP);
+  const int nkt = (int)((K + L::BK - 1) / L::BK);
+  lds_char* const lds = (lds_char*)lds_raw;
+  lds_char* const lds_s = lds + L::STAGES * L::STAGE;
+
+  // x: wave w loads rows 8 (XQ w + q) + lane / 8, chunk slot lane % 8 holding chunk
+  // slot ^ ((row >> 1) & 7). Rows past the expert's read as zeros.
+  const bool gather = p.arow != nullptr;
+  const int64_t first = t.seg0 + i0;
+  const char* const xbase = static_cast<const char*>(p.x) + (gather ? 0 : first * K * ES);
+  const i32x4 rx = make_rsrc(xbase, (gather ? p.src_rows : (rows < T_BM ? rows : T_BM)) * K * ES);
+  constexpr int XQ = T_BM / 32;  // instructions per wave
+  uint32_t xoff[XQ];
+  int xk[XQ];
+#pragma unroll
+  for (int q = 0; q < XQ; ++q) {
+    const int r = 8 * XQ * wave + 8 * q + (lane >> 3);
+    const int c = (lane & 7) ^ ((r >> 1) & 7);
+    xk[q] = c * (16 / ES);
+    xoff[q] = DM_OOB;
+    if (r < rows) xoff[q] = (uint32_t)((gather ? mx_source_row(p, first + r) : r) * K * ES + 16 * c);
+  }
+  // W: rows of WR bytes. Tile row r is weight row `weight_row(r)`; those past the last read it again
+  // (their columns are not stored). A wave's instruction covers 1 KiB.
+  const int64_t width = GATED ? 2 * p.N : p.N;
+  const uint8_t* const wbase = p.w + (int64_t)t.e * width * (K / 2);
+  const uint8_t* const sbase = p.ws + (int64_t)t.e * width * groups;
+  const i32x4 rw = make_rsrc(wbase, width * (K / 2));
+  const i32x4 rs = make_rsrc(sbase, width * groups);
+  auto weight_row = [&](int r) -> int64_t {
+    int64_t n = GATED ? j0 + 32 * (r >> 6) + (r & 31) : j0 + r;  // gated: 32 gates, their 32 ups
+    n = n < p.N ? n : p.N - 1;
+    return GATED && (r & 32) ? n + p.N : n;
+  };
+  constexpr int WQ = L::WB / 4096;  // instructions per wave
+  constexpr int CW = L::WR / 16;    // chunks of a row
+  uint32_t woff[WQ];
+  int wk[WQ];
+#pragma unroll
+  for (int q = 0; q < WQ; ++q) {
+    const int r = (64 / CW) * (WQ * wave + q) + lane / CW;
+    const int c = (lane % CW) ^ (MX ? (r >> 2) & 3 : (r >> 3) & 1);
+    wk[q] = 32 * c;
+    woff[q] = (uint32_t)(weight_row(r) * (K / 2) + 16 * c);
+  }
+  // Scales: thread t takes weight row t and row t of x.
+  const uint32_t soff = (uint32_t)(weight_row(tid < T_BN ? tid : 0) * groups);
+  const uint8_t* const xsbase = MX ? p.xs + (gather ? 0 : first * groups) : nullptr;
+  const i32x4 rxs = make_rsrc(xsbase, MX ? (gather ? p.src_rows : (rows < T_BM ? rows : T_BM)) * groups : 0);
+  uint32_t xsoff = DM_OOB;
+  if (MX && tid < T_BM && tid < rows)
+    xsoff = (uint32_t)((gather ? mx_source_row(p, first + tid) : tid) * groups);
+
+  // The words of 128 elements from group g0 on into scale buffer b.
+  auto load_scales = [&](int g0, int b) {
+    const uint32_t at = lds_addr_of(lds_s) + (uint32_t)(b * L::SB);
+    if constexpr (KA) {
+      if (wave < T_BN / 64) dma4(soff, advance_rsrc(rs, (uint32_t)g0), at + 256u * wave);
+      if (MX && wave < T_BM / 64)
+        dma4(xsoff, advance_rsrc(rxs, (uint32_t)g0), at + T_BN * 4 + 256u * wave);
+    } else {
+      uint32_t* const to = reinterpret_cast<uint32_t*>(lds_raw + L::STAGES * L::STAGE + b * L::SB);
+      if (tid < T_BN) to[tid] = scale_word(sbase + soff + g0, groups - g0);
+      if constexpr (MX)
+        if (tid < T_BM) to[T_BN + tid] = xsoff == DM_OOB ? 0x7f7f7f7fu : scale_word(xsbase + xsoff + g0, groups - g0);
+    }
+  };
+  auto issue = [&](int kt, int stage) {
+    const uint32_t base = lds_addr_of(lds) + (uint32_t)(stage * L::STAGE);
+    const i32x4 rxk = advance_rsrc(rx, (uint32_t)(kt * L::BK * ES));
+    const i32x4 rwk = advance_rsrc(rw, (uint32_t)(kt * (L::BK / 2)));
+#pragma unroll
+    for (int q = 0; q < XQ; ++q)
+      dma16(KA || kt * L::BK + xk[q] < (int)K ? xoff[q] : DM_OOB, rxk,
+            base + (uint32_t)(XQ * wave + q) * 1024u);
+#pragma unroll
+    for (int q = 0; q < WQ; ++q)
+      dma16(KA || kt * L::BK + wk[q] < (int)K ? woff[q] : DM_OOB, rwk,
+            base + L::XB + (uint32_t)(WQ * wave + q) * 1024u);
+    if (MX || (kt & 1) == 0)
+      load_scales(kt * (L::BK / MX_GROUP), MX ? stage : (kt >> 1) & 1);
+  };
+
+  // Wave w multiplies half w / 2 of the rows by half w % 2 of the weight rows.
+  const int m0 = T_BM / 2 * (wave >> 1), n0 = T_BN / 2 * (wave & 1);
+  const int r32 = lane & 31, g = lane >> 5;
+  f32x16 acc[MI][NJ] = {};
+  auto multiply = [&](int kt, int stage) {
+    lds_char* const st = lds + stage * L::STAGE;
+    const char* const sw = lds_raw + L::STAGES * L::STAGE + (MX ? stage : (kt >> 1) & 1) * L::SB;
+    const int shift = MX ? 8 * g : 8 * (2 * (kt & 1) + g);
+    uint32_t ws[NJ], xs[MI];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      ws[j] = *reinterpret_cast<const uint32_t*>(sw + 4 * (n0 + 32 * j + r32)) >> shift;
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+        xs[i] = *reinterpret_cast<const uint32_t*>(sw + 4 * (T_BN + m0 + 32 * i + r32)) >> shift;
+      auto step = [&](auto sc) {
+        constexpr int s = decltype(sc)::value;
+        uint4 w[NJ], x[MI][2];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int r = m0 + 32 * i + r32;
+          const uint32_t at = (uint32_t)(r * 128), sz = (uint32_t)((r >> 1) & 7);
+          x[i][0] = read_k(st, at + (((4 * s + g) ^ sz) << 4));
+          x[i][1] = read_k(st, at + (((4 * s + 2 + g) ^ sz) << 4));
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int r = n0 + 32 * j + r32;
+          w[j] = read_k(st, L::XB + (uint32_t)(r * 64 + (((2 * s + g) ^ ((r >> 2) & 3)) << 4)));
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+            acc[i][j] = mx_mma32<2 * s, 2 * s>(w[j], x[i][0], x[i][1], ws[j], xs[i], acc[i][j]);
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+    } else {
+      uint4 w[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int r = n0 + 32 * j + r32;
+        w[j] = read_k(st, L::XB + (uint32_t)(r * 32 + ((g ^ ((r >> 3) & 1)) << 4)));
+        ws[j] &= 255u;
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        uint4 x[MI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int r = m0 + 32 * i + r32;
+          x[i] = read_k(st, (uint32_t)(r * 128 + (((4 * g + s) ^ ((r >> 1) & 7)) << 4)));
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const uint32_t q = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w;
+          const uint4 a = mx_bf16x8(q, ws[j]);
+#pragma unroll
+          for (int i = 0; i < MI; ++i) acc[i][j] = Mma<TT_BF16>::run(a, x[i], acc[i][j]);
+        }
+      }
+    }
+  };
+
+  // This block's k-tiles: from an even one where the words of scales span two.
+  const int pairs = MX ? nkt : (nkt + 1) / 2;
+  const int k0 = (MX ? 1 : 2) * (int)((int64_t)pairs * part / parts);
+  const int k1r = (MX ? 1 : 2) * (int)((int64_t)pairs * (part + 1) / parts);
+  const int k1 = k1r < nkt ? k1r : nkt;
+#pragma unroll
+  for (int s = 0; s < L::STAGES - 1; ++s)
+    if (k0 + s < k1) issue(k0 + s, s);
+  int stage = 0;
+  for (int kt = k0; kt < k1; ++kt) {
+    // k-tile kt has landed once at most the loads of later ones are outstanding, at least the x and
+    // W pieces of each.
+    const int later = KA ? k1 - 1 - kt : 0;
+    if (L::STAGES >= 4 && later >= 2) TT_WAIT_VMCNT(2 * (XQ + WQ));
+    else if (L::STAGES >= 3 && later >= 1) TT_WAIT_VMCNT(XQ + WQ);
+    else TT_WAIT_VMCNT(0);
+    TT_LDS_BARRIER();
+    const int next = stage == 0 ? L::STAGES - 1 : stage - 1;  // the stage of kt - 1
+    if (kt + L::STAGES - 1 < k1) issue(kt + L::STAGES - 1, next);
+    multiply(kt, stage);
+    stage = stage == L::STAGES - 1 ? 0 : stage + 1;
+  }
+
+  if (parts > 1) {
+    // A part of the reduction: the sums as the registers hold them, for mx_join_kernel.
+    float* const to = p.part + ((int64_t)slot * 4 + wave) * (MI * NJ * 1024) + lane * 4;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(to + ((i * NJ + j) * 4 + q) * 256) =
+              float4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                     acc[i][j][4 * q + 3]};
+    return;
+  }
+  TT_LDS_BARRIER();  // every wave is past its fragment reads
+  mx_tile_store<GATED, OUT8, MI, NJ>(p, acc, lds + wave * (MI * NJ * 2048), t.seg0 + i0, rows, m0,
+                                     j0 + (GATED ? n0 / 2 : n0));
+}
+
+// Sum of a dense product's parts, in order, and the epilogue: a wave per wave of a tile.
+template <bool GATED, bool OUT8, int T_BM, int T_BN>
+__global__ __launch_bounds__(64) void mx_join_kernel(MxArgs p, int tiles_i, int parts) {
+  constexpr int MI = T_BM / 64, NJ = T_BN / 64;
+  __shared__ __align__(16) char lds_raw[MI * NJ * 2048];
+  const int tile = (int)(blockIdx.x >> 2), wave = (int)(blockIdx.x & 3), lane = lane_id();
+  const int64_t i0 = (int64_t)(tile % tiles_i) * T_BM;
+  const int64_t j0 = (int64_t)(tile / tiles_i) * (GATED ? T_BN / 2 : T_BN);
+  f32x16 acc[MI][NJ] = {};
+  for (int z = 0; z < parts; ++z) {
+    const float* const from =
+        p.part + (((int64_t)tile * parts + z) * 4 + wave) * (MI * NJ * 1024) + lane * 4;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 v = *reinterpret_cast<const float4*>(from + ((i * NJ + j) * 4 + q) * 256);
+          acc[i][j][4 * q] += v.x;
+          acc[i][j][4 * q + 1] += v.y;
+          acc[i][j][4 * q + 2] += v.z;
+          acc[i][j][4 * q + 3] += v.w;
+        }
+  }
+  const int n0 = T_BN / 2 * (wave & 1);
+  mx_tile_store<GATED, OUT8, MI, NJ>(p, acc, (lds_char*)lds_raw, i0, p.M - i0, T_BM / 2 * (wave >> 1),
+                                     j0 + (GATED ? n0 / 2 : n0));
+}
+
+template <bool MX, bool GATED, bool OUT8, bool KA, int BM, int BN>
+int launch(const MxArgs& p, int parts, hipStream_t s) {
+  constexpr int CB = GATED ? BN / 2 : BN;
   const int64_t tiles_j = (p.N + CB - 1) / CB;
-  int64_t tiles_i = (p.M + T_BM - 1) / T_BM;
-  if (p.counts != nullptr) tiles_i = p.M / T_BM + (p.E < p.M ? p.E : p.M);
-  TT_REQUIRE(tiles_i * tiles_j < (1ll << 31) && tt_grid_ok(tiles_i * tiles_j, T_NT),
-             "mx product: grid too large");
-  hipLaunchKernelGGL((mx_tile_kernel<MX, GATED, OUT8, KA>), dim3((unsigned)(tiles_i * tiles_j)),
-                     dim3(T_NT), 0, s, p, (int)tiles_j);
-  return tt_check_launch("mx_tile");
+  int64_t tiles_i = (p.M + BM - 1) / BM;
+  if (p.counts != nullptr) tiles_i = p.M / BM + (p.E < p.M ? p.E : p.M);
+  const int64_t blocks = tiles_i * tiles_j * parts;
+  TT_REQUIRE(blocks < (1ll << 31) && tt_grid_ok(blocks, T_NT), "mx product: grid too large");
+  hipLaunchKernelGGL((mx_tile_kernel<MX, GATED, OUT8, KA, BM, BN>), dim3((unsigned)blocks),
+                     dim3(T_NT), 0, s, p, (int)tiles_j, parts);
+  const int rc = tt_check_launch("mx_tile");
+  if (rc != TT_OK || parts == 1) return rc;
+  hipLaunchKernelGGL((mx_join_kernel<GATED, OUT8, BM, BN>), dim3((unsigned)(tiles_i * tiles_j * 4)),
+                     dim3(64), 0, s, p, (int)tiles_i, parts);
+  return tt_check_launch("mx_join");
 }
 
 template <bool MX, bool GATED, bool OUT8>
-int aligned(const MxArgs& p, hipStream_t s) {
+int shaped(const MxArgs& p, MxPlan plan, hipStream_t s) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs);
-  return p.K % 128 == 0 && (at & 3) == 0 ? launch<MX, GATED, OUT8, true>(p, s)
-                                         : launch<MX, GATED, OUT8, false>(p, s);
+  if (p.K % 128 != 0 || (at & 3) != 0) return launch<MX, GATED, OUT8, false, 128, 128>(p, plan.parts, s);
+  if (plan.bm == 64) return launch<MX, GATED, OUT8, true, 64, 128>(p, plan.parts, s);
+  if (plan.bn == 128) return launch<MX, GATED, OUT8, true, 128, 128>(p, plan.parts, s);
+  return launch<MX, GATED, OUT8, true, 128, 256>(p, plan.parts, s);
 }
 
 template <bool MX, bool GATED>
-int out(const MxArgs& p, hipStream_t s) {
-  return p.ys != nullptr ? aligned<MX, GATED, true>(p, s) : aligned<MX, GATED, false>(p, s);
+int out(const MxArgs& p, MxPlan plan, hipStream_t s) {
+  return p.ys != nullptr ? shaped<MX, GATED, true>(p, plan, s) : shaped<MX, GATED, false>(p, plan, s);
 }
 
 }  // namespace
@@ -337,12 +412,12 @@ int out(const MxArgs& p, hipStream_t s) {
 bool tt_mx_tile_takes(const MxArgs& p, bool gated) {
   const int64_t es = p.xs != nullptr ? 1 : 2, width = gated ? 2 * p.N : p.N;
   // 32-bit offsets within an expert's weights, a tile's rows, and a gathered source.
-  return p.K > 0 && width * (p.K / 2) < (1ll << 31) && T_BM * p.K * es < (1ll << 31) &&
+  return p.K > 0 && width * (p.K / 2) < (1ll << 31) && 128 * p.K * es < (1ll << 31) &&
          (p.arow == nullptr || p.src_rows * p.K * es < (1ll << 31)) &&
          (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
 }
 
-int tt_mx_tile(const MxArgs& p, bool gated, hipStream_t s) {
-  if (p.xs != nullptr) return gated ? out<true, true>(p, s) : out<true, false>(p, s);
-  return gated ? out<false, true>(p, s) : out<false, false>(p, s);
+int tt_mx_tile(const MxArgs& p, bool gated, MxPlan plan, hipStream_t s) {
+  if (p.xs != nullptr) return gated ? out<true, true>(p, plan, s) : out<true, false>(p, plan, s);
+  return gated ? out<false, true>(p, plan, s) : out<false, false>(p, plan, s);
 }

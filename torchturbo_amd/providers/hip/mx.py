@@ -92,10 +92,12 @@ def product(values, xs, codes, scales, counts, *, gated=False, act=0, probs=None
     n = codes.shape[-2] // (2 if gated else 1)
     y = torch.empty((m, n), dtype=torch.float8_e4m3fn if mx_out else torch.bfloat16, device=dev)
     ys = torch.empty((m, n // GROUP), dtype=torch.uint8, device=dev) if mx_out else None
+    size = L.load().tt_mx_product_workspace(m, k, n, counts is not None, gated) if m > 16 else 0
+    ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
     L.call("tt_mx_product", L.ptr(values), L.ptr(xs), L.ptr(row_map), values.shape[0],
            L.ptr(codes), L.ptr(scales), m, k, n, experts, L.ptr(counts), int(gated), act,
            L.ptr(probs), 0 if probs is None else L.dtype_code(probs.dtype), L.ptr(y), L.ptr(ys),
-           L.stream(dev))
+           L.ptr(ws), size, L.stream(dev))
     return (y, ys) if mx_out else y
 
 
