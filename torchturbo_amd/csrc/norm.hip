@@ -8,9 +8,10 @@
 //
 //   dh = rho (a - xh mean(a xh)) + g_sum,  dw = sum over rows of gy xh.
 //
-// All of it is bound by memory: every tensor is read or written once. A row stays in the
-// registers of its threads between the sum of squares and the product: a wave per row up to 2048
-// features, 256 threads to 8192, 1024 to 16384; longer rows are read twice. Blocks go on to further rows with the weight kept, so that it is read once per
+// All of it is bound by memory: every tensor is read or written once (4.2 to 5.1 TB/s; a large copy
+// on this card reaches 5.2). A row stays in the registers of its threads between the sum of squares
+// and the product: a wave per row up to 2048 features, 256 threads to 8192, 1024 to 16384; longer
+// rows are read twice. Blocks go on to further rows with the weight kept, so that it is read once per
 // block, and dw is summed in registers: one partial row per block, joined by a second kernel in the
 // order of the blocks.
 #include <initializer_list>
@@ -53,6 +54,22 @@ __device__ __forceinline__ void load_weight(float (&w)[8], const void* p, int dt
     default: load8<F32T, VEC>(w, static_cast<const float*>(p) + at, left); break;
   }
 }
+
+// Eight elements as they lie in memory.
+template <class T>
+struct Raw8 {
+  uint4 v[sizeof(typename T::storage) / 2];
+  __device__ __forceinline__ void load(const typename T::storage* p) {
+    v[0] = *reinterpret_cast<const uint4*>(p);
+    if constexpr (sizeof(typename T::storage) == 4) v[1] = *reinterpret_cast<const uint4*>(p + 4);
+  }
+  __device__ __forceinline__ void unpack(float (&f)[8]) const {
+    typename T::storage s[8];
+    __builtin_memcpy(s, v, sizeof(s));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = T::to_f32(s[j]);
+  }
+};
 
 struct NormArgs {
   const void *x, *residual, *weight;
@@ -103,7 +120,23 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_fwd_kernel(NormArgs p)
     }
   };
   const int64_t stride = (int64_t)gridDim.x * ROWS;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / RT; row < p.T; row += stride) {
+  // The next row of a thread, in flight while the one before is worked on.
+  constexpr bool AHEAD = VEC && IT > 0;
+  Raw8<T> xn[AHEAD ? KEEP : 1], en[AHEAD ? KEEP : 1];
+  auto fetch = [&](int64_t row) {
+    if (row >= p.T) return;
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c) {
+      const int64_t at = ((int64_t)c * RT + t) * 8;
+      if (at < H) {
+        xn[c].load(static_cast<const S*>(p.x) + row * H + at);
+        if (p.residual != nullptr) en[c].load(static_cast<const S*>(p.residual) + row * H + at);
+      }
+    }
+  };
+  const int64_t row0 = (int64_t)blockIdx.x * ROWS + threadIdx.x / RT;
+  if constexpr (AHEAD) fetch(row0);
+  for (int64_t row = row0; row < p.T; row += stride) {
     float h[KEEP][8];
     float s = 0.f;
     if constexpr (IT > 0) {
@@ -111,7 +144,17 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_fwd_kernel(NormArgs p)
       for (int c = 0; c < IT; ++c) {
         const int64_t at = ((int64_t)c * RT + t) * 8;
         if (at < H) {
-          load_sum(h[c], row, at);
+          if constexpr (AHEAD) {
+            xn[c].unpack(h[c]);
+            if (p.residual != nullptr) {
+              float r[8];
+              en[c].unpack(r);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) h[c][j] += r[j];
+            }
+          } else {
+            load_sum(h[c], row, at);
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) h[c][j] = 0.f;
@@ -121,6 +164,7 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_fwd_kernel(NormArgs p)
       for (int c = 0; c < IT; ++c)
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += h[c][j] * h[c][j];
+      if constexpr (AHEAD) fetch(row + stride);
     } else {
       for (int c = 0; c < its; ++c) {
         const int64_t at = ((int64_t)c * RT + t) * 8;
@@ -198,8 +242,26 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_bwd_kernel(NormBwdArgs
     for (int j = 0; j < 8; ++j) xh[j] *= rho;
   };
   const int64_t stride = (int64_t)gridDim.x * ROWS;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / RT; row < p.T; row += stride) {
-    const float rho = p.rstd[row];
+  // The next row of a thread, in flight while the one before is worked on.
+  constexpr bool AHEAD = VEC && IT > 0;
+  Raw8<T> hn[AHEAD ? KEEP : 1], gn[AHEAD ? KEEP : 1];
+  float rn = 0.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= p.T) return;
+    rn = p.rstd[row];
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c) {
+      const int64_t at = ((int64_t)c * RT + t) * 8;
+      if (at < H) {
+        hn[c].load(static_cast<const S*>(p.h) + row * H + at);
+        gn[c].load(static_cast<const S*>(p.gy) + row * H + at);
+      }
+    }
+  };
+  const int64_t row0 = (int64_t)blockIdx.x * ROWS + threadIdx.x / RT;
+  if constexpr (AHEAD) fetch(row0);
+  for (int64_t row = row0; row < p.T; row += stride) {
+    const float rho = AHEAD ? rn : p.rstd[row];
     float xh[KEEP][8], g[KEEP][8];
     float s = 0.f;
     if constexpr (IT > 0) {
@@ -207,7 +269,14 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_bwd_kernel(NormBwdArgs
       for (int c = 0; c < IT; ++c) {
         const int64_t at = ((int64_t)c * RT + t) * 8;
         if (at < H) {
-          load_pair(xh[c], g[c], rho, row, at);
+          if constexpr (AHEAD) {
+            hn[c].unpack(xh[c]);
+            gn[c].unpack(g[c]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) xh[c][j] *= rho;
+          } else {
+            load_pair(xh[c], g[c], rho, row, at);
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) xh[c][j] = g[c][j] = 0.f;
@@ -220,6 +289,7 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_bwd_kernel(NormBwdArgs
           s += g[c][j] * w[c][j] * xh[c][j];
           dw[c][j] += g[c][j] * xh[c][j];
         }
+      if constexpr (AHEAD) fetch(row + stride);
     } else {
       for (int c = 0; c < its; ++c) {
         const int64_t at = ((int64_t)c * RT + t) * 8;
@@ -298,22 +368,24 @@ __global__ __launch_bounds__(256) void rms_norm_dw_kernel(NormBwdArgs p) {
   p.part[(int64_t)blockIdx.y * p.H + j] = v;
 }
 
-// dw [H] from `parts` partial rows: a block takes 32 features and eight threads each a share of the
+// dw [H] from `parts` partial rows: a block takes 32 features and 32 threads each a share of the
 // rows, whose sums are added in order.
-__global__ __launch_bounds__(256) void rms_norm_join_kernel(const float* __restrict__ part,
-                                                            int parts, int64_t H,
-                                                            void* __restrict__ dw, int dtype) {
-  __shared__ float sums[8][32];
+__global__ __launch_bounds__(1024) void rms_norm_join_kernel(const float* __restrict__ part,
+                                                             int parts, int64_t H,
+                                                             void* __restrict__ dw, int dtype) {
+  __shared__ float sums[32][33];
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
   const int64_t j = (int64_t)blockIdx.x * 32 + c;
   float v = 0.f;
-  if (j < H)
-    for (int i = r; i < parts; i += 8) v += part[(int64_t)i * H + j];
+  if (j < H) {
+#pragma unroll 8
+    for (int i = r; i < parts; i += 32) v += part[(int64_t)i * H + j];
+  }
   sums[r][c] = v;
   __syncthreads();
   if (r != 0 || j >= H) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) v += sums[i][c];
+  for (int i = 1; i < 32; ++i) v += sums[i][c];
   store_from_f32(dw, dtype, j, v);
 }
 
@@ -325,9 +397,11 @@ int row_chunks(int64_t H) {
   return H <= 16384 ? (int)(((H + 7) / 8 + rt - 1) / rt) : 0;
 }
 
-// Blocks of a launch: enough to fill the card several times over (a wave per SIMD and more), each
-// with several rows where there are many.
-constexpr int64_t FWD_BLOCKS = 256 * 8, BWD_BLOCKS = 256 * 2;
+// Blocks of a launch: as many as a CU holds with a row in work and the next in flight (more start
+// later and wait for their first row; fewer leave memory idle). us at 16384 x 2048 / 4096 x 7168, bf16
+// with residual: forward in 512, 768, 2048 blocks 69 / 61 / 59 and 66 / 57 / 58, backward in 256, 512, 640
+// blocks 87 / 65 / 87 and 87 / 64 / 87; with no row in flight ahead 60 and 58, 97 and 98.
+constexpr int64_t FWD_BLOCKS = 256 * 3, BWD_BLOCKS = 256 * 2;
 int64_t blocks_for(int64_t T, int64_t H, int64_t most) {
   const int rows = row_threads(H) >= 256 ? 1 : 256 / row_threads(H);
   const int64_t want = (T + rows - 1) / rows;
@@ -444,7 +518,7 @@ extern "C" int tt_rms_norm_bwd(const void* h, const void* weight, int weight_dty
     default: rc = vec ? bwd_shape<F32T, true>(p, s) : bwd_shape<F32T, false>(p, s); break;
   }
   if (rc != TT_OK || dweight == nullptr) return rc;
-  hipLaunchKernelGGL(rms_norm_join_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, s,
+  hipLaunchKernelGGL(rms_norm_join_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, s,
                      p.part, (int)blocks_for(rows, cols, BWD_BLOCKS), cols, dweight, weight_dtype);
   return tt_check_launch("rms_norm_join");
 }

@@ -14,7 +14,7 @@ import torch
 GROUP = 32
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False, slots=True)
 class MxRows:
     # [..., K] float8_e4m3fn.
     codes: torch.Tensor
@@ -31,7 +31,7 @@ class MxRows:
                       self.scales.view(*lead, self.scales.shape[-1]))
 
 
-@dataclass(frozen=True)
+@dataclass(eq=False, slots=True)
 class NormRows:
     """What ``rms_norm_mx`` gives."""
 

@@ -38,66 +38,87 @@ from .linear import ACTIVATIONS, FLOATS, _autograd_sees, _rows
 
 def _aligned(t, size):
     """``t``, contiguous at a multiple of ``size`` bytes (copied where a view is not)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % size == 0 else t.clone()
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t if t.data_ptr() % size == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _bytes(op, name, t, kind):
-    if t.dtype not in (torch.uint8, kind):
+    if t.dtype is not kind:
         raise ValueError(f"{op}: {name} must be uint8 or {kind}, got {t.dtype}")
-    return t if t.dtype is torch.uint8 else t.view(torch.uint8)
+    return t.view(torch.uint8)
 
 
 def check_weights(op, codes, scales, dims):
     """Codes ``[..., N, K / 2]`` and scales as uint8, contiguous; ``ValueError`` otherwise."""
-    codes = _bytes(op, "codes", codes, torch.float4_e2m1fn_x2)
-    scales = _bytes(op, "scales", scales, torch.float8_e8m0fnu)
-    if codes.dim() != dims:
+    if codes.dtype is not torch.uint8:
+        codes = _bytes(op, "codes", codes, torch.float4_e2m1fn_x2)
+    if scales.dtype is not torch.uint8:
+        scales = _bytes(op, "scales", scales, torch.float8_e8m0fnu)
+    shape = codes.shape
+    if len(shape) != dims:
         raise ValueError(f"{op} expects codes of {dims} dimensions ([..., out, in / 2]), got "
-                         f"{list(codes.shape)}")
-    k = 2 * codes.shape[-1]
-    want = (*codes.shape[:-1], k // GROUP)
-    if k % GROUP or tuple(scales.shape) != want:
-        raise ValueError(f"{op}: codes {list(codes.shape)} need scales {list(want)} and whole groups "
-                         f"of {GROUP} elements, got {list(scales.shape)}")
-    return _aligned(codes, 16), scales.contiguous()
+                         f"{list(shape)}")
+    k = 2 * shape[-1]
+    if k % GROUP or scales.shape != (*shape[:-1], k // GROUP):
+        raise ValueError(f"{op}: codes {list(shape)} need scales {[*shape[:-1], k // GROUP]} and whole "
+                         f"groups of {GROUP} elements, got {list(scales.shape)}")
+    return _aligned(codes, 16), scales if scales.is_contiguous() else scales.contiguous()
 
 
 def check_rows(op, x, k):
     """``(values [T, K], scales or None, leading shape)`` of bf16 rows or ``MxRows``."""
-    if isinstance(x, MxRows):
-        codes, scales = x.codes, _bytes(op, "the rows' scales", x.scales, torch.float8_e8m0fnu)
-        if codes.dtype is not torch.float8_e4m3fn or codes.dim() == 0 or codes.shape[-1] % GROUP \
-                or tuple(scales.shape) != (*codes.shape[:-1], codes.shape[-1] // GROUP):
+    if type(x) is MxRows:
+        codes, scales = x.codes, x.scales
+        if scales.dtype is not torch.uint8:
+            scales = _bytes(op, "the rows' scales", scales, torch.float8_e8m0fnu)
+        shape = codes.shape
+        if codes.dtype is not torch.float8_e4m3fn or not shape or shape[-1] % GROUP \
+                or scales.shape != (*shape[:-1], shape[-1] // GROUP):
             raise ValueError(f"{op}: rows in 8 bits are float8_e4m3fn [..., K] with uint8 scales "
-                             f"[..., K / {GROUP}], got {codes.dtype} {list(codes.shape)} and "
+                             f"[..., K / {GROUP}], got {codes.dtype} {list(shape)} and "
                              f"{list(scales.shape)}")
-        values = _rows(codes, codes.shape[-1])
+        values = _rows(codes, shape[-1])
         scales = _rows(scales, scales.shape[-1])
     else:
-        if x.dtype is not torch.bfloat16 or x.dim() == 0:
-            raise ValueError(f"{op} takes bf16 rows [..., in] or MxRows, got {x.dtype}")
-        codes, values, scales = x, _rows(x, x.shape[-1]), None
-    if k is not None and values.shape[1] != k:
-        raise ValueError(f"{op}: x has {values.shape[1]} features, weight expects {k}")
-    return _aligned(values, 16), scales, codes.shape[:-1]
+        if not isinstance(x, torch.Tensor) or x.dtype is not torch.bfloat16 or x.dim() == 0:
+            raise ValueError(f"{op} takes bf16 rows [..., in] or MxRows, got "
+                             f"{getattr(x, 'dtype', type(x).__name__)}")
+        shape, scales = x.shape, None
+        values = _rows(x, shape[-1])
+    if k is not None and shape[-1] != k:
+        raise ValueError(f"{op}: x has {shape[-1]} features, weight expects {k}")
+    return _aligned(values, 16), scales, shape[:-1]
+
+
+def _device(first, *others):
+    """The tensors' one GPU, or ``require_cuda``'s refusal."""
+    index = first.get_device()
+    if index >= 0:
+        for t in others:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return first.device
+    return require_cuda(first, *others)
 
 
 def product(values, xs, codes, scales, counts, *, gated=False, act=0, probs=None, row_map=None,
             mx_out=False):
     """``tt_mx_product`` of checked operands: bf16 [M, N], or its codes and scales."""
-    m = values.shape[0] if row_map is None else row_map.shape[0]
-    k, dev = values.shape[1], values.device
+    source, k = values.shape
+    m, dev, ptr = source if row_map is None else row_map.shape[0], values.device, L.ptr
     experts = 1 if counts is None else codes.shape[0]
     n = codes.shape[-2] // (2 if gated else 1)
     y = torch.empty((m, n), dtype=torch.float8_e4m3fn if mx_out else torch.bfloat16, device=dev)
     ys = torch.empty((m, n // GROUP), dtype=torch.uint8, device=dev) if mx_out else None
-    size = L.load().tt_mx_product_workspace(m, k, n, counts is not None, gated) if m > 16 else 0
+    # Scratch of a split reduction; a few rows have none.
+    size = L.load().tt_mx_product_workspace(m, k, n, 0, gated) if counts is None and m > 16 else 0
     ws = torch.empty((size,), dtype=torch.uint8, device=dev) if size else None
-    L.call("tt_mx_product", L.ptr(values), L.ptr(xs), L.ptr(row_map), values.shape[0],
-           L.ptr(codes), L.ptr(scales), m, k, n, experts, L.ptr(counts), int(gated), act,
-           L.ptr(probs), 0 if probs is None else L.dtype_code(probs.dtype), L.ptr(y), L.ptr(ys),
-           L.ptr(ws), size, L.stream(dev))
+    L.call("tt_mx_product", values.data_ptr(), ptr(xs), ptr(row_map), source, codes.data_ptr(),
+           scales.data_ptr(), m, k, n, experts, ptr(counts), gated, act, ptr(probs),
+           0 if probs is None else L.dtype_code(probs.dtype), y.data_ptr(), ptr(ys), ptr(ws), size,
+           L.stream(dev))
     return (y, ys) if mx_out else y
 
 
@@ -143,7 +164,7 @@ class HipLinearMxfp4(OpImpl):
         if mx_out and n % GROUP:
             raise ValueError(f"{op}: outputs in 8 bits are whole groups of {GROUP}, got {n}")
         values, xs, lead = check_rows(op, x, 2 * codes.shape[1])
-        require_cuda(values, xs, codes, scales)
+        _device(values, xs, codes, scales)
         if _autograd_sees(values):
             if mx_out:
                 raise _no_gradient(op, "outputs in 8 bits")
@@ -157,8 +178,8 @@ class HipLinearMxfp4(OpImpl):
         y = product(values, xs, codes, scales, None, gated=bool(gated),
                     act=ACTIVATIONS[activation_func], mx_out=mx_out)
         if mx_out:
-            return MxRows(y[0].view(*lead, n), y[1].view(*lead, n // GROUP))
-        return y.view(*lead, n)
+            return MxRows(*y) if len(lead) == 1 else MxRows(*y).view(*lead)
+        return y if len(lead) == 1 else y.view(*lead, n)
 
 
 @register_op(op_name="grouped_matmul_mxfp4", impl_name="hip_grouped_matmul_mxfp4",
@@ -194,7 +215,7 @@ class HipGroupedMatmulMxfp4(OpImpl):
                 raise ValueError(f"{op}: probs must be a float tensor of shape [{m}], got "
                                  f"{probs.dtype} {list(probs.shape)}")
             probs = probs.reshape(-1).contiguous()
-        dev = require_cuda(values, xs, codes, scales, row_map, probs)
+        dev = _device(values, xs, codes, scales, row_map, probs)
         counts = device_counts(tokens_per_expert, experts, dev, m=m)
         if _autograd_sees(values, probs):
             if mx_out:
@@ -216,27 +237,26 @@ def _quantized(op, x, bits):
     if x.dtype not in FLOATS or x.dim() == 0 or x.shape[-1] % GROUP:
         raise ValueError(f"{op} takes f32, bf16 or f16 rows of whole groups of {GROUP} elements, got "
                          f"{x.dtype} {list(x.shape)}")
-    require_cuda(x)
-    x2 = _rows(x.detach(), x.shape[-1])
+    dev = _device(x)
+    x2 = _rows(x, x.shape[-1])
     t, k = x2.shape
     lead = x.shape[:-1]
-    codes = torch.empty((*lead, k * bits // 8), device=x.device,
+    codes = torch.empty((*lead, k * bits // 8), device=dev,
                         dtype=torch.uint8 if bits == 4 else torch.float8_e4m3fn)
-    scales = torch.empty((*lead, k // GROUP), dtype=torch.uint8, device=x.device)
-    L.call(f"tt_mxfp{bits}_quantize", L.ptr(x2), L.dtype_code(x.dtype), t, k, L.ptr(codes),
-           L.ptr(scales), L.stream(x.device))
+    scales = torch.empty((*lead, k // GROUP), dtype=torch.uint8, device=dev)
+    L.call("tt_mxfp4_quantize" if bits == 4 else "tt_mxfp8_quantize", x2.data_ptr(),
+           L.dtype_code(x.dtype), t, k, codes.data_ptr(), scales.data_ptr(), L.stream(dev))
     return codes, scales
 
 
 def _dequantized(op, codes, scales, k, dtype, bits):
     if dtype not in FLOATS:
         raise ValueError(f"{op} gives f32, bf16 or f16, not {dtype}")
-    require_cuda(codes, scales)
-    codes, scales = _aligned(codes, 8), scales.contiguous()
-    out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=codes.device)
-    rows = out.numel() // k if k else 0
-    L.call(f"tt_mxfp{bits}_dequantize", L.ptr(codes), L.ptr(scales), rows, k, L.ptr(out),
-           L.dtype_code(dtype), L.stream(codes.device))
+    dev = _device(codes, scales)
+    out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=dev)
+    L.call("tt_mxfp4_dequantize" if bits == 4 else "tt_mxfp8_dequantize", codes.data_ptr(),
+           scales.data_ptr(), out.numel() // k if k else 0, k, out.data_ptr(), L.dtype_code(dtype),
+           L.stream(dev))
     return out
 
 
@@ -282,4 +302,4 @@ class HipDequantizeMxfp8(OpImpl):
             raise ValueError(f"dequantize_mxfp8 takes MxRows, got {type(rows).__name__}")
         values, scales, lead = check_rows("dequantize_mxfp8", rows, None)
         out = _dequantized("dequantize_mxfp8", values, scales, values.shape[1], dtype, 8)
-        return out.view(*lead, values.shape[1])
+        return out if len(lead) == 1 else out.view(*lead, values.shape[1])

@@ -22,16 +22,16 @@ from ...dispatch import MxRows, NormRows, OpImpl, OpImplKind, register_op
 from ...dispatch.mx import GROUP
 from ...runtime import TurboDevice
 from . import PRIORITY
-from ._functions import require_cuda
 from .available import hip_available
 from .linear import FLOATS, _autograd_sees, _rows
+from .mx import _device
 
 
 def _forward(x, weight, eps, residual, with_y, with_rstd, with_mx):
     """(y, sum, rstd, codes, scales) of rows [T, H]; None for a part not wanted."""
     (t, h), dev = x.shape, x.device
     y = torch.empty_like(x) if with_y else None
-    total = torch.empty_like(x) if residual is not None else None
+    total = None if residual is None else torch.empty_like(x)
     rstd = torch.empty((t,), dtype=torch.float32, device=dev) if with_rstd else None
     codes = scales = None
     if with_mx:
@@ -87,9 +87,9 @@ def _operands(op, x, weight, residual):
                          f"{residual.dtype} {list(residual.shape)}")
     if x.shape[-1] >= 1 << 31:
         raise ValueError(f"{op} takes fewer than 2^31 features")
-    require_cuda(x, weight, residual)
+    _device(x, weight, residual)
     h = x.shape[-1]
-    return (_rows(x, h), weight.contiguous(), None if residual is None else _rows(residual, h))
+    return _rows(x, h), weight.contiguous(), None if residual is None else _rows(residual, h)
 
 
 @register_op(op_name="rms_norm", impl_name="hip_rms_norm", kind=OpImplKind.CUSTOM,
@@ -104,8 +104,9 @@ class HipRmsNorm(OpImpl):
             y, h = RmsNorm.apply(x2, w, r, float(eps))
         else:
             y, h = _forward(x2, w, float(eps), r, True, False, False)[:2]
-        y = y.view(x.shape)
-        return y if residual is None else (y, h.view(x.shape))
+        if x.dim() != 2:
+            y, h = y.view(x.shape), None if h is None else h.view(x.shape)
+        return y if residual is None else (y, h)
 
 
 @register_op(op_name="rms_norm_mx", impl_name="hip_rms_norm_mx", kind=OpImplKind.CUSTOM,
@@ -123,7 +124,8 @@ class HipRmsNormMx(OpImpl):
             raise RuntimeError("rms_norm_mx has no gradient: call it under torch.no_grad(), or "
                                "rms_norm in its place")
         y, h, _, codes, scales = _forward(x2, w, float(eps), r, with_y, False, True)
-        lead = x.shape[:-1]
-        return NormRows(MxRows(codes.view(x.shape), scales.view(*lead, x.shape[-1] // GROUP)),
-                        y.view(x.shape) if with_y else None,
+        rows = MxRows(codes, scales)
+        if x.dim() == 2:
+            return NormRows(rows, y, h)
+        return NormRows(rows.view(*x.shape[:-1]), y.view(x.shape) if with_y else None,
                         None if h is None else h.view(x.shape))
