@@ -7,6 +7,8 @@ from .lora import GroupedLoRALinear, GroupedMLPLoRA
 from .module import ModuleSpec, build_module
 from .moe_config import MoEConfig, get_base_moe_config
 from .moe_layer import MoELayer, MoERuntimeInputs, MoESubmodules
+from .mxfp4 import Mxfp4GroupedMLP, Mxfp4SharedExpertMLP
+from .norm import RMSNorm
 from .router import MoEAuxLossAutoScaler, RouterGatingLinearFunction, TopKRouter
 from .shared_experts import SharedExpertMLP
 from .token_dispatcher import MoEAlltoAllTokenDispatcher
@@ -24,6 +26,9 @@ __all__ = [
     "MoERuntimeInputs",
     "MoESubmodules",
     "ModuleSpec",
+    "Mxfp4GroupedMLP",
+    "Mxfp4SharedExpertMLP",
+    "RMSNorm",
     "RouterGatingLinearFunction",
     "SafetensorsCheckpoint",
     "SharedExpertMLP",

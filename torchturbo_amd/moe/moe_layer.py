@@ -16,10 +16,12 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
-from ..dispatch import ops
+from ..dispatch import op_resolves, ops
 from .experts import Fp8GroupedMLP, GroupedMLP
 from .module import ModuleSpec, attached, build_module
 from .moe_config import MoEConfig
+from .mxfp4 import Mxfp4GroupedMLP
+from .norm import RMSNorm
 from .router import TopKRouter
 from .shared_experts import SharedExpertMLP
 from .token_dispatcher import MoEAlltoAllTokenDispatcher
@@ -29,6 +31,8 @@ from .token_dispatcher import MoEAlltoAllTokenDispatcher
 class MoESubmodules:
     experts: Union[ModuleSpec, type] = None
     shared_experts: Union[ModuleSpec, type] = None
+    # Norm of the layer's input (RMSNorm); the reference leaves it to the decoder layer.
+    norm: Union[ModuleSpec, type] = None
 
 
 @dataclass
@@ -60,6 +64,7 @@ class BaseMoELayer(torch.nn.Module):
         self.shared_expert = None
         self.shared_expert_gate = None
         self.token_dispatcher = None
+        self.norm = None
         self.layer_number = layer_number
         self._runtime_inputs = MoERuntimeInputs()
 
@@ -85,6 +90,7 @@ class MoELayer(BaseMoELayer):
                                     layer_number=layer_number)
         if self.use_shared_expert:
             self.shared_experts = build_module(submodules.shared_experts, config=config)
+        self.norm = build_module(getattr(submodules, "norm", None), config=config)
 
     def _gathering_experts(self, tokens, expert_indices) -> bool:
         """Whether the permutation and unpermutation can be folded into the
@@ -152,7 +158,59 @@ class MoELayer(BaseMoELayer):
         d.hidden_shape, d.hidden_shape_before_permute = hidden_states.shape, tokens.shape
         return output.view(hidden_states.shape)
 
-    def _experts_and_combine(self, hidden_states, probs, routing_map, expert_indices):
+    def _mxfp4_inference(self, hidden_states) -> bool:
+        """Whether 4-bit experts may read the tokens' rows through the routing index: no gradients,
+        nothing attached to the experts, and the HIP providers for the ops this stands in for."""
+        if (torch.is_grad_enabled() or not hidden_states.is_cuda
+                or type(self.experts) is not Mxfp4GroupedMLP or attached(self.experts, "inference")
+                or type(self.token_dispatcher) is not MoEAlltoAllTokenDispatcher
+                or self.num_local_experts != self.config.num_moe_experts):
+            return False
+        wanted = (("moe_permutation", "hip_moe_mask_permutation"),
+                  ("moe_unpermutation", "hip_moe_mask_unpermutation"),
+                  ("grouped_matmul_mxfp4", "hip_grouped_matmul_mxfp4"))
+        try:
+            return all(ops.selected_impl_name(op) == impl for op, impl in wanted)
+        except RuntimeError:
+            return False
+
+    def _mxfp4_experts(self, hidden_states, probs, expert_indices, rows):
+        """The output of 4-bit experts without gradients, their rows gathered by the products
+        (``rows``: the tokens in 8 bits, or None); None where the conditions do not hold."""
+        if expert_indices is None or not self._mxfp4_inference(hidden_states):
+            return None
+        from ..providers.hip import fused_experts
+        output, counts = fused_experts.mxfp4_forward(
+            self.experts, hidden_states.view(-1, hidden_states.shape[-1]), rows, probs,
+            expert_indices)
+        if output is None:
+            return None
+        d = self.token_dispatcher
+        d.tokens_per_expert = counts
+        d.hidden_shape = hidden_states.shape
+        d.hidden_shape_before_permute = (hidden_states.numel() // hidden_states.shape[-1],
+                                         hidden_states.shape[-1])
+        return output.view(hidden_states.shape)
+
+    def _normalised(self, hidden_states, residual):
+        """(normalised input, the same in 8 bits or None, input + residual or None)."""
+        norm = self.norm
+        if norm is None:
+            if residual is not None:
+                raise ValueError("MoELayer takes a residual only with a norm (MoESubmodules.norm)")
+            return hidden_states, None, None
+        if (type(norm) is RMSNorm and not attached(norm) and self._mxfp4_inference(hidden_states)
+                and self.experts.rows_in_8_bits and op_resolves("rms_norm_mx")
+                and ops.selected_impl_name("rms_norm") == "hip_rms_norm"):
+            # The router's rows and the experts' in one pass.
+            out = ops.rms_norm_mx(hidden_states, norm.weight, norm.eps, residual=residual, with_y=True)
+            return out.y, out.rows, out.sum
+        if residual is None:
+            return norm(hidden_states), None, None
+        y, total = norm(hidden_states, residual)
+        return y, None, total
+
+    def _experts_and_combine(self, hidden_states, probs, routing_map, expert_indices, rows=None):
         flat = hidden_states.view(-1, hidden_states.shape[-1])
         if self._gathering_experts(flat, expert_indices):
             # One GPU, every expert local: the GEMMs gather the token rows
@@ -164,6 +222,8 @@ class MoELayer(BaseMoELayer):
             output = tokens.view(hidden_states.shape).to(hidden_states.dtype)
         else:
             output = self._inference_experts(hidden_states, probs, expert_indices)
+            if output is None:
+                output = self._mxfp4_experts(hidden_states, probs, expert_indices, rows)
             if output is None:
                 output = self._dispatched_experts(hidden_states, probs, routing_map,
                                                   expert_indices)
@@ -206,16 +266,21 @@ class MoELayer(BaseMoELayer):
         tokens = d.combine_postprocess(tokens)
         return tokens.to(hidden_states.dtype)
 
-    def forward(self, hidden_states, input_ids=None):
+    def forward(self, hidden_states, input_ids=None, residual=None):
+        """``(output, logits)``; with a norm and a ``residual`` stream ``(output, logits, hidden_states
+        + residual)``, the output being that of the normalised sum."""
+        hidden_states, rows, total = self._normalised(hidden_states, residual)
         probs, routing_map, expert_indices, logits = self.router(
             hidden_states, input_ids, self._runtime_inputs.padding_mask,
             self._runtime_inputs.accumulate_tokens_per_expert)
         logits = logits.view(-1, logits.shape[-1])
-        return self._experts_and_combine(hidden_states, probs, routing_map, expert_indices), logits
+        output = self._experts_and_combine(hidden_states, probs, routing_map, expert_indices, rows)
+        return (output, logits) if residual is None else (output, logits, total)
 
     def forward_with_logits(self, hidden_states, logits, input_ids=None):
         """Same path with caller-supplied router logits [T, E]."""
+        hidden_states, rows, _ = self._normalised(hidden_states, None)
         probs, routing_map, expert_indices = self.router.routing(
             logits, input_ids, self._runtime_inputs.padding_mask,
             self._runtime_inputs.accumulate_tokens_per_expert)
-        return self._experts_and_combine(hidden_states, probs, routing_map, expert_indices)
+        return self._experts_and_combine(hidden_states, probs, routing_map, expert_indices, rows)

@@ -316,3 +316,30 @@ def experts_forward(tokens, probs, expert_indices, num_experts, ffn, weights, sc
            L.dtype_code(s1.dtype) if s1 is not None else 0, ffn, act, float(limit),
            int(clamp_after), L.ptr(counts), L.ptr(out), L.ptr(ws), nbytes, L.stream(dev))
     return out, counts
+
+
+def mxfp4_forward(experts, tokens, rows, probs, expert_indices):
+    """(output [T, H], per-expert counts) of ``Mxfp4GroupedMLP`` experts for the routed tokens,
+    without gradients: the first product gathers each packed row from its token (``rows``: the
+    tokens in 8 bits, where they are at hand), so neither is permuted in memory. (None, None) for
+    operands that the separate ops refuse or serve another way."""
+    if (checks.enabled() or torch.compiler.is_compiling()
+            or torch._C._are_functorch_transforms_active()
+            or torch.autograd.forward_ad._current_level >= 0):
+        return None, None
+    if tokens.dim() != 2 or expert_indices.dim() != 2:
+        return None, None
+    T, k = expert_indices.shape
+    E = experts.num_local_experts
+    if (T * k == 0 or tokens.shape[0] != T or probs.shape != (T, E)
+            or tokens.dtype != torch.bfloat16):
+        return None, None
+    x = tokens
+    if rows is not None and experts.rows_in_8_bits:
+        x = rows.view(T)
+    packed_rows, token_of_row, packed_probs, counts = route_index(expert_indices, E, probs)
+    y = experts.inference(x, counts, packed_probs, row_map=token_of_row)
+    out = torch.empty_like(tokens)
+    L.call("tt_unpermute_gather", L.ptr(y), L.dtype_code(y.dtype), T, tokens.shape[1], k,
+           L.ptr(packed_rows), None, None, 0, E, L.ptr(out), L.stream(tokens.device))
+    return out, counts
