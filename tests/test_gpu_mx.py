@@ -175,6 +175,26 @@ def test_every_tile_on_integers(hip_ops, m, k, n, mx):
     assert torch.equal(got.cpu(), want), (got.cpu() != want).nonzero()[:8]
 
 
+@pytest.mark.parametrize("m, k, n, gated", [(2000, 4096, 7200, False), (1900, 4224, 3616, True)])
+@pytest.mark.parametrize("mx_out", [False, True])
+def test_largest_tile(hip_ops, m, k, n, gated, mx_out):
+    """Long reductions of rows in 8 bits, against fp32 products of whole numbers (exact)."""
+    x, codes, scales = _integers(m, k, 2 * n if gated else n, True)
+    w = hip_ops.dequantize_mxfp4(codes.to(DEV), scales.to(DEV), torch.float32)
+    a = (x.codes.to(DEV).float() @ w.t()).double()
+    act = F.silu if gated else None
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), activation_func=act, gated=gated,
+                               mx_out=mx_out)
+    y = o_mx.epilogue(a, act, gated)
+    if gated or mx_out:
+        exact = torch.zeros_like(a).cpu()
+        y, a = y.cpu(), a.cpu()
+        bound = _epilogue_bound(a, exact, act or (lambda v: v), gated, 0 * y if mx_out else y)
+        _within_8_bits(got, y, bound) if mx_out else _within(got, y, bound)
+    else:
+        assert torch.equal(got, a.to(BF16))
+
+
 @pytest.mark.parametrize("m, k, n, gated", [(40, 6400, 64, True), (300, 128, 2400, True),
                                             (1700, 128, 2112, True), (40, 6400, 160, False),
                                             (1700, 224, 4224, False)])

@@ -26,8 +26,9 @@ bool few_rows(int64_t M, int64_t K, int64_t W, int E, bool grouped) {
 // 7168 -> 2 x 2048 100 / 70 / 78 / 93, 2048 rows 112 / 119 / 163, 4096 204 / 264 / 325. 128 experts of
 // 2048 -> 2 x 768 with 32 rows each 95 / 96 / 77, with 64 115 / 117 / 104, with 128 148 / 164 / 161; 64
 // of 7168 -> 2 x 2048 with 64 479 / 494 / 528, E4M3 rows 375 / 339 / 363, with 256 625 / 714 / 873.
-MxPlan plan(int64_t M, int64_t K, int64_t W, int E, bool grouped) {
+MxPlan plan(bool x8, int64_t M, int64_t K, int64_t W, int E, bool grouped) {
   const int64_t per = grouped ? M / E : M;
+  if (x8 && K >= 4096 && per >= 384 && tiles(M, W, 256, 256) >= 224) return MxPlan{256, 256, 1};
   if (per > 96 && tiles(M, W, 128, 256) >= 224) return MxPlan{128, 256, 1};
   if (per > 48 && tiles(M, W, 128, 128) >= 160) return MxPlan{128, 128, 1};
   int parts = 1;
@@ -81,7 +82,7 @@ extern "C" int tt_mx_product(const void* x, const uint8_t* x_scales, const int32
   const bool grouped = tokens_per_expert != nullptr;
   if (few_rows(M, K, W, num_experts, grouped) || !tt_mx_tile_takes(p, gated != 0))
     return tt_mx_rows(p, gated != 0, s);
-  MxPlan pl = plan(M, K, W, num_experts, grouped);
+  MxPlan pl = plan(x_scales != nullptr, M, K, W, num_experts, grouped);
   if (pl.parts > 1) {
     if (workspace != nullptr && workspace_bytes >= part_bytes(pl, M, W) &&
         (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)
@@ -97,5 +98,5 @@ extern "C" size_t tt_mx_product_workspace(int64_t M, int64_t K, int64_t N,
   if (M <= 0 || K <= 0 || N <= 0 || grouped) return 0;
   const int64_t W = gated ? 2 * N : N;
   if (few_rows(M, K, W, 1, false)) return 0;
-  return part_bytes(plan(M, K, W, 1, false), M, W);
+  return part_bytes(plan(false, M, K, W, 1, false), M, W);
 }

@@ -3,7 +3,9 @@
 // A block computes 128 rows by 256 weight rows (gated: 128 columns, a wave's blocks of 32 weight
 // rows alternating between gates and their ups), four waves of 64 x 128 each on 32-wide matrix
 // instructions; 128 x 128 or 64 x 128 where the launch would have too few blocks, and dense products
-// of fewer still split their reduction, the parts' sums joined in order by a second kernel. k-tiles go from memory straight to LDS, swizzled so that fragment reads are
+// of fewer still split their reduction, the parts' sums joined in order by a second kernel. Long
+// reductions of E4M3 rows take 256 x 256 in one block of eight waves with three stages: half the reads,
+// and loads two k-tiles ahead. k-tiles go from memory straight to LDS, swizzled so that fragment reads are
 // free of bank conflicts; two blocks share a CU, so that one's matrix instructions cover the
 // other's waits, prologue and epilogue. Rows of 4-bit weights are a quarter of bf16 rows' bytes
 // (half of E4M3 rows'), which is why the tile is twice as wide in them.
@@ -20,13 +22,12 @@
 
 namespace {
 
-constexpr int T_NT = 256;
-
 template <bool MX, int BM_, int BN_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_;           // rows of x and of W
+  static constexpr int NW = BM == 256 ? 8 : 4;       // waves: NW / 2 along the rows, two along W's
   static constexpr int BK = MX ? 128 : 64;
-  static constexpr int STAGES = MX ? (BM == 64 ? 4 : 2) : 3;
+  static constexpr int STAGES = !MX || BM == 256 ? 3 : BM == 64 ? 4 : 2;
   static constexpr int XB = BM * 128;                // rows of x: 128 bytes per k-tile
   static constexpr int WR = MX ? 64 : 32;            // bytes of a weight row per k-tile
   static constexpr int WB = BN * WR;
@@ -36,7 +37,7 @@ struct Tile {
   static constexpr int SB = (BN + (MX ? BM : 0)) * 4;
   static constexpr int SBS = MX ? STAGES : 2;
   static constexpr int LDS = STAGES * STAGE + SBS * SB;
-  static constexpr int MI = BM / 64, NJ = BN / 64;   // 32-wide blocks of a wave
+  static constexpr int MI = BM / NW / 16, NJ = BN / 64;   // 32-wide blocks of a wave
 };
 
 // Bytes 0..3 of a scale word: groups past the reduction's end are 127 (their codes are zeros).
@@ -128,16 +129,16 @@ __device__ __forceinline__ void mx_tile_store(const MxArgs& p, const f32x16 (&ac
 
 // KA: K is a multiple of 128 and scales are 4-byte aligned.
 template <bool MX, bool GATED, bool OUT8, bool KA, int T_BM, int T_BN>
-__global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j, int parts) {
+__global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) void mx_tile_kernel(MxArgs p, int tiles_j, int parts) {
   typedef Tile<MX, T_BM, T_BN> L;
   constexpr int CB = GATED ? T_BN / 2 : T_BN;  // output columns
   constexpr int ES = MX ? 1 : 2;               // bytes of an element of x
-  constexpr int MI = L::MI, NJ = L::NJ;
+  constexpr int MI = L::MI, NJ = L::NJ, NW = L::NW, NT = 64 * NW;
   __shared__ __align__(16) char lds_raw[L::LDS];
   RowTile t;
   int slot = 0, part = 0;  // of a dense product
   if (p.counts != nullptr) {
-    if (!row_tile<T_BM, T_NT>(p.counts, p.E, tiles_j, lds_raw, t)) return;
+    if (!row_tile<T_BM, NT>(p.counts, p.E, tiles_j, lds_raw, t)) return;
     // Counts that sum to more than M end at its last row.
     if (t.seg0 + t.nrows > p.M) t.nrows = p.M - t.seg0;
     if ((int64_t)t.mt * T_BM >= t.nrows) return;
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j,
   const int64_t first = t.seg0 + i0;
   const char* const xbase = static_cast<const char*>(p.x) + (gather ? 0 : first * K * ES);
   const i32x4 rx = make_rsrc(xbase, (gather ? p.src_rows : (rows < T_BM ? rows : T_BM)) * K * ES);
-  constexpr int XQ = T_BM / 32;  // instructions per wave
+  constexpr int XQ = T_BM / 8 / NW;  // instructions per wave
   uint32_t xoff[XQ];
   int xk[XQ];
 #pragma unroll
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j,
     n = n < p.N ? n : p.N - 1;
     return GATED && (r & 32) ? n + p.N : n;
   };
-  constexpr int WQ = L::WB / 4096;  // instructions per wave
+  constexpr int WQ = L::WB / 1024 / NW;  // instructions per wave
   constexpr int CW = L::WR / 16;    // chunks of a row
   uint32_t woff[WQ];
   int wk[WQ];
@@ -200,26 +201,27 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j,
     wk[q] = 32 * c;
     woff[q] = (uint32_t)(weight_row(r) * (K / 2) + 16 * c);
   }
-  // Scales: thread t takes weight row t and row t of x.
+  // Scales: thread t takes weight row t, and row t of x (of eight waves the last four do).
+  const int xt = tid - (NW == 8 ? 256 : 0), xw = wave - (NW == 8 ? 4 : 0);
   const uint32_t soff = (uint32_t)(weight_row(tid < T_BN ? tid : 0) * groups);
   const uint8_t* const xsbase = MX ? p.xs + (gather ? 0 : first * groups) : nullptr;
   const i32x4 rxs = make_rsrc(xsbase, MX ? (gather ? p.src_rows : (rows < T_BM ? rows : T_BM)) * groups : 0);
   uint32_t xsoff = DM_OOB;
-  if (MX && tid < T_BM && tid < rows)
-    xsoff = (uint32_t)((gather ? mx_source_row(p, first + tid) : tid) * groups);
+  if (MX && xt >= 0 && xt < T_BM && xt < rows)
+    xsoff = (uint32_t)((gather ? mx_source_row(p, first + xt) : xt) * groups);
 
   // The words of 128 elements from group g0 on into scale buffer b.
   auto load_scales = [&](int g0, int b) {
     const uint32_t at = lds_addr_of(lds_s) + (uint32_t)(b * L::SB);
     if constexpr (KA) {
       if (wave < T_BN / 64) dma4(soff, advance_rsrc(rs, (uint32_t)g0), at + 256u * wave);
-      if (MX && wave < T_BM / 64)
-        dma4(xsoff, advance_rsrc(rxs, (uint32_t)g0), at + T_BN * 4 + 256u * wave);
+      if (MX && xw >= 0 && xw < T_BM / 64)
+        dma4(xsoff, advance_rsrc(rxs, (uint32_t)g0), at + T_BN * 4 + 256u * xw);
     } else {
       uint32_t* const to = reinterpret_cast<uint32_t*>(lds_raw + L::STAGES * L::STAGE + b * L::SB);
       if (tid < T_BN) to[tid] = scale_word(sbase + soff + g0, groups - g0);
       if constexpr (MX)
-        if (tid < T_BM) to[T_BN + tid] = xsoff == DM_OOB ? 0x7f7f7f7fu : scale_word(xsbase + xsoff + g0, groups - g0);
+        if (xt >= 0 && xt < T_BM) to[T_BN + xt] = xsoff == DM_OOB ? 0x7f7f7f7fu : scale_word(xsbase + xsoff + g0, groups - g0);
     }
   };
   auto issue = [&](int kt, int stage) {
@@ -238,8 +240,8 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j,
       load_scales(kt * (L::BK / MX_GROUP), MX ? stage : (kt >> 1) & 1);
   };
 
-  // Wave w multiplies half w / 2 of the rows by half w % 2 of the weight rows.
-  const int m0 = T_BM / 2 * (wave >> 1), n0 = T_BN / 2 * (wave & 1);
+  // Wave w multiplies part w / 2 of the rows by half w % 2 of the weight rows.
+  const int m0 = 32 * MI * (wave >> 1), n0 = T_BN / 2 * (wave & 1);
   const int r32 = lane & 31, g = lane >> 5;
   f32x16 acc[MI][NJ] = {};
   auto multiply = [&](int kt, int stage) {
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j,
 
   if (parts > 1) {
     // A part of the reduction: the sums as the registers hold them, for mx_join_kernel.
-    float* const to = p.part + ((int64_t)slot * 4 + wave) * (MI * NJ * 1024) + lane * 4;
+    float* const to = p.part + ((int64_t)slot * NW + wave) * (MI * NJ * 1024) + lane * 4;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -346,7 +348,7 @@ __global__ __launch_bounds__(T_NT, 2) void mx_tile_kernel(MxArgs p, int tiles_j,
                                      j0 + (GATED ? n0 / 2 : n0));
 }
 
-// Sum of a dense product's parts, in order, and the epilogue: a wave per wave of a tile.
+// Sum of a dense product's parts, in order, and the epilogue: a wave per wave of a tile's four.
 template <bool GATED, bool OUT8, int T_BM, int T_BN>
 __global__ __launch_bounds__(64) void mx_join_kernel(MxArgs p, int tiles_i, int parts) {
   constexpr int MI = T_BM / 64, NJ = T_BN / 64;
@@ -378,28 +380,33 @@ __global__ __launch_bounds__(64) void mx_join_kernel(MxArgs p, int tiles_i, int 
 
 template <bool MX, bool GATED, bool OUT8, bool KA, int BM, int BN>
 int launch(const MxArgs& p, int parts, hipStream_t s) {
-  constexpr int CB = GATED ? BN / 2 : BN;
+  constexpr int CB = GATED ? BN / 2 : BN, NT = 64 * Tile<MX, BM, BN>::NW;
   const int64_t tiles_j = (p.N + CB - 1) / CB;
   int64_t tiles_i = (p.M + BM - 1) / BM;
   if (p.counts != nullptr) tiles_i = p.M / BM + (p.E < p.M ? p.E : p.M);
   const int64_t blocks = tiles_i * tiles_j * parts;
-  TT_REQUIRE(blocks < (1ll << 31) && tt_grid_ok(blocks, T_NT), "mx product: grid too large");
+  TT_REQUIRE(blocks < (1ll << 31) && tt_grid_ok(blocks, NT), "mx product: grid too large");
   hipLaunchKernelGGL((mx_tile_kernel<MX, GATED, OUT8, KA, BM, BN>), dim3((unsigned)blocks),
-                     dim3(T_NT), 0, s, p, (int)tiles_j, parts);
+                     dim3(NT), 0, s, p, (int)tiles_j, parts);
   const int rc = tt_check_launch("mx_tile");
-  if (rc != TT_OK || parts == 1) return rc;
-  hipLaunchKernelGGL((mx_join_kernel<GATED, OUT8, BM, BN>), dim3((unsigned)(tiles_i * tiles_j * 4)),
-                     dim3(64), 0, s, p, (int)tiles_i, parts);
-  return tt_check_launch("mx_join");
+  if constexpr (BM == 64 && KA) {  // the only tile whose reductions are split
+    if (rc != TT_OK || parts == 1) return rc;
+    hipLaunchKernelGGL((mx_join_kernel<GATED, OUT8, BM, BN>), dim3((unsigned)(tiles_i * tiles_j * 4)),
+                       dim3(64), 0, s, p, (int)tiles_i, parts);
+    return tt_check_launch("mx_join");
+  }
+  return rc;
 }
 
 template <bool MX, bool GATED, bool OUT8>
 int shaped(const MxArgs& p, MxPlan plan, hipStream_t s) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs);
-  if (p.K % 128 != 0 || (at & 3) != 0) return launch<MX, GATED, OUT8, false, 128, 128>(p, plan.parts, s);
+  if (p.K % 128 != 0 || (at & 3) != 0) return launch<MX, GATED, OUT8, false, 128, 128>(p, 1, s);
+  if constexpr (MX)
+    if (plan.bm == 256) return launch<MX, GATED, OUT8, true, 256, 256>(p, 1, s);
   if (plan.bm == 64) return launch<MX, GATED, OUT8, true, 64, 128>(p, plan.parts, s);
-  if (plan.bn == 128) return launch<MX, GATED, OUT8, true, 128, 128>(p, plan.parts, s);
-  return launch<MX, GATED, OUT8, true, 128, 256>(p, plan.parts, s);
+  if (plan.bn == 128) return launch<MX, GATED, OUT8, true, 128, 128>(p, 1, s);
+  return launch<MX, GATED, OUT8, true, 128, 256>(p, 1, s);
 }
 
 template <bool MX, bool GATED>
