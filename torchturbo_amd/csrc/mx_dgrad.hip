@@ -5,22 +5,36 @@
 // need W transposed: a block turns a 64 x 128 piece of codes into bf16 (exact, two codes an
 // instruction, each thread one group with its scale) and writes it to LDS as it lies; the transposing
 // LDS reads then give each lane eight reduction elements of a column. dy goes straight from memory
-// to LDS. Both are double-buffered: the next k-tile's loads are in flight while a tile is
-// multiplied. Every product is exact in fp32; sums run in fp32 and dx is rounded once.
+// to LDS, two stages deep: the next k-tile's loads (W's in registers) are in flight while a tile is
+// multiplied. One copy of W's piece leaves room for three blocks on a CU, which cover one another's
+// barriers (1531 x 2048 -> 5632 66 -> 54 us, 8192 rows of 128 experts 1536 -> 2048 155 -> 127, against
+// two copies and two blocks). Every product is exact in fp32; sums run in fp32 and dx is rounded once.
 #include "mx_gemm.h"
 
 namespace {
 
 constexpr int D_NT = 256, D_BM = 128, D_BN = 128, D_BK = 64;
-constexpr int D_A = D_BM * D_BK * 2, D_B = D_BN * D_BK * 2, D_STAGE = D_A + D_B;
+constexpr int D_A = D_BM * D_BK * 2, D_B = D_BN * D_BK * 2;  // two stages of dy, one of W
+
+// The block's tile of a dense product: eight row tiles at a time, so that the blocks an XCD has at
+// work read few panels of either operand.
+__device__ __forceinline__ void dense_tile(RowTile& t, int64_t M, int tiles_i, int tiles_j) {
+  const int at = xcd_remap(blockIdx.x, tiles_i * tiles_j), group = 8 * tiles_j;
+  const int m0 = at / group * 8, gm = tiles_i - m0 < 8 ? tiles_i - m0 : 8;
+  t.e = 0;
+  t.mt = m0 + at % group % gm;
+  t.nt = at % group / gm;
+  t.seg0 = 0;
+  t.nrows = M;
+}
 
 // ALIGNED: rows of dy are multiples of 16 bytes at 16-byte addresses.
 template <bool ALIGNED>
-__global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
+__global__ __launch_bounds__(D_NT, 3) void mx_dgrad_kernel(
     const char* __restrict__ dy, const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
     char* __restrict__ dx, int64_t M, int64_t K, int64_t N, int E,
     const int64_t* __restrict__ counts, int tiles_j) {
-  __shared__ __align__(16) char lds_raw[2 * D_STAGE];
+  __shared__ __align__(16) char lds_raw[2 * D_A + D_B];
   RowTile t;
   if (counts != nullptr) {
     if (!row_tile<D_BM, D_NT>(counts, E, tiles_j, lds_raw, t)) return;
@@ -28,13 +42,7 @@ __global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
     if (t.seg0 + t.nrows > M) t.nrows = M - t.seg0;
     if ((int64_t)t.mt * D_BM >= t.nrows) return;
   } else {
-    t.e = 0;
-    const int tiles_i = (int)((M + D_BM - 1) / D_BM);
-    const int slot = xcd_remap(blockIdx.x, tiles_i * tiles_j);
-    t.mt = slot % tiles_i;
-    t.nt = slot / tiles_i;
-    t.seg0 = 0;
-    t.nrows = M;
+    dense_tile(t, M, (int)((M + D_BM - 1) / D_BM), tiles_j);
   }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,7 +84,7 @@ __global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
       wv = *reinterpret_cast<const uint4*>(wp + n * (K / 2));
       wsv = wsp[n * groups];
     }
-    lds_char* const a = lds + buf * D_STAGE;
+    lds_char* const a = lds + buf * D_A;
     if constexpr (ALIGNED) {
       const uint32_t base = lds_addr_of(a) + (uint32_t)(4 * wave) * 1024u;
       const i32x4 rk = advance_rsrc(ra, (uint32_t)kt * (D_BK * 2));
@@ -102,8 +110,8 @@ __global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
     }
   };
   // The k-row's chunk c (eight columns) lies in slot c ^ (4 (row % 4)) ^ (row / 4 % 4).
-  auto put = [&](int buf) {
-    lds_char* const b = lds + buf * D_STAGE + D_A + wr * 256;
+  auto put = [&]() {
+    lds_char* const b = lds + 2 * D_A + wr * 256;
     const uint32_t q[4] = {wv.x, wv.y, wv.z, wv.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -124,30 +132,27 @@ __global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
     for (int b = 0; b < 2; ++b) {
       const int col = n0 + 32 * b + 16 * (g & 1) + 4 * (i & 3);
       const int kr = 16 * s + 8 * (g >> 1) + (i >> 2);
-      fb[s][b] = D_A + (uint32_t)(kr * 256 + (col & 7) * 2 +
+      fb[s][b] = 2 * D_A + (uint32_t)(kr * 256 + (col & 7) * 2 +
                                   (((col >> 3) ^ (4 * (kr & 3)) ^ ((kr >> 2) & 3)) << 4));
     }
   }
   f32x16 acc[2][2] = {};
-  if (nkt > 0) {
-    load(0, 0);
-    put(0);
-  }
-  TT_WAIT_VMCNT(0);
-  TT_LDS_BARRIER();
+  if (nkt > 0) load(0, 0);
   for (int kt = 0; kt < nkt; ++kt) {
-    const int buf = kt & 1;
-    if (kt + 1 < nkt) load(kt + 1, buf ^ 1);
-    lds_char* const st = lds + buf * D_STAGE;
+    put();  // the k-tile's codes, loaded during the one before
+    TT_WAIT_VMCNT(0);
+    TT_LDS_BARRIER();
+    if (kt + 1 < nkt) load(kt + 1, (kt & 1) ^ 1);
+    lds_char* const st = lds + (kt & 1) * D_A;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       uint4 b[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(st + fb[s][j]));
+        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds + fb[s][j]));
         // Four k-rows on: 1024 bytes, and the other slot of a pair.
         const i16x4 v1 =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(st + (fb[s][j] ^ 16) + 1024));
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds + (fb[s][j] ^ 16) + 1024));
         const uint2 p0 = __builtin_bit_cast(uint2, v0), p1 = __builtin_bit_cast(uint2, v1);
         b[j] = uint4{p0.x, p0.y, p1.x, p1.y};
       }
@@ -158,8 +163,6 @@ __global__ __launch_bounds__(D_NT, 2) void mx_dgrad_kernel(
         for (int j = 0; j < 2; ++j) acc[i][j] = Mma<TT_BF16>::run(b[j], a, acc[i][j]);
       }
     }
-    if (kt + 1 < nkt) put(buf ^ 1);
-    TT_WAIT_VMCNT(0);
     TT_LDS_BARRIER();
   }
   // The tile through LDS, rows of 256 bytes, chunk c of row r in slot c ^ (r % 16). Register 4 q + e
@@ -209,13 +212,7 @@ __global__ __launch_bounds__(D_NT, 1) void mx_dgrad_big_kernel(
     if (t.seg0 + t.nrows > M) t.nrows = M - t.seg0;
     if ((int64_t)t.mt * G_BM >= t.nrows) return;
   } else {
-    t.e = 0;
-    const int tiles_i = (int)((M + G_BM - 1) / G_BM);
-    const int slot = xcd_remap(blockIdx.x, tiles_i * tiles_j);
-    t.mt = slot % tiles_i;
-    t.nt = slot / tiles_i;
-    t.seg0 = 0;
-    t.nrows = M;
+    dense_tile(t, M, (int)((M + G_BM - 1) / G_BM), tiles_j);
   }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);

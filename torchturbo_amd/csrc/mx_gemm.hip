@@ -22,15 +22,19 @@ bool few_rows(int64_t M, int64_t K, int64_t W, int E, bool grouped) {
 // experts that fill it); then 128 x 128; the smallest, for dense products split until the blocks fill
 // the CUs, while a part keeps 1536 elements (the second kernel and its reads cost some 5 us). us, bf16
 // rows, 128 x 256 / 128 x 128 / 64 x 128 / 64 x 128 in 2 / in 4 parts: 128 x 7168 -> 2 x 2048 98 / 67 /
-// 46 / 30 / 22, 256 rows 99 / 68 / 46 / 31 / 30, 1531 x 5632 -> 2048 92 / 57 / 59 / 61 / 67, 1024 x
+// 44 / 30 / 22, 256 rows 99 / 68 / 46 / 31 / 30, 1531 x 5632 -> 2048 92 / 58 / 54 / 61 / 67, 1024 x
 // 7168 -> 2 x 2048 100 / 70 / 78 / 93, 2048 rows 112 / 119 / 163, 4096 204 / 264 / 325. 128 experts of
 // 2048 -> 2 x 768 with 32 rows each 95 / 96 / 77, with 64 115 / 117 / 104, with 128 148 / 164 / 161; 64
 // of 7168 -> 2 x 2048 with 64 479 / 494 / 528, E4M3 rows 375 / 339 / 363, with 256 625 / 714 / 873.
+// Long reductions of E4M3 rows, 128 x 256 / 256 x 256: 4096 x 4096 -> 2 x 14336 434 / 403, 4096 x 7168
+// -> 2 x 2048 114 / 97, 8192 x 7168 -> 2 x 7168 736 / 657, 4096 x 2048 -> 7168 77 / 83, 64 experts of
+// 7168 -> 2 x 2048 with 512 rows each 1020 / 985, with 256 618 / 653; bf16 rows 769 / 762, 198 / 187,
+// 1320 / 1305, 120 / 132, 1796 / 1876: not worth a kernel.
 MxPlan plan(bool x8, int64_t M, int64_t K, int64_t W, int E, bool grouped) {
   const int64_t per = grouped ? M / E : M;
   if (x8 && K >= 4096 && per >= 384 && tiles(M, W, 256, 256) >= 224) return MxPlan{256, 256, 1};
   if (per > 96 && tiles(M, W, 128, 256) >= 224) return MxPlan{128, 256, 1};
-  if (per > 48 && tiles(M, W, 128, 128) >= 160) return MxPlan{128, 128, 1};
+  if (per > 48 && tiles(M, W, 128, 128) >= 224) return MxPlan{128, 128, 1};
   int parts = 1;
   if (!grouped)
     while (parts < 4 && tiles(M, W, 64, 128) * parts * 2 <= 256 && K / (parts * 2) >= 1536) parts *= 2;

@@ -25,7 +25,8 @@ namespace {
 template <bool MX, int BM_, int BN_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_;           // rows of x and of W
-  static constexpr int NW = BM == 256 ? 8 : 4;       // waves: NW / 2 along the rows, two along W's
+  static constexpr int NW = BM == 256 ? 8 : 4;       // waves: MW along the rows, two along W's
+  static constexpr int MW = BM == 256 ? 4 : 2, WN = BN / 2;
   static constexpr int BK = MX ? 128 : 64;
   static constexpr int STAGES = !MX || BM == 256 ? 3 : BM == 64 ? 4 : 2;
   static constexpr int XB = BM * 128;                // rows of x: 128 bytes per k-tile
@@ -37,7 +38,7 @@ struct Tile {
   static constexpr int SB = (BN + (MX ? BM : 0)) * 4;
   static constexpr int SBS = MX ? STAGES : 2;
   static constexpr int LDS = STAGES * STAGE + SBS * SB;
-  static constexpr int MI = BM / NW / 16, NJ = BN / 64;   // 32-wide blocks of a wave
+  static constexpr int MI = BM / MW / 32, NJ = WN / 32;   // 32-wide blocks of a wave
 };
 
 // Bytes 0..3 of a scale word: groups past the reduction's end are 127 (their codes are zeros).
@@ -136,7 +137,7 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
   constexpr int MI = L::MI, NJ = L::NJ, NW = L::NW, NT = 64 * NW;
   __shared__ __align__(16) char lds_raw[L::LDS];
   RowTile t;
-  int slot = 0, part = 0;  // of a dense product
+  int tile = 0, part = 0;  // of a dense product
   if (p.counts != nullptr) {
     if (!row_tile<T_BM, NT>(p.counts, p.E, tiles_j, lds_raw, t)) return;
     // Counts that sum to more than M end at its last row.
@@ -145,10 +146,14 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
   } else {
     t.e = 0;
     const int tiles_i = (int)((p.M + T_BM - 1) / T_BM);
-    slot = xcd_remap(blockIdx.x, tiles_i * tiles_j * parts);
+    const int slot = xcd_remap(blockIdx.x, tiles_i * tiles_j * parts);
     part = slot % parts;
-    t.mt = slot / parts % tiles_i;
-    t.nt = slot / parts / tiles_i;
+    // Eight row tiles at a time: the blocks that an XCD has at work read few panels of either operand.
+    const int at = slot / parts, group = 8 * tiles_j, m0 = at / group * 8;
+    const int gm = tiles_i - m0 < 8 ? tiles_i - m0 : 8;
+    t.mt = m0 + at % group % gm;
+    t.nt = at % group / gm;
+    tile = t.nt * tiles_i + t.mt;
     t.seg0 = 0;
     t.nrows = p.M;
   }
@@ -240,8 +245,8 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
       load_scales(kt * (L::BK / MX_GROUP), MX ? stage : (kt >> 1) & 1);
   };
 
-  // Wave w multiplies part w / 2 of the rows by half w % 2 of the weight rows.
-  const int m0 = 32 * MI * (wave >> 1), n0 = T_BN / 2 * (wave & 1);
+  // A wave multiplies its part of the rows by its part of the weight rows.
+  const int m0 = 32 * MI * (wave >> 1), n0 = L::WN * (wave & 1);
   const int r32 = lane & 31, g = lane >> 5;
   f32x16 acc[MI][NJ] = {};
   auto multiply = [&](int kt, int stage) {
@@ -331,7 +336,7 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
 
   if (parts > 1) {
     // A part of the reduction: the sums as the registers hold them, for mx_join_kernel.
-    float* const to = p.part + ((int64_t)slot * NW + wave) * (MI * NJ * 1024) + lane * 4;
+    float* const to = p.part + (((int64_t)tile * parts + part) * NW + wave) * (MI * NJ * 1024) + lane * 4;
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
