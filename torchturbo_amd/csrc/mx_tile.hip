@@ -50,11 +50,11 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* p, int left) {
 }
 
 // Epilogue of a wave's MI x NJ blocks: register 4 q + e of lane l in block (i, j) is row
-// m0 + 32 i + l % 32 of the tile's (`rows` valid, the first is output row `first`), weight row
+// m0 + MS i + l % 32 of the tile's (`rows` valid, the first is output row `first`), weight row
 // 32 j + 8 q + 4 (l / 32) + e of the wave's; gated: odd blocks are the ups of the even ones. Output
 // columns from c0. Rows go through the wave's own LDS at `out`, RB bytes each, chunk c of row r in
 // slot c ^ (r % (RB / 16)).
-template <bool GATED, bool OUT8, int MI, int NJ>
+template <bool GATED, bool OUT8, int MI, int NJ, int MS>
 __device__ __forceinline__ void mx_tile_store(const MxArgs& p, const f32x16 (&acc)[MI][NJ],
                                               lds_char* out, int64_t first, int64_t rows, int m0,
                                               int64_t c0) {
@@ -64,8 +64,8 @@ __device__ __forceinline__ void mx_tile_store(const MxArgs& p, const f32x16 (&ac
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int r = 32 * i + r32;
-    const int64_t row = first + m0 + r;
-    const bool valid = m0 + r < rows;
+    const int64_t row = first + m0 + MS * i + r32;
+    const bool valid = m0 + MS * i + r32 < rows;
     float f = 1.f;
     if (p.probs != nullptr && valid) f = load_as_f32(p.probs, p.pdt, row);
 #pragma unroll
@@ -113,10 +113,10 @@ __device__ __forceinline__ void mx_tile_store(const MxArgs& p, const f32x16 (&ac
   const bool whole = OUT8 || (p.N & 7) == 0;
 #pragma unroll
   for (int q = 0; q < MI * LR / 2; ++q) {
-    const int r = q * (64 / LR) + lane / LR;
-    if (m0 + r >= rows || col >= p.N) continue;
+    const int r = q * (64 / LR) + lane / LR, at = m0 + MS * (r >> 5) + (r & 31);
+    if (at >= rows || col >= p.N) continue;
     const uint4 v = read_k(out, (uint32_t)(r * RB + (((lane % LR) ^ (r & (LR - 1))) << 4)));
-    char* const to = static_cast<char*>(p.y) + ((first + m0 + r) * p.N + col) * (OUT8 ? 1 : 2);
+    char* const to = static_cast<char*>(p.y) + ((first + at) * p.N + col) * (OUT8 ? 1 : 2);
     if (whole) {
       *reinterpret_cast<uint4*>(to) = v;
     } else {
@@ -245,28 +245,31 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
       load_scales(kt * (L::BK / MX_GROUP), MX ? stage : (kt >> 1) & 1);
   };
 
-  // A wave multiplies its part of the rows by its part of the weight rows.
-  const int m0 = 32 * MI * (wave >> 1), n0 = L::WN * (wave & 1);
+  // A wave multiplies rows m0 + MS i .. + 31 by its half of the weight rows: the rows of a partial
+  // tile spread over all waves, and blocks i past the last one are left out.
+  constexpr int MS = 32 * L::MW;
+  const int m0 = 32 * (wave >> 1), n0 = L::WN * (wave & 1);
   const int r32 = lane & 31, g = lane >> 5;
   f32x16 acc[MI][NJ] = {};
-  auto multiply = [&](int kt, int stage) {
+  auto multiply = [&](int kt, int stage, auto blocks) {
+    constexpr int MN = decltype(blocks)::value;
     lds_char* const st = lds + stage * L::STAGE;
     const char* const sw = lds_raw + L::STAGES * L::STAGE + (MX ? stage : (kt >> 1) & 1) * L::SB;
     const int shift = MX ? 8 * g : 8 * (2 * (kt & 1) + g);
-    uint32_t ws[NJ], xs[MI];
+    uint32_t ws[NJ], xs[MN];
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
       ws[j] = *reinterpret_cast<const uint32_t*>(sw + 4 * (n0 + 32 * j + r32)) >> shift;
     if constexpr (MX) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
-        xs[i] = *reinterpret_cast<const uint32_t*>(sw + 4 * (T_BN + m0 + 32 * i + r32)) >> shift;
+      for (int i = 0; i < MN; ++i)
+        xs[i] = *reinterpret_cast<const uint32_t*>(sw + 4 * (T_BN + m0 + MS * i + r32)) >> shift;
       auto step = [&](auto sc) {
         constexpr int s = decltype(sc)::value;
-        uint4 w[NJ], x[MI][2];
+        uint4 w[NJ], x[MN][2];
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          const int r = m0 + 32 * i + r32;
+        for (int i = 0; i < MN; ++i) {
+          const int r = m0 + MS * i + r32;
           const uint32_t at = (uint32_t)(r * 128), sz = (uint32_t)((r >> 1) & 7);
           x[i][0] = read_k(st, at + (((4 * s + g) ^ sz) << 4));
           x[i][1] = read_k(st, at + (((4 * s + 2 + g) ^ sz) << 4));
@@ -279,7 +282,7 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int i = 0; i < MI; ++i)
+          for (int i = 0; i < MN; ++i)
             acc[i][j] = mx_mma32<2 * s, 2 * s>(w[j], x[i][0], x[i][1], ws[j], xs[i], acc[i][j]);
       };
       step(std::integral_constant<int, 0>{});
@@ -294,10 +297,10 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        uint4 x[MI];
+        uint4 x[MN];
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          const int r = m0 + 32 * i + r32;
+        for (int i = 0; i < MN; ++i) {
+          const int r = m0 + MS * i + r32;
           x[i] = read_k(st, (uint32_t)(r * 128 + (((4 * g + s) ^ ((r >> 1) & 7)) << 4)));
         }
 #pragma unroll
@@ -305,7 +308,7 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
           const uint32_t q = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w;
           const uint4 a = mx_bf16x8(q, ws[j]);
 #pragma unroll
-          for (int i = 0; i < MI; ++i) acc[i][j] = Mma<TT_BF16>::run(a, x[i], acc[i][j]);
+          for (int i = 0; i < MN; ++i) acc[i][j] = Mma<TT_BF16>::run(a, x[i], acc[i][j]);
         }
       }
     }
@@ -319,20 +322,24 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
 #pragma unroll
   for (int s = 0; s < L::STAGES - 1; ++s)
     if (k0 + s < k1) issue(k0 + s, s);
-  int stage = 0;
-  for (int kt = k0; kt < k1; ++kt) {
-    // k-tile kt has landed once at most the loads of later ones are outstanding, at least the x and
-    // W pieces of each.
-    const int later = KA ? k1 - 1 - kt : 0;
-    if (L::STAGES >= 4 && later >= 2) TT_WAIT_VMCNT(2 * (XQ + WQ));
-    else if (L::STAGES >= 3 && later >= 1) TT_WAIT_VMCNT(XQ + WQ);
-    else TT_WAIT_VMCNT(0);
-    TT_LDS_BARRIER();
-    const int next = stage == 0 ? L::STAGES - 1 : stage - 1;  // the stage of kt - 1
-    if (kt + L::STAGES - 1 < k1) issue(kt + L::STAGES - 1, next);
-    multiply(kt, stage);
-    stage = stage == L::STAGES - 1 ? 0 : stage + 1;
-  }
+  auto run = [&](auto blocks) {
+    int stage = 0;
+    for (int kt = k0; kt < k1; ++kt) {
+      // k-tile kt has landed once at most the loads of later ones are outstanding, at least the x and
+      // W pieces of each.
+      const int later = KA ? k1 - 1 - kt : 0;
+      if (L::STAGES >= 4 && later >= 2) TT_WAIT_VMCNT(2 * (XQ + WQ));
+      else if (L::STAGES >= 3 && later >= 1) TT_WAIT_VMCNT(XQ + WQ);
+      else TT_WAIT_VMCNT(0);
+      TT_LDS_BARRIER();
+      const int next = stage == 0 ? L::STAGES - 1 : stage - 1;  // the stage of kt - 1
+      if (kt + L::STAGES - 1 < k1) issue(kt + L::STAGES - 1, next);
+      multiply(kt, stage, blocks);
+      stage = stage == L::STAGES - 1 ? 0 : stage + 1;
+    }
+  };
+  if (MI > 1 && rows <= MS) run(std::integral_constant<int, 1>{});
+  else run(std::integral_constant<int, MI>{});
 
   if (parts > 1) {
     // A part of the reduction: the sums as the registers hold them, for mx_join_kernel.
@@ -349,7 +356,7 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
     return;
   }
   TT_LDS_BARRIER();  // every wave is past its fragment reads
-  mx_tile_store<GATED, OUT8, MI, NJ>(p, acc, lds + wave * (MI * NJ * 2048), t.seg0 + i0, rows, m0,
+  mx_tile_store<GATED, OUT8, MI, NJ, MS>(p, acc, lds + wave * (MI * NJ * 2048), t.seg0 + i0, rows, m0,
                                      j0 + (GATED ? n0 / 2 : n0));
 }
 
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(64) void mx_join_kernel(MxArgs p, int tiles_i, int 
         }
   }
   const int n0 = T_BN / 2 * (wave & 1);
-  mx_tile_store<GATED, OUT8, MI, NJ>(p, acc, (lds_char*)lds_raw, i0, p.M - i0, T_BM / 2 * (wave >> 1),
+  mx_tile_store<GATED, OUT8, MI, NJ, 64>(p, acc, (lds_char*)lds_raw, i0, p.M - i0, 32 * (wave >> 1),
                                      j0 + (GATED ? n0 / 2 : n0));
 }
 
