@@ -8,14 +8,14 @@ int64_t tiles(int64_t rows, int64_t cols, int bm, int bn) {
 }
 
 // Whether a product takes the kernel of few rows, which reads x once per weight tile from memory.
-// us, rows / tiles (the plan's), bf16 rows: dense 17 x 7168 -> 2 x 2048 17.6 / 21.1, 24 x 2048 ->
-// 7168 8.6 / 15.0, 64 x 7168 -> 2 x 2048 21.9 / 21.3, 64 x 4096 -> 2 x 14336 79 / 31; 128 experts
-// of 2048 -> 2 x 768 with 512 rows 59 / 57, with 1024 74 / 64, of 768 -> 2048 with 512 28 / 40; 64 of
-// 7168 -> 2 x 2048 with 256 rows 279 / 263. E4M3 rows: 15.2 / 15.4, 7.4 / 9.9, 18.7 / 15.7, 66 / 24;
-// 54 / 46, 68 / 53, 26 / 32; 269 / 201.
-bool few_rows(int64_t M, int64_t K, int64_t W, int E, bool grouped) {
-  if (grouped) return M <= (int64_t)E * (K <= 1024 ? 8 : 3);
-  return M <= 16 || (M <= 32 && W < 512 * 16);
+// us, rows / tiles (the plan's), bf16 rows: dense 17 x 7168 -> 2 x 2048 14.6 / 20.5, 64 x 7168 -> 2 x
+// 2048 19.3 / 20.8, 24 x 2048 -> 7168 7.3 / 16.1, 32 x 4096 -> 2 x 14336 44 / 31; 128 experts of 2048 ->
+// 2 x 768 with 512 rows 50 / 57, with 768 53 / 63, with 1024 62 / 65, of 768 -> 2048 with 512 31 / 32,
+// with 1024 38 / 36; 64 of 7168 -> 2 x 2048 with 256 rows 224 / 273. E4M3 rows: 10.9 / 15.5, 13.2 / 15.9,
+// 6.0 / 10.0, 31 / 22; 45 / 46, 47 / 52, 55 / 52, 29 / 32, 35 / 36; 205 / 201.
+bool few_rows(int64_t M, int64_t W, int E, bool grouped) {
+  if (grouped) return M <= (int64_t)6 * E;
+  return M <= 16 || (M <= 64 && W < 512 * 16);
 }
 
 // Tile and parts. The largest tile reads least, but wants a block for nearly each of the 256 CUs (and
@@ -84,7 +84,7 @@ extern "C" int tt_mx_product(const void* x, const uint8_t* x_scales, const int32
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t W = gated ? 2 * N : N;
   const bool grouped = tokens_per_expert != nullptr;
-  if (few_rows(M, K, W, num_experts, grouped) || !tt_mx_tile_takes(p, gated != 0))
+  if (few_rows(M, W, num_experts, grouped) || !tt_mx_tile_takes(p, gated != 0))
     return tt_mx_rows(p, gated != 0, s);
   MxPlan pl = plan(x_scales != nullptr, M, K, W, num_experts, grouped);
   if (pl.parts > 1) {
@@ -101,6 +101,6 @@ extern "C" size_t tt_mx_product_workspace(int64_t M, int64_t K, int64_t N,
                                           int32_t grouped, int32_t gated) {
   if (M <= 0 || K <= 0 || N <= 0 || grouped) return 0;
   const int64_t W = gated ? 2 * N : N;
-  if (few_rows(M, K, W, 1, false)) return 0;
+  if (few_rows(M, W, 1, false)) return 0;
   return part_bytes(plan(false, M, K, W, 1, false), M, W);
 }
