@@ -467,6 +467,35 @@ def test_experts_of_many_rows_and_offsets_past_32_bits(hip_ops):
     assert torch.equal(dx.cpu(), (dy[:, -64:].double().cpu() @ w).to(BF16))
 
 
+@pytest.mark.parametrize("mx", [False, True])
+def test_one_expert_of_rows_past_32_bits(hip_ops, mx):
+    """Few rows an expert, all of them one expert's: 4 GiB lie behind its first rows."""
+    m, n, k = 8208 * (2 if mx else 1), 8, 1 << 18
+    e = m // 6
+    codes = torch.full((e, n, k // 2), 0x22, dtype=torch.uint8, device=DEV)  # ones
+    scales = torch.full((e, n, k // 32), 127, dtype=torch.uint8, device=DEV)
+    x = torch.ones((m, k), dtype=BF16, device=DEV)
+    if mx:
+        x = MxRows(x.to(torch.float8_e4m3fn), torch.full((m, k // 32), 127, dtype=torch.uint8, device=DEV))
+    y = hip_ops.grouped_matmul_mxfp4(x, codes, scales, [0] * (e - 1) + [m])
+    assert bool((y == float(k)).all())
+    y = hip_ops.grouped_matmul_mxfp4(x, codes, scales, [m - 16] + [0] * (e - 2) + [16])
+    assert bool((y == float(k)).all())
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_rows_gathered_past_32_bits(hip_ops, m):
+    n, k, source = 64, 1024, (1 << 21) + 64
+    few, codes, scales = _integers(64, k, 2 * n, False, seed=3)
+    x = torch.zeros((source, k), dtype=BF16, device=DEV)
+    x[-64:] = few.to(DEV)
+    pick = torch.randint(0, 64, (m,), generator=torch.Generator().manual_seed(m))
+    row_map = (pick + source - 64).to(torch.int32).to(DEV)
+    w = codes.view(2, n, -1), scales.view(2, n, -1)
+    y = hip_ops.grouped_matmul_mxfp4(x, *(t.to(DEV) for t in w), [m - 7, 7], row_map=row_map)
+    assert torch.equal(y.cpu(), o_mx.grouped(few[pick], *w, torch.tensor([m - 7, 7])).to(BF16))
+
+
 def test_more_experts_than_rows_and_repeats(hip_ops):
     e, k, n = 1000, 64, 32
     x, codes, scales = _integers(10, k, n * e, False)

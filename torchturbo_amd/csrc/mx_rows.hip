@@ -82,7 +82,8 @@ __global__ __launch_bounds__(64 * W) void mx_rows_kernel(MxArgs p, int tiles_j) 
   using Off = typename Operand<NEAR>::Off;
   const int64_t width = (GATED ? 2 : 1) * p.N;
   const bool gather = p.arow != nullptr;
-  const int64_t first = gather ? 0 : t.seg0 + i0, held = gather ? p.src_rows : rows;
+  const int64_t first = gather ? 0 : t.seg0 + i0;
+  const int64_t held = gather ? p.src_rows : (rows < 16 * MB ? rows : 16 * MB);
   constexpr int ES = MX ? 1 : 2;
   const Operand<NEAR> w(p.w + (int64_t)t.e * width * (K / 2), width * (K / 2)),
       ws(p.ws + (int64_t)t.e * width * groups, width * groups),
