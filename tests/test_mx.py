@@ -147,6 +147,19 @@ def test_refusals(call, message):
         call()
 
 
+def test_rows_in_8_bits_have_no_gradient():
+    """Codes that ask for one (or a transform that follows them) are refused before any product."""
+    rows = MxRows(R8.codes.clone().requires_grad_(), R8.scales)
+    calls = (lambda r: HipLinearMxfp4()(r, Q, S),
+             lambda r: HipGroupedMatmulMxfp4()(r, QE, SE, [4, 0, 0]))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="rows in 8 bits have no gradient"):
+            call(rows)
+        with torch.autograd.forward_ad.dual_level(), torch.no_grad(), \
+                pytest.raises(RuntimeError, match="rows in 8 bits have no gradient"):
+            call(R8)
+
+
 AT = ctypes.c_void_p(4096)  # an address that no kernel ever gets: every such call is refused
 ODD = ctypes.c_void_p(4104)
 

@@ -35,7 +35,6 @@ from .available import hip_available
 from .linear import ACTIVATIONS, FLOATS, _autograd_sees, _rows
 
 
-
 def _aligned(t, size):
     """``t``, contiguous at a multiple of ``size`` bytes (copied where a view is not)."""
     if not t.is_contiguous():
@@ -164,8 +163,11 @@ class HipLinearMxfp4(OpImpl):
         if mx_out and n % GROUP:
             raise ValueError(f"{op}: outputs in 8 bits are whole groups of {GROUP}, got {n}")
         values, xs, lead = check_rows(op, x, 2 * codes.shape[1])
+        sees = _autograd_sees(values)
+        if sees and xs is not None:
+            raise _no_gradient(op, "rows in 8 bits")
         _device(values, xs, codes, scales)
-        if _autograd_sees(values):
+        if sees:
             if mx_out:
                 raise _no_gradient(op, "outputs in 8 bits")
             y = MxProduct.apply(values, codes, scales, None)
@@ -215,13 +217,14 @@ class HipGroupedMatmulMxfp4(OpImpl):
                 raise ValueError(f"{op}: probs must be a float tensor of shape [{m}], got "
                                  f"{probs.dtype} {list(probs.shape)}")
             probs = probs.reshape(-1).contiguous()
+        sees = _autograd_sees(values, probs)
+        if sees and xs is not None:
+            raise _no_gradient(op, "rows in 8 bits")
         dev = _device(values, xs, codes, scales, row_map, probs)
         counts = device_counts(tokens_per_expert, experts, dev, m=m)
-        if _autograd_sees(values, probs):
+        if sees:
             if mx_out:
                 raise _no_gradient(op, "outputs in 8 bits")
-            if xs is not None:
-                raise _no_gradient(op, "rows in 8 bits")
             if row_map is not None:
                 raise _no_gradient(op, "rows taken through row_map")
             y = MxProduct.apply(values, codes, scales, counts)
