@@ -4,14 +4,15 @@
 // rows alternating between gates and their ups), four waves of 64 x 128 each on 32-wide matrix
 // instructions; 128 x 128 or 64 x 128 where the launch would have too few blocks, and dense products
 // of fewer still split their reduction, the parts' sums joined in order by a second kernel. Long
-// reductions of E4M3 rows take 256 x 256 in one block of eight waves with three stages: half the reads,
-// and loads two k-tiles ahead. k-tiles go from memory straight to LDS, swizzled so that fragment reads are
-// free of bank conflicts; two blocks share a CU, so that one's matrix instructions cover the
-// other's waits, prologue and epilogue. Rows of 4-bit weights are a quarter of bf16 rows' bytes
-// (half of E4M3 rows'), which is why the tile is twice as wide in them.
+// reductions of E4M3 rows take 256 x 256 in one block of eight waves with three stages: half the
+// reads, and loads two k-tiles ahead. k-tiles go from memory straight to LDS, swizzled so that
+// fragment reads are free of bank conflicts; otherwise two blocks share a CU, so that one's matrix
+// instructions cover the other's waits, prologue and epilogue. Rows of 4-bit weights are a quarter of
+// bf16 rows' bytes (half of E4M3 rows'), which is why the tile is twice as wide in them.
 //
-// E4M3 rows: k-tiles of 128, two stages (four of the smallest tile); codes are multiplied as they are, with the groups' bytes as
-// the instruction's scales (a row's four bytes of a k-tile are one word in LDS).
+// E4M3 rows: k-tiles of 128, two stages (four of the smallest tile); codes are multiplied as they
+// are, with the groups' bytes as the instruction's scales (a row's four bytes of a k-tile are one
+// word in LDS).
 // bf16 rows: k-tiles of 64, three stages; a lane's 16 bytes of codes are one group of a weight row,
 // which it turns into four bf16 fragments with the group's scale. The order of the reduction
 // within a k-tile is free as long as both operands agree: lane half g of step s takes elements

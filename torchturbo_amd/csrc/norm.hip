@@ -8,8 +8,8 @@
 //
 //   dh = rho (a - xh mean(a xh)) + g_sum,  dw = sum over rows of gy xh.
 //
-// All of it is bound by memory: every tensor is read or written once (4.2 to 5.1 TB/s; a large copy
-// on this card reaches 5.2). A row stays in the registers of its threads between the sum of squares
+// All of it is bound by memory: every tensor is read or written once (4.4 to 4.9 TB/s; a large copy
+// on this card reaches 5.1). A row stays in the registers of its threads between the sum of squares
 // and the product: a wave per row up to 2048 features, 256 threads to 8192, 1024 to 16384; longer
 // rows are read twice. Blocks go on to further rows with the weight kept, so that it is read once per
 // block, and dw is summed in registers: one partial row per block, joined by a second kernel in the
