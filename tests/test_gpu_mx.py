@@ -195,6 +195,28 @@ def test_largest_tile(hip_ops, m, k, n, gated, mx_out):
         assert torch.equal(got, a.to(BF16))
 
 
+@pytest.mark.parametrize("m, k, n, gated", [(1531, 1152, 2048, False), (700, 1664, 2112, True),
+                                            (1980, 1024, 2000, False), (110, 1152, 20480, False)])
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("mx_out", [False, True])
+def test_reduction_shared_by_two_sets_of_waves(hip_ops, m, k, n, gated, mx, mx_out):
+    """Odd and even numbers of steps, partial tiles; against fp32 products of whole numbers (exact)."""
+    n -= n % 32 if mx_out else 0
+    x, codes, scales = _integers(m, k, 2 * n if gated else n, mx)
+    w = hip_ops.dequantize_mxfp4(codes.to(DEV), scales.to(DEV), torch.float32)
+    a = (o_mx.values_of(x).float().to(DEV) @ w.t()).double()
+    act = F.silu if gated else None
+    got = hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), activation_func=act, gated=gated,
+                               mx_out=mx_out)
+    y = o_mx.epilogue(a, act, gated)
+    if gated or mx_out:
+        y, a = y.cpu(), a.cpu()
+        bound = _epilogue_bound(a, torch.zeros_like(a), act or (lambda v: v), gated, 0 * y if mx_out else y)
+        _within_8_bits(got, y, bound) if mx_out else _within(got, y, bound)
+    else:
+        assert torch.equal(got, a.to(BF16))
+
+
 @pytest.mark.parametrize("m, k, n, gated", [(40, 6400, 64, True), (300, 128, 2400, True),
                                             (1700, 128, 2112, True), (40, 6400, 160, False),
                                             (1700, 224, 4224, False)])

@@ -23,9 +23,10 @@ struct MxArgs {
   float* part;            // sums of the parts of a split reduction
 };
 
-// Tile of a product of many rows, and the parts that its reduction is split into (1: none).
+// Tile of a product of many rows, the parts that its reduction is split into (1: none), and the sets
+// of waves that share a block's reduction.
 struct MxPlan {
-  int bm, bn, parts;
+  int bm, bn, parts, halves = 1;
 };
 
 namespace {

@@ -26,6 +26,11 @@ bool few_rows(int64_t M, int64_t W, int E, bool grouped) {
 // 7168 -> 2 x 2048 100 / 70 / 78 / 93, 2048 rows 112 / 119 / 163, 4096 204 / 264 / 325. 128 experts of
 // 2048 -> 2 x 768 with 32 rows each 95 / 96 / 77, with 64 115 / 117 / 104, with 128 148 / 164 / 161; 64
 // of 7168 -> 2 x 2048 with 64 479 / 494 / 528, E4M3 rows 375 / 339 / 363, with 256 625 / 714 / 873.
+// Dense products of 160 to 256 tiles of 128 x 128 (one for most CUs), two sets of waves with half of the
+// reduction each / the better of 128 x 128 and 64 x 128: 1531 x 5632 -> 2048 47 / 56, E4M3 rows 34 / 39,
+// 2048 x 2048 -> 2048 23.5 / 24.2, 14.5 / 16.3, 1024 x 7168 -> 2 x 2048 67 / 75, 44 / 50, 128 x 4096 -> 2 x
+// 14336 42 / 48, 31 / 35, 1531 x 768 -> 2048 11.6 / 11.7; with 128 tiles (1024 x 5632 -> 2048) 45 / 39,
+// with 512 (2048 x 7168 -> 2 x 2048) 129 / 119.
 // Long reductions of E4M3 rows, 128 x 256 / 256 x 256: 4096 x 4096 -> 2 x 14336 434 / 403, 4096 x 7168
 // -> 2 x 2048 114 / 97, 8192 x 7168 -> 2 x 7168 736 / 657, 4096 x 2048 -> 7168 77 / 83, 64 experts of
 // 7168 -> 2 x 2048 with 512 rows each 1020 / 985, with 256 618 / 653; bf16 rows 769 / 762, 198 / 187,
@@ -34,7 +39,9 @@ MxPlan plan(bool x8, int64_t M, int64_t K, int64_t W, int E, bool grouped) {
   const int64_t per = grouped ? M / E : M;
   if (x8 && K >= 4096 && per >= 384 && tiles(M, W, 256, 256) >= 224) return MxPlan{256, 256, 1};
   if (per > 96 && tiles(M, W, 128, 256) >= 224) return MxPlan{128, 256, 1};
-  if (per > 48 && tiles(M, W, 128, 128) >= 224) return MxPlan{128, 128, 1};
+  const int64_t t = tiles(M, W, 128, 128);
+  if (!grouped && per > 96 && K >= 1024 && t >= 160 && t <= 256) return MxPlan{128, 128, 1, 2};
+  if (per > 48 && t >= 224) return MxPlan{128, 128, 1};
   int parts = 1;
   if (!grouped)
     while (parts < 4 && tiles(M, W, 64, 128) * parts * 2 <= 256 && K / (parts * 2) >= 1536) parts *= 2;

@@ -3,7 +3,8 @@
 // A block computes 128 rows by 256 weight rows (gated: 128 columns, a wave's blocks of 32 weight
 // rows alternating between gates and their ups), four waves of 64 x 128 each on 32-wide matrix
 // instructions; 128 x 128 or 64 x 128 where the launch would have too few blocks, and dense products
-// of fewer still split their reduction, the parts' sums joined in order by a second kernel. Long
+// of fewer still split their reduction, the parts' sums joined in order by a second kernel. Where
+// 128 x 128 gives most CUs one block, two sets of four waves take half of the reduction each. Long
 // reductions of E4M3 rows take 256 x 256 in one block of eight waves with three stages: half the
 // reads, and loads two k-tiles ahead. k-tiles go from memory straight to LDS, swizzled so that
 // fragment reads are free of bank conflicts; otherwise two blocks share a CU, so that one's matrix
@@ -129,18 +130,21 @@ __device__ __forceinline__ void mx_tile_store(const MxArgs& p, const f32x16 (&ac
   }
 }
 
-// KA: K is a multiple of 128 and scales are 4-byte aligned.
-template <bool MX, bool GATED, bool OUT8, bool KA, int T_BM, int T_BN>
-__global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) void mx_tile_kernel(MxArgs p, int tiles_j, int parts) {
+// KA: K is a multiple of 128 and scales are 4-byte aligned. KS = 2: two sets of waves with stages of their
+// own take a half of the reduction each, and exchange halves of their sums at its end.
+template <bool MX, bool GATED, bool OUT8, bool KA, int T_BM, int T_BN, int KS>
+__global__ __launch_bounds__((T_BM == 256 || KS == 2 ? 512 : 256), (T_BM == 256 || KS == 2 ? 1 : 2))
+void mx_tile_kernel(MxArgs p, int tiles_j, int parts) {
   typedef Tile<MX, T_BM, T_BN> L;
   constexpr int CB = GATED ? T_BN / 2 : T_BN;  // output columns
   constexpr int ES = MX ? 1 : 2;               // bytes of an element of x
-  constexpr int MI = L::MI, NJ = L::NJ, NW = L::NW, NT = 64 * NW;
-  __shared__ __align__(16) char lds_raw[L::LDS];
+  constexpr int MI = L::MI, NJ = L::NJ, NW = L::NW, NT = 64 * NW * KS;
+  static_assert(KS == 1 || (KA && MI == 2 && NW == 4), "halves exchange one of two blocks of rows");
+  __shared__ __align__(16) char lds_block[KS * L::LDS];
   RowTile t;
   int tile = 0, part = 0;  // of a dense product
   if (p.counts != nullptr) {
-    if (!row_tile<T_BM, NT>(p.counts, p.E, tiles_j, lds_raw, t)) return;
+    if (!row_tile<T_BM, NT>(p.counts, p.E, tiles_j, lds_block, t)) return;
     // Counts that sum to more than M end at its last row.
     if (t.seg0 + t.nrows > p.M) t.nrows = p.M - t.seg0;
     if ((int64_t)t.mt * T_BM >= t.nrows) return;
@@ -158,7 +162,9 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
     t.seg0 = 0;
     t.nrows = p.M;
   }
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int half = KS == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  const int tid = threadIdx.x - 256 * half, lane = tid & 63;
+  char* const lds_raw = lds_block + half * L::LDS;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t K = p.K, i0 = (int64_t)t.mt * T_BM, j0 = (int64_t)t.nt * CB;
   const int64_t rows = t.nrows - i0;  // valid rows of the tile, at least one
@@ -317,15 +323,19 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
 
   // This block's k-tiles: from an even one where the words of scales span two.
   const int pairs = MX ? nkt : (nkt + 1) / 2;
-  const int k0 = (MX ? 1 : 2) * (int)((int64_t)pairs * part / parts);
-  const int k1r = (MX ? 1 : 2) * (int)((int64_t)pairs * (part + 1) / parts);
+  const int first_pair = (int)((int64_t)pairs * part / parts);
+  const int last_pair = (int)((int64_t)pairs * (part + 1) / parts);
+  const int mid = KS == 2 ? (first_pair + last_pair + 1) / 2 : last_pair;
+  const int k0 = (MX ? 1 : 2) * (half ? mid : first_pair);
+  const int k1r = (MX ? 1 : 2) * (half ? last_pair : mid);
   const int k1 = k1r < nkt ? k1r : nkt;
+  const int steps = KS == 2 ? (MX ? 1 : 2) * (mid - first_pair) : k1 - k0;  // of both halves
 #pragma unroll
   for (int s = 0; s < L::STAGES - 1; ++s)
     if (k0 + s < k1) issue(k0 + s, s);
   auto run = [&](auto blocks) {
     int stage = 0;
-    for (int kt = k0; kt < k1; ++kt) {
+    for (int kt = k0; kt < k0 + steps; ++kt) {
       // k-tile kt has landed once at most the loads of later ones are outstanding, at least the x and
       // W pieces of each.
       const int later = KA ? k1 - 1 - kt : 0;
@@ -335,7 +345,7 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
       TT_LDS_BARRIER();
       const int next = stage == 0 ? L::STAGES - 1 : stage - 1;  // the stage of kt - 1
       if (kt + L::STAGES - 1 < k1) issue(kt + L::STAGES - 1, next);
-      multiply(kt, stage, blocks);
+      if (KS == 1 || kt < k1) multiply(kt, stage, blocks);
       stage = stage == L::STAGES - 1 ? 0 : stage + 1;
     }
   };
@@ -357,6 +367,40 @@ __global__ __launch_bounds__((T_BM == 256 ? 512 : 256), (T_BM == 256 ? 1 : 2)) v
     return;
   }
   TT_LDS_BARRIER();  // every wave is past its fragment reads
+  if constexpr (KS == 2) {
+    // A half keeps block `half` of its rows and gives the other one away.
+    lds_char* const all = (lds_char*)lds_block;
+    constexpr uint32_t BLOCK = NJ * 4096;  // bytes of a wave's block of sums
+    const uint32_t to = (4u * (1 - half) + wave) * BLOCK, from = (4u * half + wave) * BLOCK;
+    static_assert(8 * BLOCK + 8 * NJ * 2048 <= 2 * L::LDS, "sums and outputs side by side");
+    f32x16 sum[1][NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        typedef __attribute__((address_space(3))) f32x4_t lds_f32x4;
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = half ? acc[0][j][4 * q + e] : acc[1][j][4 * q + e];
+          sum[0][j][4 * q + e] = half ? acc[1][j][4 * q + e] : acc[0][j][4 * q + e];
+        }
+        *reinterpret_cast<lds_f32x4*>(all + to + (4 * j + q) * 1024 + lane * 16) = v;
+      }
+    TT_LDS_BARRIER();
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4_t v = __builtin_bit_cast(f32x4_t, read_k(all, from + (4 * j + q) * 1024 + lane * 16));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[0][j][4 * q + e] += v[e];
+      }
+    mx_tile_store<GATED, OUT8, 1, NJ, MS>(p, sum, all + 8 * BLOCK + (4 * half + wave) * (NJ * 2048),
+                                          t.seg0 + i0, rows, m0 + MS * half,
+                                          j0 + (GATED ? n0 / 2 : n0));
+    return;
+  }
   mx_tile_store<GATED, OUT8, MI, NJ, MS>(p, acc, lds + wave * (MI * NJ * 2048), t.seg0 + i0, rows, m0,
                                      j0 + (GATED ? n0 / 2 : n0));
 }
@@ -391,15 +435,15 @@ __global__ __launch_bounds__(64) void mx_join_kernel(MxArgs p, int tiles_i, int 
                                      j0 + (GATED ? n0 / 2 : n0));
 }
 
-template <bool MX, bool GATED, bool OUT8, bool KA, int BM, int BN>
+template <bool MX, bool GATED, bool OUT8, bool KA, int BM, int BN, int KS = 1>
 int launch(const MxArgs& p, int parts, hipStream_t s) {
-  constexpr int CB = GATED ? BN / 2 : BN, NT = 64 * Tile<MX, BM, BN>::NW;
+  constexpr int CB = GATED ? BN / 2 : BN, NT = 64 * Tile<MX, BM, BN>::NW * KS;
   const int64_t tiles_j = (p.N + CB - 1) / CB;
   int64_t tiles_i = (p.M + BM - 1) / BM;
   if (p.counts != nullptr) tiles_i = p.M / BM + (p.E < p.M ? p.E : p.M);
   const int64_t blocks = tiles_i * tiles_j * parts;
   TT_REQUIRE(blocks < (1ll << 31) && tt_grid_ok(blocks, NT), "mx product: grid too large");
-  hipLaunchKernelGGL((mx_tile_kernel<MX, GATED, OUT8, KA, BM, BN>), dim3((unsigned)blocks),
+  hipLaunchKernelGGL((mx_tile_kernel<MX, GATED, OUT8, KA, BM, BN, KS>), dim3((unsigned)blocks),
                      dim3(NT), 0, s, p, (int)tiles_j, parts);
   const int rc = tt_check_launch("mx_tile");
   if constexpr (BM == 64 && KA) {  // the only tile whose reductions are split
@@ -418,6 +462,7 @@ int shaped(const MxArgs& p, MxPlan plan, hipStream_t s) {
   if constexpr (MX)
     if (plan.bm == 256) return launch<MX, GATED, OUT8, true, 256, 256>(p, 1, s);
   if (plan.bm == 64) return launch<MX, GATED, OUT8, true, 64, 128>(p, plan.parts, s);
+  if (plan.halves == 2) return launch<MX, GATED, OUT8, true, 128, 128, 2>(p, 1, s);
   if (plan.bn == 128) return launch<MX, GATED, OUT8, true, 128, 128>(p, 1, s);
   return launch<MX, GATED, OUT8, true, 128, 256>(p, 1, s);
 }
