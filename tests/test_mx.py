@@ -18,7 +18,7 @@ from torchturbo_amd.moe import (GroupedMLP, MoEConfig, MoELayer, MoESubmodules, 
                                 Mxfp4GroupedMLP, Mxfp4SharedExpertMLP, RMSNorm, SharedExpertMLP)
 from torchturbo_amd.providers.hip.mx import (HipDequantizeMxfp4, HipDequantizeMxfp8,
                                              HipGroupedMatmulMxfp4, HipLinearMxfp4,
-                                             HipQuantizeMxfp4, HipQuantizeMxfp8)
+                                             HipQuantizeMxfp4, HipQuantizeMxfp8, _device)
 from torchturbo_amd.providers.hip.norm import HipRmsNorm, HipRmsNormMx
 from torchturbo_amd.runtime import CpuRuntime
 
@@ -145,6 +145,20 @@ W = torch.ones(64)
 def test_refusals(call, message):
     with pytest.raises(ValueError, match=message):
         call()
+
+
+def test_tensors_of_another_gpu_than_the_current_one(monkeypatch):
+    class Elsewhere:
+        device = torch.device("cuda", 1)
+
+        def get_device(self):
+            return 1
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="cuda:1, which is not the current device"):
+        _device(Elsewhere(), None, Elsewhere())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    assert _device(Elsewhere(), None, Elsewhere()) == Elsewhere.device
 
 
 def test_rows_in_8_bits_have_no_gradient():

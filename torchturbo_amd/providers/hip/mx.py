@@ -91,13 +91,17 @@ def check_rows(op, x, k):
 
 
 def _device(first, *others):
-    """The tensors' one GPU, or ``require_cuda``'s refusal."""
+    """The tensors' one GPU, or ``require_cuda``'s refusal. It has to be the current one: launches
+    on another's default stream would go to the current GPU."""
     index = first.get_device()
     if index >= 0:
         for t in others:
             if t is not None and t.get_device() != index:
                 break
         else:
+            if index != torch.cuda.current_device():
+                raise ValueError(f"tensors are on cuda:{index}, which is not the current device "
+                                 "(torch.cuda.set_device)")
             return first.device
     return require_cuda(first, *others)
 
