@@ -151,6 +151,24 @@ def test_linear_integers_to_the_bit(hip_ops, m, k, n, mx):
     assert torch.equal(got.cpu(), want), (got.cpu() != want).nonzero()[:8]
 
 
+@pytest.mark.parametrize("k", [128, 256, 384, 640, 896, 1664, 4224])
+@pytest.mark.parametrize("mx", [False, True])
+def test_few_rows_of_ragged_reductions(hip_ops, k, mx):
+    """Loads of four steps' scales that end in the next row or behind the operand, and scales at odd
+    addresses, which take another path; few and many tiles, alone and as experts."""
+    for m, n in ((1, 17), (3, 1040), (24, 48)):
+        x, codes, scales = _integers(m, k, n, mx, seed=k + n)
+        want = o_mx.linear(x, codes, scales).to(BF16)
+        odd = torch.empty(scales.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(scales.shape)
+        odd.copy_(scales)
+        for s in (scales.to(DEV), odd):
+            assert torch.equal(hip_ops.linear_mxfp4(_dev(x), codes.to(DEV), s).cpu(), want), (m, n)
+    x, codes, scales = _integers(7, k, 3 * 33, mx, seed=k)
+    codes, scales = codes.view(3, 33, -1), scales.view(3, 33, -1)
+    got = hip_ops.grouped_matmul_mxfp4(_dev(x), codes.to(DEV), scales.to(DEV), [2, 0, 5])
+    assert torch.equal(got.cpu(), o_mx.grouped(x, codes, scales, [2, 0, 5]).to(BF16))
+
+
 @pytest.mark.parametrize("m, k, n", SIZES)
 @pytest.mark.parametrize("mx", [False, True])
 def test_linear(hip_ops, m, k, n, mx):

@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * W) void mx_rows_kernel(MxArgs p, int tiles_j) 
   u32x4 wv[2][NB], xv[2][MB][XV], ws4[2][NB], xs4[2][MB];
   uint32_t ws1[2][NB], xs1[2][MB];
   const int limit = 4 * s1 < groups ? 4 * s1 : groups;
-  // The scales of steps s to s + 3.
+  // The scales of steps s to s + 3; words behind the operand's last one read as zeros.
   auto fetch_scales = [&](int s, int d) {
     if constexpr (NEAR) {
 #pragma unroll
