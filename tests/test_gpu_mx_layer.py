@@ -167,3 +167,18 @@ def test_empty_batch(process_ops):
         with torch.no_grad():
             out, _, total = layer(_tokens((0, H)), residual=_tokens((0, H)))
         assert out.shape == total.shape == (0, H)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_column_major_tokens(process_ops, eight, norm):
+    """A dense [T, H] whose tokens lie along the fast dimension: the output is that of its copy."""
+    process_ops(CudaRuntime(), OpPolicy.CUSTOM)
+    layer = _layer(eight, norm=norm)
+    x = _tokens((65, H))
+    turned = x.t().contiguous().t()
+    assert not turned.is_contiguous() and torch.equal(turned, x)
+    with torch.no_grad():
+        out, logits = layer(turned)
+        want, want_logits = layer(x)
+    assert torch.equal(logits, want_logits) and torch.equal(out, want)

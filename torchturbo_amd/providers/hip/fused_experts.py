@@ -339,7 +339,8 @@ def mxfp4_forward(experts, tokens, rows, probs, expert_indices):
         x = rows.view(T)
     packed_rows, token_of_row, packed_probs, counts = route_index(expert_indices, E, probs)
     y = experts.inference(x, counts, packed_probs, row_map=token_of_row)
-    out = torch.empty_like(tokens)
+    # Row-major whatever the tokens' strides are: the kernel gets an address.
+    out = torch.empty_like(tokens, memory_format=torch.contiguous_format)
     L.call("tt_unpermute_gather", L.ptr(y), L.dtype_code(y.dtype), T, tokens.shape[1], k,
            L.ptr(packed_rows), None, None, 0, E, L.ptr(out), L.stream(tokens.device))
     return out, counts
