@@ -522,6 +522,7 @@ int tt_lora_wgrad_dropout(const void* x, const float* dh, int dtype, int64_t m, 
  * tt_rms_norm_fwd: h = x + residual (or x), y = h (mean(h^2) + eps)^(-1/2) weight over the
  *   last of [rows, cols], each of y, sum (h, rounded), rstd [rows] and codes / scales (y in
  *   E4M3, cols a multiple of 32) skipped when NULL. weight [cols] may have another dtype.
+ * tt_rms_norm_fwd_rounded: the same, codes / scales being tt_mxfp8_quantize's of y as rounded.
  * tt_rms_norm_bwd: with h as rounded, a = gy weight, xh = h rstd: dx = rstd (a - xh
  *   mean(a xh)) + gsum (or without, NULL), dweight = the sum over rows of gy xh, joined in a
  *   fixed order; either skipped when NULL. workspace (dweight): tt_rms_norm_bwd_workspace
@@ -546,6 +547,10 @@ int tt_mx_dgrad(const void* dy, const uint8_t* codes, const uint8_t* scales, int
 int tt_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
                     int dtype, int64_t rows, int64_t cols, float eps, void* y, void* sum,
                     float* rstd, uint8_t* codes, uint8_t* scales, void* stream);
+int tt_rms_norm_fwd_rounded(const void* x, const void* residual, const void* weight,
+                            int weight_dtype, int dtype, int64_t rows, int64_t cols, float eps,
+                            void* y, void* sum, float* rstd, uint8_t* codes, uint8_t* scales,
+                            void* stream);
 size_t tt_rms_norm_bwd_workspace(int64_t rows, int64_t cols);
 int tt_rms_norm_bwd(const void* h, const void* weight, int weight_dtype, const float* rstd,
                     const void* gy, const void* gsum, int dtype, int64_t rows, int64_t cols,

@@ -26,7 +26,8 @@ class TorchRmsNorm(OpImpl):
 @register_op(op_name="rms_norm_mx", impl_name="torch_rms_norm_mx", kind=OpImplKind.NATIVE,
              priority=0, devices=())
 class TorchRmsNormMx(OpImpl):
-    def __call__(self, x, weight, eps=1e-6, *, residual=None, with_y=False):
+    def __call__(self, x, weight, eps=1e-6, *, residual=None, with_y=False, rounded=False):
         y, h = norm(x, weight, eps, residual)
-        return NormRows(quantize_mxfp8(y), y.to(x.dtype) if with_y else None,
+        return NormRows(quantize_mxfp8(y.to(x.dtype) if rounded else y),
+                        y.to(x.dtype) if with_y else None,
                         None if residual is None else h.to(x.dtype))

@@ -14,6 +14,7 @@ import torch.nn.functional as F
 from oracle.native_providers import mx as o_mx
 from oracle.native_providers import norm as o_norm
 from tests.conftest import assert_bf16_close
+from torchturbo_amd import checks
 from torchturbo_amd.dispatch import OpPolicy, ops
 from torchturbo_amd.moe import (GroupedMLP, MoEConfig, MoELayer, MoESubmodules, ModuleSpec,
                                 Mxfp4GroupedMLP, Mxfp4SharedExpertMLP, RMSNorm)
@@ -183,3 +184,24 @@ def test_column_major_tokens(process_ops, eight, norm):
     with torch.no_grad():
         out, want = (layer.forward_with_logits(t, logits) for t in (turned, x))
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 64, 700])
+@pytest.mark.parametrize("residual", [False, True])
+def test_the_norms_rows_are_those_of_its_output(process_ops, tokens, residual):
+    """With rows in 8 bits: a hook on the experts or on the norm, or checks of the inputs, send the layer
+    another way; its output stays the same."""
+    process_ops(CudaRuntime(), OpPolicy.CUSTOM)
+    layer = _layer(True)
+    x, r = _tokens((tokens, H)), _tokens((tokens, H), 2) if residual else None
+    with torch.no_grad():
+        want = layer(x, residual=r)
+        others = []
+        for module in (layer.experts, layer.norm):
+            handle = module.register_forward_hook(lambda *a: None)
+            others.append(layer(x, residual=r))
+            handle.remove()
+        with checks.checking():
+            others.append(layer(x, residual=r))
+    for other in others:
+        assert all(torch.equal(a, b) for a, b in zip(want, other))

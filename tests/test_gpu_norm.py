@@ -247,3 +247,20 @@ def test_graph_replay(hip_ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, step(x, r, w)))
+
+
+@pytest.mark.parametrize("shape, dtype", MX_SHAPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("with_y", [False, True])
+def test_rounded_rows_are_the_quantisers(hip_ops, shape, dtype, residual, with_y):
+    """To the bit: the codes and scales of y as it is stored."""
+    x, r, w = _dev(*_inputs(shape, DTYPES[dtype], residual))
+    out = hip_ops.rms_norm_mx(x, w, 1e-5, residual=r, with_y=with_y, rounded=True)
+    y = hip_ops.rms_norm(x, w, 1e-5, residual=r)
+    if residual:
+        assert torch.equal(out.sum, y[1])
+        y = y[0]
+    assert torch.equal(out.y, y) if with_y else out.y is None
+    want = o_mx.quantize_mxfp8(y.cpu())
+    assert torch.equal(out.rows.codes.cpu().view(torch.uint8), want.codes.view(torch.uint8))
+    assert torch.equal(out.rows.scales.cpu(), want.scales)

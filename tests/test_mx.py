@@ -398,3 +398,19 @@ def test_layer_with_a_norm(process_ops, residual):
     layer(x)
     handle.remove()
     assert calls == [1]
+
+
+def test_rounded_rows_of_the_norm(process_ops):
+    """The rows that ``quantize_mxfp8`` gives for the output; not asked for, a provider without them serves."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    g = torch.Generator().manual_seed(7)
+    x, w = torch.randn(40, 64, generator=g).to(BF16), torch.rand(64, generator=g).to(BF16)
+    out = ops.rms_norm_mx(x, w, with_y=True, rounded=True)
+    want = ops.quantize_mxfp8(ops.rms_norm(x, w))
+    assert torch.equal(out.y, ops.rms_norm(x, w))
+    assert torch.equal(out.rows.codes.float(), want.codes.float())
+    assert torch.equal(out.rows.scales, want.scales)
+    plain = ops.rms_norm_mx(x, w).rows
+    assert (plain.codes.float() != want.codes.float()).any()  # the unrounded y's differ here and there
+    with pytest.raises(ValueError, match="NULL tensor"):
+        L.call("tt_rms_norm_fwd_rounded", *_norm(x=None)[1])

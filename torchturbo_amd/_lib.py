@@ -98,6 +98,7 @@ _PROTOS: dict[str, list] = {
     "tt_mx_product_workspace": [I64, I64, I64, I32, I32],
     "tt_mx_dgrad": [P, P, P, I64, I64, I64, I32, P, P, P],
     "tt_rms_norm_fwd": [P, P, P, c_int, c_int, I64, I64, c_float, P, P, P, P, P, P],
+    "tt_rms_norm_fwd_rounded": [P, P, P, c_int, c_int, I64, I64, c_float, P, P, P, P, P, P],
     "tt_rms_norm_bwd_workspace": [I64, I64],
     "tt_rms_norm_bwd": [P, P, c_int, P, P, P, c_int, I64, I64, P, P, P, c_size_t, P],
 }

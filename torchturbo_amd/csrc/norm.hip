@@ -3,7 +3,9 @@
 //   h = x + residual,  rho = (mean(h^2) + eps)^(-1/2),  y = h rho w
 //
 // and, for the experts' products, y in E4M3 with one power of two per 32 features (mx.h). The
-// statistics and the product are formed in fp32 from the unrounded sum; sum and y are rounded once.
+// statistics and the product are formed in fp32 from the unrounded sum; sum and y are rounded once, and
+// so are the codes, of the unrounded y or (rounded) of y as it is stored: then they are those that the
+// quantiser gives for the stored y.
 // The backward, with a = gy w and xh = h rho from the rounded sum that it is given:
 //
 //   dh = rho (a - xh mean(a xh)) + g_sum,  dw = sum over rows of gy xh.
@@ -79,6 +81,7 @@ struct NormArgs {
   void *y, *sum;
   float* rstd;
   uint8_t *codes, *scales;
+  int rounded;  // codes of y as rounded to the input's dtype
 };
 
 template <class T, bool VEC, int RT, int IT>
@@ -113,6 +116,10 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_fwd_kernel(NormArgs p)
     if (p.sum != nullptr) store8<T, VEC>(static_cast<S*>(p.sum) + row * H + at, h, H - at);
     if (p.y != nullptr) store8<T, VEC>(static_cast<S*>(p.y) + row * H + at, y, H - at);
     if (p.codes != nullptr) {  // H is a multiple of 32: a group's four lanes come together
+      if (p.rounded) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = T::to_f32(T::from_f32(y[j]));
+      }
       uint32_t byte;
       const uint2 q = mx_rows8(y, byte);
       *reinterpret_cast<uint2*>(p.codes + row * H + at) = q;
@@ -466,10 +473,11 @@ bool is_float(int dtype) { return dtype == TT_F32 || dtype == TT_BF16 || dtype =
 
 }  // namespace
 
-extern "C" int tt_rms_norm_fwd(const void* x, const void* residual, const void* weight,
-                               int weight_dtype, int dtype, int64_t rows, int64_t cols, float eps,
-                               void* y, void* sum, float* rstd, uint8_t* codes, uint8_t* scales,
-                               void* stream) {
+namespace {
+
+int norm_fwd(const void* x, const void* residual, const void* weight, int weight_dtype, int dtype,
+             int64_t rows, int64_t cols, float eps, void* y, void* sum, float* rstd, uint8_t* codes,
+             uint8_t* scales, int rounded, void* stream) {
   TT_REQUIRE(is_float(dtype) && is_float(weight_dtype), "rms_norm: tensors must be f32, bf16 or f16");
   TT_REQUIRE(rows >= 0 && cols >= 0 && cols < (1ll << 31), "rms_norm: bad sizes");
   TT_REQUIRE((codes == nullptr) == (scales == nullptr), "rms_norm: codes and scales, or neither");
@@ -479,7 +487,8 @@ extern "C" int tt_rms_norm_fwd(const void* x, const void* residual, const void* 
   TT_REQUIRE(x != nullptr && weight != nullptr, "rms_norm: NULL tensor");
   TT_REQUIRE((residual != nullptr) || (sum == nullptr), "rms_norm: a sum needs a residual");
   TT_REQUIRE((reinterpret_cast<uintptr_t>(codes) & 7) == 0, "rms_norm: codes must be 8-byte aligned");
-  const NormArgs p = {x, residual, weight, weight_dtype, rows, cols, eps, y, sum, rstd, codes, scales};
+  const NormArgs p = {x,   residual, weight, weight_dtype, rows,   cols,   eps,
+                      y,   sum,      rstd,   codes,        scales, rounded};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool vec = aligned(cols, {x, residual, weight, y, sum});
   switch (dtype) {
@@ -487,6 +496,24 @@ extern "C" int tt_rms_norm_fwd(const void* x, const void* residual, const void* 
     case TT_F16: return vec ? fwd_shape<F16T, true>(p, s) : fwd_shape<F16T, false>(p, s);
     default: return vec ? fwd_shape<F32T, true>(p, s) : fwd_shape<F32T, false>(p, s);
   }
+}
+
+}  // namespace
+
+extern "C" int tt_rms_norm_fwd(const void* x, const void* residual, const void* weight,
+                               int weight_dtype, int dtype, int64_t rows, int64_t cols, float eps,
+                               void* y, void* sum, float* rstd, uint8_t* codes, uint8_t* scales,
+                               void* stream) {
+  return norm_fwd(x, residual, weight, weight_dtype, dtype, rows, cols, eps, y, sum, rstd, codes,
+                  scales, 0, stream);
+}
+
+extern "C" int tt_rms_norm_fwd_rounded(const void* x, const void* residual, const void* weight,
+                                       int weight_dtype, int dtype, int64_t rows, int64_t cols,
+                                       float eps, void* y, void* sum, float* rstd, uint8_t* codes,
+                                       uint8_t* scales, void* stream) {
+  return norm_fwd(x, residual, weight, weight_dtype, dtype, rows, cols, eps, y, sum, rstd, codes,
+                  scales, 1, stream);
 }
 
 extern "C" size_t tt_rms_norm_bwd_workspace(int64_t rows, int64_t cols) {

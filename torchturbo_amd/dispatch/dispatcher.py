@@ -264,10 +264,12 @@ class OpDispatcher:
         return self._dispatch("rms_norm", x, weight, eps, residual=residual, impl=impl)
 
     def rms_norm_mx(self, x, weight, eps: float = 1e-6, *, residual=None, with_y: bool = False,
-                    impl: str | None = None):
-        """``rms_norm`` with its output in 8 bits (``NormRows``). No reference counterpart."""
+                    rounded: bool = False, impl: str | None = None):
+        """``rms_norm`` with its output in 8 bits (``NormRows``); rounded: the rows are
+        ``quantize_mxfp8`` of the output in x's dtype. No reference counterpart."""
+        more = {"rounded": True} if rounded else {}  # providers may lack what is not asked for
         return self._dispatch("rms_norm_mx", x, weight, eps, residual=residual, with_y=with_y,
-                              impl=impl)
+                              impl=impl, **more)
 
     def linear_mxfp4(self, x, codes, scales, *, activation_func=None, gated: bool = False,
                      mx_out: bool = False, impl: str | None = None):

@@ -201,9 +201,12 @@ class MoELayer(BaseMoELayer):
             return hidden_states, None, None
         if (type(norm) is RMSNorm and not attached(norm) and self._mxfp4_inference(hidden_states)
                 and self.experts.rows_in_8_bits and op_resolves("rms_norm_mx")
+                and ops.selected_impl_name("rms_norm_mx") == "hip_rms_norm_mx"
                 and ops.selected_impl_name("rms_norm") == "hip_rms_norm"):
-            # The router's rows and the experts' in one pass.
-            out = ops.rms_norm_mx(hidden_states, norm.weight, norm.eps, residual=residual, with_y=True)
+            # The router's rows and the experts' in one pass: the rows that the experts would
+            # quantise themselves, so that a hook or a check does not change the output.
+            out = ops.rms_norm_mx(hidden_states, norm.weight, norm.eps, residual=residual,
+                                  with_y=True, rounded=True)
             return out.y, out.rows, out.sum
         if residual is None:
             return norm(hidden_states), None, None

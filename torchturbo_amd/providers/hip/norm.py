@@ -4,7 +4,9 @@
   of ``h = x + residual`` over the last dimension; with a residual ``(y, h)``, else
   ``y``. Gradients flow to x, residual and weight from y and h.
 * ``rms_norm_mx``: the same forward with y in 8 bits (``NormRows``), for the products
-  with 4-bit weights, and y itself where a router reads it. Without gradients.
+  with 4-bit weights, and y itself where a router reads it. Without gradients. The rows
+  are those of the unrounded y, or with ``rounded`` of y as it is given back: what
+  ``quantize_mxfp8(y)`` gives, so that it does not matter who quantises.
 
 x and residual share one dtype (f32, bf16 or f16), the weight may have another of the
 three. The statistics and the product are formed in fp32 from the unrounded sum; y and
@@ -27,7 +29,7 @@ from .linear import FLOATS, _autograd_sees, _rows
 from .mx import _device
 
 
-def _forward(x, weight, eps, residual, with_y, with_rstd, with_mx):
+def _forward(x, weight, eps, residual, with_y, with_rstd, with_mx, rounded=False):
     """(y, sum, rstd, codes, scales) of rows [T, H]; None for a part not wanted."""
     (t, h), dev = x.shape, x.device
     y = torch.empty_like(x) if with_y else None
@@ -37,9 +39,9 @@ def _forward(x, weight, eps, residual, with_y, with_rstd, with_mx):
     if with_mx:
         codes = torch.empty((t, h), dtype=torch.float8_e4m3fn, device=dev)
         scales = torch.empty((t, h // GROUP), dtype=torch.uint8, device=dev)
-    L.call("tt_rms_norm_fwd", L.ptr(x), L.ptr(residual), L.ptr(weight), L.dtype_code(weight.dtype),
-           L.dtype_code(x.dtype), t, h, eps, L.ptr(y), L.ptr(total), L.ptr(rstd), L.ptr(codes),
-           L.ptr(scales), L.stream(dev))
+    L.call("tt_rms_norm_fwd_rounded" if rounded else "tt_rms_norm_fwd", L.ptr(x), L.ptr(residual),
+           L.ptr(weight), L.dtype_code(weight.dtype), L.dtype_code(x.dtype), t, h, eps, L.ptr(y),
+           L.ptr(total), L.ptr(rstd), L.ptr(codes), L.ptr(scales), L.stream(dev))
     return y, total, rstd, codes, scales
 
 
@@ -115,7 +117,7 @@ class HipRmsNormMx(OpImpl):
     def available(self) -> bool:
         return hip_available()
 
-    def __call__(self, x, weight, eps=1e-6, *, residual=None, with_y=False):
+    def __call__(self, x, weight, eps=1e-6, *, residual=None, with_y=False, rounded=False):
         if x.dim() and x.shape[-1] % GROUP:
             raise ValueError(f"rms_norm_mx: the features must be whole groups of {GROUP}, got "
                              f"{x.shape[-1]}")
@@ -123,7 +125,7 @@ class HipRmsNormMx(OpImpl):
         if _autograd_sees(x2, w, r):
             raise RuntimeError("rms_norm_mx has no gradient: call it under torch.no_grad(), or "
                                "rms_norm in its place")
-        y, h, _, codes, scales = _forward(x2, w, float(eps), r, with_y, False, True)
+        y, h, _, codes, scales = _forward(x2, w, float(eps), r, with_y, False, True, rounded)
         rows = MxRows(codes, scales)
         if x.dim() == 2:
             return NormRows(rows, y, h)
