@@ -264,3 +264,24 @@ def test_rounded_rows_are_the_quantisers(hip_ops, shape, dtype, residual, with_y
     want = o_mx.quantize_mxfp8(y.cpu())
     assert torch.equal(out.rows.codes.cpu().view(torch.uint8), want.codes.view(torch.uint8))
     assert torch.equal(out.rows.scales.cpu(), want.scales)
+
+
+@pytest.mark.parametrize("rows", [1, 33])
+def test_weight_gradient_of_more_features_than_a_launch_has_threads_for(hip_ops, rows):
+    """2^27 features: one block of 1024 threads per 32 of them, or a thread for each in every part, would be
+    2^32 threads and more. Rows of +-1 have rstd 1, so with gradients of small whole numbers all is
+    exact."""
+    n = 1 << 27
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    w = torch.ones(n, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    x = torch.empty(rows, n, dtype=torch.bfloat16, device=DEV)
+    gy = torch.empty_like(x)
+    want = torch.zeros(n, device=DEV)
+    for r in range(rows):
+        x[r] = torch.randint(0, 2, (n,), generator=g, device=DEV, dtype=torch.int8) * 2 - 1
+        gy[r] = torch.randint(-3, 4, (n,), generator=g, device=DEV, dtype=torch.int8)
+        want += x[r].float() * gy[r].float()
+    y = hip_ops.rms_norm(x, w, 0.0)
+    assert all(torch.equal(a, b) for a, b in zip(y.detach(), x))
+    dw, = torch.autograd.grad(y, w, gy)
+    assert torch.equal(dw, want.to(torch.bfloat16))  # at most 99: exact

@@ -362,38 +362,42 @@ __global__ __launch_bounds__(Shape<RT>::NT) void rms_norm_bwd_kernel(NormBwdArgs
 }
 
 // dw's partial rows for features past the registers' reach: block (x, y) sums feature columns x of
-// the rows y, y + gridDim.y, ... .
+// the rows y, y + gridDim.y, ..., and further columns in turn.
 template <class T>
 __global__ __launch_bounds__(256) void rms_norm_dw_kernel(NormBwdArgs p) {
   typedef typename T::storage S;
-  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (j >= p.H) return;
-  float v = 0.f;
-  for (int64_t row = blockIdx.y; row < p.T; row += gridDim.y)
-    v += T::to_f32(static_cast<const S*>(p.gy)[row * p.H + j]) *
-         (T::to_f32(static_cast<const S*>(p.h)[row * p.H + j]) * p.rstd[row]);
-  p.part[(int64_t)blockIdx.y * p.H + j] = v;
+  for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < p.H; j += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+    for (int64_t row = blockIdx.y; row < p.T; row += gridDim.y)
+      v += T::to_f32(static_cast<const S*>(p.gy)[row * p.H + j]) *
+           (T::to_f32(static_cast<const S*>(p.h)[row * p.H + j]) * p.rstd[row]);
+    p.part[(int64_t)blockIdx.y * p.H + j] = v;
+  }
 }
 
 // dw [H] from `parts` partial rows: a block takes 32 features and 32 threads each a share of the
-// rows, whose sums are added in order.
+// rows, whose sums are added in order; further features in turn.
 __global__ __launch_bounds__(1024) void rms_norm_join_kernel(const float* __restrict__ part,
                                                              int parts, int64_t H,
                                                              void* __restrict__ dw, int dtype) {
   __shared__ float sums[32][33];
   const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int64_t j = (int64_t)blockIdx.x * 32 + c;
-  float v = 0.f;
-  if (j < H) {
+  for (int64_t j0 = (int64_t)blockIdx.x * 32; j0 < H; j0 += (int64_t)gridDim.x * 32) {
+    const int64_t j = j0 + c;
+    float v = 0.f;
+    if (j < H) {
 #pragma unroll 8
-    for (int i = r; i < parts; i += 32) v += part[(int64_t)i * H + j];
-  }
-  sums[r][c] = v;
-  __syncthreads();
-  if (r != 0 || j >= H) return;
+      for (int i = r; i < parts; i += 32) v += part[(int64_t)i * H + j];
+    }
+    __syncthreads();  // the sums before have been read
+    sums[r][c] = v;
+    __syncthreads();
+    if (r == 0 && j < H) {
 #pragma unroll
-  for (int i = 1; i < 32; ++i) v += sums[i][c];
-  store_from_f32(dw, dtype, j, v);
+      for (int i = 1; i < 32; ++i) v += sums[i][c];
+      store_from_f32(dw, dtype, j, v);
+    }
+  }
 }
 
 // Threads per row for H features, and chunks per thread: at most four (two of 1024 threads, whose
@@ -409,6 +413,13 @@ int row_chunks(int64_t H) {
 // with residual: forward in 512, 768, 2048 blocks 69 / 61 / 59 and 66 / 57 / 58, backward in 256, 512, 640
 // blocks 87 / 65 / 87 and 87 / 64 / 87; with no row in flight ahead 60 and 58, 97 and 98.
 constexpr int64_t FWD_BLOCKS = 256 * 3, BWD_BLOCKS = 256 * 2;
+// Blocks along the features in the kernels of the weight's gradient, which keep their launches below
+// 2^32 threads (with BWD_BLOCKS parts of 256 threads, and alone of 1024) at any number of features.
+constexpr int64_t COLUMN_BLOCKS = 1 << 14;
+unsigned column_blocks(int64_t H, int per) {
+  const int64_t want = (H + per - 1) / per;
+  return (unsigned)(want < COLUMN_BLOCKS ? want : COLUMN_BLOCKS);
+}
 int64_t blocks_for(int64_t T, int64_t H, int64_t most) {
   const int rows = row_threads(H) >= 256 ? 1 : 256 / row_threads(H);
   const int64_t want = (T + rows - 1) / rows;
@@ -431,7 +442,7 @@ int launch_bwd(const NormBwdArgs& p, hipStream_t s) {
   int rc = tt_check_launch("rms_norm_bwd");
   if (IT > 0 || rc != TT_OK || p.part == nullptr) return rc;
   hipLaunchKernelGGL((rms_norm_dw_kernel<T>),
-                     dim3((unsigned)((p.H + 255) / 256), (unsigned)blocks), dim3(256), 0, s, p);
+                     dim3(column_blocks(p.H, 256), (unsigned)blocks), dim3(256), 0, s, p);
   return tt_check_launch("rms_norm_dw");
 }
 
@@ -545,7 +556,7 @@ extern "C" int tt_rms_norm_bwd(const void* h, const void* weight, int weight_dty
     default: rc = vec ? bwd_shape<F32T, true>(p, s) : bwd_shape<F32T, false>(p, s); break;
   }
   if (rc != TT_OK || dweight == nullptr) return rc;
-  hipLaunchKernelGGL(rms_norm_join_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, s,
-                     p.part, (int)blocks_for(rows, cols, BWD_BLOCKS), cols, dweight, weight_dtype);
+  hipLaunchKernelGGL(rms_norm_join_kernel, dim3(column_blocks(cols, 32)), dim3(1024), 0, s, p.part,
+                     (int)blocks_for(rows, cols, BWD_BLOCKS), cols, dweight, weight_dtype);
   return tt_check_launch("rms_norm_join");
 }
