@@ -414,3 +414,17 @@ def test_rounded_rows_of_the_norm(process_ops):
     assert (plain.codes.float() != want.codes.float()).any()  # the unrounded y's differ here and there
     with pytest.raises(ValueError, match="NULL tensor"):
         L.call("tt_rms_norm_fwd_rounded", *_norm(x=None)[1])
+
+
+def test_shared_expert_refuses_weights_of_other_shapes(process_ops):
+    """Also those that would fill every row by broadcasting; nothing is written then."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    small = Mxfp4SharedExpertMLP(_config(moe_shared_expert_intermediate_size=128))
+    w1, w2 = torch.randn(256, 64), torch.randn(64, 128)
+    small.quantize(w1, w2)
+    state = {k: v.clone() for k, v in small.state_dict().items()}
+    for a, b in ((w1[:1], w2[:1]), (w1[:1], w2), (w1, w2[:1]), (w1, w2[:, :64]), (w1[:128], w2),
+                 (w1[None], w2), (w1[0], w2), (w1, w2.t())):
+        with pytest.raises(ValueError, match=r"do not fit \[256, 64\] and \[64, 128\]"):
+            small.quantize(-a, -b)
+        assert all(torch.equal(v, state[k]) for k, v in small.state_dict().items())

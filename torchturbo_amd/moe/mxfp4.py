@@ -123,6 +123,10 @@ class Mxfp4SharedExpertMLP(_Mxfp4Weights):
     @torch.no_grad()
     def quantize(self, weight1, weight2) -> None:
         """Quantise ``SharedExpertMLP``'s weights (``[2F or F, H]`` and ``[H, F]``)."""
+        shapes = [[*q.shape[:-1], 2 * q.shape[-1]] for q in (self.q1, self.q2)]
+        if [list(weight1.shape), list(weight2.shape)] != shapes:
+            raise ValueError(f"weights {list(weight1.shape)} and {list(weight2.shape)} do not fit "
+                             f"{shapes[0]} and {shapes[1]}")
         self._quantize(1, weight1)
         self._quantize(2, weight2)
 
