@@ -428,3 +428,16 @@ def test_shared_expert_refuses_weights_of_other_shapes(process_ops):
         with pytest.raises(ValueError, match=r"do not fit \[256, 64\] and \[64, 128\]"):
             small.quantize(-a, -b)
         assert all(torch.equal(v, state[k]) for k, v in small.state_dict().items())
+
+
+def test_a_refused_checkpoint_leaves_the_weights(process_ops):
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    experts = Mxfp4GroupedMLP(4, False, _config())
+    state = {k: v.clone() for k, v in experts.state_dict().items()}
+    ones = [torch.ones_like(t) for t in (experts.q1, experts.s1, experts.q2, experts.s2)]
+    for bad in (ones[3][:2], ones[3].int()):
+        with pytest.raises(ValueError, match="s2"):
+            experts.load_quantized(*ones[:3], bad)
+        assert all(torch.equal(v, state[k]) for k, v in experts.state_dict().items())
+    experts.load_quantized(*ones)
+    assert all((v == 1).all() for v in experts.state_dict().values())

@@ -39,6 +39,7 @@ class _Mxfp4Weights(torch.nn.Module):
     @torch.no_grad()
     def load_quantized(self, q1, s1, q2, s2) -> None:
         """Copy codes and scales (uint8, or torch's ``float4_e2m1fn_x2`` and ``float8_e8m0fnu``)."""
+        checked = []
         for name, t in (("q1", q1), ("s1", s1), ("q2", q2), ("s2", s2)):
             own = getattr(self, name)
             if t.dtype not in (torch.uint8, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu):
@@ -47,6 +48,8 @@ class _Mxfp4Weights(torch.nn.Module):
             t = t if t.dtype == torch.uint8 else t.view(torch.uint8)
             if t.shape != own.shape:
                 raise ValueError(f"{name} has shape {list(t.shape)}, expected {list(own.shape)}")
+            checked.append((own, t))
+        for own, t in checked:
             own.copy_(t)
 
     def _quantize(self, which: int, weight) -> None:
