@@ -441,3 +441,30 @@ def test_a_refused_checkpoint_leaves_the_weights(process_ops):
         assert all(torch.equal(v, state[k]) for k, v in experts.state_dict().items())
     experts.load_quantized(*ones)
     assert all((v == 1).all() for v in experts.state_dict().values())
+
+
+def test_8_bit_conversions_do_not_cut_a_gradient():
+    """Gradients, tangents and transforms are refused before any GPU is looked for; what none follows
+    reaches the device's check."""
+    x = torch.randn(4, 64)
+    calls = ((HipQuantizeMxfp8(), x, lambda v: v), (HipDequantizeMxfp8(), R8.codes,
+                                                    lambda v: MxRows(v, R8.scales)))
+    for op, plain, form in calls:
+        leaf = plain.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            op(form(leaf))
+        for v in (plain, leaf.detach()):
+            with pytest.raises(ValueError, match="need device tensors"):
+                op(form(v))
+        with torch.no_grad(), pytest.raises(ValueError, match="need device tensors"):
+            op(form(leaf))
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(ValueError, match="need device tensors"):
+                op(form(plain))
+            dual = torch.autograd.forward_ad.make_dual(plain, torch.ones_like(plain))
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                op(form(dual))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.func.vmap(lambda v: HipQuantizeMxfp8()(v).codes)(x[None])
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.func.jvp(lambda v: HipQuantizeMxfp8()(v).codes.float(), (x,), (x,))

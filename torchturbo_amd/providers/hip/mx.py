@@ -17,7 +17,8 @@ K / 32]``, ``2^(byte - 127)``, 255 for NaN); rows in 8 bits are ``MxRows``. torc
 ``x`` is bf16 or ``MxRows``; the output bf16, or with ``mx_out`` ``MxRows``. Every product of two
 elements is exact, sums run in fp32 and are rounded once. The weights are frozen: gradients flow
 to a bf16 ``x`` (and to ``probs``). With gradients the activation is a pass of its own over the
-product, rounded to bf16, as in ``GroupedMLP``; rows in 8 bits, in or out, have none.
+product, rounded to bf16, as in ``GroupedMLP``; rows in 8 bits, in or out, have none, and making
+them (or values) of a tensor that asks for one is refused.
 """
 
 from __future__ import annotations
@@ -240,10 +241,22 @@ class HipGroupedMatmulMxfp4(OpImpl):
         return MxRows(*y) if mx_out else y
 
 
+def _followed(t):
+    """Whether a gradient, a tangent or a function transform follows ``t`` itself."""
+    ad = torch.autograd.forward_ad
+    return (torch.is_grad_enabled() and t.requires_grad
+            or torch._C._are_functorch_transforms_active()
+            and torch._C._functorch.is_functorch_wrapped_tensor(t)
+            or ad._current_level >= 0 and ad.unpack_dual(t).tangent is not None)
+
+
 def _quantized(op, x, bits):
     if x.dtype not in FLOATS or x.dim() == 0 or x.shape[-1] % GROUP:
         raise ValueError(f"{op} takes f32, bf16 or f16 rows of whole groups of {GROUP} elements, got "
                          f"{x.dtype} {list(x.shape)}")
+    # Codes of weights are whole numbers, which nobody takes for differentiable; those of rows are floats.
+    if bits == 8 and _followed(x):
+        raise _no_gradient(op, "rows in 8 bits")
     dev = _device(x)
     x2 = _rows(x, x.shape[-1])
     t, k = x2.shape
@@ -308,5 +321,7 @@ class HipDequantizeMxfp8(OpImpl):
         if not isinstance(rows, MxRows):
             raise ValueError(f"dequantize_mxfp8 takes MxRows, got {type(rows).__name__}")
         values, scales, lead = check_rows("dequantize_mxfp8", rows, None)
+        if _followed(values):
+            raise _no_gradient("dequantize_mxfp8", "rows in 8 bits")
         out = _dequantized("dequantize_mxfp8", values, scales, values.shape[1], dtype, 8)
         return out if len(lead) == 1 else out.view(*lead, values.shape[1])
