@@ -468,3 +468,36 @@ def test_8_bit_conversions_do_not_cut_a_gradient():
         torch.func.vmap(lambda v: HipQuantizeMxfp8()(v).codes)(x[None])
     with pytest.raises(RuntimeError, match="no gradient"):
         torch.func.jvp(lambda v: HipQuantizeMxfp8()(v).codes.float(), (x,), (x,))
+
+
+def test_a_subclass_keeps_what_it_calls_norm(process_ops):
+    """A norm that no submodule spec asked for is the subclass's own: the layer does not apply it."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    subs = MoESubmodules(experts=ModuleSpec(module=GroupedMLP))
+
+    class Normed(MoELayer):
+        def __init__(self, cfg):
+            super().__init__(cfg, None, submodules=subs)
+            self.norm = RMSNorm(cfg)
+
+        def forward(self, x, input_ids=None):
+            return super().forward(self.norm(x), input_ids)
+
+    class Measured(MoELayer):
+        def norm(self, x):
+            return x.norm()
+
+    plain = _filled(MoELayer(_config(), None, submodules=subs))
+    x = torch.randn(6, 64, generator=torch.Generator().manual_seed(8))
+    normed = Normed(_config())
+    normed.load_state_dict(plain.state_dict(), strict=False)
+    with torch.no_grad():
+        normed.norm.weight.uniform_(0.5, 1.5)
+        want, logits = plain(normed.norm(x))
+        assert all(torch.equal(a, b) for a, b in zip(normed(x), (want, logits)))
+        measured = Measured(_config(), None, submodules=subs)
+        measured.load_state_dict(plain.state_dict())
+        assert measured.norm(x) == x.norm()
+        assert torch.equal(measured(x)[0], plain(x)[0]) and plain.norm is None
+    with pytest.raises(ValueError, match="only with a norm"):
+        MoELayer.forward(normed, x, residual=x)

@@ -64,7 +64,6 @@ class BaseMoELayer(torch.nn.Module):
         self.shared_expert = None
         self.shared_expert_gate = None
         self.token_dispatcher = None
-        self.norm = None
         self.layer_number = layer_number
         self._runtime_inputs = MoERuntimeInputs()
 
@@ -74,6 +73,10 @@ class BaseMoELayer(torch.nn.Module):
 
 class MoELayer(BaseMoELayer):
     """Mixture-of-experts layer without token dropping."""
+
+    # Whether the layer normalises its input: only where its submodules ask for a norm (a `norm` that
+    # they did not ask for is a subclass's own).
+    _norms_input = False
 
     def __init__(self, config: MoEConfig, ep_group=None, submodules: Optional[MoESubmodules] = None,
                  use_te: bool = False, layer_number: Optional[int] = None, sp_group=None):
@@ -90,7 +93,10 @@ class MoELayer(BaseMoELayer):
                                     layer_number=layer_number)
         if self.use_shared_expert:
             self.shared_experts = build_module(submodules.shared_experts, config=config)
-        self.norm = build_module(getattr(submodules, "norm", None), config=config)
+        norm = build_module(getattr(submodules, "norm", None), config=config)
+        self._norms_input = norm is not None
+        if self._norms_input or not hasattr(type(self), "norm"):
+            self.norm = norm
 
     def _gathering_experts(self, tokens, expert_indices) -> bool:
         """Whether the permutation and unpermutation can be folded into the
@@ -194,7 +200,7 @@ class MoELayer(BaseMoELayer):
 
     def _normalised(self, hidden_states, residual):
         """(normalised input, the same in 8 bits or None, input + residual or None)."""
-        norm = self.norm
+        norm = self.norm if self._norms_input else None
         if norm is None:
             if residual is not None:
                 raise ValueError("MoELayer takes a residual only with a norm (MoESubmodules.norm)")
