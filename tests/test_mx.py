@@ -501,3 +501,23 @@ def test_a_subclass_keeps_what_it_calls_norm(process_ops):
         assert torch.equal(measured(x)[0], plain(x)[0]) and plain.norm is None
     with pytest.raises(ValueError, match="only with a norm"):
         MoELayer.forward(normed, x, residual=x)
+
+
+def test_a_subclass_that_combines_by_itself(process_ops):
+    """An override with the arguments that the layer had before there were rows in 8 bits serves a layer
+    without them."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    subs = MoESubmodules(experts=ModuleSpec(module=GroupedMLP))
+
+    class Halved(MoELayer):
+        def _experts_and_combine(self, hidden_states, probs, routing_map, expert_indices):
+            return super()._experts_and_combine(hidden_states, probs, routing_map, expert_indices) / 2
+
+    plain = _filled(MoELayer(_config(), None, submodules=subs))
+    halved = Halved(_config(), None, submodules=subs)
+    halved.load_state_dict(plain.state_dict())
+    x = torch.randn(6, 64, generator=torch.Generator().manual_seed(9))
+    with torch.no_grad():
+        want, logits = plain(x)
+        assert torch.equal(halved(x)[0], want / 2)
+        assert torch.equal(halved.forward_with_logits(x, logits), want / 2)

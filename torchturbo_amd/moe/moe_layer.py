@@ -219,6 +219,11 @@ class MoELayer(BaseMoELayer):
         y, total = norm(hidden_states, residual)
         return y, None, total
 
+    def _combined(self, hidden_states, probs, routing_map, expert_indices, rows):
+        # Subclasses that override the call know no rows, unless there are some.
+        more = () if rows is None else (rows,)
+        return self._experts_and_combine(hidden_states, probs, routing_map, expert_indices, *more)
+
     def _experts_and_combine(self, hidden_states, probs, routing_map, expert_indices, rows=None):
         flat = hidden_states.view(-1, hidden_states.shape[-1])
         if self._gathering_experts(flat, expert_indices):
@@ -283,7 +288,7 @@ class MoELayer(BaseMoELayer):
             hidden_states, input_ids, self._runtime_inputs.padding_mask,
             self._runtime_inputs.accumulate_tokens_per_expert)
         logits = logits.view(-1, logits.shape[-1])
-        output = self._experts_and_combine(hidden_states, probs, routing_map, expert_indices, rows)
+        output = self._combined(hidden_states, probs, routing_map, expert_indices, rows)
         return (output, logits) if residual is None else (output, logits, total)
 
     def forward_with_logits(self, hidden_states, logits, input_ids=None):
@@ -292,4 +297,4 @@ class MoELayer(BaseMoELayer):
         probs, routing_map, expert_indices = self.router.routing(
             logits, input_ids, self._runtime_inputs.padding_mask,
             self._runtime_inputs.accumulate_tokens_per_expert)
-        return self._experts_and_combine(hidden_states, probs, routing_map, expert_indices, rows)
+        return self._combined(hidden_states, probs, routing_map, expert_indices, rows)
