@@ -521,3 +521,20 @@ def test_a_subclass_that_combines_by_itself(process_ops):
         want, logits = plain(x)
         assert torch.equal(halved(x)[0], want / 2)
         assert torch.equal(halved.forward_with_logits(x, logits), want / 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, BF16])
+def test_shared_expert_with_8_bit_rows_keeps_the_dtype(process_ops, dtype):
+    """Its products give bf16; the output is in the input's dtype, as SharedExpertMLP's, and so is the
+    layer's."""
+    process_ops(CpuRuntime(), OpPolicy.NATIVE, oracle=True)
+    cfg = _config(moe_shared_expert_intermediate_size=128, params_dtype=dtype)
+    eight = {"rows_in_8_bits": True}
+    layer = MoELayer(cfg, None, submodules=MoESubmodules(
+        experts=ModuleSpec(Mxfp4GroupedMLP, eight), shared_experts=ModuleSpec(Mxfp4SharedExpertMLP, eight)))
+    layer.shared_experts.quantize(torch.randn(256, 64), torch.randn(64, 128))
+    x = torch.randn(6, 64, generator=torch.Generator().manual_seed(10)).to(dtype)
+    with torch.no_grad():
+        shared = layer.shared_experts(x)
+        assert shared.dtype == dtype and shared.any() and torch.equal(shared.to(BF16).to(dtype), shared)
+        assert layer(x)[0].dtype == dtype

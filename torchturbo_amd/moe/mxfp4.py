@@ -139,7 +139,8 @@ class Mxfp4SharedExpertMLP(_Mxfp4Weights):
         x = ops.quantize_mxfp8(hidden_states) if eight else hidden_states
         h = ops.linear_mxfp4(x, self.q1, self.s1, activation_func=cfg.activation_func,
                              gated=cfg.gated_linear_unit, mx_out=eight)
-        return ops.linear_mxfp4(h, self.q2, self.s2)
+        # Products of rows in 8 bits are bf16 whatever the input was.
+        return ops.linear_mxfp4(h, self.q2, self.s2).to(hidden_states.dtype)
 
 
 __all__ = ["Mxfp4GroupedMLP", "Mxfp4SharedExpertMLP"]
