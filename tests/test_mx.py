@@ -538,3 +538,11 @@ def test_shared_expert_with_8_bit_rows_keeps_the_dtype(process_ops, dtype):
         shared = layer.shared_experts(x)
         assert shared.dtype == dtype and shared.any() and torch.equal(shared.to(BF16).to(dtype), shared)
         assert layer(x)[0].dtype == dtype
+
+
+def test_no_workspace_for_reductions_that_are_not_split():
+    """Split reductions are multiples of 128: other sizes ask for no scratch, which no kernel would touch."""
+    size = L.load().tt_mx_product_workspace
+    for K in (7136, 7104, 7200):
+        assert size(128, K, 2048, 0, 1) == size(128, K, 2048, 0, 0) == 0
+    assert size(128, 7040, 2048, 0, 1) > 0

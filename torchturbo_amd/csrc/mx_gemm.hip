@@ -106,7 +106,8 @@ extern "C" int tt_mx_product(const void* x, const uint8_t* x_scales, const int32
 
 extern "C" size_t tt_mx_product_workspace(int64_t M, int64_t K, int64_t N,
                                           int32_t grouped, int32_t gated) {
-  if (M <= 0 || K <= 0 || N <= 0 || grouped) return 0;
+  // Only reductions in whole steps of 128 are split (mx_tile.hip).
+  if (M <= 0 || K <= 0 || K % 128 != 0 || N <= 0 || grouped) return 0;
   const int64_t W = gated ? 2 * N : N;
   if (few_rows(M, W, 1, false)) return 0;
   return part_bytes(plan(false, M, K, W, 1, false), M, W);
