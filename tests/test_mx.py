@@ -546,3 +546,18 @@ def test_no_workspace_for_reductions_that_are_not_split():
     for K in (7136, 7104, 7200):
         assert size(128, K, 2048, 0, 1) == size(128, K, 2048, 0, 0) == 0
     assert size(128, 7040, 2048, 0, 1) > 0
+
+
+def test_counts_of_another_gpu_are_refused(monkeypatch):
+    """The kernels read the counts where they are: those of another GPU than the rows' are refused."""
+    from torchturbo_amd.providers.hip import mx as provider
+
+    def launched(*a, **k):
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(provider, "_device", lambda *t: torch.device("cuda", 0))
+    monkeypatch.setattr(provider, "device_counts", lambda c, *a, **k: c)  # device counts come back as they are
+    monkeypatch.setattr(provider, "product", launched)
+    counts = torch.tensor([4, 0, 0], device="meta")  # on a device that is not cuda:0
+    with pytest.raises(ValueError, match="tokens_per_expert is on meta, the rows on cuda:0"):
+        HipGroupedMatmulMxfp4()(X, QE, SE, counts)

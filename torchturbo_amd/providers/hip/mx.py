@@ -227,6 +227,8 @@ class HipGroupedMatmulMxfp4(OpImpl):
             raise _no_gradient(op, "rows in 8 bits")
         dev = _device(values, xs, codes, scales, row_map, probs)
         counts = device_counts(tokens_per_expert, experts, dev, m=m)
+        if counts.device != dev:
+            raise ValueError(f"{op}: tokens_per_expert is on {counts.device}, the rows on {dev}")
         if sees:
             if mx_out:
                 raise _no_gradient(op, "outputs in 8 bits")
