@@ -205,3 +205,28 @@ def test_the_norms_rows_are_those_of_its_output(process_ops, tokens, residual):
             others.append(layer(x, residual=r))
     for other in others:
         assert all(torch.equal(a, b) for a, b in zip(want, other))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_every_token_against_64_bits(process_ops, eight):
+    """The bound of the block's norm for each token by itself: a token that took another's rows or experts
+    would be off by its whole norm. Roundings are uniform errors, so that a token's error comes to
+    1 / sqrt(3) of the sum of its steps and less, and with 256 features hardly varies."""
+    process_ops(CudaRuntime(), OpPolicy.CUSTOM)
+    layer = _layer(eight)
+    x, r = _tokens((600, H)), _tokens((600, H), 2)
+    with torch.no_grad():
+        got = layer(x, residual=r)[0].double().cpu()
+        probs, _, ids, _ = layer.router(layer.norm(x, r)[0])
+    y, _ = o_norm.norm(x.cpu(), layer.norm.weight.cpu(), 1e-6, r.cpu())
+    e, s = layer.experts, layer.shared_experts
+    ids, probs = ids.cpu(), probs.double().cpu()
+    want = o_mx.linear(o_mx.linear(y, s.q1.cpu(), s.s1.cpu(), F.silu, True), s.q2.cpu(), s.s2.cpu())
+    for i in range(E):
+        t, _ = (ids == i).nonzero(as_tuple=True)
+        a = o_mx.linear(y[t], e.q1[i].cpu(), e.s1[i].cpu(), F.silu, True) * probs[t, i].unsqueeze(1)
+        want[t] += o_mx.linear(a, e.q2[i].cpu(), e.s2[i].cpu())
+    steps = 4 * 2.0 ** -8 + (2 * 2.0 ** -4 if eight else 0.0)
+    error = (got - want).norm(dim=1) / want.norm(dim=1)
+    print(f"largest {error.max():.4f}, mean {error.mean():.4f}, bound {steps:.4f}")
+    assert (error <= steps).all()
