@@ -513,11 +513,14 @@ int tt_lora_wgrad_dropout(const void* x, const float* dh, int dtype, int64_t m, 
  *   W = N, or gated 2 N with the gates' rows first. epilogue: act (0 none, 1 SiLU, 2 GELU) of
  *   the product, gated: act of the first half times the second half; times probs[r] (f32 /
  *   bf16 / f16, or NULL). y: bf16, or with y_scales E4M3 codes and their E8M0 bytes (N a
- *   multiple of 32). Products are exact, sums run in fp32 and are rounded once.
+ *   multiple of 32). Sums run in fp32 and are rounded once. Products of bf16 rows are exact; of each
+ *   eight consecutive products of E4M3 rows the matrix instruction keeps what is at least 2^-13 of their
+ *   largest. M < 2^31, N < 2^30.
  *   tt_mx_product_workspace: bytes of scratch of a call of these sizes (0: none), 16-byte
  *   aligned; with less it does not split its reduction.
  * tt_mx_dgrad: dx [M, K] = dy [M, N] W[e], bf16, of weights that stay as they are.
- * x, codes and dx are 16-byte aligned; K is a multiple of 32; any M, N.
+ *   N < 2^24.
+ * x, codes and dx are 16-byte aligned; K is a multiple of 32.
  *
  * tt_rms_norm_fwd: h = x + residual (or x), y = h (mean(h^2) + eps)^(-1/2) weight over the
  *   last of [rows, cols], each of y, sum (h, rounded), rstd [rows] and codes / scales (y in

@@ -9,6 +9,11 @@
 // multiplied. One copy of W's piece leaves room for three blocks on a CU, which cover one another's
 // barriers (1531 x 2048 -> 5632 66 -> 54 us, 8192 rows of 128 experts 1536 -> 2048 155 -> 127, against
 // two copies and two blocks). Every product is exact in fp32; sums run in fp32 and dx is rounded once.
+//
+// Two limits: rows of dy off 16 bytes come by single elements through registers (1531 x 2047 -> 5632
+// 168 us for 56 at 2048, 8192 x 4095 -> 4096, which loses the larger tile too, 1009 for 232), and the
+// reduction is never split, so that few rows take the time of K / 128 blocks' loops (1 to 512 rows of 2048
+// -> 5632 23 to 26 us, 16 rows of 14336 -> 4096 144, 1 to 64 rows for each of 128 experts 1536 -> 2048 103 to 115).
 #include "mx_gemm.h"
 
 namespace {

@@ -11,6 +11,11 @@
 // instructions cover the other's waits, prologue and epilogue. Rows of 4-bit weights are a quarter of
 // bf16 rows' bytes (half of E4M3 rows'), which is why the tile is twice as wide in them.
 //
+// Reductions off 128 and scales off four bytes take 128 x 128, unsplit: the scales of a k-tile come by
+// single bytes through registers, and every k-tile waits for all of its loads. us at 7136 -> 2 x 2048, for
+// those at 7168: 128 rows 116 / 23, 1531 rows 155 / 109, 4096 rows 320 / 214; E4M3 rows 93 / 20, 155 / 64,
+// 316 / 105; 32 experts of 64 rows, 2016 -> 2 x 1024, for 2048 52 / 35, of 512 rows 213 / 147.
+//
 // E4M3 rows: k-tiles of 128, two stages (four of the smallest tile); codes are multiplied as they
 // are, with the groups' bytes as the instruction's scales (a row's four bytes of a k-tile are one
 // word in LDS).

@@ -10,10 +10,12 @@
 //
 //   dh = rho (a - xh mean(a xh)) + g_sum,  dw = sum over rows of gy xh.
 //
-// All of it is bound by memory: every tensor is read or written once (4.4 to 4.9 TB/s; a large copy
-// on this card reaches 5.1). A row stays in the registers of its threads between the sum of squares
-// and the product: a wave per row up to 2048 features, 256 threads to 8192, 1024 to 16384; longer
-// rows are read twice. Blocks go on to further rows with the weight kept, so that it is read once per
+// All of it is bound by memory: every tensor is read or written once (4.3 to 4.9 TB/s up to 8192 bf16
+// features, 5.7 in fp32; a large copy on this card reaches 5.1). Rows of features off eight and tensors off
+// 16 bytes are read and written by single elements, with no row in flight ahead (16384 x 2047 forward 186 us
+// for 56 at 2048, backward 211 for 56; fp32 4096 x 4095 142 for 46 and 131 for 48). A row stays in
+// the registers of its threads between the sum of squares and the product: a wave per row up to 2048
+// features, 256 threads to 8192, 1024 to 16384; longer rows are read twice. Blocks go on to further rows with the weight kept, so that it is read once per
 // block, and dw is summed in registers: one partial row per block, joined by a second kernel in the
 // order of the blocks.
 #include <initializer_list>
@@ -411,7 +413,8 @@ int row_chunks(int64_t H) {
 // Blocks of a launch: as many as a CU holds with a row in work and the next in flight (more start
 // later and wait for their first row; fewer leave memory idle). us at 16384 x 2048 / 4096 x 7168, bf16
 // with residual: forward in 512, 768, 2048 blocks 69 / 61 / 59 and 66 / 57 / 58, backward in 256, 512, 640
-// blocks 87 / 65 / 87 and 87 / 64 / 87; with no row in flight ahead 60 and 58, 97 and 98.
+// blocks 87 / 65 / 87 and 87 / 64 / 87; with no row in flight ahead 60 and 58, 97 and 98. Rows of 1024 threads
+// take the same numbers, of which a CU holds fewer at once: 2048 x 16384 56 and 79, 1024 x 32768 75 and 112.
 constexpr int64_t FWD_BLOCKS = 256 * 3, BWD_BLOCKS = 256 * 2;
 // Blocks along the features in the kernels of the weight's gradient, which keep their launches below
 // 2^32 threads (with BWD_BLOCKS parts of 256 threads, and alone of 1024) at any number of features.
