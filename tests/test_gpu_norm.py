@@ -285,3 +285,18 @@ def test_weight_gradient_of_more_features_than_a_launch_has_threads_for(hip_ops,
     assert all(torch.equal(a, b) for a, b in zip(y.detach(), x))
     dw, = torch.autograd.grad(y, w, gy)
     assert torch.equal(dw, want.to(torch.bfloat16))  # at most 99: exact
+
+
+def test_a_tensor_as_its_own_residual(hip_ops):
+    """Both of its gradients add up: h = 2 x, so dx is twice the sum's gradient."""
+    x, _, w = _inputs((6, 160), torch.float32, False)
+    leaf, wd = x.to(DEV).requires_grad_(), w.to(DEV)
+    y, h = hip_ops.rms_norm(leaf, wd, residual=leaf)
+    y.sum().add(h.sum()).backward()  # gradients of stride zero
+    other = (2 * x).to(DEV).requires_grad_()
+    want = hip_ops.rms_norm(other, wd)
+    dx, = torch.autograd.grad(want, other, torch.ones_like(want))
+    assert torch.equal(y, want) and torch.equal(h, other)
+    # 1 added within the kernel, or here: each rounds once, before the exact doubling.
+    bound = 2.0 ** -23 * (dx.abs() + 1) * 2
+    assert ((leaf.grad - 2 * (dx + 1)).abs() <= bound).all()
